@@ -1,0 +1,348 @@
+"""Measured cases of the block-scaled fp8 and gated feed-forward operators.
+
+Each case is a dict of plain values.  ``kind`` names the call a program makes:
+
+* ``quantize``    ``quantize_fp8``: e4m3 values with one fp32 scale for each 1 x 128 run of a row (activations,
+                  ``block_rows`` 1) or each 128 x 128 block (weights, ``block_rows`` 128);
+* ``matmul``      ``grouped_mm_fp8`` over expert-sorted rows, or ``matmul_fp8`` where G is 0: the product of operands
+                  quantised that way, weights stored [N, K] as linear layers and checkpoints store them;
+* ``gated_fp8``   ``grouped_mm_fp8_swiglu``: packed Gate+Up in fp8 with silu(gate) * up and the quantisation of the
+                  result for the down projection in the same launch;
+* ``train``       ``gate_up_swiglu_forward`` and ``gate_up_swiglu_backward``: the 16-bit gated block of a training step,
+                  its output and the gradients of its input and its weights.
+
+Rows are routed to the G experts unevenly; the row counts are a fixed function of the case and the seed says which
+expert gets which count.
+"""
+
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+_DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+_SIZES = {"bf16": 2, "fp16": 2, "fp32": 4}
+_BLOCK = 128
+_E4M3_MAX = 448.0
+_AMAX_FLOOR = 2.0 ** -96  # amax of a block of zeros
+
+
+def _kernels():
+    package = os.path.join(_ROOT, "moe-gemm-parallel-bench_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import kernels
+
+    return kernels
+
+
+def _case(kind, g, rows, k, n, dtype="bf16", **more):
+    """``n``: output columns (quantize: none; gated_fp8 and train: F, the width of the gate and of the up half)."""
+    return dict(kind=kind, G=g, rows=rows, K=k, N=n, dtype=dtype, **more)
+
+
+def listed():
+    return [
+        # One token's hidden state before a quantised projection: launch latency.
+        _case("quantize", 0, 1, 7168, 0, block_rows=1, name="quantize_token"),
+        # A prefill batch of 16384 routed rows: one read and half a write of HBM.
+        _case("quantize", 0, 16384, 7168, 0, block_rows=1, name="quantize_prefill"),
+        # fp32 master weights of 8 experts (packed W13, 2880 = 22.5 blocks), quantised after a load or an update.
+        _case("quantize", 8, 5760, 2880, 0, "fp32", block_rows=128, name="quantize_weights"),
+        # A dense linear layer at one token: 29 MB of weights, too few output tiles for the CUs.
+        _case("matmul", 0, 1, 7168, 4096, name="linear_token"),
+        # Packed W13 of one of 8 expert-parallel ranks in decode, about 8 rows an expert: 0.94 GB of weights.
+        _case("matmul", 32, 256, 7168, 4096, name="w13_decode"),
+        # W2 of the same rank in prefill, about 512 rows an expert.
+        _case("matmul", 32, 16384, 2048, 7168, name="w2_prefill"),
+        # Sizes that are no multiple of a tile or a block, few and uneven rows, fp16 out.
+        _case("matmul", 16, 1777, 2880, 2880, "fp16", name="ragged_fp16"),
+        # Gate+Up of a decode step, 64 tokens x top-8 over 128 small experts.
+        _case("gated_fp8", 128, 512, 2048, 768, name="gated_decode"),
+        # Gate+Up of one of 8 expert-parallel ranks in prefill.
+        _case("gated_fp8", 32, 16384, 7168, 2048, name="gated_prefill"),
+        # Training step of the smallest group of the test configurations: launch latency.
+        _case("train", 8, 512, 512, 512, name="train_small"),
+        # Training step over uneven experts, an odd row count and sizes off the tiles, fp16.
+        _case("train", 16, 4001, 2880, 2880, "fp16", name="train_ragged_fp16"),
+        # Training step of one of 8 expert-parallel ranks: the largest case.
+        _case("train", 32, 16384, 7168, 2048, name="train_prefill"),
+    ]
+
+
+_FLOP_CAP = {"quantize": 3e9, "matmul": 4e11, "gated_fp8": 4e11, "train": 6e11}
+_WEIGHT_CAP = 4e8  # weight elements
+
+
+def _log_uniform(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    while True:
+        kind = rng.choice(("quantize", "matmul", "gated_fp8", "train"))
+        if kind == "quantize":
+            block_rows = rng.choice((1, 1, 128))
+            # Any row count and any width, odd ones among them.
+            case = _case(kind, 0 if block_rows == 1 else _log_uniform(rng, 1, 32), _log_uniform(rng, 1, 16384),
+                         _log_uniform(rng, 128, 8192), 0, rng.choice(("bf16", "fp16", "fp32")), block_rows=block_rows)
+            n = max(1, case["G"]) * case["rows"] * case["K"]
+            if n <= 1.2e8:
+                return case
+            continue
+        g = _log_uniform(rng, 2, 128)
+        if kind == "matmul" and rng.random() < 0.3:
+            g = 0
+        step = 8 if kind == "train" else 16  # model widths
+        k = max(256, _log_uniform(rng, 256, 7168) // step * step)
+        n = max(128, _log_uniform(rng, 128, 4096) // 8 * 8)
+        case = _case(kind, g, _log_uniform(rng, 1, 16384), k, n, rng.choice(("bf16", "bf16", "fp16")))
+        wide = n if kind == "matmul" else 2 * n
+        if work(case)["flops"] <= _FLOP_CAP[kind] and max(1, g) * k * wide <= _WEIGHT_CAP:
+            return case
+
+
+def _counts(case):
+    """Rows of each expert, largest first: uneven expert popularity, whole rows by largest remainder."""
+    g, rows = case["G"], case["rows"]
+    popularity = np.exp(1.2 * (0.5 - (np.arange(g) + 0.5) / g))
+    share = rows * popularity / popularity.sum()
+    counts = np.floor(share).astype(int)
+    rest = rows - int(counts.sum())
+    counts[np.argsort(-(share - counts), kind="stable")[:rest]] += 1
+    return counts.tolist()
+
+
+def _active(case):
+    return sum(c > 0 for c in _counts(case)) if case["G"] else 1
+
+
+def _scale_of(amax):
+    return amax.clamp_min(_AMAX_FLOOR)
+
+
+def _padded_blocks(x, block_rows):
+    """x [..., R, K] as [..., R / block_rows, block_rows, K / 128, 128], zeros past its end."""
+    rows, k = x.shape[-2:]
+    pad = (0, -k % _BLOCK, 0, -rows % block_rows)
+    x = torch.nn.functional.pad(x, pad)
+    return x.reshape(*x.shape[:-2], x.shape[-2] // block_rows, block_rows, x.shape[-1] // _BLOCK, _BLOCK)
+
+
+def _quantized(x, block_rows):
+    """(e4m3 values, fp32 scales) of x [..., R, K]: scale = max|x| / 448 of each block, value = x * (448 / max|x|)."""
+    rows, k = x.shape[-2:]
+    blocks = _padded_blocks(x.float(), block_rows)
+    amax = _scale_of(blocks.abs().amax(dim=(-3, -1)))
+    values = blocks * (_E4M3_MAX / amax)[..., :, None, :, None]
+    values = values.reshape(*values.shape[:-4], -1, values.shape[-2] * _BLOCK)[..., :rows, :k]
+    return values.to(torch.float8_e4m3fn), amax / _E4M3_MAX
+
+
+def _dequantized(q, scale, block_rows):
+    """fp32 values of block-quantised q [..., R, K]."""
+    blocks = _padded_blocks(q.float(), block_rows) * scale[..., :, None, :, None]
+    rows, k = q.shape[-2:]
+    return blocks.reshape(*blocks.shape[:-4], -1, blocks.shape[-2] * _BLOCK)[..., :rows, :k]
+
+
+def _rows16(q):
+    """q on rows that start at multiples of 16 bytes, as ``quantize_fp8`` returns them."""
+    k = q.shape[-1]
+    buffer = torch.zeros((*q.shape[:-1], -(-k // 16) * 16), dtype=torch.uint8, device=q.device)
+    buffer[..., :k] = q.view(torch.uint8)
+    return buffer.view(torch.float8_e4m3fn)[..., :k]
+
+
+def prepare(case, seed):
+    """Activations: N(0, 1) with a channel spread of about e and a few large channels; weights N(0, 1 / sqrt(K)) with a
+    spread over their rows; gradients N(0, 1)."""
+    generator = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, dtype=torch.float32):
+        return torch.randn(shape, device="cuda", generator=generator, dtype=dtype)
+
+    kind, g, rows, k, n, dtype = (case[f] for f in ("kind", "G", "rows", "K", "N", "dtype"))
+    dtype = _DTYPES[dtype]
+    state = dict(case=case)
+    channels = normal(k).mul_(0.7).exp_()
+    channels[torch.randint(0, k, (max(1, k // 500),), device="cuda", generator=generator)] *= 20.0
+    if kind == "quantize":
+        shape = (g, rows, k) if g else (rows, k)
+        state["x"] = normal(*shape).mul_(channels).to(dtype)
+        return state
+    wide = n if kind == "matmul" else 2 * n
+    if g:
+        order = torch.randperm(g, generator=torch.Generator().manual_seed(seed)).tolist()
+        counts = _counts(case)
+        state["counts"] = [counts[i] for i in order]
+        state["offs"] = torch.tensor(np.cumsum(state["counts"]), device="cuda", dtype=torch.int32)
+    if kind == "train":
+        state["x"] = normal(rows, k).to(dtype)
+        state["w"] = normal(g, k, wide, dtype=dtype).mul_(1.0 / math.sqrt(k))
+        state["dh"] = normal(rows, n).to(dtype)
+        return state
+    state["a"], scale = _quantized(normal(rows, k).mul_(channels), 1)
+    state["a"] = _rows16(state["a"])
+    state["a_scale"] = scale.t().contiguous().t()  # a column of scales is contiguous, as quantize_fp8 returns them
+    groups = [_quantized(normal(wide, k, dtype=torch.bfloat16).mul_(1.0 / math.sqrt(k))
+                         * normal(wide, 1).mul_(0.3).exp_(), _BLOCK) for _ in range(max(1, g))]
+    weight, w_scale = torch.stack([q.view(torch.uint8) for q, _ in groups]), torch.stack([s for _, s in groups])
+    weight = _rows16(weight.view(torch.float8_e4m3fn))
+    state["w"], state["w_scale"] = (weight, w_scale) if g else (weight[0], w_scale[0])
+    return state
+
+
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+def _own(state):
+    ops = _kernels()
+    case = state["case"]
+    kind, dtype = case["kind"], _DTYPES[case["dtype"]]
+    if kind == "quantize":
+        q, scale = ops.quantize_fp8(state["x"], block_rows=case["block_rows"])
+        return {"q": q, "scale": scale}
+    if kind == "matmul":
+        if not case["G"]:
+            return ops.matmul_fp8(state["a"], state["a_scale"], state["w"], state["w_scale"], out_dtype=dtype)
+        return ops.grouped_mm_fp8(state["a"], state["a_scale"], state["w"], state["w_scale"], state["offs"],
+                                  out_dtype=dtype)
+    if kind == "gated_fp8":
+        q, scale = ops.grouped_mm_fp8_swiglu(state["a"], state["a_scale"], state["w"], state["w_scale"], state["offs"])
+        return {"q": q, "scale": scale}
+    h, saved = ops.gate_up_swiglu_forward(state["x"], state["w"], state["offs"])
+    dx, dw = ops.gate_up_swiglu_backward(state["dh"], state["x"], state["w"], state["offs"], saved)
+    return {"h": h, "dx": dx, "dw": dw}
+
+
+def _silu(x):
+    return x / (1.0 + torch.exp(-x))
+
+
+def _plain(state):
+    case = state["case"]
+    kind, dtype = case["kind"], _DTYPES[case["dtype"]]
+    if kind == "quantize":
+        q, scale = _quantized(state["x"], case["block_rows"])
+        return {"q": q, "scale": scale}
+    if kind == "train":
+        return _plain_train(state["x"].float(), state["w"].float(), state["dh"].float(), state["counts"], dtype)
+    a = _dequantized(state["a"], state["a_scale"], 1)
+    w = _dequantized(state["w"], state["w_scale"], _BLOCK)
+    if not case["G"]:
+        return (a @ w.t()).to(dtype)
+    product = torch.cat([rows @ weight.t() for rows, weight in zip(a.split(state["counts"]), w)])
+    if kind == "matmul":
+        return product.to(dtype)
+    gate, up = product.chunk(2, dim=1)
+    q, scale = _quantized(_silu(gate) * up, 1)
+    return {"q": q, "scale": scale}
+
+
+def _plain_train(x, w, dh, counts, dtype):
+    xs = x.split(counts)
+    gate, up = torch.cat([rows @ weight for rows, weight in zip(xs, w)]).chunk(2, dim=1)
+    sigmoid = 1.0 / (1.0 + torch.exp(-gate))
+    h = gate * sigmoid * up
+    dgate = dh * up * (sigmoid * (1.0 + gate * (1.0 - sigmoid)))
+    dup = dh * (gate * sigmoid)
+    ds = torch.cat([dgate, dup], dim=1).split(counts)
+    dx = torch.cat([d @ weight.t() for d, weight in zip(ds, w)])
+    dw = torch.stack([rows.t() @ d for rows, d in zip(xs, ds)])
+    return {"h": h.to(dtype), "dx": dx.to(dtype), "dw": dw.to(dtype)}
+
+
+def exact(case, seed):
+    """The definitions in 64 bits; fp8 values are given before their rounding to 8 bits."""
+    state = prepare(case, seed)
+    kind, k = case["kind"], case["K"]
+
+    def block_values(values, block_rows):
+        rows, width = values.shape
+        amax = torch.zeros((-(-rows // block_rows), -(-width // _BLOCK)), dtype=torch.float64, device="cuda")
+        for j in range(amax.shape[1]):
+            part = values[:, j * _BLOCK:(j + 1) * _BLOCK].abs().amax(dim=1)
+            if block_rows == 1:
+                amax[:, j] = part
+            else:
+                for i in range(amax.shape[0]):
+                    amax[i, j] = part[i * block_rows:(i + 1) * block_rows].max()
+        amax = amax.clamp(min=_AMAX_FLOOR)
+        wide = amax.repeat_interleave(block_rows, 0)[:rows].repeat_interleave(_BLOCK, 1)[:, :width]
+        return values / wide * _E4M3_MAX, amax / _E4M3_MAX
+
+    if kind == "quantize":
+        if not case["G"]:
+            q, scale = block_values(state["x"].double(), case["block_rows"])
+            return {"q": q, "scale": scale}
+        if state["x"].numel() > 2e8:
+            return None
+        parts = [block_values(x.double(), case["block_rows"]) for x in state["x"]]
+        return {"q": torch.stack([q for q, _ in parts]), "scale": torch.stack([s for _, s in parts])}
+
+    def experts():
+        if not case["G"]:
+            yield 0, 0, case["rows"]
+            return
+        first = 0
+        for e, count in enumerate(state["counts"]):
+            yield e, first, first + count
+            first += count
+
+    if kind == "train":
+        rows, n = case["rows"], case["N"]
+        h = torch.empty((rows, n), dtype=torch.float64, device="cuda")
+        dx = torch.empty((rows, k), dtype=torch.float64, device="cuda")
+        dw = torch.empty((case["G"], k, 2 * n), dtype=torch.float64, device="cuda")
+        for e, lo, hi in experts():
+            x, w, dh = state["x"][lo:hi].double(), state["w"][e].double(), state["dh"][lo:hi].double()
+            gate, up = x @ w[:, :n], x @ w[:, n:]
+            act = torch.sigmoid(gate)
+            h[lo:hi] = gate * act * up
+            dgate = dh * up * (act + gate * act * (1.0 - act))
+            dup = dh * gate * act
+            dx[lo:hi] = dgate @ w[:, :n].t() + dup @ w[:, n:].t()
+            dw[e, :, :n] = x.t() @ dgate
+            dw[e, :, n:] = x.t() @ dup
+        return {"h": h, "dx": dx, "dw": dw}
+
+    def spread(scale, block_rows, rows):
+        return scale.double().repeat_interleave(block_rows, 0)[:rows].repeat_interleave(_BLOCK, 1)[:, :k]
+
+    wide = state["w"].shape[-2]
+    a = state["a"].float().double() * spread(state["a_scale"], 1, case["rows"])
+    product = torch.empty((case["rows"], wide), dtype=torch.float64, device="cuda")
+    for e, lo, hi in experts():
+        w, s = (state["w"][e], state["w_scale"][e]) if case["G"] else (state["w"], state["w_scale"])
+        product[lo:hi] = a[lo:hi] @ (w.float().double() * spread(s, _BLOCK, wide)).t()
+    if kind == "matmul":
+        return product
+    gate, up = product[:, :case["N"]], product[:, case["N"]:]
+    q, scale = block_values(gate * torch.sigmoid(gate) * up, 1)
+    return {"q": q, "scale": scale}
+
+
+def work(case):
+    kind, rows, k, n = case["kind"], case["rows"], case["K"], case["N"]
+    blocks = -(-k // _BLOCK)
+    if kind == "quantize":
+        g = max(1, case["G"])
+        values = g * rows * k
+        scales = g * -(-rows // case["block_rows"]) * blocks
+        return {"bytes": values * (_SIZES[case["dtype"]] + 1) + 4 * scales, "flops": 3 * values}
+    active, es = _active(case), _SIZES[case["dtype"]]
+    if kind == "train":
+        weights = k * 2 * n
+        rows_bytes = rows * (2 * k + 2 * n) * es  # x and dx, h and dh
+        return {"bytes": rows_bytes + (active + case["G"]) * weights * es, "flops": 3 * 2 * rows * weights}
+    wide = n if kind == "matmul" else 2 * n
+    read = rows * (k + 4 * blocks) + active * (wide * k + 4 * blocks * -(-wide // _BLOCK))
+    written = rows * n * es if kind == "matmul" else rows * (n + 4 * -(-n // _BLOCK))
+    return {"bytes": read + written, "flops": 2 * rows * k * wide}
