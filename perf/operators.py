@@ -6,10 +6,13 @@ Each case is a dict of plain values.  ``kind`` names the call a program makes:
                   ``block_rows`` 1) or each 128 x 128 block (weights, ``block_rows`` 128);
 * ``matmul``      ``grouped_mm_fp8`` over expert-sorted rows, or ``matmul_fp8`` where G is 0: the product of operands
                   quantised that way, weights stored [N, K] as linear layers and checkpoints store them;
-* ``gated_fp8``   ``grouped_mm_fp8_swiglu``: packed Gate+Up in fp8 with silu(gate) * up and the quantisation of the
-                  result for the down projection in the same launch;
+* ``expert``      ``grouped_mm_fp8_swiglu`` and ``grouped_mm_fp8``: an expert layer in serving, packed Gate+Up with
+                  silu(gate) * up and its quantisation in one launch, then the down projection;
 * ``train``       ``gate_up_swiglu_forward`` and ``gate_up_swiglu_backward``: the 16-bit gated block of a training step,
                   its output and the gradients of its input and its weights.
+
+``fast`` cases let the 8-bit matrix instructions sum (``fast_accum``), as a serving program does in prefill; the others
+ask for fp32 sums throughout, the default.
 
 Rows are routed to the G experts unevenly; the row counts are a fixed function of the case and the seed says which
 expert gets which count.
@@ -42,7 +45,7 @@ def _kernels():
 
 
 def _case(kind, g, rows, k, n, dtype="bf16", **more):
-    """``n``: output columns (quantize: none; gated_fp8 and train: F, the width of the gate and of the up half)."""
+    """``n``: output columns (quantize: none; expert and train: F, the width of the gate and of the up half)."""
     return dict(kind=kind, G=g, rows=rows, K=k, N=n, dtype=dtype, **more)
 
 
@@ -59,13 +62,13 @@ def listed():
         # Packed W13 of one of 8 expert-parallel ranks in decode, about 8 rows an expert: 0.94 GB of weights.
         _case("matmul", 32, 256, 7168, 4096, name="w13_decode"),
         # W2 of the same rank in prefill, about 512 rows an expert.
-        _case("matmul", 32, 16384, 2048, 7168, name="w2_prefill"),
+        _case("matmul", 32, 16384, 2048, 7168, fast=True, name="w2_prefill"),
         # Sizes that are no multiple of a tile or a block, few and uneven rows, fp16 out.
         _case("matmul", 16, 1777, 2880, 2880, "fp16", name="ragged_fp16"),
-        # Gate+Up of a decode step, 64 tokens x top-8 over 128 small experts.
-        _case("gated_fp8", 128, 512, 2048, 768, name="gated_decode"),
-        # Gate+Up of one of 8 expert-parallel ranks in prefill.
-        _case("gated_fp8", 32, 16384, 7168, 2048, name="gated_prefill"),
+        # The experts of a decode step, 64 tokens x top-8 over 128 small experts.
+        _case("expert", 128, 512, 2048, 768, name="expert_decode"),
+        # The experts of one of 8 expert-parallel ranks in prefill.
+        _case("expert", 32, 16384, 7168, 2048, fast=True, name="expert_prefill"),
         # Training step of the smallest group of the test configurations: launch latency.
         _case("train", 8, 512, 512, 512, name="train_small"),
         # Training step over uneven experts, an odd row count and sizes off the tiles, fp16.
@@ -75,7 +78,7 @@ def listed():
     ]
 
 
-_FLOP_CAP = {"quantize": 3e9, "matmul": 4e11, "gated_fp8": 4e11, "train": 6e11}
+_FLOP_CAP = {"quantize": 3e9, "matmul": 4e11, "expert": 6e11, "train": 6e11}
 _WEIGHT_CAP = 4e8  # weight elements
 
 
@@ -85,7 +88,7 @@ def _log_uniform(rng, low, high):
 
 def draw(rng):
     while True:
-        kind = rng.choice(("quantize", "matmul", "gated_fp8", "train"))
+        kind = rng.choice(("quantize", "matmul", "expert", "train"))
         if kind == "quantize":
             block_rows = rng.choice((1, 1, 128))
             # Any row count and any width, odd ones among them.
@@ -102,6 +105,8 @@ def draw(rng):
         k = max(256, _log_uniform(rng, 256, 7168) // step * step)
         n = max(128, _log_uniform(rng, 128, 4096) // 8 * 8)
         case = _case(kind, g, _log_uniform(rng, 1, 16384), k, n, rng.choice(("bf16", "bf16", "fp16")))
+        if kind != "train":
+            case["fast"] = case["dtype"] == "bf16" and rng.random() < 0.5
         wide = n if kind == "matmul" else 2 * n
         if work(case)["flops"] <= _FLOP_CAP[kind] and max(1, g) * k * wide <= _WEIGHT_CAP:
             return case
@@ -190,11 +195,17 @@ def prepare(case, seed):
     state["a"], scale = _quantized(normal(rows, k).mul_(channels), 1)
     state["a"] = _rows16(state["a"])
     state["a_scale"] = scale.t().contiguous().t()  # a column of scales is contiguous, as quantize_fp8 returns them
-    groups = [_quantized(normal(wide, k, dtype=torch.bfloat16).mul_(1.0 / math.sqrt(k))
-                         * normal(wide, 1).mul_(0.3).exp_(), _BLOCK) for _ in range(max(1, g))]
-    weight, w_scale = torch.stack([q.view(torch.uint8) for q, _ in groups]), torch.stack([s for _, s in groups])
-    weight = _rows16(weight.view(torch.float8_e4m3fn))
-    state["w"], state["w_scale"] = (weight, w_scale) if g else (weight[0], w_scale[0])
+
+    def weights(out, width):
+        made = [_quantized(normal(out, width, dtype=torch.bfloat16).mul_(1.0 / math.sqrt(width))
+                           * normal(out, 1).mul_(0.3).exp_(), _BLOCK) for _ in range(max(1, g))]
+        q = _rows16(torch.stack([q.view(torch.uint8) for q, _ in made]).view(torch.float8_e4m3fn))
+        scale = torch.stack([s for _, s in made])
+        return (q, scale) if g else (q[0], scale[0])
+
+    state["w"], state["w_scale"] = weights(wide, k)
+    if kind == "expert":
+        state["w2"], state["w2_scale"] = weights(k, n)
     return state
 
 
@@ -209,14 +220,18 @@ def _own(state):
     if kind == "quantize":
         q, scale = ops.quantize_fp8(state["x"], block_rows=case["block_rows"])
         return {"q": q, "scale": scale}
-    if kind == "matmul":
+    if kind in ("matmul", "expert"):
+        fast = case.get("fast", False)
         if not case["G"]:
-            return ops.matmul_fp8(state["a"], state["a_scale"], state["w"], state["w_scale"], out_dtype=dtype)
-        return ops.grouped_mm_fp8(state["a"], state["a_scale"], state["w"], state["w_scale"], state["offs"],
-                                  out_dtype=dtype)
-    if kind == "gated_fp8":
-        q, scale = ops.grouped_mm_fp8_swiglu(state["a"], state["a_scale"], state["w"], state["w_scale"], state["offs"])
-        return {"q": q, "scale": scale}
+            return ops.matmul_fp8(state["a"], state["a_scale"], state["w"], state["w_scale"], out_dtype=dtype,
+                                  fast_accum=fast)
+        offs = state["offs"]
+        if kind == "matmul":
+            return ops.grouped_mm_fp8(state["a"], state["a_scale"], state["w"], state["w_scale"], offs, out_dtype=dtype,
+                                      fast_accum=fast)
+        h, scale = ops.grouped_mm_fp8_swiglu(state["a"], state["a_scale"], state["w"], state["w_scale"], offs,
+                                             fast_accum=fast)
+        return ops.grouped_mm_fp8(h, scale, state["w2"], state["w2_scale"], offs, out_dtype=dtype, fast_accum=fast)
     h, saved = ops.gate_up_swiglu_forward(state["x"], state["w"], state["offs"])
     dx, dw = ops.gate_up_swiglu_backward(state["dh"], state["x"], state["w"], state["offs"], saved)
     return {"h": h, "dx": dx, "dw": dw}
@@ -242,8 +257,9 @@ def _plain(state):
     if kind == "matmul":
         return product.to(dtype)
     gate, up = product.chunk(2, dim=1)
-    q, scale = _quantized(_silu(gate) * up, 1)
-    return {"q": q, "scale": scale}
+    h = _dequantized(*_quantized(_silu(gate) * up, 1), 1)
+    w2 = _dequantized(state["w2"], state["w2_scale"], _BLOCK)
+    return torch.cat([rows @ weight.t() for rows, weight in zip(h.split(state["counts"]), w2)]).to(dtype)
 
 
 def _plain_train(x, w, dh, counts, dtype):
@@ -260,7 +276,7 @@ def _plain_train(x, w, dh, counts, dtype):
 
 
 def exact(case, seed):
-    """The definitions in 64 bits; fp8 values are given before their rounding to 8 bits."""
+    """The definitions in 64 bits; quantised outputs are given before their rounding to 8 bits."""
     state = prepare(case, seed)
     kind, k = case["kind"], case["K"]
 
@@ -313,20 +329,23 @@ def exact(case, seed):
             dw[e, :, n:] = x.t() @ dup
         return {"h": h, "dx": dx, "dw": dw}
 
-    def spread(scale, block_rows, rows):
-        return scale.double().repeat_interleave(block_rows, 0)[:rows].repeat_interleave(_BLOCK, 1)[:, :k]
+    def values(q, scale, block_rows):
+        wide = scale.double().repeat_interleave(block_rows, 0)[:q.shape[0]]
+        return q.float().double() * wide.repeat_interleave(_BLOCK, 1)[:, :q.shape[1]]
 
-    wide = state["w"].shape[-2]
-    a = state["a"].float().double() * spread(state["a_scale"], 1, case["rows"])
-    product = torch.empty((case["rows"], wide), dtype=torch.float64, device="cuda")
-    for e, lo, hi in experts():
-        w, s = (state["w"][e], state["w_scale"][e]) if case["G"] else (state["w"], state["w_scale"])
-        product[lo:hi] = a[lo:hi] @ (w.float().double() * spread(s, _BLOCK, wide)).t()
+    def product(a, weight, scale):
+        out = torch.empty((case["rows"], weight.shape[-2]), dtype=torch.float64, device="cuda")
+        for e, lo, hi in experts():
+            w, s = (weight[e], scale[e]) if case["G"] else (weight, scale)
+            out[lo:hi] = a[lo:hi] @ values(w, s, _BLOCK).t()
+        return out
+
+    first = product(values(state["a"], state["a_scale"], 1), state["w"], state["w_scale"])
     if kind == "matmul":
-        return product
-    gate, up = product[:, :case["N"]], product[:, case["N"]:]
+        return first
+    gate, up = first[:, :case["N"]], first[:, case["N"]:]
     q, scale = block_values(gate * torch.sigmoid(gate) * up, 1)
-    return {"q": q, "scale": scale}
+    return product(values(q.to(torch.float8_e4m3fn), scale, 1), state["w2"], state["w2_scale"])
 
 
 def work(case):
@@ -342,7 +361,11 @@ def work(case):
         weights = k * 2 * n
         rows_bytes = rows * (2 * k + 2 * n) * es  # x and dx, h and dh
         return {"bytes": rows_bytes + (active + case["G"]) * weights * es, "flops": 3 * 2 * rows * weights}
-    wide = n if kind == "matmul" else 2 * n
-    read = rows * (k + 4 * blocks) + active * (wide * k + 4 * blocks * -(-wide // _BLOCK))
-    written = rows * n * es if kind == "matmul" else rows * (n + 4 * -(-n // _BLOCK))
-    return {"bytes": read + written, "flops": 2 * rows * k * wide}
+
+    def weight(out, width):
+        return out * width + 4 * -(-out // _BLOCK) * -(-width // _BLOCK)
+
+    read = rows * (k + 4 * blocks)
+    if kind == "matmul":
+        return {"bytes": read + active * weight(n, k) + rows * n * es, "flops": 2 * rows * k * n}
+    return {"bytes": read + active * (weight(2 * n, k) + weight(k, n)) + rows * k * es, "flops": 2 * rows * k * 3 * n}
