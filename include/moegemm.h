@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define MOEGEMM_ABI_VERSION 9
+#define MOEGEMM_ABI_VERSION 10
 
 #define MOEGEMM_OK 0
 #define MOEGEMM_ERR_INVALID (-1)   /* bad shape, pointer, dtype or parameter (Python: ValueError) */
@@ -322,6 +322,58 @@ int moegemm_matmul(const void* a, const void* b, void* c, int32_t m, int32_t n, 
                    int64_t stride_cm, int64_t stride_cn, int32_t dtype, int32_t input_precision,
                    int32_t block_m, int32_t block_n, int32_t block_k, int32_t group_size_m,
                    int32_t num_warps, int32_t num_stages, int32_t grid_size, int32_t b_stream, void* stream);
+
+/*
+ * Block-scaled fp8 (OCP e4m3): values with one fp32 scale for each 1 x 128 run of a row (activations) or
+ * each 128 x 128 block (weights), the format that model_configs/deepseek-v3.json names
+ * (quantization_config: fp8, e4m3, weight_block_size [128, 128]).  No counterpart in the reference,
+ * whose kernels take fp16, bf16 and fp32 only.
+ *
+ * moegemm_quantize_fp8: for each block, amax = max(max|x|, 2^-96), scale = amax / 448 and
+ * q = e4m3(x * (448 / amax)), round to nearest even.  A block that holds a NaN or an infinity becomes NaN.
+ * x is [batch, rows, k] (dtype; unit stride along k), q its bytes and scale
+ * [batch, rows / block_rows, k / 128], rounded up, with the given strides (elements).  block_rows is
+ * 1 or 128; q rows start at multiples of 8 bytes.
+ */
+int moegemm_quantize_fp8(const void* x, void* q, float* scale, int32_t batch, int32_t rows, int32_t k,
+                         int64_t stride_xb, int64_t stride_xr, int64_t stride_qb, int64_t stride_qr, int64_t stride_sb,
+                         int64_t stride_sr, int64_t stride_sk, int32_t dtype, int32_t block_rows, void* stream);
+
+/* Compiled variants of the fp8 products (gated: of moegemm_grouped_mm_fp8_swiglu), and whether one sums on the
+ * 8-bit matrix instructions (1), in fp32 (0), < 0 on a bad index. */
+int moegemm_fp8_variant_count(int32_t gated);
+int moegemm_fp8_variant_fast(int32_t gated, int32_t variant);
+
+/*
+ * C[r0:r1] = (A_q * scale_a)[r0:r1] @ (W_q[e] * scale_w[e])^T for each group e of rows r0 = offs[e-1] (0 for
+ * e = 0) to r1 = offs[e], offsets as in moegemm_grouped_mm_offs; offs NULL: one group of all rows.
+ * a is e4m3 [rows, k] with scale_a [rows, k / 128], w e4m3 [group_count, n, k] (a linear layer's weight,
+ * unit stride along k) with scale_w [group_count, n / 128, k / 128], rounded up.  Sums are fp32, out is
+ * out_dtype [rows, n] with unit column stride; k and n are arbitrary.  a, w and their pitches are multiples of 16
+ * bytes and pitches under 2^23.  Rows at or past offs[group_count-1] are not written.  fast_accum 1 lets the 8-bit matrix
+ * instructions form the sums inside a block, which keep about 14 bits below the largest of eight products, at
+ * twice the rate; 0 keeps them in fp32.  `variant` -1
+ * lets the library choose by rows, groups and columns; grid_size is the persistent grid (CUs; <= 0: 256).
+ */
+int moegemm_grouped_mm_fp8(const void* a, const float* scale_a, const void* w, const float* scale_w, void* out,
+                           const int32_t* offs, int32_t group_count, int32_t rows, int32_t n, int32_t k,
+                           int64_t stride_am, int64_t stride_sam, int64_t stride_sak, int64_t stride_wg,
+                           int64_t stride_wn, int64_t stride_swg, int64_t stride_swn, int64_t stride_swk,
+                           int64_t stride_om, int32_t out_dtype, int32_t fast_accum, int32_t variant,
+                           int32_t grid_size, void* stream);
+
+/*
+ * Packed Gate+Up in fp8 with the activation and the quantisation for the next product in the epilogue:
+ * w is [group_count, n = 2F, k], rows [gate | up] (F a multiple of 8); h = silu(a gate^T) * (a up^T) in fp32 is
+ * quantised as by moegemm_quantize_fp8 with block_rows 1 into out, e4m3 [rows, F] (row pitch stride_om), and
+ * out_scale [rows, F / 128].  Operands, offsets and rows that are not written as in moegemm_grouped_mm_fp8.
+ */
+int moegemm_grouped_mm_fp8_swiglu(const void* a, const float* scale_a, const void* w, const float* scale_w, void* out,
+                                  float* out_scale, const int32_t* offs, int32_t group_count, int32_t rows, int32_t n,
+                                  int32_t k, int64_t stride_am, int64_t stride_sam, int64_t stride_sak,
+                                  int64_t stride_wg, int64_t stride_wn, int64_t stride_swg, int64_t stride_swn,
+                                  int64_t stride_swk, int64_t stride_om, int64_t stride_osm, int64_t stride_osk,
+                                  int32_t fast_accum, int32_t variant, int32_t grid_size, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,7 @@
 #include <string>
 
 #include "../../include/moegemm.h"
+#include "error.h"
 #include "registry.h"
 
 using namespace moegemm;
@@ -306,6 +307,19 @@ int fail_transposed_homogeneous() {
 }
 
 }  // namespace
+
+namespace moegemm {
+
+int report(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+
+}  // namespace moegemm
 
 extern "C" {
 

@@ -1,0 +1,750 @@
+// Products of e4m3 operands with one fp32 scale for each block of 128 along K (gfx950).
+//
+//   C[m, n] = sum_b sa[m, b] sw[n / 128, b] * (sum_{k in block b} a[m, k] w[n, k])
+//
+// a [rows, K] carries a scale for each row and block of 128 columns, w [N, K] (a linear layer's
+// weight) one for each 128 x 128 block.  The inner sum runs on the matrix cores from a zero
+// accumulator; one fp32 FMA per output and block adds it, scaled, to the running sum.  Scales are
+// arbitrary fp32 numbers, so the matrix instructions' own power-of-two block scales cannot carry them.
+//
+// Two ways to form the inner sum:
+//  * exact: e4m3 values are widened to bf16 (exactly) in registers and multiplied with the bf16
+//    instructions, whose sums keep fp32's bits: 2^16 + 2^-7 comes back whole;
+//  * FAST: the 8-bit instructions (32x32x64), at twice the rate.  They add eight products at a time
+//    and drop what is below 2^-13 of the largest (2^16 + 8 came back whole, 2^16 + 4 as 2^16, where
+//    both products are among the same eight), then in fp32.  Fewer than 32 bits, so the caller has to
+//    ask for it; an output is off by at most 2^-10 sum |a w|.
+//
+// Operands are swapped (D^T = W A^T, as in gemm_kernel.h): a lane owns one output row m, so a
+// block's scale is one value per lane and fragment, and four consecutive columns n per register
+// quad, which the epilogue stores as vectors.  Within a block the order of k does not matter, so
+// fragments take their 32 bytes as two 16-byte chunks 64 bytes apart (or as the LDS swizzle likes
+// them), the same two for both operands.
+//
+// Rows are grouped by cumulative end offsets on the device as in MODE_OFFSETS (gemm_kernel.h), or
+// form one group (offs null).  Two kernels:
+//  * Fp8Tile (prefill): operands reach LDS by DMA, one 128-byte K slice (= one scale block) per
+//    stage, 16-byte chunks XOR-swizzled, read with ds_read_b128;
+//  * Fp8Stream (decode, few rows a group): weights go from HBM straight into registers, each byte
+//    read once, the waves of a workgroup split K and join their sums through LDS.  Exact sums only:
+//    HBM is the bound, and widening costs no time.
+#pragma once
+
+#include "gemm_fast.h"
+
+namespace moegemm {
+
+typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+typedef int32_t i32x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kScaleBlock = 128;
+constexpr float kE4m3Max = 448.0f;
+constexpr float kAmaxFloor = 0x1p-96f;  // amax of a block of zeros: a finite scale and its reciprocal
+
+struct Fp8Params {
+  const uint8_t* a;   // [rows, k], lda bytes between rows
+  const float* sa;    // [rows, blocks of k]
+  const uint8_t* w;   // [groups, n, k]
+  const float* sw;    // [groups, blocks of n, blocks of k]
+  void* out;          // [rows, n] (plain) or e4m3 [rows, n / 2] (gated)
+  float* out_scale;   // gated: [rows, blocks of n / 2]
+  const int32_t* offs;
+  int64_t lda, sam, sak;            // scale strides in elements
+  int64_t swg, ldw, ssg, ssn, ssk;  // weight strides in bytes, its scales' in elements
+  int64_t ldo, osm, osk;            // output row pitch in elements, output scale strides
+  int32_t groups, rows, n, k;
+  int32_t n_tiles;                  // column tiles (the launch's)
+};
+
+// Rows of group e: [row0, row0 + m), offsets clamped to [0, rows], a decreasing offset empty.
+__device__ __forceinline__ int group_rows(const int32_t* offs, int rows, int e, int& m) {
+  if (!offs) {
+    m = rows;
+    return 0;
+  }
+  const int lo = e == 0 ? 0 : min(max(offs[e - 1], 0), rows);
+  const int hi = min(max(offs[e], 0), rows);
+  m = max(hi - lo, 0);
+  return lo;
+}
+
+struct GroupTile {
+  int e, row0, m, local;
+};
+
+// The group of tile t when each group holds ceil(m / bm) * n_tiles tiles; false past the last one.
+// Each wave looks it up for itself, 64 groups at a time (wave-uniform result).
+__device__ __forceinline__ bool find_group_tile(const int32_t* offs, int groups, int rows, int bm, int n_tiles, int t,
+                                                GroupTile& g) {
+  const int lane = threadIdx.x & 63;
+  int64_t base = 0;
+  for (int first = 0; first < groups; first += 64) {
+    int m = 0, row0 = 0;
+    if (first + lane < groups) row0 = group_rows(offs, rows, first + lane, m);
+    const int64_t count = (int64_t)((m + bm - 1) / bm) * n_tiles;
+    int64_t sum = count;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t below = __shfl_up(sum, d);
+      if (lane >= d) sum += below;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > t);
+    if (past) {
+      const int hit = __builtin_ctzll(past);
+      g.e = first + hit;
+      g.row0 = __builtin_amdgcn_readlane(row0, hit);
+      g.m = __builtin_amdgcn_readlane(m, hit);
+      const int64_t before = base + __shfl(sum - count, hit);
+      g.local = uniform((int32_t)(t - before));
+      return true;
+    }
+    base = uniform((int64_t)(base + __shfl(sum, 63)));
+  }
+  return false;
+}
+
+__device__ __forceinline__ f32x16_t mfma_fp8(i32x8_t w, i32x8_t a, f32x16_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, 0, 0, 0, 0, 0, 0);
+}
+
+// The 8 e4m3 values of two dwords as bf16: exact, e4m3's range and 4 bits fit.
+__device__ __forceinline__ bf16x8_t widen(int32_t lo, int32_t hi) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// A lane's 32 bytes of a fragment, as they are (FAST) or widened.
+template <bool FAST>
+struct Fragment;
+template <>
+struct Fragment<true> {
+  i32x8_t v;
+  __device__ __forceinline__ void set(i32x8_t x) { v = x; }
+};
+template <>
+struct Fragment<false> {
+  bf16x8_t v[4];
+  __device__ __forceinline__ void set(i32x8_t x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = widen(x[2 * i], x[2 * i + 1]);
+  }
+};
+template <class ACC>
+__device__ __forceinline__ ACC block_sum(const Fragment<true>& w, const Fragment<true>& a, ACC c) {
+  return mfma_fp8(w.v, a.v, c);
+}
+template <class ACC>
+__device__ __forceinline__ ACC block_sum(const Fragment<false>& w, const Fragment<false>& a, ACC c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(ACC) == 64)
+      c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.v[i], a.v[i], c, 0, 0, 0);
+    else
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], a.v[i], c, 0, 0, 0);
+  }
+  return c;
+}
+
+__device__ __forceinline__ i32x8_t join(i32x4_t lo, i32x4_t hi) {
+  return i32x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// The first `bytes` (any int) of a 16-byte chunk, zeros behind them.
+__device__ __forceinline__ i32x4_t keep_bytes(i32x4_t v, int bytes) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int left = bytes - 4 * i;
+    const uint32_t mask = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+    v[i] = (int32_t)((uint32_t)v[i] & mask);
+  }
+  return v;
+}
+
+// silu(g) * u as the definition has it; the e4m3 rounding behind it is far coarser than rcp's 1 ulp.
+__device__ __forceinline__ float gated(float g, float u) {
+  return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * u;
+}
+
+// max of |x| as bit patterns: a NaN is larger than everything else, so it reaches the scale.
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+// amax with its floor (as bits; positive floats order like their bits).
+__device__ __forceinline__ float floored(uint32_t amax_bits) {
+  return __builtin_bit_cast(float, max(amax_bits, __builtin_bit_cast(uint32_t, kAmaxFloor)));
+}
+
+__device__ __forceinline__ int32_t pack_e4m3(f32x4_t v) {
+  int32_t r = 0;
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], r, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], r, true);
+}
+
+// One dword per lane by LDS-DMA: lane l's dword lands at `lds` + 4 l (see dma_copy16).
+__device__ __forceinline__ void dma_copy4(u32x4_t rsrc, uint32_t voffset, uint32_t lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+               :
+               : "v"(voffset), "s"(rsrc), "s"(lds)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
+// E: the output type (EBf16, EF16, EF32) of a plain product.  GATED: w is [gate | up] of n = 2F rows,
+// and a tile's BN weight rows are BN/2 = 128 gate rows and the 128 up rows that go with them.
+template <class E, int BM_, int BN_, int WM_, int WN_, int STAGES_, bool GATED_, bool FAST_>
+struct Fp8Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
+  static constexpr bool GATED = GATED_, FAST = FAST_;
+  static constexpr int NW = WM * WN, NT = NW * 64;
+  static constexpr int WTM = BM / WM, WTN = BN / WN, FM = WTM / 32, FN = WTN / 32;
+  static constexpr int A_BYTES = BM * kScaleBlock, B_BYTES = BN * kScaleBlock;
+  static constexpr int IA = A_BYTES / 1024, IB = B_BYTES / 1024;  // 1 KiB copies per stage: 8 rows of 128 bytes
+  static constexpr int QA = IA / NW, QB = IB / NW;
+  static constexpr int SA_WAVES = BM / 64;      // waves that copy the row scales of a stage
+  static constexpr int SCALE_BYTES = NW * 256;  // 64 dwords a wave: row scales, the weight's, unused ones
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SCALE_BYTES;
+  static constexpr int PER_STAGE = QA + QB + 1;  // copies of a wave per stage
+  static constexpr int RED_BYTES = GATED ? BM * WN * 4 : 0;  // row maxima of the waves that share a row
+  static constexpr int LDS_BYTES = STAGES * STAGE_BYTES + RED_BYTES;
+  static constexpr int OUT_COLS = GATED ? BN / 2 : BN;  // output columns of a tile
+  static_assert(IA % NW == 0 && IB % NW == 0, "every wave issues the same copies");
+  static_assert(SA_WAVES < NW, "one wave is left to copy the weight's scales");
+  static_assert(!GATED || (BN == 256 && FN % 2 == 0), "a gated tile is one 128-column block of the output");
+  static_assert(LDS_BYTES <= 160 * 1024, "LDS of one CU");
+  static_assert(STAGES * PER_STAGE < 64, "vmcnt is 6 bits");
+
+  struct Copies {
+    u32x4_t ra, rb, rb2;       // rb2: the up rows of a gated tile
+    uint32_t a_off[QA], b_off[QB];
+    uint32_t kch;              // this lane's k in a slice
+    uint32_t s_off;            // scale copy of this wave, or kOutOfRange
+    const float* s_base;
+    int64_t s_step;            // elements between blocks
+    uint32_t s_bytes;
+    uint32_t lds, lds_scale;
+    int k;
+  };
+
+  __device__ static __forceinline__ void setup(Copies& c, const Fp8Params& p, const GroupTile& g, int tm, int tn,
+                                               const char* smem) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int m0 = tm * BM;
+    const int valid_m = min(BM, g.m - m0);
+    c.k = p.k;
+    c.ra = make_rsrc(p.a + ((int64_t)g.row0 + m0) * p.lda, (uint32_t)valid_m * (uint32_t)p.lda);
+    const uint8_t* w = p.w + (int64_t)g.e * p.swg;
+    const int f = p.n >> 1;
+    const int n0 = tn * OUT_COLS;
+    const int valid_n = GATED ? min(BN / 2, f - n0) : min(BN, p.n - n0);
+    c.rb = make_rsrc(w + (int64_t)n0 * p.ldw, (uint32_t)valid_n * (uint32_t)p.ldw);
+    if constexpr (GATED) c.rb2 = make_rsrc(w + (int64_t)(f + n0) * p.ldw, (uint32_t)valid_n * (uint32_t)p.ldw);
+    c.lds = lds_address(smem) + (uint32_t)wave * 1024u;
+    c.lds_scale = lds_address(smem) + (uint32_t)(A_BYTES + B_BYTES + wave * 256);
+    // Row r of a panel keeps chunk c at c ^ swz_a(r, 8); wave w copies rows 8 (w + q NW) .. + 7.
+    const int r0 = wave * 8 + lane / 8;
+    const int ch = (lane & 7) ^ swz_a(r0, 8);  // swz_a of 8 chunks repeats every 32 rows, and NW * 8 is 32 or 64
+    c.kch = (uint32_t)ch * 16u;
+#pragma unroll
+    for (int q = 0; q < QA; ++q) c.a_off[q] = (uint32_t)(r0 + q * NW * 8) * (uint32_t)p.lda + c.kch;
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+      const int r = r0 + q * NW * 8;
+      c.b_off[q] = (uint32_t)(GATED && q >= QB / 2 ? r - BN / 2 : r) * (uint32_t)p.ldw + c.kch;
+    }
+    // Scales: waves 0 .. BM/64 - 1 fetch 64 rows' each, the next one the weight's (at most 4 values).
+    c.s_off = kOutOfRange;
+    if (wave < SA_WAVES) {
+      const int row = wave * 64 + lane;
+      c.s_base = p.sa + ((int64_t)g.row0 + m0) * p.sam;
+      c.s_step = p.sak;
+      if (row < valid_m) c.s_off = (uint32_t)row * (uint32_t)p.sam * 4u;
+    } else {
+      // Lane j: scale block of the tile's weight rows 128 j (plain); gated: the gate's, then the one or
+      // two blocks of the up rows, which start at any multiple of 8.
+      const int last = (p.n + kScaleBlock - 1) / kScaleBlock - 1;
+      int nb;
+      if constexpr (GATED)
+        nb = lane == 0 ? n0 / kScaleBlock : min((f + n0) / kScaleBlock + lane - 1, last);
+      else
+        nb = min(n0 / kScaleBlock + lane, last);
+      c.s_base = p.sw + (int64_t)g.e * p.ssg;
+      c.s_step = p.ssk;
+      if (wave == SA_WAVES && lane < 4) c.s_off = (uint32_t)nb * (uint32_t)p.ssn * 4u;
+    }
+    c.s_base = uniform(c.s_base);
+    c.s_step = uniform(c.s_step);
+  }
+
+  __device__ static __forceinline__ void issue(const Copies& c, int stage, int kt) {
+    const uint32_t base = c.lds + (uint32_t)(stage * STAGE_BYTES);
+    const uint32_t k0 = (uint32_t)kt * kScaleBlock;
+    const bool in_k = (int)(k0 + c.kch) < c.k;
+#pragma unroll
+    for (int q = 0; q < QA; ++q)
+      dma_copy16(c.ra, in_k ? c.a_off[q] + k0 : kOutOfRange, base + (uint32_t)(q * NW * 1024));
+#pragma unroll
+    for (int q = 0; q < QB; ++q)
+      dma_copy16(GATED && q >= QB / 2 ? c.rb2 : c.rb, in_k ? c.b_off[q] + k0 : kOutOfRange,
+                 base + (uint32_t)(A_BYTES + q * NW * 1024));
+    const bool in = (int)k0 < c.k;
+    dma_copy4(make_rsrc(c.s_base + (in ? kt : 0) * c.s_step, kOutOfRange), in ? c.s_off : kOutOfRange,
+              c.lds_scale + (uint32_t)(stage * STAGE_BYTES));
+  }
+
+  // 32 bytes of panel row x0 + lane % 32 for the j-th 64-byte half of the slice.  TAIL: bytes at or past
+  // `left` of the slice are zeroed (a K that is no multiple of 16 ends inside a chunk).
+  template <bool TAIL>
+  __device__ static __forceinline__ i32x8_t frag(const char* panel, int x0, int j, int left) {
+    const int lane = threadIdx.x & 63;
+    const int row = x0 + (lane & 31);
+    const int s = swz_a(row, 8);
+    const int c0 = j * 4 + (lane >> 5), c1 = c0 + 2;
+    i32x4_t lo = *reinterpret_cast<const i32x4_t*>(panel + row * kScaleBlock + ((c0 ^ s) << 4));
+    i32x4_t hi = *reinterpret_cast<const i32x4_t*>(panel + row * kScaleBlock + ((c1 ^ s) << 4));
+    if constexpr (TAIL) {
+      lo = keep_bytes(lo, left - c0 * 16);
+      hi = keep_bytes(hi, left - c1 * 16);
+    }
+    return join(lo, hi);
+  }
+
+  // First panel row of B fragment fn: gated waves hold their gate rows' fragments, then the up rows'.
+  __device__ static __forceinline__ int b_row(int fn, int wave_n) {
+    if constexpr (GATED)
+      return (fn < FN / 2 ? 0 : BN / 2) + wave_n * (WTN / 2) + (fn % (FN / 2)) * 32;
+    else
+      return wave_n * WTN + fn * 32;
+  }
+
+  // One slice.  `up_split`: up columns of the tile before the scale block boundary inside them.
+  template <bool TAIL>
+  __device__ static __forceinline__ void compute(f32x16_t (&acc)[FM][FN], const char* stage, int wave_m, int wave_n,
+                                                 int left, int up_split) {
+    const int lane = threadIdx.x & 63;
+    const float* scales = reinterpret_cast<const float*>(stage + A_BYTES + B_BYTES);
+    const float* sw = scales + SA_WAVES * 64;
+    Fragment<FAST> b[FN][2];
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) b[fn][j].set(frag<TAIL>(stage + A_BYTES, b_row(fn, wave_n), j, left));
+    // A fragment's sum is added while the next one's is formed: its FMAs run beside matrix instructions.
+    f32x16_t t[2];
+    float sa[FM];
+    Fragment<FAST> a[2];
+#pragma unroll
+    for (int x = 0; x <= FM * FN; ++x) {
+      if (x < FM * FN) {
+        const int fm = x / FN, fn = x % FN;
+        if (fn == 0) {
+          sa[fm] = scales[wave_m * WTM + fm * 32 + (lane & 31)];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) a[j].set(frag<TAIL>(stage, wave_m * WTM + fm * 32, j, left));
+        }
+        t[x & 1] = f32x16_t{};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) t[x & 1] = block_sum(b[fn][j], a[j], t[x & 1]);
+      }
+      if (x > 0) add_scaled(acc[(x - 1) / FN][(x - 1) % FN], t[(x - 1) & 1], sa[(x - 1) / FN], sw, (x - 1) % FN, wave_n,
+                            up_split);
+    }
+  }
+
+  // acc += t * scales for B fragment fn.
+  __device__ static __forceinline__ void add_scaled(f32x16_t& acc, const f32x16_t& t, float sa, const float* sw, int fn,
+                                                    int wave_n, int up_split) {
+    if (GATED && fn >= FN / 2) {
+      // Quad q of the fragment is up columns col + 8 q .. + 7: the block boundary falls between quads.
+      const int col = wave_n * (WTN / 2) + (fn - FN / 2) * 32;
+      const float s0 = sa * sw[1], s1 = sa * sw[2];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float s = col + q * 8 < up_split ? s0 : s1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[q * 4 + i] += t[q * 4 + i] * s;
+      }
+    } else {
+      const float s = sa * sw[GATED ? 0 : (wave_n * WTN + fn * 32) / kScaleBlock];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[i] += t[i] * s;
+    }
+  }
+
+  __device__ static __forceinline__ void store_plain(const f32x16_t (&acc)[FM][FN], const Fp8Params& p,
+                                                     const GroupTile& g, int tm, int tn, int wave_m, int wave_n) {
+    const int lane = threadIdx.x & 63;
+    constexpr int ES = sizeof(typename E::raw);
+    const bool vec = p.n % 4 == 0 && p.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (4 * ES - 1)) == 0;
+    const bool vec8 = ES == 2 && p.n % 8 == 0 && p.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      const int row = tm * BM + wave_m * WTM + fm * 32 + (lane & 31);
+      char* out = static_cast<char*>(p.out) + ((int64_t)g.row0 + row) * p.ldo * ES;
+      const bool in_m = row < g.m;
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn) {
+        const int n0 = tn * BN + wave_n * WTN + fn * 32;
+        if constexpr (ES == 2) {
+          if (vec8) {
+            // Lanes l and l + 32 hold columns 0-3 and 4-7 of an octet of the same row: they exchange
+            // halves of two octets, so that each stores 16 bytes.
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+              const u32x2_t x = pack4<E>(f32x4_t{acc[fm][fn][q * 4], acc[fm][fn][q * 4 + 1], acc[fm][fn][q * 4 + 2],
+                                                 acc[fm][fn][q * 4 + 3]});
+              const u32x2_t y = pack4<E>(f32x4_t{acc[fm][fn][q * 4 + 4], acc[fm][fn][q * 4 + 5],
+                                                 acc[fm][fn][q * 4 + 6], acc[fm][fn][q * 4 + 7]});
+              const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+              const auto s1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+              const int n = n0 + q * 8 + (lane >> 5) * 8;
+              if (in_m && n < p.n)
+                *MOEGEMM_GLOBAL(u32x4_t, out + (int64_t)n * 2) = u32x4_t{s0[0], s1[0], s0[1], s1[1]};
+            }
+            continue;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n0 + q * 8 + (lane >> 5) * 4;
+          const f32x4_t v = {acc[fm][fn][q * 4], acc[fm][fn][q * 4 + 1], acc[fm][fn][q * 4 + 2],
+                             acc[fm][fn][q * 4 + 3]};
+          if (!in_m) continue;
+          if (vec) {
+            if (n < p.n) store4<E>(out + (int64_t)n * ES, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (n + i < p.n) store1<E>(out + (int64_t)(n + i) * ES, v[i]);
+          }
+        }
+      }
+    }
+  }
+
+  // silu(gate) * up of the tile's 128 output columns, their maximum per row over the waves that share
+  // it (through `red`), and the quantised row.
+  __device__ static __forceinline__ void store_gated(f32x16_t (&acc)[FM][FN], const Fp8Params& p, const GroupTile& g,
+                                                     int tm, int tn, int wave_m, int wave_n, uint32_t* red) {
+    const int lane = threadIdx.x & 63;
+    const int f = p.n >> 1;
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int fn = 0; fn < FN / 2; ++fn)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float h = gated(acc[fm][fn][i], acc[fm][fn + FN / 2][i]);
+          acc[fm][fn][i] = h;
+          top = max(top, abs_bits(h));  // columns past F are zeros
+        }
+      const auto other = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+      top = max(other[0], other[1]);
+      if (lane < 32) red[(wave_m * WTM + fm * 32 + lane) * WN + wave_n] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      const int local = wave_m * WTM + fm * 32 + (lane & 31);
+      const int row = tm * BM + local;
+      uint32_t top = 0;
+#pragma unroll
+      for (int w = 0; w < WN; ++w) top = max(top, red[local * WN + w]);
+      const float amax = floored(top);
+      const float inverse = kE4m3Max / amax;
+      const bool in_m = row < g.m;
+      if (in_m && wave_n == 0 && lane < 32)
+        p.out_scale[((int64_t)g.row0 + row) * p.osm + (int64_t)tn * p.osk] = amax / kE4m3Max;
+      uint8_t* out = static_cast<uint8_t*>(p.out) + ((int64_t)g.row0 + row) * p.ldo;
+#pragma unroll
+      for (int fn = 0; fn < FN / 2; ++fn)
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          f32x4_t v, u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[i] = acc[fm][fn][q * 4 + i] * inverse;
+            u[i] = acc[fm][fn][q * 4 + 4 + i] * inverse;
+          }
+          const auto s = __builtin_amdgcn_permlane32_swap(pack_e4m3(v), pack_e4m3(u), false, false);
+          const int n = tn * (BN / 2) + wave_n * (WTN / 2) + fn * 32 + q * 8 + (lane >> 5) * 8;
+          if (in_m && n < f) *MOEGEMM_GLOBAL(u32x2_t, out + n) = u32x2_t{s[0], s[1]};
+        }
+    }
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
+  __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wave_m = wave / T::WN, wave_n = wave % T::WN;
+  const int grid = gridDim.x;
+  // Each round of `grid` tiles is split into eight contiguous runs, one per XCD (workgroup b runs on
+  // XCD b % 8), so that the tiles that share an expert's panels read them through one L2.
+  int t = (int)blockIdx.x;
+  if ((grid & 7) == 0) t = (t & 7) * (grid >> 3) + (t >> 3);
+  const int kt_count = (p.k + kScaleBlock - 1) / kScaleBlock;
+  const int last_bytes = p.k - (kt_count - 1) * kScaleBlock;
+  const int f = p.n >> 1;
+  GroupTile g;
+  for (; find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g); t += grid) {
+    int tm, tn;
+    group_m_order(g.local, (g.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm, tn);
+    typename T::Copies c;
+    T::setup(c, p, g, tm, tn, smem);
+    const int up_split = kScaleBlock - (f + tn * T::OUT_COLS) % kScaleBlock;
+    f32x16_t acc[T::FM][T::FN];
+#pragma unroll
+    for (int fm = 0; fm < T::FM; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < T::FN; ++fn) acc[fm][fn] = f32x16_t{};
+#pragma unroll
+    for (int s = 0; s < T::STAGES - 1; ++s) T::issue(c, s, s);
+    int stage = 0;
+    for (int kt = 0; kt < kt_count; ++kt) {
+      // Slice kt has landed once only the STAGES - 2 younger slices' copies are outstanding, for every
+      // wave after the barrier, which also says that slice kt - 1 has been read: its buffer is refilled.
+      wait_vmcnt<(T::STAGES - 2) * T::PER_STAGE>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      compiler_fence();
+      const int refill = stage == 0 ? T::STAGES - 1 : stage - 1;
+      T::issue(c, refill, kt + T::STAGES - 1);
+      const char* cur = smem + stage * T::STAGE_BYTES;
+      if (kt + 1 == kt_count && (last_bytes & 15))
+        T::template compute<true>(acc, cur, wave_m, wave_n, last_bytes, up_split);
+      else
+        T::template compute<false>(acc, cur, wave_m, wave_n, 0, up_split);
+      stage = stage + 1 == T::STAGES ? 0 : stage + 1;
+    }
+    wait_vmcnt<0>();
+    if constexpr (T::GATED)
+      T::store_gated(acc, p, g, tm, tn, wave_m, wave_n,
+                     reinterpret_cast<uint32_t*>(smem + T::STAGES * T::STAGE_BYTES));
+    else
+      T::store_plain(acc, p, g, tm, tn, wave_m, wave_n);
+    __syncthreads();  // every wave is done with the slices before the next tile's copies
+  }
+}
+
+// Decode: 16 FM rows of a group by 16 FN columns per wave, WN waves along the columns, WK waves that
+// take K blocks wk, wk + WK, ...  Each wave keeps U blocks of weights and rows in flight in registers.
+template <class E, int FM_, int FN_, int WN_, int WK_, int U_, bool GATED_>
+struct Fp8Stream {
+  static constexpr int FM = FM_, FN = FN_, WN = WN_, WK = WK_, U = U_;
+  static constexpr bool GATED = GATED_;
+  static constexpr int NW = WN * WK, NT = NW * 64;
+  static constexpr int BM = 16 * FM, BN = 16 * FN * WN;
+  static constexpr int OUT_COLS = GATED ? BN / 2 : BN;
+  static constexpr int FRAGS = FM * FN * WN;  // accumulator fragments of a tile
+  static constexpr int RED_BYTES = WK * FRAGS * 1024;
+  static constexpr int LDS_BYTES = RED_BYTES + (GATED ? BM * 8 * 4 : 0);
+  static_assert(!GATED || (OUT_COLS == kScaleBlock && FN % 2 == 0), "a gated tile is one block of the output");
+};
+
+template <class T, class E>
+__global__ void __launch_bounds__(T::NT) fp8_stream_kernel(Fp8Params p) {
+  constexpr int FM = T::FM, FN = T::FN, WN = T::WN, WK = T::WK, U = T::U;
+  constexpr bool GATED = T::GATED;
+  __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wn = wave % WN, wk = wave / WN;
+  const int e = (int)blockIdx.x / p.n_tiles, tn = (int)blockIdx.x % p.n_tiles;
+  int m;
+  const int row0 = group_rows(p.offs, p.rows, e, m);
+  if (m == 0) return;
+  const int f = p.n >> 1;
+  const int blocks = (p.k + kScaleBlock - 1) / kScaleBlock;
+  const int kch = (lane >> 4) * 16;  // this lane's chunks start at kch and kch + 64 of a block
+  const int n0 = tn * T::OUT_COLS + wn * (GATED ? 8 : 16) * FN;  // the wave's first output column
+  const uint8_t* w = p.w + (int64_t)e * p.swg;
+  const float* sw = p.sw + (int64_t)e * p.ssg;
+  // Weight rows of fragment fn, in one buffer resource from the fragment's first row; gated waves hold
+  // their gate fragments, then the up ones.
+  auto first_row = [&](int fn) {
+    if constexpr (GATED) return (fn < FN / 2 ? 0 : f) + n0 + (fn % (FN / 2)) * 16;
+    return n0 + fn * 16;
+  };
+  auto valid_rows = [&](int fn) {
+    const int end = GATED ? f - (n0 + (fn % (FN > 1 ? FN / 2 : 1)) * 16) : p.n - (n0 + fn * 16);
+    return min(max(end, 0), 16);
+  };
+  const uint32_t w_off = (uint32_t)(lane & 15) * (uint32_t)p.ldw + (uint32_t)kch;
+  const int last_n = (p.n + kScaleBlock - 1) / kScaleBlock - 1;
+
+  for (int m0 = 0; m0 < m; m0 += T::BM) {
+    const int valid_m = min(T::BM, m - m0);
+    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a) + ((int64_t)row0 + m0) * p.lda,
+                                                      (short)0, (int)((uint32_t)valid_m * (uint32_t)p.lda),
+                                                      (int)kBufferFlags);
+    f32x4_t acc[FM][FN];
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn) acc[fm][fn] = f32x4_t{};
+
+    i32x4_t wv[U][FN][2], av[U][FM][2];
+    float sv[U][FM];
+    // Blocks at or past the end load zeros (values and row scales) and add nothing.
+    auto load = [&](int u, int kb) {
+      const uint32_t k0 = (uint32_t)kb * kScaleBlock;
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn) {
+        const auto rw = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(w) + (int64_t)first_row(fn) * p.ldw, (short)0,
+            (int)((uint32_t)valid_rows(fn) * (uint32_t)p.ldw), (int)kBufferFlags);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool in = (int)k0 + kch + j * 64 < p.k;
+          wv[u][fn][j] = __builtin_bit_cast(
+              i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? w_off + k0 + j * 64 : kOutOfRange, 0, kNonTemporal));
+        }
+      }
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm) {
+        const int r = fm * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool in = (int)k0 + kch + j * 64 < p.k;
+          av[u][fm][j] = __builtin_bit_cast(
+              i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                           ra, in ? (uint32_t)r * (uint32_t)p.lda + kch + k0 + j * 64 : kOutOfRange, 0, 0));
+        }
+        sv[u][fm] = 0.0f;
+        if (kb < blocks && r < valid_m)
+          sv[u][fm] = p.sa[((int64_t)row0 + m0 + r) * p.sam + (int64_t)kb * p.sak];
+      }
+    };
+    auto consume = [&](int u, int kb) {
+      if (kb >= blocks) return;
+      if (kb + 1 == blocks && (p.k & 15)) {
+        const int left = p.k - kb * kScaleBlock - kch;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int fn = 0; fn < FN; ++fn) wv[u][fn][j] = keep_bytes(wv[u][fn][j], left - j * 64);
+#pragma unroll
+          for (int fm = 0; fm < FM; ++fm) av[u][fm][j] = keep_bytes(av[u][fm][j], left - j * 64);
+        }
+      }
+      Fragment<false> a[FM];
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm) a[fm].set(join(av[u][fm][0], av[u][fm][1]));
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn) {
+        Fragment<false> b;
+        b.set(join(wv[u][fn][0], wv[u][fn][1]));
+        // A fragment's 16 weight rows lie in one scale block, except up rows that start at a multiple of 8.
+        const int r = first_row(fn);
+        const float s0 = sw[(int64_t)min(r / kScaleBlock, last_n) * p.ssn + (int64_t)kb * p.ssk];
+        float s_w = s0;
+        if constexpr (GATED) {
+          if (fn >= FN / 2) {
+            const float s1 = sw[(int64_t)min((r + 15) / kScaleBlock, last_n) * p.ssn + (int64_t)kb * p.ssk];
+            s_w = (r + (lane >> 4) * 4) / kScaleBlock == r / kScaleBlock ? s0 : s1;
+          }
+        }
+#pragma unroll
+        for (int fm = 0; fm < FM; ++fm) {
+          const f32x4_t t = block_sum(b, a[fm], f32x4_t{});
+          const float s = sv[u][fm] * s_w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[fm][fn][i] += t[i] * s;
+        }
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(u, wk + u * WK);
+    for (int kb = wk; kb < blocks; kb += U * WK) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        consume(u, kb + u * WK);
+        load(u, kb + (u + U) * WK);
+      }
+    }
+
+    // Join the WK sums of every fragment in wave order: fragment id (fm, fn, wn) is summed by wave id % NW.
+    f32x4_t* red = reinterpret_cast<f32x4_t*>(smem);
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn) red[((wk * T::FRAGS) + (fm * FN + fn) * WN + wn) * 64 + lane] = acc[fm][fn];
+    __syncthreads();
+    auto total = [&](int id) {
+      f32x4_t v = red[id * 64 + lane];
+#pragma unroll
+      for (int x = 1; x < WK; ++x) v += red[(x * T::FRAGS + id) * 64 + lane];
+      return v;
+    };
+    if constexpr (!GATED) {
+      constexpr int ES = sizeof(typename E::raw);
+      const bool vec = p.n % 4 == 0 && p.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (4 * ES - 1)) == 0;
+      for (int id = wave; id < T::FRAGS; id += T::NW) {
+        const int fw = id % WN, fn = id / WN % FN, fm = id / WN / FN;
+        const f32x4_t v = total(id);
+        const int row = fm * 16 + (lane & 15);
+        const int n = tn * T::BN + fw * 16 * FN + fn * 16 + (lane >> 4) * 4;
+        if (row >= valid_m || n >= p.n) continue;
+        char* out = static_cast<char*>(p.out) + (((int64_t)row0 + m0 + row) * p.ldo + n) * ES;
+        if (vec) {
+          store4<E>(out, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + i < p.n) store1<E>(out + i * ES, v[i]);
+        }
+      }
+    } else {
+      // Output fragment id (fm, fn < FN / 2, wn): 8 of them make up a row's 128 columns.
+      constexpr int OUTS = T::FRAGS / 2, MINE = (OUTS + T::NW - 1) / T::NW;
+      uint32_t* tops = reinterpret_cast<uint32_t*>(smem + T::RED_BYTES);  // [row][8]
+      f32x4_t h[MINE];
+#pragma unroll
+      for (int x = 0; x < MINE; ++x) {
+        const int id = wave + x * T::NW;
+        if (id >= OUTS) continue;
+        const int fw = id % WN, fn = id / WN % (FN / 2), fm = id / WN / (FN / 2);
+        const f32x4_t gate = total((fm * FN + fn) * WN + fw), up = total((fm * FN + fn + FN / 2) * WN + fw);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          h[x][i] = gated(gate[i], up[i]);
+          top = max(top, abs_bits(h[x][i]));
+        }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        if (lane < 16) tops[(fm * 16 + lane) * 8 + fw * (FN / 2) + fn] = top;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < MINE; ++x) {
+        const int id = wave + x * T::NW;
+        if (id >= OUTS) continue;
+        const int fw = id % WN, fn = id / WN % (FN / 2), fm = id / WN / (FN / 2);
+        const int row = fm * 16 + (lane & 15);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, tops[row * 8 + i]);
+        const float amax = floored(top), inverse = kE4m3Max / amax;
+        if (row >= valid_m) continue;
+        if (fw == 0 && fn == 0 && lane < 16)
+          p.out_scale[((int64_t)row0 + m0 + row) * p.osm + (int64_t)tn * p.osk] = amax / kE4m3Max;
+        const int n = tn * T::OUT_COLS + fw * 8 * FN + fn * 16 + (lane >> 4) * 4;
+        if (n < f)
+          *MOEGEMM_GLOBAL(int32_t, static_cast<uint8_t*>(p.out) + ((int64_t)row0 + m0 + row) * p.ldo + n) =
+              pack_e4m3(h[x] * inverse);
+      }
+    }
+    __syncthreads();  // the sums are read before the next rows' are written
+  }
+}
+
+}  // namespace moegemm

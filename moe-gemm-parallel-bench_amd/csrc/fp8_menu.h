@@ -1,0 +1,62 @@
+// Compiled variants of the block-scaled fp8 products, one table per output type (inst_fp8_*.hip).
+#pragma once
+
+#include "fp8_gemm.h"
+
+namespace moegemm {
+
+typedef hipError_t (*Fp8LaunchFn)(const Fp8Params&, int grid, hipStream_t stream);
+
+struct Fp8Variant {
+  int block_m, block_n;  // rows and weight rows of a tile
+  int stream;            // 1: a workgroup per (group, column tile); 0: persistent over tiles
+  int fast;              // sums on the 8-bit matrix instructions
+  Fp8LaunchFn launch;
+};
+
+template <class T>
+hipError_t launch_fp8_tile(const Fp8Params& p, int grid, hipStream_t stream) {
+  hipLaunchKernelGGL((fp8_tile_kernel<T>), dim3(grid), dim3(T::NT), 0, stream, p);
+  return hipGetLastError();
+}
+template <class T, class E>
+hipError_t launch_fp8_stream(const Fp8Params& p, int grid, hipStream_t stream) {
+  hipLaunchKernelGGL((fp8_stream_kernel<T, E>), dim3(grid), dim3(T::NT), 0, stream, p);
+  return hipGetLastError();
+}
+
+// X(E, BM, BN, WAVES_M, WAVES_N, STAGES, FAST) and Y(E, FM, FN, WAVES_N, WAVES_K, BLOCKS_IN_FLIGHT, unused).
+#define MOEGEMM_MENU_FP8(X, Y, E)                                                               \
+  X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 3, true) X(E, 128, 128, 2, 2, 3, true)     \
+  X(E, 128, 256, 2, 4, 3, false) X(E, 128, 128, 2, 2, 3, false)                                 \
+  Y(E, 1, 1, 1, 8, 4, 0) Y(E, 1, 4, 1, 4, 3, 0) Y(E, 2, 4, 1, 4, 2, 0) Y(E, 4, 4, 1, 4, 1, 0)
+#define MOEGEMM_MENU_FP8_GATED(X, Y, E)                                                         \
+  X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 3, true) X(E, 128, 256, 2, 4, 3, false)    \
+  Y(E, 1, 4, 4, 2, 3, 0) Y(E, 2, 4, 4, 2, 2, 0)
+
+#define MOEGEMM_FP8_X(E, BM, BN, WM, WN, S, FAST) \
+  Fp8Variant{BM, BN, 0, FAST, &launch_fp8_tile<Fp8Tile<E, BM, BN, WM, WN, S, false, FAST>>},
+#define MOEGEMM_FP8_Y(E, FM, FN, WN, WK, U, F) \
+  Fp8Variant{16 * FM, 16 * FN * WN, 1, 0, &launch_fp8_stream<Fp8Stream<E, FM, FN, WN, WK, U, false>, E>},
+#define MOEGEMM_FP8_GX(E, BM, BN, WM, WN, S, FAST) \
+  Fp8Variant{BM, BN, 0, FAST, &launch_fp8_tile<Fp8Tile<E, BM, BN, WM, WN, S, true, FAST>>},
+#define MOEGEMM_FP8_GY(E, FM, FN, WN, WK, U, F) \
+  Fp8Variant{16 * FM, 16 * FN * WN, 1, 0, &launch_fp8_stream<Fp8Stream<E, FM, FN, WN, WK, U, true>, E>},
+
+// The kernels of a menu, for the device pass.
+#define MOEGEMM_FP8_XK(E, BM, BN, WM, WN, S, FAST) \
+  template __global__ void fp8_tile_kernel<Fp8Tile<E, BM, BN, WM, WN, S, false, FAST>>(Fp8Params);
+#define MOEGEMM_FP8_YK(E, FM, FN, WN, WK, U, F) \
+  template __global__ void fp8_stream_kernel<Fp8Stream<E, FM, FN, WN, WK, U, false>, E>(Fp8Params);
+#define MOEGEMM_FP8_GXK(E, BM, BN, WM, WN, S, FAST) \
+  template __global__ void fp8_tile_kernel<Fp8Tile<E, BM, BN, WM, WN, S, true, FAST>>(Fp8Params);
+#define MOEGEMM_FP8_GYK(E, FM, FN, WN, WK, U, F) \
+  template __global__ void fp8_stream_kernel<Fp8Stream<E, FM, FN, WN, WK, U, true>, E>(Fp8Params);
+
+#define MOEGEMM_FP8_COUNT(E, A, B, C, D, S, F) +1
+constexpr int kNumFp8 = 0 MOEGEMM_MENU_FP8(MOEGEMM_FP8_COUNT, MOEGEMM_FP8_COUNT, );
+constexpr int kNumFp8Gated = 0 MOEGEMM_MENU_FP8_GATED(MOEGEMM_FP8_COUNT, MOEGEMM_FP8_COUNT, );
+
+extern const Fp8Variant kFp8Bf16[], kFp8F16[], kFp8F32[], kFp8Gated[];
+
+}  // namespace moegemm

@@ -1,0 +1,8 @@
+// Compiled fp8 products with fp16 output.
+#include "fp8_menu.h"
+namespace moegemm {
+MOEGEMM_MENU_FP8(MOEGEMM_FP8_XK, MOEGEMM_FP8_YK, EF16)
+#if !defined(__HIP_DEVICE_COMPILE__)
+const Fp8Variant kFp8F16[] = {MOEGEMM_MENU_FP8(MOEGEMM_FP8_X, MOEGEMM_FP8_Y, EF16)};
+#endif
+}  // namespace moegemm

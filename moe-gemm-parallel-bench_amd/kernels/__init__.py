@@ -1,5 +1,6 @@
 """gfx950 HIP grouped/single GEMM kernels and the PyTorch grouped_mm comparison provider."""
 
+from .fp8 import grouped_mm_fp8, grouped_mm_fp8_swiglu, matmul_fp8, quantize_fp8
 from .grouped_gemm import (
     GroupedWorkspace,
     build_fused_gate_up_workspace,
@@ -44,6 +45,8 @@ __all__ = [
     "build_torch_grouped_workspace",
     "grouped_candidate_configs",
     "grouped_mm",
+    "grouped_mm_fp8",
+    "grouped_mm_fp8_swiglu",
     "grouped_mm_swiglu",
     "last_grouped_mm_config",
     "last_grouped_mm_schedule",
@@ -54,6 +57,8 @@ __all__ = [
     "launch_matmul",
     "launch_torch_grouped",
     "matmul_candidate_configs",
+    "matmul_fp8",
+    "quantize_fp8",
     "select_config",
     "torch_grouped_mm_unavailable_reason",
 ]

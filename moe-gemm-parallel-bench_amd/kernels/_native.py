@@ -16,7 +16,7 @@ from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().with_name("libmoegemm.so")
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 OK = 0
 ERR_INVALID = -1
 ERR_NO_KERNEL = -2
@@ -113,6 +113,22 @@ SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32,
          _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp],
+    ),
+    "moegemm_quantize_fp8": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _vp],
+    ),
+    "moegemm_fp8_variant_count": (ctypes.c_int, [_i32]),
+    "moegemm_fp8_variant_fast": (ctypes.c_int, [_i32, _i32]),
+    "moegemm_grouped_mm_fp8": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i32, _i32, _i32, _i32, _vp],
+    ),
+    "moegemm_grouped_mm_fp8_swiglu": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i32, _i32, _i32, _vp],
     ),
 }
 
