@@ -1,6 +1,7 @@
 """gfx950 HIP grouped/single GEMM kernels and the PyTorch grouped_mm comparison provider."""
 
 from .fp8 import grouped_mm_fp8, grouped_mm_fp8_swiglu, matmul_fp8, quantize_fp8
+from .gated_ffn import gate_up_swiglu, gate_up_swiglu_backward, gate_up_swiglu_forward
 from .grouped_gemm import (
     GroupedWorkspace,
     build_fused_gate_up_workspace,
@@ -43,6 +44,9 @@ __all__ = [
     "build_grouped_workspace",
     "build_offsets_workspace",
     "build_torch_grouped_workspace",
+    "gate_up_swiglu",
+    "gate_up_swiglu_backward",
+    "gate_up_swiglu_forward",
     "grouped_candidate_configs",
     "grouped_mm",
     "grouped_mm_fp8",

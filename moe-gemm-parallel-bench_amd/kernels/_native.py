@@ -130,6 +130,23 @@ SIGNATURES = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
          _i64, _i64, _i64, _i32, _i32, _i32, _vp],
     ),
+    "moegemm_gate_up_variant_count": (ctypes.c_int, [_i32]),
+    "moegemm_gate_up_forward": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
+    ),
+    "moegemm_gate_up_gradient": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i32, _i32, _vp],
+    ),
+    "moegemm_gate_up_dx": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
+    ),
+    "moegemm_gate_up_dw": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
+    ),
 }
 
 

@@ -1,0 +1,158 @@
+"""Training form of the packed Gate+Up block over expert-sorted rows on gfx950: forward and backward.
+
+``h = silu(x W_gate) * (x W_up)`` per expert, with W [G, H, 2F] = [gate | up] as ``grouped_mm_swiglu`` takes it.
+The forward pass is one launch that also keeps the projections [g | u] in fp32; the backward pass is three: the
+elementwise gradient of [g | u], then ``dx`` and ``dW``.  The reference times the forward GEMMs only (README.md:55-57).
+
+``gate_up_swiglu`` is the differentiable call; ``gate_up_swiglu_forward`` and ``gate_up_swiglu_backward`` are
+its two halves for programs that run their own backward pass.  Offsets are read on the device at run time, calls run
+on the current stream, and repeated calls give the same bits.  ``ValueError`` for operands the kernels cannot take,
+``RuntimeError`` without library or GPU.
+"""
+
+from __future__ import annotations
+
+from . import _native
+from .fp8 import _cu_count
+from .matmul import _require_runtime
+
+
+def _rows_ok(tensor) -> bool:
+    """Unit inner stride and rows at multiples of 16 bytes."""
+    return (tensor.stride(-1) == 1 and tensor.data_ptr() % 16 == 0
+            and all(s % 8 == 0 for s, d in zip(tensor.stride()[:-1], tensor.shape[:-1]) if d > 1))
+
+
+def _validate(x, weight, offs):
+    """(rows, H, F, groups) of the block's operands."""
+    import torch
+
+    grouped = offs is not None
+    if x.ndim != 2 or weight.ndim != (3 if grouped else 2):
+        raise ValueError("expected a 2-D x [rows, H] and " + ("a 3-D weight [G, H, 2F]" if grouped else
+                                                               "a 2-D weight [H, 2F]"))
+    rows, h = x.shape
+    groups = weight.shape[0] if grouped else 1
+    if weight.shape[-2] != h:
+        raise ValueError(f"contraction mismatch: x H={h}, weight H={weight.shape[-2]}")
+    if x.dtype not in (torch.float16, torch.bfloat16) or weight.dtype != x.dtype:
+        raise ValueError("x and weight must both be fp16 or bf16")
+    if groups <= 0 or h <= 0 or h % 8 or weight.shape[-1] <= 0 or weight.shape[-1] % 16:
+        raise ValueError(f"H and F must be positive multiples of 8 (H={h}, packed width {weight.shape[-1]})")
+    tensors = (x, weight) + ((offs,) if grouped else ())
+    if len({t.device for t in tensors}) != 1 or x.device.type != "cuda":
+        raise ValueError("x, weight and offs must be on the same GPU device")
+    if grouped:
+        if offs.ndim != 1 or offs.dtype != torch.int32 or offs.shape[0] != groups:
+            raise ValueError(f"offs must be an int32 vector with one entry per group ({groups})")
+        if not offs.is_contiguous():
+            raise ValueError("offs must be contiguous (pass offs.contiguous())")
+    for name, t in (("x", x), ("weight", weight)):
+        if not _rows_ok(t):
+            raise ValueError(f"{name} needs a unit inner stride and rows at multiples of 16 bytes")
+    return int(rows), int(h), weight.shape[-1] // 2, int(groups)
+
+
+def _pitch(tensor) -> int:
+    """Row stride (of a single row, any that covers it)."""
+    return tensor.stride(-2) if tensor.shape[-2] > 1 else tensor.shape[-1]
+
+
+def _group_stride(weight) -> int:
+    return weight.stride(0) if weight.ndim == 3 and weight.shape[0] > 1 else 0
+
+
+def _offs(offs):
+    return None if offs is None else offs.data_ptr()
+
+
+def gate_up_swiglu_forward(x, weight, offs=None, *, variant: int | None = None):
+    """``(h, saved)``: h [rows, F] = silu(x @ W[:, :F]) * (x @ W[:, F:]) and the fp32 projections saved [rows, 2F].
+
+    x is expert-sorted [rows, H]; weight [G, H, 2F] with int32 end rows ``offs`` [G] on the device, or [H, 2F] without.
+    fp16 or bf16, H and F multiples of 8, rows at multiples of 16 bytes.  Rows at or past offs[-1] get h = 0; their
+    saved values are unspecified.
+    """
+    import torch
+
+    rows, h, f, groups = _validate(x, weight, offs)
+    _require_runtime(x)
+    out = torch.empty((rows, f), dtype=x.dtype, device=x.device)
+    saved = torch.empty((rows, 2 * f), dtype=torch.float32, device=x.device)
+    if rows:
+        status = _native.library().moegemm_gate_up_forward(
+            x.data_ptr(), weight.data_ptr(), out.data_ptr(), saved.data_ptr(), _offs(offs), groups, rows, h, f, _pitch(x),
+            _group_stride(weight), _pitch(weight), f, _native.dtype_code(x.dtype), -1 if variant is None else variant,
+            _cu_count(x.device), _native.current_stream_handle(x.device))
+        _native.check(status)
+    return out, saved
+
+
+def gate_up_swiglu_backward(dh, x, weight, offs, saved, *, need_dx: bool = True, need_dw: bool = True,
+                            variants: tuple[int, int] | None = None):
+    """``(dx, dw)`` of ``gate_up_swiglu_forward`` for the gradient dh [rows, F] of its h; None for one not needed.
+
+    The gradient of [g | u] is rounded once to the operand type before the two products.  dx [rows, H] is zero past
+    offs[-1], dw [G, H, 2F] (or [H, 2F]) is zero for an expert without rows.
+    """
+    import torch
+
+    rows, h, f, groups = _validate(x, weight, offs)
+    if tuple(dh.shape) != (rows, f) or dh.dtype != x.dtype or dh.device != x.device:
+        raise ValueError(f"dh must be a [{rows}, {f}] {x.dtype} matrix on x's device")
+    if (tuple(saved.shape) != (rows, 2 * f) or saved.dtype != torch.float32 or saved.device != x.device
+            or not saved.is_contiguous()):
+        raise ValueError(f"saved must be the contiguous [{rows}, {2 * f}] float32 tensor of the forward pass")
+    if not _rows_ok(dh):
+        dh = dh.contiguous()  # autograd hands out expanded and transposed gradients
+    _require_runtime(x)
+    code, cus = _native.dtype_code(x.dtype), _cu_count(x.device)
+    lib, stream = _native.library(), _native.current_stream_handle(x.device)
+    dx_variant, dw_variant = variants or (-1, -1)
+    dp = torch.empty((rows, 2 * f), dtype=x.dtype, device=x.device)
+    _native.check(lib.moegemm_gate_up_gradient(dh.data_ptr(), saved.data_ptr(), dp.data_ptr(), _offs(offs), groups, rows,
+                                               f, _pitch(dh), code, cus, stream))
+    dx = dw = None
+    if need_dx:
+        dx = torch.empty((rows, h), dtype=x.dtype, device=x.device)
+        _native.check(lib.moegemm_gate_up_dx(dp.data_ptr(), weight.data_ptr(), dx.data_ptr(), _offs(offs), groups, rows, h,
+                                             f, _group_stride(weight), _pitch(weight), h, code, dx_variant, cus, stream))
+    if need_dw:
+        dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
+        _native.check(lib.moegemm_gate_up_dw(x.data_ptr(), dp.data_ptr(), dw.data_ptr(), _offs(offs), groups, rows, h, f,
+                                             _pitch(x), h * 2 * f, 2 * f, code, dw_variant, cus, stream))
+    return dx, dw
+
+
+def gate_up_swiglu(x, weight, offs=None):
+    """Differentiable h [rows, F] = silu(x @ W_gate) * (x @ W_up) per expert (``gate_up_swiglu_forward``'s operands)."""
+    return _function().apply(x, weight, offs)
+
+
+_FUNCTION: list = []
+
+
+def _function():
+    """The autograd function, made on first use (this package imports torch lazily)."""
+    if _FUNCTION:
+        return _FUNCTION[0]
+    import torch
+
+    class GateUpSwiglu(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, offs):
+            h, saved = gate_up_swiglu_forward(x, weight, offs)
+            ctx.save_for_backward(x, weight, saved, *(() if offs is None else (offs,)))
+            return h
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, dh):
+            x, weight, saved, *offs = ctx.saved_tensors
+            need_dx, need_dw = ctx.needs_input_grad[:2]
+            dx, dw = gate_up_swiglu_backward(dh, x, weight, offs[0] if offs else None, saved, need_dx=need_dx,
+                                             need_dw=need_dw)
+            return dx, dw, None
+
+    _FUNCTION.append(GateUpSwiglu)
+    return GateUpSwiglu
