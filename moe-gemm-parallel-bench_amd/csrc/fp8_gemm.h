@@ -218,25 +218,40 @@ struct Fp8Tile {
   static_assert(LDS_BYTES <= 160 * 1024, "LDS of one CU");
   static_assert(STAGES * PER_STAGE < 64, "vmcnt is 6 bits");
 
+  // What a wave's copies are made of: lane constants of the launch, and a tile's bases (wave-uniform).
   struct Copies {
-    u32x4_t ra, rb, rb2;       // rb2: the up rows of a gated tile
-    uint32_t a_off[QA], b_off[QB];
+    uint32_t a_off, b_off;     // first copy's byte offset in a panel; later ones are NW * 8 rows further on
+    uint32_t a_step, b_step;   // NW * 8 rows in bytes
     uint32_t kch;              // this lane's k in a slice
-    uint32_t s_off;            // scale copy of this wave, or kOutOfRange
-    const float* s_base;
-    int64_t s_step;            // elements between blocks
-    uint32_t s_bytes;
     uint32_t lds, lds_scale;
     int k;
+    u32x4_t ra, rb, rb2;       // rb2: the up rows of a gated tile
+    uint32_t s_off;            // scale copy of this lane, or kOutOfRange
+    const float* s_base;
+    int64_t s_step;            // elements between blocks
   };
 
-  __device__ static __forceinline__ void setup(Copies& c, const Fp8Params& p, const GroupTile& g, int tm, int tn,
-                                               const char* smem) {
+  __device__ static __forceinline__ void start(Copies& c, const Fp8Params& p, const char* smem) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    c.k = p.k;
+    c.lds = lds_address(smem) + (uint32_t)wave * 1024u;
+    c.lds_scale = lds_address(smem) + (uint32_t)(A_BYTES + B_BYTES + wave * 256);
+    // Row r of a panel keeps chunk c at c ^ swz_a(r, 8); wave w copies rows 8 (w + q NW) .. + 7.
+    const int r0 = wave * 8 + lane / 8;
+    const int ch = (lane & 7) ^ swz_a(r0, 8);  // swz_a of 8 chunks repeats every 32 rows, and NW * 8 is 32 or 64
+    c.kch = (uint32_t)ch * 16u;
+    c.a_off = (uint32_t)r0 * (uint32_t)p.lda + c.kch;
+    c.b_off = (uint32_t)r0 * (uint32_t)p.ldw + c.kch;
+    c.a_step = (uint32_t)p.lda * (NW * 8);
+    c.b_step = (uint32_t)p.ldw * (NW * 8);
+  }
+
+  __device__ static __forceinline__ void set_tile(Copies& c, const Fp8Params& p, const GroupTile& g, int tm, int tn) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int m0 = tm * BM;
     const int valid_m = min(BM, g.m - m0);
-    c.k = p.k;
     c.ra = make_rsrc(p.a + ((int64_t)g.row0 + m0) * p.lda, (uint32_t)valid_m * (uint32_t)p.lda);
     const uint8_t* w = p.w + (int64_t)g.e * p.swg;
     const int f = p.n >> 1;
@@ -244,19 +259,6 @@ struct Fp8Tile {
     const int valid_n = GATED ? min(BN / 2, f - n0) : min(BN, p.n - n0);
     c.rb = make_rsrc(w + (int64_t)n0 * p.ldw, (uint32_t)valid_n * (uint32_t)p.ldw);
     if constexpr (GATED) c.rb2 = make_rsrc(w + (int64_t)(f + n0) * p.ldw, (uint32_t)valid_n * (uint32_t)p.ldw);
-    c.lds = lds_address(smem) + (uint32_t)wave * 1024u;
-    c.lds_scale = lds_address(smem) + (uint32_t)(A_BYTES + B_BYTES + wave * 256);
-    // Row r of a panel keeps chunk c at c ^ swz_a(r, 8); wave w copies rows 8 (w + q NW) .. + 7.
-    const int r0 = wave * 8 + lane / 8;
-    const int ch = (lane & 7) ^ swz_a(r0, 8);  // swz_a of 8 chunks repeats every 32 rows, and NW * 8 is 32 or 64
-    c.kch = (uint32_t)ch * 16u;
-#pragma unroll
-    for (int q = 0; q < QA; ++q) c.a_off[q] = (uint32_t)(r0 + q * NW * 8) * (uint32_t)p.lda + c.kch;
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-      const int r = r0 + q * NW * 8;
-      c.b_off[q] = (uint32_t)(GATED && q >= QB / 2 ? r - BN / 2 : r) * (uint32_t)p.ldw + c.kch;
-    }
     // Scales: waves 0 .. BM/64 - 1 fetch 64 rows' each, the next one the weight's (at most 4 values).
     c.s_off = kOutOfRange;
     if (wave < SA_WAVES) {
@@ -285,33 +287,42 @@ struct Fp8Tile {
     const uint32_t base = c.lds + (uint32_t)(stage * STAGE_BYTES);
     const uint32_t k0 = (uint32_t)kt * kScaleBlock;
     const bool in_k = (int)(k0 + c.kch) < c.k;
+    uint32_t a0 = in_k ? c.a_off + k0 : kOutOfRange, b0 = in_k ? c.b_off + k0 : kOutOfRange;
+    // The steps are added here: hoisted out of the loop, the offsets of eight copies took spilled registers.
+    // An out-of-range start stays out of range: the steps add less than 2 GiB to it.
+    asm volatile("" : "+v"(a0), "+v"(b0));
 #pragma unroll
-    for (int q = 0; q < QA; ++q)
-      dma_copy16(c.ra, in_k ? c.a_off[q] + k0 : kOutOfRange, base + (uint32_t)(q * NW * 1024));
+    for (int q = 0; q < QA; ++q) dma_copy16(c.ra, a0 + (uint32_t)q * c.a_step, base + (uint32_t)(q * NW * 1024));
 #pragma unroll
-    for (int q = 0; q < QB; ++q)
-      dma_copy16(GATED && q >= QB / 2 ? c.rb2 : c.rb, in_k ? c.b_off[q] + k0 : kOutOfRange,
+    for (int q = 0; q < QB; ++q) {
+      const bool up = GATED && q >= QB / 2;
+      dma_copy16(up ? c.rb2 : c.rb, b0 + (uint32_t)(up ? q - QB / 2 : q) * c.b_step,
                  base + (uint32_t)(A_BYTES + q * NW * 1024));
+    }
     const bool in = (int)k0 < c.k;
     dma_copy4(make_rsrc(c.s_base + (in ? kt : 0) * c.s_step, kOutOfRange), in ? c.s_off : kOutOfRange,
               c.lds_scale + (uint32_t)(stage * STAGE_BYTES));
   }
 
-  // 32 bytes of panel row x0 + lane % 32 for the j-th 64-byte half of the slice.  TAIL: bytes at or past
-  // `left` of the slice are zeroed (a K that is no multiple of 16 ends inside a chunk).
-  template <bool TAIL>
-  __device__ static __forceinline__ i32x8_t frag(const char* panel, int x0, int j, int left) {
+  // 32 bytes of panel row x0 + lane % 32 for the j-th 64-byte half of the slice.
+  __device__ static __forceinline__ i32x8_t frag(const char* panel, int x0, int j) {
     const int lane = threadIdx.x & 63;
     const int row = x0 + (lane & 31);
     const int s = swz_a(row, 8);
     const int c0 = j * 4 + (lane >> 5), c1 = c0 + 2;
-    i32x4_t lo = *reinterpret_cast<const i32x4_t*>(panel + row * kScaleBlock + ((c0 ^ s) << 4));
-    i32x4_t hi = *reinterpret_cast<const i32x4_t*>(panel + row * kScaleBlock + ((c1 ^ s) << 4));
-    if constexpr (TAIL) {
-      lo = keep_bytes(lo, left - c0 * 16);
-      hi = keep_bytes(hi, left - c1 * 16);
+    const char* p = panel + row * kScaleBlock;
+    return join(*reinterpret_cast<const i32x4_t*>(p + ((c0 ^ s) << 4)),
+                *reinterpret_cast<const i32x4_t*>(p + ((c1 ^ s) << 4)));
+  }
+
+  // A K that is no multiple of 16 ends inside a chunk: zeros to the bytes of a landed slice from `left` on,
+  // a thread per panel row.
+  __device__ static __forceinline__ void cut_tail(char* stage, int left) {
+    for (int r = threadIdx.x; r < BM + BN; r += NT) {
+      // Panel rows of A, then of B, are 128 bytes each; swz_a repeats every 32 rows and BM is a multiple of it.
+      i32x4_t* chunk = reinterpret_cast<i32x4_t*>(stage + r * kScaleBlock + (((left >> 4) ^ swz_a(r, 8)) << 4));
+      *chunk = keep_bytes(*chunk, left & 15);
     }
-    return join(lo, hi);
   }
 
   // First panel row of B fragment fn: gated waves hold their gate rows' fragments, then the up rows'.
@@ -322,59 +333,88 @@ struct Fp8Tile {
       return wave_n * WTN + fn * 32;
   }
 
-  // One slice.  `up_split`: up columns of the tile before the scale block boundary inside them.
-  template <bool TAIL>
-  __device__ static __forceinline__ void compute(f32x16_t (&acc)[FM][FN], const char* stage, int wave_m, int wave_n,
-                                                 int left, int up_split) {
-    const int lane = threadIdx.x & 63;
+  // What a wave holds of the slice it works on.  a is double-buffered over row fragments; the first
+  // fragments of the next slice replace these while the last ones are multiplied.
+  struct Slice {
+    Fragment<FAST> a[2][2], b[FN][2];
+    float sa[FM];
+    float sw[GATED ? 3 : 1];  // gated: the gate's scale, the up's before and from its block boundary on
+  };
+  __device__ static __forceinline__ void load_a(Slice& s, const char* stage, int wave_m, int fm) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s.a[fm & 1][j].set(frag(stage, wave_m * WTM + fm * 32, j));
+  }
+  __device__ static __forceinline__ void load_b(Slice& s, const char* stage, int wave_n, int fn) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s.b[fn][j].set(frag(stage + A_BYTES, b_row(fn, wave_n), j));
+  }
+  __device__ static __forceinline__ void load_scales(Slice& s, const char* stage, int wave_m, int wave_n) {
     const float* scales = reinterpret_cast<const float*>(stage + A_BYTES + B_BYTES);
     const float* sw = scales + SA_WAVES * 64;
-    Fragment<FAST> b[FN][2];
 #pragma unroll
-    for (int fn = 0; fn < FN; ++fn)
+    for (int fm = 0; fm < FM; ++fm) s.sa[fm] = scales[wave_m * WTM + fm * 32 + (threadIdx.x & 31)];
+    if constexpr (GATED) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) b[fn][j].set(frag<TAIL>(stage + A_BYTES, b_row(fn, wave_n), j, left));
-    // A fragment's sum is added while the next one's is formed: its FMAs run beside matrix instructions.
-    f32x16_t t[2];
-    float sa[FM];
-    Fragment<FAST> a[2];
-#pragma unroll
-    for (int x = 0; x <= FM * FN; ++x) {
-      if (x < FM * FN) {
-        const int fm = x / FN, fn = x % FN;
-        if (fn == 0) {
-          sa[fm] = scales[wave_m * WTM + fm * 32 + (lane & 31)];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) a[j].set(frag<TAIL>(stage, wave_m * WTM + fm * 32, j, left));
-        }
-        t[x & 1] = f32x16_t{};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) t[x & 1] = block_sum(b[fn][j], a[j], t[x & 1]);
-      }
-      if (x > 0) add_scaled(acc[(x - 1) / FN][(x - 1) % FN], t[(x - 1) & 1], sa[(x - 1) / FN], sw, (x - 1) % FN, wave_n,
-                            up_split);
+      for (int i = 0; i < 3; ++i) s.sw[i] = sw[i];
+    } else {
+      static_assert(kScaleBlock % WTN == 0, "a wave's columns lie in one scale block");
+      s.sw[0] = sw[wave_n * WTN / kScaleBlock];
     }
   }
 
+  // A fragment's sum of one block, waiting to be added while the next one's is formed.
+  struct Pending {
+    f32x16_t t;
+    float s0, s1;
+  };
   // acc += t * scales for B fragment fn.
-  __device__ static __forceinline__ void add_scaled(f32x16_t& acc, const f32x16_t& t, float sa, const float* sw, int fn,
-                                                    int wave_n, int up_split) {
+  __device__ static __forceinline__ void add(f32x16_t& acc, const Pending& p, int fn, int wave_n, int up_split) {
     if (GATED && fn >= FN / 2) {
       // Quad q of the fragment is up columns col + 8 q .. + 7: the block boundary falls between quads.
       const int col = wave_n * (WTN / 2) + (fn - FN / 2) * 32;
-      const float s0 = sa * sw[1], s1 = sa * sw[2];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float s = col + q * 8 < up_split ? s0 : s1;
+        const float s = col + q * 8 < up_split ? p.s0 : p.s1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[q * 4 + i] += t[q * 4 + i] * s;
+        for (int i = 0; i < 4; ++i) acc[q * 4 + i] += p.t[q * 4 + i] * s;
       }
     } else {
-      const float s = sa * sw[GATED ? 0 : (wave_n * WTN + fn * 32) / kScaleBlock];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] += t[i] * s;
+      for (int i = 0; i < 16; ++i) acc[i] += p.t[i] * p.s0;
     }
   }
+
+  // Steps [X0, X1) of a slice: step x forms fragment (x / FN, x % FN)'s block sum and adds the one before.
+  // The last two sums of a slice are added in the next one (or by `flush`).
+  template <int X0, int X1>
+  __device__ static __forceinline__ void steps(f32x16_t (&acc)[FM][FN], Slice& s, Pending (&pend)[2], const char* stage,
+                                               int wave_m, int wave_n, int up_split) {
+#pragma unroll
+    for (int x = X0; x < X1; ++x) {
+      const int fm = x / FN, fn = x % FN, last = x == 0 ? FM * FN - 1 : x - 1;
+      if (fn == 0 && fm + 1 < FM) load_a(s, stage, wave_m, fm + 1);
+      Pending& p = pend[x & 1];
+      p.t = f32x16_t{};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) p.t = block_sum(s.b[fn][j], s.a[fm & 1][j], p.t);
+      const bool up = GATED && fn >= FN / 2;
+      p.s0 = s.sa[fm] * s.sw[up ? 1 : 0];
+      p.s1 = s.sa[fm] * s.sw[up ? 2 : 0];
+      f32x16_t& to = acc[last / FN][last % FN];
+      add(to, pend[(x + 1) & 1], last % FN, wave_n, up_split);
+      // The sum is made here and now: put off past the slice's barrier, every pending sum would stay alive.
+      asm volatile("" : "+v"(to));
+      if constexpr (FAST) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 9, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 9, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  static constexpr int BEFORE = (FM - 1) * FN;  // steps before the slice's barrier: every read of it is under way
+  static_assert((FM * FN) % 2 == 0 && FM % 2 == 0, "pending sums and row fragments alternate");
 
   __device__ static __forceinline__ void store_plain(const f32x16_t (&acc)[FM][FN], const Fp8Params& p,
                                                      const GroupTile& g, int tm, int tn, int wave_m, int wave_n) {
@@ -480,8 +520,13 @@ struct Fp8Tile {
   }
 };
 
+// The slices of a workgroup's tiles form one stream: while slice i is multiplied, slice i + 1 has landed
+// or is about to, and its first fragments are read under slice i's last matrix instructions.  There is one barrier
+// per slice, before its last row of fragments, when every wave has read all of the slice: behind it the
+// slice's buffer takes slice i + 2, of this tile or the next, so a tile's end does not drain the pipeline.
 template <class T>
 __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
+  static_assert(T::STAGES == 2, "two buffers: slice i + 2 takes slice i's");
   __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wave_m = wave / T::WN, wave_n = wave % T::WN;
@@ -490,47 +535,88 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   // XCD b % 8), so that the tiles that share an expert's panels read them through one L2.
   int t = (int)blockIdx.x;
   if ((grid & 7) == 0) t = (t & 7) * (grid >> 3) + (t >> 3);
-  const int kt_count = (p.k + kScaleBlock - 1) / kScaleBlock;
-  const int last_bytes = p.k - (kt_count - 1) * kScaleBlock;
+  const int blocks = (p.k + kScaleBlock - 1) / kScaleBlock;
+  const int kt_count = max(blocks, 2);  // slices past K are zeros
+  const int last_bytes = p.k - (blocks - 1) * kScaleBlock;
+  const bool cut = (last_bytes & 15) != 0;
   const int f = p.n >> 1;
   GroupTile g;
-  for (; find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g); t += grid) {
-    int tm, tn;
-    group_m_order(g.local, (g.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm, tn);
-    typename T::Copies c;
-    T::setup(c, p, g, tm, tn, smem);
+  if (!find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g)) return;
+  int tm, tn;
+  group_m_order(g.local, (g.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm, tn);
+  typename T::Copies c;
+  T::start(c, p, smem);
+  T::set_tile(c, p, g, tm, tn);
+  T::issue(c, 0, 0);
+  T::issue(c, 1, 1);
+  wait_vmcnt<T::PER_STAGE>();
+  __builtin_amdgcn_s_barrier();
+  compiler_fence();
+  if (cut && blocks == 1) {
+    T::cut_tail(smem, last_bytes);
+    __syncthreads();
+  }
+  typename T::Slice s;
+  auto load_first = [&](const char* stage) {
+    T::load_scales(s, stage, wave_m, wave_n);
+    T::load_a(s, stage, wave_m, 0);
+#pragma unroll
+    for (int fn = 0; fn < T::FN; ++fn) T::load_b(s, stage, wave_n, fn);
+  };
+  load_first(smem);
+
+  int buffer = 0;
+  bool more = true;
+  while (more) {
     const int up_split = kScaleBlock - (f + tn * T::OUT_COLS) % kScaleBlock;
     f32x16_t acc[T::FM][T::FN];
 #pragma unroll
     for (int fm = 0; fm < T::FM; ++fm)
 #pragma unroll
       for (int fn = 0; fn < T::FN; ++fn) acc[fm][fn] = f32x16_t{};
-#pragma unroll
-    for (int s = 0; s < T::STAGES - 1; ++s) T::issue(c, s, s);
-    int stage = 0;
-    for (int kt = 0; kt < kt_count; ++kt) {
-      // Slice kt has landed once only the STAGES - 2 younger slices' copies are outstanding, for every
-      // wave after the barrier, which also says that slice kt - 1 has been read: its buffer is refilled.
-      wait_vmcnt<(T::STAGES - 2) * T::PER_STAGE>();
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    typename T::Pending pend[2] = {};
+    // One slice; `refill(buffer)` issues slice i + 2, `cut_next`: the next slice is one that K ends inside.
+    auto slice = [&](auto&& refill, bool cut_next) {
+      char* cur = smem + buffer * T::STAGE_BYTES;
+      char* next = smem + (buffer ^ 1) * T::STAGE_BYTES;
+      T::template steps<0, T::BEFORE>(acc, s, pend, cur, wave_m, wave_n, up_split);
+      // Every fragment of this slice is in registers, and the next slice has landed.
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       compiler_fence();
-      const int refill = stage == 0 ? T::STAGES - 1 : stage - 1;
-      T::issue(c, refill, kt + T::STAGES - 1);
-      const char* cur = smem + stage * T::STAGE_BYTES;
-      if (kt + 1 == kt_count && (last_bytes & 15))
-        T::template compute<true>(acc, cur, wave_m, wave_n, last_bytes, up_split);
-      else
-        T::template compute<false>(acc, cur, wave_m, wave_n, 0, up_split);
-      stage = stage + 1 == T::STAGES ? 0 : stage + 1;
-    }
-    wait_vmcnt<0>();
+      refill(buffer);
+      if (cut_next) {
+        T::cut_tail(next, last_bytes);
+        __syncthreads();
+      }
+      // Fragments of the next slice (of the next tile, behind the last one) as this one's fall free.
+      T::template steps<T::BEFORE, T::FM * T::FN>(acc, s, pend, cur, wave_m, wave_n, up_split);
+      load_first(next);
+      buffer ^= 1;
+    };
+    for (int kt = 0; kt + 2 < kt_count; ++kt) slice([&](int stage) { T::issue(c, stage, kt + 2); }, false);
+    // The last two slices refill with the next tile's first two.
+    GroupTile g_next{};
+    int tm_next = 0, tn_next = 0;
+    slice([&](int stage) {
+      t += grid;
+      more = find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g_next);
+      if (more) {
+        group_m_order(g_next.local, (g_next.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm_next, tn_next);
+        T::set_tile(c, p, g_next, tm_next, tn_next);
+        T::issue(c, stage, 0);
+      }
+    }, cut && blocks > 1);
+    slice([&](int stage) { if (more) T::issue(c, stage, 1); }, cut && blocks == 1);
+    T::add(acc[T::FM - 1][T::FN - 1], pend[(T::FM * T::FN - 1) & 1], T::FN - 1, wave_n, up_split);
     if constexpr (T::GATED)
       T::store_gated(acc, p, g, tm, tn, wave_m, wave_n,
                      reinterpret_cast<uint32_t*>(smem + T::STAGES * T::STAGE_BYTES));
     else
       T::store_plain(acc, p, g, tm, tn, wave_m, wave_n);
-    __syncthreads();  // every wave is done with the slices before the next tile's copies
+    g = g_next;
+    tm = tm_next;
+    tn = tn_next;
   }
 }
 

@@ -27,11 +27,11 @@ hipError_t launch_fp8_stream(const Fp8Params& p, int grid, hipStream_t stream) {
 
 // X(E, BM, BN, WAVES_M, WAVES_N, STAGES, FAST) and Y(E, FM, FN, WAVES_N, WAVES_K, BLOCKS_IN_FLIGHT, unused).
 #define MOEGEMM_MENU_FP8(X, Y, E)                                                               \
-  X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 3, true) X(E, 128, 128, 2, 2, 3, true)     \
-  X(E, 128, 256, 2, 4, 3, false) X(E, 128, 128, 2, 2, 3, false)                                 \
+  X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, true) X(E, 128, 128, 2, 2, 2, true)     \
+  X(E, 128, 256, 2, 4, 2, false) X(E, 128, 128, 2, 2, 2, false)                                 \
   Y(E, 1, 1, 1, 8, 4, 0) Y(E, 1, 4, 1, 4, 3, 0) Y(E, 2, 4, 1, 4, 2, 0) Y(E, 4, 4, 1, 4, 1, 0)
 #define MOEGEMM_MENU_FP8_GATED(X, Y, E)                                                         \
-  X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 3, true) X(E, 128, 256, 2, 4, 3, false)    \
+  X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, false)    \
   Y(E, 1, 4, 4, 2, 3, 0) Y(E, 2, 4, 4, 2, 2, 0)
 
 #define MOEGEMM_FP8_X(E, BM, BN, WM, WN, S, FAST) \
