@@ -205,15 +205,16 @@ struct Fp8Tile {
   static constexpr int A_BYTES = BM * kScaleBlock, B_BYTES = BN * kScaleBlock;
   static constexpr int IA = A_BYTES / 1024, IB = B_BYTES / 1024;  // 1 KiB copies per stage: 8 rows of 128 bytes
   static constexpr int QA = IA / NW, QB = IB / NW;
-  static constexpr int SA_WAVES = BM / 64;      // waves that copy the row scales of a stage
-  static constexpr int SCALE_BYTES = NW * 256;  // 64 dwords a wave: row scales, the weight's, unused ones
+  // Scales of a stage, in copies of 64 dwords: row scales, then the weight's, then unused ones.
+  static constexpr int SA_COPIES = BM / 64;
+  static constexpr int QS = (SA_COPIES + NW) / NW;  // copies a wave makes
+  static constexpr int SCALE_BYTES = QS * NW * 256;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SCALE_BYTES;
-  static constexpr int PER_STAGE = QA + QB + 1;  // copies of a wave per stage
+  static constexpr int PER_STAGE = QA + QB + QS;  // copies of a wave per stage
   static constexpr int RED_BYTES = GATED ? BM * WN * 4 : 0;  // row maxima of the waves that share a row
   static constexpr int LDS_BYTES = STAGES * STAGE_BYTES + RED_BYTES;
   static constexpr int OUT_COLS = GATED ? BN / 2 : BN;  // output columns of a tile
   static_assert(IA % NW == 0 && IB % NW == 0, "every wave issues the same copies");
-  static_assert(SA_WAVES < NW, "one wave is left to copy the weight's scales");
   static_assert(!GATED || (BN == 256 && FN % 2 == 0), "a gated tile is one 128-column block of the output");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS of one CU");
   static_assert(STAGES * PER_STAGE < 64, "vmcnt is 6 bits");
@@ -222,27 +223,25 @@ struct Fp8Tile {
   struct Copies {
     uint32_t a_off, b_off;     // first copy's byte offset in a panel; later ones are NW * 8 rows further on
     uint32_t a_step, b_step;   // NW * 8 rows in bytes
-    uint32_t kch;              // this lane's k in a slice
     uint32_t lds, lds_scale;
-    int k;
+    int blocks;
     u32x4_t ra, rb, rb2;       // rb2: the up rows of a gated tile
-    uint32_t s_off;            // scale copy of this lane, or kOutOfRange
-    const float* s_base;
-    int64_t s_step;            // elements between blocks
+    uint32_t s_off[QS];        // scale copies of this lane, or kOutOfRange
+    const float* s_base[QS];
+    int64_t s_step[QS];        // elements between blocks
   };
 
   __device__ static __forceinline__ void start(Copies& c, const Fp8Params& p, const char* smem) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    c.k = p.k;
+    c.blocks = (p.k + kScaleBlock - 1) / kScaleBlock;
     c.lds = lds_address(smem) + (uint32_t)wave * 1024u;
     c.lds_scale = lds_address(smem) + (uint32_t)(A_BYTES + B_BYTES + wave * 256);
     // Row r of a panel keeps chunk c at c ^ swz_a(r, 8); wave w copies rows 8 (w + q NW) .. + 7.
     const int r0 = wave * 8 + lane / 8;
     const int ch = (lane & 7) ^ swz_a(r0, 8);  // swz_a of 8 chunks repeats every 32 rows, and NW * 8 is 32 or 64
-    c.kch = (uint32_t)ch * 16u;
-    c.a_off = (uint32_t)r0 * (uint32_t)p.lda + c.kch;
-    c.b_off = (uint32_t)r0 * (uint32_t)p.ldw + c.kch;
+    c.a_off = (uint32_t)r0 * (uint32_t)p.lda + (uint32_t)ch * 16u;
+    c.b_off = (uint32_t)r0 * (uint32_t)p.ldw + (uint32_t)ch * 16u;
     c.a_step = (uint32_t)p.lda * (NW * 8);
     c.b_step = (uint32_t)p.ldw * (NW * 8);
   }
@@ -252,44 +251,39 @@ struct Fp8Tile {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int m0 = tm * BM;
     const int valid_m = min(BM, g.m - m0);
-    c.ra = make_rsrc(p.a + ((int64_t)g.row0 + m0) * p.lda, (uint32_t)valid_m * (uint32_t)p.lda);
+    // A panel ends with the chunk that holds its last row's last k; what a copy reads past K inside it
+    // (the next row's start) is cut in LDS.
+    const uint32_t row_bytes = ((uint32_t)p.k + 15u) & ~15u;
+    c.ra = make_rsrc(p.a + ((int64_t)g.row0 + m0) * p.lda, (uint32_t)(valid_m - 1) * (uint32_t)p.lda + row_bytes);
     const uint8_t* w = p.w + (int64_t)g.e * p.swg;
     const int f = p.n >> 1;
     const int n0 = tn * OUT_COLS;
     const int valid_n = GATED ? min(BN / 2, f - n0) : min(BN, p.n - n0);
-    c.rb = make_rsrc(w + (int64_t)n0 * p.ldw, (uint32_t)valid_n * (uint32_t)p.ldw);
-    if constexpr (GATED) c.rb2 = make_rsrc(w + (int64_t)(f + n0) * p.ldw, (uint32_t)valid_n * (uint32_t)p.ldw);
-    // Scales: waves 0 .. BM/64 - 1 fetch 64 rows' each, the next one the weight's (at most 4 values).
-    c.s_off = kOutOfRange;
-    if (wave < SA_WAVES) {
-      const int row = wave * 64 + lane;
-      c.s_base = p.sa + ((int64_t)g.row0 + m0) * p.sam;
-      c.s_step = p.sak;
-      if (row < valid_m) c.s_off = (uint32_t)row * (uint32_t)p.sam * 4u;
-    } else {
-      // Lane j: scale block of the tile's weight rows 128 j (plain); gated: the gate's, then the one or
-      // two blocks of the up rows, which start at any multiple of 8.
-      const int last = (p.n + kScaleBlock - 1) / kScaleBlock - 1;
-      int nb;
-      if constexpr (GATED)
-        nb = lane == 0 ? n0 / kScaleBlock : min((f + n0) / kScaleBlock + lane - 1, last);
-      else
-        nb = min(n0 / kScaleBlock + lane, last);
-      c.s_base = p.sw + (int64_t)g.e * p.ssg;
-      c.s_step = p.ssk;
-      if (wave == SA_WAVES && lane < 4) c.s_off = (uint32_t)nb * (uint32_t)p.ssn * 4u;
+    const uint32_t b_bytes = (uint32_t)(valid_n - 1) * (uint32_t)p.ldw + row_bytes;
+    c.rb = make_rsrc(w + (int64_t)n0 * p.ldw, b_bytes);
+    if constexpr (GATED) c.rb2 = make_rsrc(w + (int64_t)(f + n0) * p.ldw, b_bytes);
+    // Scales: copy j < SA_COPIES fetches the scales of rows 64 j .. + 63, the next one the weight's (lane i:
+    // scale block of the tile's weight rows 128 i; gated: the gate's, then the one or two blocks of the up
+    // rows, which start at any multiple of 8).
+    const int last = (p.n + kScaleBlock - 1) / kScaleBlock - 1;
+    const int first = (GATED && lane > 0 ? f + n0 : n0) / kScaleBlock + (GATED && lane > 0 ? lane - 1 : lane);
+    const uint32_t w_off = lane < 4 ? (uint32_t)min(first, last) * (uint32_t)p.ssn * 4u : kOutOfRange;
+#pragma unroll
+    for (int q = 0; q < QS; ++q) {
+      const int j = wave + q * NW, row = j * 64 + lane;
+      const bool rows = j < SA_COPIES;
+      c.s_base[q] = uniform(rows ? p.sa + ((int64_t)g.row0 + m0) * p.sam : p.sw + (int64_t)g.e * p.ssg);
+      c.s_step[q] = uniform(rows ? p.sak : p.ssk);
+      if (rows) c.s_off[q] = row < valid_m ? (uint32_t)row * (uint32_t)p.sam * 4u : kOutOfRange;
+      else c.s_off[q] = j == SA_COPIES ? w_off : kOutOfRange;
     }
-    c.s_base = uniform(c.s_base);
-    c.s_step = uniform(c.s_step);
   }
 
   __device__ static __forceinline__ void issue(const Copies& c, int stage, int kt) {
     const uint32_t base = c.lds + (uint32_t)(stage * STAGE_BYTES);
     const uint32_t k0 = (uint32_t)kt * kScaleBlock;
-    const bool in_k = (int)(k0 + c.kch) < c.k;
-    uint32_t a0 = in_k ? c.a_off + k0 : kOutOfRange, b0 = in_k ? c.b_off + k0 : kOutOfRange;
+    uint32_t a0 = c.a_off + k0, b0 = c.b_off + k0;
     // The steps are added here: hoisted out of the loop, the offsets of eight copies took spilled registers.
-    // An out-of-range start stays out of range: the steps add less than 2 GiB to it.
     asm volatile("" : "+v"(a0), "+v"(b0));
 #pragma unroll
     for (int q = 0; q < QA; ++q) dma_copy16(c.ra, a0 + (uint32_t)q * c.a_step, base + (uint32_t)(q * NW * 1024));
@@ -299,60 +293,76 @@ struct Fp8Tile {
       dma_copy16(up ? c.rb2 : c.rb, b0 + (uint32_t)(up ? q - QB / 2 : q) * c.b_step,
                  base + (uint32_t)(A_BYTES + q * NW * 1024));
     }
-    const bool in = (int)k0 < c.k;
-    dma_copy4(make_rsrc(c.s_base + (in ? kt : 0) * c.s_step, kOutOfRange), in ? c.s_off : kOutOfRange,
-              c.lds_scale + (uint32_t)(stage * STAGE_BYTES));
+#pragma unroll
+    for (int q = 0; q < QS; ++q)
+      dma_copy4(make_rsrc(c.s_base[q] + min(kt, c.blocks - 1) * c.s_step[q], kOutOfRange), c.s_off[q],
+                c.lds_scale + (uint32_t)(stage * STAGE_BYTES + q * NW * 256));
   }
 
-  // 32 bytes of panel row x0 + lane % 32 for the j-th 64-byte half of the slice.
-  __device__ static __forceinline__ i32x8_t frag(const char* panel, int x0, int j) {
-    const int lane = threadIdx.x & 63;
-    const int row = x0 + (lane & 31);
-    const int s = swz_a(row, 8);
-    const int c0 = j * 4 + (lane >> 5), c1 = c0 + 2;
-    const char* p = panel + row * kScaleBlock;
-    return join(*reinterpret_cast<const i32x4_t*>(p + ((c0 ^ s) << 4)),
-                *reinterpret_cast<const i32x4_t*>(p + ((c1 ^ s) << 4)));
+  // This lane's first 16-byte chunk in the 32 rows of a fragment: every panel row group of 32 has the same
+  // swizzle, so one offset serves both panels, and the lane's other three chunks of the row differ from it
+  // in bits 5 and 6 only.
+  __device__ static __forceinline__ uint32_t lane_offset() {
+    const int lane = threadIdx.x & 63, row = lane & 31;
+    return (uint32_t)(row * kScaleBlock + (((lane >> 5) ^ swz_a(row, 8)) << 4));
+  }
+  // LDS addresses of the four chunks in the row group that starts `rows` bytes into LDS (a multiple of 128).
+  struct Chunks {
+    uint32_t at[4];
+  };
+  __device__ static __forceinline__ Chunks chunks(uint32_t lane, uint32_t rows) {
+    Chunks c;
+    c.at[0] = rows + lane;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) c.at[i] = c.at[0] ^ (uint32_t)(i << 5);
+    return c;
   }
 
-  // A K that is no multiple of 16 ends inside a chunk: zeros to the bytes of a landed slice from `left` on,
-  // a thread per panel row.
+  // 32 bytes of a panel row for the j-th 64-byte half of the slice, `rows32` row groups on.
+  __device__ static __forceinline__ i32x8_t frag(const char* smem, const Chunks& c, int rows32, int j) {
+    const char* p = smem + rows32 * 32 * kScaleBlock;
+    return join(*reinterpret_cast<const i32x4_t*>(p + c.at[2 * j]),
+                *reinterpret_cast<const i32x4_t*>(p + c.at[2 * j + 1]));
+  }
+
+  // Zeros to the bytes of a landed slice from `left` (< 128, any sign) on: a K that is no multiple of 128
+  // ends inside it.  A thread per panel row.
   __device__ static __forceinline__ void cut_tail(char* stage, int left) {
     for (int r = threadIdx.x; r < BM + BN; r += NT) {
       // Panel rows of A, then of B, are 128 bytes each; swz_a repeats every 32 rows and BM is a multiple of it.
-      i32x4_t* chunk = reinterpret_cast<i32x4_t*>(stage + r * kScaleBlock + (((left >> 4) ^ swz_a(r, 8)) << 4));
-      *chunk = keep_bytes(*chunk, left & 15);
+      for (int c = max(left, 0) >> 4; c < 8; ++c) {
+        i32x4_t* chunk = reinterpret_cast<i32x4_t*>(stage + r * kScaleBlock + ((c ^ swz_a(r, 8)) << 4));
+        *chunk = keep_bytes(*chunk, left - c * 16);
+      }
     }
   }
 
-  // First panel row of B fragment fn: gated waves hold their gate rows' fragments, then the up rows'.
-  __device__ static __forceinline__ int b_row(int fn, int wave_n) {
-    if constexpr (GATED)
-      return (fn < FN / 2 ? 0 : BN / 2) + wave_n * (WTN / 2) + (fn % (FN / 2)) * 32;
-    else
-      return wave_n * WTN + fn * 32;
-  }
+  // First panel row of a wave's columns: gated waves hold their gate rows' fragments, then the up rows',
+  // which lie BN / 2 rows after the gate rows.
+  __device__ static __forceinline__ int b_row(int wave_n) { return wave_n * (GATED ? WTN / 2 : WTN); }
 
   // What a wave holds of the slice it works on.  a is double-buffered over row fragments; the first
   // fragments of the next slice replace these while the last ones are multiplied.
   struct Slice {
     Fragment<FAST> a[2][2], b[FN][2];
-    float sa[FM];
+    float sa[2];
     float sw[GATED ? 3 : 1];  // gated: the gate's scale, the up's before and from its block boundary on
   };
-  __device__ static __forceinline__ void load_a(Slice& s, const char* stage, int wave_m, int fm) {
+  // `a`: the chunks of the wave's first row group of the slice; `stage` its LDS offset.
+  __device__ static __forceinline__ void load_a(Slice& s, const char* smem, const Chunks& a, uint32_t stage, int wave_m,
+                                                int fm) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) s.a[fm & 1][j].set(frag(stage, wave_m * WTM + fm * 32, j));
+    for (int j = 0; j < 2; ++j) s.a[fm & 1][j].set(frag(smem, a, fm, j));
+    s.sa[fm & 1] = *reinterpret_cast<const float*>(smem + stage + A_BYTES + B_BYTES + (wave_m * WTM + fm * 32) * 4 +
+                                                   (threadIdx.x & 31) * 4);
   }
-  __device__ static __forceinline__ void load_b(Slice& s, const char* stage, int wave_n, int fn) {
+  __device__ static __forceinline__ void load_b(Slice& s, const char* smem, const Chunks& b, int fn) {
+    constexpr int UP = GATED ? (BN / 2 - WTN / 2) / 32 : 0;  // row groups from a wave's gate rows' end to its up rows
 #pragma unroll
-    for (int j = 0; j < 2; ++j) s.b[fn][j].set(frag(stage + A_BYTES, b_row(fn, wave_n), j));
+    for (int j = 0; j < 2; ++j) s.b[fn][j].set(frag(smem, b, fn + (GATED && fn >= FN / 2 ? UP : 0), j));
   }
-  __device__ static __forceinline__ void load_scales(Slice& s, const char* stage, int wave_m, int wave_n) {
-    const float* scales = reinterpret_cast<const float*>(stage + A_BYTES + B_BYTES);
-    const float* sw = scales + SA_WAVES * 64;
-#pragma unroll
-    for (int fm = 0; fm < FM; ++fm) s.sa[fm] = scales[wave_m * WTM + fm * 32 + (threadIdx.x & 31)];
+  __device__ static __forceinline__ void load_weight_scales(Slice& s, const char* smem, uint32_t stage, int wave_n) {
+    const float* sw = reinterpret_cast<const float*>(smem + stage + A_BYTES + B_BYTES) + SA_COPIES * 64;
     if constexpr (GATED) {
 #pragma unroll
       for (int i = 0; i < 3; ++i) s.sw[i] = sw[i];
@@ -387,19 +397,19 @@ struct Fp8Tile {
   // Steps [X0, X1) of a slice: step x forms fragment (x / FN, x % FN)'s block sum and adds the one before.
   // The last two sums of a slice are added in the next one (or by `flush`).
   template <int X0, int X1>
-  __device__ static __forceinline__ void steps(f32x16_t (&acc)[FM][FN], Slice& s, Pending (&pend)[2], const char* stage,
-                                               int wave_m, int wave_n, int up_split) {
+  __device__ static __forceinline__ void steps(f32x16_t (&acc)[FM][FN], Slice& s, Pending (&pend)[2], const char* smem,
+                                               const Chunks& a, uint32_t stage, int wave_m, int wave_n, int up_split) {
 #pragma unroll
     for (int x = X0; x < X1; ++x) {
       const int fm = x / FN, fn = x % FN, last = x == 0 ? FM * FN - 1 : x - 1;
-      if (fn == 0 && fm + 1 < FM) load_a(s, stage, wave_m, fm + 1);
+      if (fn == 0 && fm + 1 < FM) load_a(s, smem, a, stage, wave_m, fm + 1);
       Pending& p = pend[x & 1];
       p.t = f32x16_t{};
 #pragma unroll
       for (int j = 0; j < 2; ++j) p.t = block_sum(s.b[fn][j], s.a[fm & 1][j], p.t);
       const bool up = GATED && fn >= FN / 2;
-      p.s0 = s.sa[fm] * s.sw[up ? 1 : 0];
-      p.s1 = s.sa[fm] * s.sw[up ? 2 : 0];
+      p.s0 = s.sa[fm & 1] * s.sw[up ? 1 : 0];
+      p.s1 = s.sa[fm & 1] * s.sw[up ? 2 : 0];
       f32x16_t& to = acc[last / FN][last % FN];
       add(to, pend[(x + 1) & 1], last % FN, wave_n, up_split);
       // The sum is made here and now: put off past the slice's barrier, every pending sum would stay alive.
@@ -536,9 +546,8 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   int t = (int)blockIdx.x;
   if ((grid & 7) == 0) t = (t & 7) * (grid >> 3) + (t >> 3);
   const int blocks = (p.k + kScaleBlock - 1) / kScaleBlock;
-  const int kt_count = max(blocks, 2);  // slices past K are zeros
-  const int last_bytes = p.k - (blocks - 1) * kScaleBlock;
-  const bool cut = (last_bytes & 15) != 0;
+  const int kt_count = max(blocks, 2);
+  const bool cut = p.k % kScaleBlock != 0;  // slices from K / 128 on are cut in LDS
   const int f = p.n >> 1;
   GroupTile g;
   if (!find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g)) return;
@@ -553,17 +562,21 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   __builtin_amdgcn_s_barrier();
   compiler_fence();
   if (cut && blocks == 1) {
-    T::cut_tail(smem, last_bytes);
+    T::cut_tail(smem, p.k);
     __syncthreads();
   }
+  const uint32_t lane = T::lane_offset();
   typename T::Slice s;
-  auto load_first = [&](const char* stage) {
-    T::load_scales(s, stage, wave_m, wave_n);
-    T::load_a(s, stage, wave_m, 0);
+  typename T::Chunks ca;
+  auto load_first = [&](uint32_t stage) {
+    T::load_weight_scales(s, smem, stage, wave_n);
+    ca = T::chunks(lane, stage + (uint32_t)(wave_m * T::WTM * kScaleBlock));
+    T::load_a(s, smem, ca, stage, wave_m, 0);
+    const typename T::Chunks cb = T::chunks(lane, stage + (uint32_t)(T::A_BYTES + T::b_row(wave_n) * kScaleBlock));
 #pragma unroll
-    for (int fn = 0; fn < T::FN; ++fn) T::load_b(s, stage, wave_n, fn);
+    for (int fn = 0; fn < T::FN; ++fn) T::load_b(s, smem, cb, fn);
   };
-  load_first(smem);
+  load_first(0);
 
   int buffer = 0;
   bool more = true;
@@ -575,26 +588,25 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
 #pragma unroll
       for (int fn = 0; fn < T::FN; ++fn) acc[fm][fn] = f32x16_t{};
     typename T::Pending pend[2] = {};
-    // One slice; `refill(buffer)` issues slice i + 2, `cut_next`: the next slice is one that K ends inside.
-    auto slice = [&](auto&& refill, bool cut_next) {
-      char* cur = smem + buffer * T::STAGE_BYTES;
-      char* next = smem + (buffer ^ 1) * T::STAGE_BYTES;
-      T::template steps<0, T::BEFORE>(acc, s, pend, cur, wave_m, wave_n, up_split);
+    // One slice; `refill(buffer)` issues slice i + 2; the next slice keeps `left` bytes of its rows.
+    auto slice = [&](auto&& refill, int left) {
+      const uint32_t cur = (uint32_t)(buffer * T::STAGE_BYTES), next = (uint32_t)((buffer ^ 1) * T::STAGE_BYTES);
+      T::template steps<0, T::BEFORE>(acc, s, pend, smem, ca, cur, wave_m, wave_n, up_split);
       // Every fragment of this slice is in registers, and the next slice has landed.
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       compiler_fence();
       refill(buffer);
-      if (cut_next) {
-        T::cut_tail(next, last_bytes);
+      if (left < kScaleBlock) {
+        T::cut_tail(smem + next, left);
         __syncthreads();
       }
       // Fragments of the next slice (of the next tile, behind the last one) as this one's fall free.
-      T::template steps<T::BEFORE, T::FM * T::FN>(acc, s, pend, cur, wave_m, wave_n, up_split);
+      T::template steps<T::BEFORE, T::FM * T::FN>(acc, s, pend, smem, ca, cur, wave_m, wave_n, up_split);
       load_first(next);
       buffer ^= 1;
     };
-    for (int kt = 0; kt + 2 < kt_count; ++kt) slice([&](int stage) { T::issue(c, stage, kt + 2); }, false);
+    for (int kt = 0; kt + 2 < kt_count; ++kt) slice([&](int stage) { T::issue(c, stage, kt + 2); }, kScaleBlock);
     // The last two slices refill with the next tile's first two.
     GroupTile g_next{};
     int tm_next = 0, tn_next = 0;
@@ -606,8 +618,8 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
         T::set_tile(c, p, g_next, tm_next, tn_next);
         T::issue(c, stage, 0);
       }
-    }, cut && blocks > 1);
-    slice([&](int stage) { if (more) T::issue(c, stage, 1); }, cut && blocks == 1);
+    }, p.k - (kt_count - 1) * kScaleBlock);
+    slice([&](int stage) { if (more) T::issue(c, stage, 1); }, p.k);
     T::add(acc[T::FM - 1][T::FN - 1], pend[(T::FM * T::FN - 1) & 1], T::FN - 1, wave_n, up_split);
     if constexpr (T::GATED)
       T::store_gated(acc, p, g, tm, tn, wave_m, wave_n,
