@@ -72,11 +72,25 @@ struct GroupTile {
   int e, row0, m, local;
 };
 
+// threadIdx.x, computed where it is used.  The tile loops' lookups, tails and epilogues depend on the lane and not on
+// the tile: hoisted out of the loop, their offsets took a hundred spilled registers.
+__device__ __forceinline__ int thread_here() {
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));
+  return thread;
+}
+
+__device__ __forceinline__ int64_t value_of(int64_t x, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)(uint32_t)x);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)(uint32_t)((uint64_t)x >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
 // The group of tile t when each group holds ceil(m / bm) * n_tiles tiles; false past the last one.
 // Each wave looks it up for itself, 64 groups at a time (wave-uniform result).
 __device__ __forceinline__ bool find_group_tile(const int32_t* offs, int groups, int rows, int bm, int n_tiles, int t,
                                                 GroupTile& g) {
-  const int lane = threadIdx.x & 63;
+  const int lane = thread_here() & 63;
   int64_t base = 0;
   for (int first = 0; first < groups; first += 64) {
     int m = 0, row0 = 0;
@@ -85,7 +99,7 @@ __device__ __forceinline__ bool find_group_tile(const int32_t* offs, int groups,
     int64_t sum = count;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t below = __shfl_up(sum, d);
+      const int64_t below = value_of(sum, lane - d);
       if (lane >= d) sum += below;
     }
     const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > t);
@@ -94,11 +108,11 @@ __device__ __forceinline__ bool find_group_tile(const int32_t* offs, int groups,
       g.e = first + hit;
       g.row0 = __builtin_amdgcn_readlane(row0, hit);
       g.m = __builtin_amdgcn_readlane(m, hit);
-      const int64_t before = base + __shfl(sum - count, hit);
-      g.local = uniform((int32_t)(t - before));
+      const int before = __builtin_amdgcn_readlane((int)(base + sum - count), hit);  // at most t
+      g.local = t - before;
       return true;
     }
-    base = uniform((int64_t)(base + __shfl(sum, 63)));
+    base = uniform(value_of(base + sum, 63));
   }
   return false;
 }
@@ -200,6 +214,7 @@ template <class E, int BM_, int BN_, int WM_, int WN_, int STAGES_, bool GATED_,
 struct Fp8Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
   static constexpr bool GATED = GATED_, FAST = FAST_;
+  using E16 = typename std::conditional<E::is_f32, EBf16, E>::type;  // 16-bit stores' type
   static constexpr int NW = WM * WN, NT = NW * 64;
   static constexpr int WTM = BM / WM, WTN = BN / WN, FM = WTM / 32, FN = WTN / 32;
   static constexpr int A_BYTES = BM * kScaleBlock, B_BYTES = BN * kScaleBlock;
@@ -247,7 +262,7 @@ struct Fp8Tile {
   }
 
   __device__ static __forceinline__ void set_tile(Copies& c, const Fp8Params& p, const GroupTile& g, int tm, int tn) {
-    const int lane = threadIdx.x & 63;
+    const int lane = thread_here() & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int m0 = tm * BM;
     const int valid_m = min(BM, g.m - m0);
@@ -328,7 +343,7 @@ struct Fp8Tile {
   // Zeros to the bytes of a landed slice from `left` (< 128, any sign) on: a K that is no multiple of 128
   // ends inside it.  A thread per panel row.
   __device__ static __forceinline__ void cut_tail(char* stage, int left) {
-    for (int r = threadIdx.x; r < BM + BN; r += NT) {
+    for (int r = thread_here(); r < BM + BN; r += NT) {
       // Panel rows of A, then of B, are 128 bytes each; swz_a repeats every 32 rows and BM is a multiple of it.
       for (int c = max(left, 0) >> 4; c < 8; ++c) {
         i32x4_t* chunk = reinterpret_cast<i32x4_t*>(stage + r * kScaleBlock + ((c ^ swz_a(r, 8)) << 4));
@@ -428,52 +443,59 @@ struct Fp8Tile {
 
   __device__ static __forceinline__ void store_plain(const f32x16_t (&acc)[FM][FN], const Fp8Params& p,
                                                      const GroupTile& g, int tm, int tn, int wave_m, int wave_n) {
-    const int lane = threadIdx.x & 63;
+    const int lane = thread_here() & 63;
     constexpr int ES = sizeof(typename E::raw);
+    const int m0 = tm * BM, n0 = tn * BN;
+    char* base = static_cast<char*>(p.out) + (((int64_t)g.row0 + m0) * p.ldo + n0) * ES;
+    const int valid_m = min(BM, g.m - m0), valid_n = p.n - n0;
+    if (ES == 2 && p.n % 8 == 0 && p.ldo % 8 == 0 && p.ldo < (1 << 22) && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0) {
+      // Lanes l and l + 32 hold columns 0-3 and 4-7 of an octet of the same row: they exchange halves of two
+      // octets, so that each stores 16 bytes.  One buffer resource ends with the tile's last valid row.
+      const uint32_t pitch = (uint32_t)p.ldo * ES;
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+          base, (short)0, (int)((uint32_t)(valid_m - 1) * pitch + (uint32_t)valid_n * ES), (int)kBufferFlags);
+      const int row = wave_m * WTM + (lane & 31), col = wave_n * WTN + (lane >> 5) * 8;
+      uint32_t offset = (uint32_t)row * pitch + (uint32_t)col * ES;
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm) {
+#pragma unroll
+        for (int fn = 0; fn < FN; ++fn)
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            const f32x16_t& v = acc[fm][fn];
+            const u32x2_t x = pack4<E16>(f32x4_t{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]});
+            const u32x2_t y = pack4<E16>(f32x4_t{v[q * 4 + 4], v[q * 4 + 5], v[q * 4 + 6], v[q * 4 + 7]});
+            const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+            const int c = fn * 32 + q * 8;
+            __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{s0[0], s1[0], s0[1], s1[1]}, rs,
+                                                   col + c < valid_n ? offset + (uint32_t)(c * ES) : kOutOfRange, 0, 0);
+          }
+        offset += 32 * pitch;
+      }
+      return;
+    }
     const bool vec = p.n % 4 == 0 && p.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (4 * ES - 1)) == 0;
-    const bool vec8 = ES == 2 && p.n % 8 == 0 && p.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
-      const int row = tm * BM + wave_m * WTM + fm * 32 + (lane & 31);
-      char* out = static_cast<char*>(p.out) + ((int64_t)g.row0 + row) * p.ldo * ES;
-      const bool in_m = row < g.m;
+      const int row = wave_m * WTM + fm * 32 + (lane & 31);
+      char* out = base + (int64_t)row * p.ldo * ES;
+      if (row >= valid_m) continue;
 #pragma unroll
-      for (int fn = 0; fn < FN; ++fn) {
-        const int n0 = tn * BN + wave_n * WTN + fn * 32;
-        if constexpr (ES == 2) {
-          if (vec8) {
-            // Lanes l and l + 32 hold columns 0-3 and 4-7 of an octet of the same row: they exchange
-            // halves of two octets, so that each stores 16 bytes.
-#pragma unroll
-            for (int q = 0; q < 4; q += 2) {
-              const u32x2_t x = pack4<E>(f32x4_t{acc[fm][fn][q * 4], acc[fm][fn][q * 4 + 1], acc[fm][fn][q * 4 + 2],
-                                                 acc[fm][fn][q * 4 + 3]});
-              const u32x2_t y = pack4<E>(f32x4_t{acc[fm][fn][q * 4 + 4], acc[fm][fn][q * 4 + 5],
-                                                 acc[fm][fn][q * 4 + 6], acc[fm][fn][q * 4 + 7]});
-              const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
-              const auto s1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
-              const int n = n0 + q * 8 + (lane >> 5) * 8;
-              if (in_m && n < p.n)
-                *MOEGEMM_GLOBAL(u32x4_t, out + (int64_t)n * 2) = u32x4_t{s0[0], s1[0], s0[1], s1[1]};
-            }
-            continue;
-          }
-        }
+      for (int fn = 0; fn < FN; ++fn)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int n = n0 + q * 8 + (lane >> 5) * 4;
+          const int n = wave_n * WTN + fn * 32 + q * 8 + (lane >> 5) * 4;
           const f32x4_t v = {acc[fm][fn][q * 4], acc[fm][fn][q * 4 + 1], acc[fm][fn][q * 4 + 2],
                              acc[fm][fn][q * 4 + 3]};
-          if (!in_m) continue;
           if (vec) {
-            if (n < p.n) store4<E>(out + (int64_t)n * ES, v);
+            if (n < valid_n) store4<E>(out + (int64_t)n * ES, v);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (n + i < p.n) store1<E>(out + (int64_t)(n + i) * ES, v[i]);
+              if (n + i < valid_n) store1<E>(out + (int64_t)(n + i) * ES, v[i]);
           }
         }
-      }
     }
   }
 
@@ -481,7 +503,7 @@ struct Fp8Tile {
   // it (through `red`), and the quantised row.
   __device__ static __forceinline__ void store_gated(f32x16_t (&acc)[FM][FN], const Fp8Params& p, const GroupTile& g,
                                                      int tm, int tn, int wave_m, int wave_n, uint32_t* red) {
-    const int lane = threadIdx.x & 63;
+    const int lane = thread_here() & 63;
     const int f = p.n >> 1;
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
@@ -581,6 +603,12 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   int buffer = 0;
   bool more = true;
   while (more) {
+    // The next tile is looked up before this one's sums take the registers.
+    GroupTile g_next{};
+    int tm_next = 0, tn_next = 0;
+    t += grid;
+    more = find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g_next);
+    if (more) group_m_order(g_next.local, (g_next.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm_next, tn_next);
     const int up_split = kScaleBlock - (f + tn * T::OUT_COLS) % kScaleBlock;
     f32x16_t acc[T::FM][T::FN];
 #pragma unroll
@@ -588,16 +616,16 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
 #pragma unroll
       for (int fn = 0; fn < T::FN; ++fn) acc[fm][fn] = f32x16_t{};
     typename T::Pending pend[2] = {};
-    // One slice; `refill(buffer)` issues slice i + 2; the next slice keeps `left` bytes of its rows.
-    auto slice = [&](auto&& refill, int left) {
+    // One slice; `refill` issues slice i + 2 into its buffer and says how many bytes of the next slice's rows
+    // lie inside K.
+    auto slice = [&](auto&& refill) {
       const uint32_t cur = (uint32_t)(buffer * T::STAGE_BYTES), next = (uint32_t)((buffer ^ 1) * T::STAGE_BYTES);
       T::template steps<0, T::BEFORE>(acc, s, pend, smem, ca, cur, wave_m, wave_n, up_split);
       // Every fragment of this slice is in registers, and the next slice has landed.
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       compiler_fence();
-      refill(buffer);
-      if (left < kScaleBlock) {
+      if (const int left = refill(); left < kScaleBlock) {
         T::cut_tail(smem + next, left);
         __syncthreads();
       }
@@ -606,20 +634,17 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
       load_first(next);
       buffer ^= 1;
     };
-    for (int kt = 0; kt + 2 < kt_count; ++kt) slice([&](int stage) { T::issue(c, stage, kt + 2); }, kScaleBlock);
+    // The loop is kept free of branches: the copies are issued between matrix instructions.
+    for (int kt = 0; kt + 2 < kt_count; ++kt) slice([&] {
+      T::issue(c, buffer, kt + 2);
+      return kScaleBlock;
+    });
     // The last two slices refill with the next tile's first two.
-    GroupTile g_next{};
-    int tm_next = 0, tn_next = 0;
-    slice([&](int stage) {
-      t += grid;
-      more = find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g_next);
-      if (more) {
-        group_m_order(g_next.local, (g_next.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm_next, tn_next);
-        T::set_tile(c, p, g_next, tm_next, tn_next);
-        T::issue(c, stage, 0);
-      }
-    }, p.k - (kt_count - 1) * kScaleBlock);
-    slice([&](int stage) { if (more) T::issue(c, stage, 1); }, p.k);
+    for (int ahead = 0; ahead < 2; ++ahead) slice([&] {
+      if (ahead == 0 && more) T::set_tile(c, p, g_next, tm_next, tn_next);
+      if (more) T::issue(c, buffer, ahead);
+      return p.k - (ahead == 0 ? kt_count - 1 : 0) * kScaleBlock;
+    });
     T::add(acc[T::FM - 1][T::FN - 1], pend[(T::FM * T::FN - 1) & 1], T::FN - 1, wave_n, up_split);
     if constexpr (T::GATED)
       T::store_gated(acc, p, g, tm, tn, wave_m, wave_n,
