@@ -72,6 +72,10 @@ struct GroupTile {
   int e, row0, m, local;
 };
 
+__device__ __forceinline__ float uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
 // threadIdx.x, computed where it is used.  The tile loops' lookups, tails and epilogues depend on the lane and not on
 // the tile: hoisted out of the loop, their offsets took a hundred spilled registers.
 __device__ __forceinline__ int thread_here() {
@@ -230,7 +234,7 @@ struct Fp8Tile {
   static constexpr int LDS_BYTES = STAGES * STAGE_BYTES + RED_BYTES;
   static constexpr int OUT_COLS = GATED ? BN / 2 : BN;  // output columns of a tile
   static_assert(IA % NW == 0 && IB % NW == 0, "every wave issues the same copies");
-  static_assert(!GATED || (BN == 256 && FN % 2 == 0), "a gated tile is one 128-column block of the output");
+  static_assert(!GATED || (BN == 256 && FN == 2), "a gated tile is one 128-column block of the output");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS of one CU");
   static_assert(STAGES * PER_STAGE < 64, "vmcnt is 6 bits");
 
@@ -277,12 +281,12 @@ struct Fp8Tile {
     const uint32_t b_bytes = (uint32_t)(valid_n - 1) * (uint32_t)p.ldw + row_bytes;
     c.rb = make_rsrc(w + (int64_t)n0 * p.ldw, b_bytes);
     if constexpr (GATED) c.rb2 = make_rsrc(w + (int64_t)(f + n0) * p.ldw, b_bytes);
-    // Scales: copy j < SA_COPIES fetches the scales of rows 64 j .. + 63, the next one the weight's (lane i:
-    // scale block of the tile's weight rows 128 i; gated: the gate's, then the one or two blocks of the up
-    // rows, which start at any multiple of 8).
+    // Scales: copy j < SA_COPIES fetches the scales of rows 64 j .. + 63, the next one the weight's.  Plain: lane i
+    // has the tile's weight rows from 128 i on.  Gated: lanes 0 to 15 have eight up rows each (up rows start at any
+    // multiple of 8, so a scale block may end between any two of them), lane 16 the gate rows.
     const int last = (p.n + kScaleBlock - 1) / kScaleBlock - 1;
-    const int first = (GATED && lane > 0 ? f + n0 : n0) / kScaleBlock + (GATED && lane > 0 ? lane - 1 : lane);
-    const uint32_t w_off = lane < 4 ? (uint32_t)min(first, last) * (uint32_t)p.ssn * 4u : kOutOfRange;
+    const int block = GATED && lane < 16 ? (f + n0 + 8 * lane) / kScaleBlock : n0 / kScaleBlock + (GATED ? 0 : lane);
+    const uint32_t w_off = lane < (GATED ? 17 : 4) ? (uint32_t)min(block, last) * (uint32_t)p.ssn * 4u : kOutOfRange;
 #pragma unroll
     for (int q = 0; q < QS; ++q) {
       const int j = wave + q * NW, row = j * 64 + lane;
@@ -294,6 +298,16 @@ struct Fp8Tile {
     }
   }
 
+  // Copies of a slice are spread over the steps in which its buffer is free: the FN steps after the barrier of the
+  // slice that held it and the first EARLY steps of the next one, weights (which come from HBM) first.  Issued
+  // in one burst they kept every wave from its matrix instructions until the last was accepted.
+  static constexpr int BEFORE = (FM - 1) * FN;  // steps before a slice's barrier: every read of it is under way
+  static constexpr int EARLY = FM * FN >= 8 ? 3 : 0;
+  static constexpr int PARTS = FN + EARLY;
+  static constexpr int first_copy(int part) { return (part * PER_STAGE + PARTS - 1) / PARTS; }
+
+  // Part [PART0, PART1) of slice kt's copies.
+  template <int PART0, int PART1>
   __device__ static __forceinline__ void issue(const Copies& c, int stage, int kt) {
     const uint32_t base = c.lds + (uint32_t)(stage * STAGE_BYTES);
     const uint32_t k0 = (uint32_t)kt * kScaleBlock;
@@ -301,17 +315,20 @@ struct Fp8Tile {
     // The steps are added here: hoisted out of the loop, the offsets of eight copies took spilled registers.
     asm volatile("" : "+v"(a0), "+v"(b0));
 #pragma unroll
-    for (int q = 0; q < QA; ++q) dma_copy16(c.ra, a0 + (uint32_t)q * c.a_step, base + (uint32_t)(q * NW * 1024));
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-      const bool up = GATED && q >= QB / 2;
-      dma_copy16(up ? c.rb2 : c.rb, b0 + (uint32_t)(up ? q - QB / 2 : q) * c.b_step,
-                 base + (uint32_t)(A_BYTES + q * NW * 1024));
+    for (int i = first_copy(PART0); i < first_copy(PART1); ++i) {
+      if (i < QB) {
+        const bool up = GATED && i >= QB / 2;
+        dma_copy16(up ? c.rb2 : c.rb, b0 + (uint32_t)(up ? i - QB / 2 : i) * c.b_step,
+                   base + (uint32_t)(A_BYTES + i * NW * 1024));
+      } else if (i < QB + QA) {
+        const int q = i - QB;
+        dma_copy16(c.ra, a0 + (uint32_t)q * c.a_step, base + (uint32_t)(q * NW * 1024));
+      } else {
+        const int q = i - QB - QA;
+        dma_copy4(make_rsrc(c.s_base[q] + min(kt, c.blocks - 1) * c.s_step[q], kOutOfRange), c.s_off[q],
+                  c.lds_scale + (uint32_t)(stage * STAGE_BYTES + q * NW * 256));
+      }
     }
-#pragma unroll
-    for (int q = 0; q < QS; ++q)
-      dma_copy4(make_rsrc(c.s_base[q] + min(kt, c.blocks - 1) * c.s_step[q], kOutOfRange), c.s_off[q],
-                c.lds_scale + (uint32_t)(stage * STAGE_BYTES + q * NW * 256));
   }
 
   // This lane's first 16-byte chunk in the 32 rows of a fragment: every panel row group of 32 has the same
@@ -361,7 +378,7 @@ struct Fp8Tile {
   struct Slice {
     Fragment<FAST> a[2][2], b[FN][2];
     float sa[2];
-    float sw[GATED ? 3 : 1];  // gated: the gate's scale, the up's before and from its block boundary on
+    float sw[GATED ? 5 : 1];  // wave-uniform; gated: of each eight up rows of the wave's 32, then the gate's
   };
   // `a`: the chunks of the wave's first row group of the slice; `stage` its LDS offset.
   __device__ static __forceinline__ void load_a(Slice& s, const char* smem, const Chunks& a, uint32_t stage, int wave_m,
@@ -380,53 +397,59 @@ struct Fp8Tile {
     const float* sw = reinterpret_cast<const float*>(smem + stage + A_BYTES + B_BYTES) + SA_COPIES * 64;
     if constexpr (GATED) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) s.sw[i] = sw[i];
+      for (int i = 0; i < 4; ++i) s.sw[i] = uniform(sw[wave_n * (WTN / 16) + i]);
+      s.sw[4] = uniform(sw[16]);
     } else {
       static_assert(kScaleBlock % WTN == 0, "a wave's columns lie in one scale block");
-      s.sw[0] = sw[wave_n * WTN / kScaleBlock];
+      s.sw[0] = uniform(sw[wave_n * WTN / kScaleBlock]);
     }
   }
 
   // A fragment's sum of one block, waiting to be added while the next one's is formed.
   struct Pending {
     f32x16_t t;
-    float s0, s1;
+    float s;     // the sum's scale; up rows of a gated tile: the row scale alone, and
+    float w[4];  // the weight's (wave-uniform) for each quad of registers, eight up rows
   };
-  // acc += t * scales for B fragment fn.
-  __device__ static __forceinline__ void add(f32x16_t& acc, const Pending& p, int fn, int wave_n, int up_split) {
+  // acc += t * scale for B fragment fn.
+  __device__ static __forceinline__ void add(f32x16_t& acc, const Pending& p, int fn) {
     if (GATED && fn >= FN / 2) {
-      // Quad q of the fragment is up columns col + 8 q .. + 7: the block boundary falls between quads.
-      const int col = wave_n * (WTN / 2) + (fn - FN / 2) * 32;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float s = col + q * 8 < up_split ? p.s0 : p.s1;
+        const float s = p.s * p.w[q];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[q * 4 + i] += p.t[q * 4 + i] * s;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] += p.t[i] * p.s0;
+      for (int i = 0; i < 16; ++i) acc[i] += p.t[i] * p.s;
     }
   }
 
   // Steps [X0, X1) of a slice: step x forms fragment (x / FN, x % FN)'s block sum and adds the one before.
-  // The last two sums of a slice are added in the next one (or by `flush`).
-  template <int X0, int X1>
+  // The last sum of a slice is added in the next one.  `copies(part)` issues a part of a slice's copies.
+  template <int X0, int X1, class Issue>
   __device__ static __forceinline__ void steps(f32x16_t (&acc)[FM][FN], Slice& s, Pending (&pend)[2], const char* smem,
-                                               const Chunks& a, uint32_t stage, int wave_m, int wave_n, int up_split) {
-#pragma unroll
-    for (int x = X0; x < X1; ++x) {
-      const int fm = x / FN, fn = x % FN, last = x == 0 ? FM * FN - 1 : x - 1;
+                                               const Chunks& a, uint32_t stage, Issue&& copies, int wave_m) {
+    unroll_steps<X0, X1>([&](auto step) {
+      constexpr int x = decltype(step)::value;
+      constexpr int fm = x / FN, fn = x % FN, last = x == 0 ? FM * FN - 1 : x - 1;
+      constexpr int part = x >= BEFORE ? x - BEFORE : x < EARLY ? FN + x : -1;
+      if constexpr (part >= 0) copies(std::integral_constant<int, part>{});
       if (fn == 0 && fm + 1 < FM) load_a(s, smem, a, stage, wave_m, fm + 1);
       Pending& p = pend[x & 1];
       p.t = f32x16_t{};
 #pragma unroll
       for (int j = 0; j < 2; ++j) p.t = block_sum(s.b[fn][j], s.a[fm & 1][j], p.t);
-      const bool up = GATED && fn >= FN / 2;
-      p.s0 = s.sa[fm & 1] * s.sw[up ? 1 : 0];
-      p.s1 = s.sa[fm & 1] * s.sw[up ? 2 : 0];
+      if constexpr (GATED && fn >= FN / 2) {
+        p.s = s.sa[fm & 1];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) p.w[q] = s.sw[q];
+      } else {
+        p.s = s.sa[fm & 1] * s.sw[GATED ? 4 : 0];
+      }
       f32x16_t& to = acc[last / FN][last % FN];
-      add(to, pend[(x + 1) & 1], last % FN, wave_n, up_split);
+      add(to, pend[(x + 1) & 1], last % FN);
       // The sum is made here and now: put off past the slice's barrier, every pending sum would stay alive.
       asm volatile("" : "+v"(to));
       if constexpr (FAST) {
@@ -436,9 +459,15 @@ struct Fp8Tile {
         __builtin_amdgcn_sched_group_barrier(0x002, 9, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
+    });
+  }
+  template <int X0, int X1, class F>
+  __device__ static __forceinline__ void unroll_steps(F&& f) {
+    if constexpr (X0 < X1) {
+      f(std::integral_constant<int, X0>{});
+      unroll_steps<X0 + 1, X1>(f);
     }
   }
-  static constexpr int BEFORE = (FM - 1) * FN;  // steps before the slice's barrier: every read of it is under way
   static_assert((FM * FN) % 2 == 0 && FM % 2 == 0, "pending sums and row fragments alternate");
 
   __device__ static __forceinline__ void store_plain(const f32x16_t (&acc)[FM][FN], const Fp8Params& p,
@@ -570,7 +599,6 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   const int blocks = (p.k + kScaleBlock - 1) / kScaleBlock;
   const int kt_count = max(blocks, 2);
   const bool cut = p.k % kScaleBlock != 0;  // slices from K / 128 on are cut in LDS
-  const int f = p.n >> 1;
   GroupTile g;
   if (!find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g)) return;
   int tm, tn;
@@ -578,9 +606,9 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   typename T::Copies c;
   T::start(c, p, smem);
   T::set_tile(c, p, g, tm, tn);
-  T::issue(c, 0, 0);
-  T::issue(c, 1, 1);
-  wait_vmcnt<T::PER_STAGE>();
+  T::template issue<0, T::PARTS>(c, 0, 0);
+  T::template issue<0, T::FN>(c, 1, 1);  // the rest of it under slice 0's first steps
+  wait_vmcnt<T::first_copy(T::FN)>();
   __builtin_amdgcn_s_barrier();
   compiler_fence();
   if (cut && blocks == 1) {
@@ -609,43 +637,46 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
     t += grid;
     more = find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g_next);
     if (more) group_m_order(g_next.local, (g_next.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm_next, tn_next);
-    const int up_split = kScaleBlock - (f + tn * T::OUT_COLS) % kScaleBlock;
     f32x16_t acc[T::FM][T::FN];
 #pragma unroll
     for (int fm = 0; fm < T::FM; ++fm)
 #pragma unroll
       for (int fn = 0; fn < T::FN; ++fn) acc[fm][fn] = f32x16_t{};
     typename T::Pending pend[2] = {};
-    // One slice; `refill` issues slice i + 2 into its buffer and says how many bytes of the next slice's rows
-    // lie inside K.
-    auto slice = [&](auto&& refill) {
+    // One slice.  `early(part)` issues the rest of slice i + 1's copies into the other buffer, `late(part)`
+    // the first of slice i + 2's into this one; `left()` says how many bytes of the next slice's rows lie inside K.
+    auto slice = [&](auto&& early, auto&& late, auto&& left) {
       const uint32_t cur = (uint32_t)(buffer * T::STAGE_BYTES), next = (uint32_t)((buffer ^ 1) * T::STAGE_BYTES);
-      T::template steps<0, T::BEFORE>(acc, s, pend, smem, ca, cur, wave_m, wave_n, up_split);
+      T::template steps<0, T::BEFORE>(acc, s, pend, smem, ca, cur, early, wave_m);
       // Every fragment of this slice is in registers, and the next slice has landed.
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       compiler_fence();
-      if (const int left = refill(); left < kScaleBlock) {
-        T::cut_tail(smem + next, left);
+      if (const int bytes = left(); bytes < kScaleBlock) {
+        T::cut_tail(smem + next, bytes);
         __syncthreads();
       }
       // Fragments of the next slice (of the next tile, behind the last one) as this one's fall free.
-      T::template steps<T::BEFORE, T::FM * T::FN>(acc, s, pend, smem, ca, cur, wave_m, wave_n, up_split);
+      T::template steps<T::BEFORE, T::FM * T::FN>(acc, s, pend, smem, ca, cur, late, wave_m);
       load_first(next);
       buffer ^= 1;
     };
+    auto issue = [&](auto part, int stage, int kt) {
+      T::template issue<decltype(part)::value, decltype(part)::value + 1>(c, stage, kt);
+    };
     // The loop is kept free of branches: the copies are issued between matrix instructions.
-    for (int kt = 0; kt + 2 < kt_count; ++kt) slice([&] {
-      T::issue(c, buffer, kt + 2);
-      return kScaleBlock;
-    });
+    for (int kt = 0; kt + 2 < kt_count; ++kt)
+      slice([&](auto part) { issue(part, buffer ^ 1, kt + 1); }, [&](auto part) { issue(part, buffer, kt + 2); },
+            [] { return kScaleBlock; });
     // The last two slices refill with the next tile's first two.
-    for (int ahead = 0; ahead < 2; ++ahead) slice([&] {
-      if (ahead == 0 && more) T::set_tile(c, p, g_next, tm_next, tn_next);
-      if (more) T::issue(c, buffer, ahead);
-      return p.k - (ahead == 0 ? kt_count - 1 : 0) * kScaleBlock;
-    });
-    T::add(acc[T::FM - 1][T::FN - 1], pend[(T::FM * T::FN - 1) & 1], T::FN - 1, wave_n, up_split);
+    for (int ahead = 0; ahead < 2; ++ahead)
+      slice([&](auto part) { if (ahead == 0 || more) issue(part, buffer ^ 1, ahead == 0 ? kt_count - 1 : 0); },
+            [&](auto part) { if (more) issue(part, buffer, ahead); },
+            [&] {
+              if (ahead == 0 && more) T::set_tile(c, p, g_next, tm_next, tn_next);
+              return p.k - (ahead == 0 ? kt_count - 1 : 0) * kScaleBlock;
+            });
+    T::add(acc[T::FM - 1][T::FN - 1], pend[(T::FM * T::FN - 1) & 1], T::FN - 1);
     if constexpr (T::GATED)
       T::store_gated(acc, p, g, tm, tn, wave_m, wave_n,
                      reinterpret_cast<uint32_t*>(smem + T::STAGES * T::STAGE_BYTES));
