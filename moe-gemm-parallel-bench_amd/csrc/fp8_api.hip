@@ -73,7 +73,8 @@ int choose(const Fp8Variant* table, int count, int64_t rows, int64_t groups, int
   if (mean <= (gated ? 32 : 64)) {
     const int bm = mean <= 12 ? 16 : mean <= 24 || gated ? 32 : 64;
     if (bm == 16 && !gated && groups * cdiv(out_cols, 64) < 2 * cus) return find(16, 16, 1);
-    return find(bm, gated ? 0 : 64, 1);
+    if (bm == 16 && !gated) return find(16, 64, 1);
+    return find(bm, 0, 1);
   }
   if (fast && rows / groups >= 192 && cdiv(rows, 256) * cdiv(cols, 256) * 4 >= 3 * cus) return find(256, 256, 0);
   if (!gated && cdiv(rows, 128) * cdiv(cols, 256) < cus) return find(128, 128, 0);
@@ -95,7 +96,8 @@ int launch_product(const Fp8Variant* table, int count, Fp8Params& p, int64_t out
   p.n_tiles = (int32_t)col_tiles;
   int64_t grid;
   if (v.stream) {
-    grid = (int64_t)p.groups * col_tiles;
+    if ((int64_t)p.groups * col_tiles > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "unit count exceeds int32");
+    grid = std::min<int64_t>((int64_t)p.groups * col_tiles, cus);
   } else {
     const int64_t bound = std::min(p.rows / v.block_m + (int64_t)p.groups, p.groups * cdiv(p.rows, v.block_m)) * col_tiles;
     if (bound > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");

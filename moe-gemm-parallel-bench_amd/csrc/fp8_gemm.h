@@ -25,9 +25,8 @@
 // form one group (offs null).  Two kernels:
 //  * Fp8Tile (prefill): operands reach LDS by DMA, one 128-byte K slice (= one scale block) per
 //    stage, 16-byte chunks XOR-swizzled, read with ds_read_b128;
-//  * Fp8Stream (decode, few rows a group): weights go from HBM straight into registers, each byte
-//    read once, the waves of a workgroup split K and join their sums through LDS.  Exact sums only:
-//    HBM is the bound, and widening costs no time.
+//  * Fp8Stream (decode, few rows a group): each wave streams weights through a ring of its own in LDS, every
+//    byte read once.  Exact sums only: HBM is the bound, and widening costs no time.
 #pragma once
 
 #include "gemm_fast.h"
@@ -688,166 +687,200 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   }
 }
 
-// Decode: 16 FM rows of a group by 16 FN columns per wave, WN waves along the columns, WK waves that
-// take K blocks wk, wk + WK, ...  Each wave keeps U blocks of weights and rows in flight in registers.
-template <class E, int FM_, int FN_, int WN_, int WK_, int U_, bool GATED_>
+// Decode: 16 FM rows of a group by 16 FN weight rows per wave, WN waves along the columns, WK waves that take
+// the K blocks wk, wk + WK, ...  Bound by HBM: each weight byte is read once.
+//
+// Every wave streams on its own: a ring of STAGES slots in LDS, one K block of its weights, rows and scales each,
+// filled by DMA in whole 128-byte lines and refilled as soon as its fragments are in registers.  No barrier
+// and no wait of other waves is involved, and the ring runs on over the units (group, column tile, row tile) of the
+// workgroup, so nothing drains between them.  Loads of fragments straight into registers read half lines:
+// 256 rows over 32 experts of [4096, 7168] took 171 to 197 us that way whatever the tile and depth.
+template <class E, int FM_, int FN_, int WN_, int WK_, int STAGES_, bool GATED_>
 struct Fp8Stream {
-  static constexpr int FM = FM_, FN = FN_, WN = WN_, WK = WK_, U = U_;
+  static constexpr int FM = FM_, FN = FN_, WN = WN_, WK = WK_, STAGES = STAGES_;
   static constexpr bool GATED = GATED_;
   static constexpr int NW = WN * WK, NT = NW * 64;
   static constexpr int BM = 16 * FM, BN = 16 * FN * WN;
   static constexpr int OUT_COLS = GATED ? BN / 2 : BN;
   static constexpr int FRAGS = FM * FN * WN;  // accumulator fragments of a tile
-  static constexpr int RED_BYTES = WK * FRAGS * 1024;
-  static constexpr int LDS_BYTES = RED_BYTES + (GATED ? BM * 8 * 4 : 0);
-  static_assert(!GATED || (OUT_COLS == kScaleBlock && FN % 2 == 0), "a gated tile is one block of the output");
+  static constexpr int W_BYTES = FN * 16 * kScaleBlock, A_BYTES = FM * 16 * kScaleBlock;
+  static constexpr int SLOT_BYTES = W_BYTES + A_BYTES + 512;  // and two copies of scales: rows, weights
+  static constexpr int COPIES = 2 * FN + 2 * FM + 2;
+  static constexpr int RING_BYTES = NW * STAGES * SLOT_BYTES;
+  static constexpr int RED_BYTES = WK > 1 ? WK * FRAGS * 1024 : 0;
+  static constexpr int LDS_BYTES = RING_BYTES + RED_BYTES + (GATED ? BM * 8 * 4 : 0);
+  static_assert(!GATED || (OUT_COLS == kScaleBlock && FN == 4 && WK == 1), "a gated tile is one block of the output");
+  static_assert(LDS_BYTES <= 160 * 1024, "LDS of one CU");
+  static_assert(STAGES * COPIES < 64, "vmcnt is 6 bits");
 };
 
 template <class T, class E>
 __global__ void __launch_bounds__(T::NT) fp8_stream_kernel(Fp8Params p) {
-  constexpr int FM = T::FM, FN = T::FN, WN = T::WN, WK = T::WK, U = T::U;
+  constexpr int FM = T::FM, FN = T::FN, WN = T::WN, WK = T::WK, STAGES = T::STAGES;
   constexpr bool GATED = T::GATED;
   __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wn = wave % WN, wk = wave / WN;
-  const int e = (int)blockIdx.x / p.n_tiles, tn = (int)blockIdx.x % p.n_tiles;
-  int m;
-  const int row0 = group_rows(p.offs, p.rows, e, m);
-  if (m == 0) return;
   const int f = p.n >> 1;
   const int blocks = (p.k + kScaleBlock - 1) / kScaleBlock;
-  const int kch = (lane >> 4) * 16;  // this lane's chunks start at kch and kch + 64 of a block
-  const int n0 = tn * T::OUT_COLS + wn * (GATED ? 8 : 16) * FN;  // the wave's first output column
-  const uint8_t* w = p.w + (int64_t)e * p.swg;
-  const float* sw = p.sw + (int64_t)e * p.ssg;
-  // Weight rows of fragment fn, in one buffer resource from the fragment's first row; gated waves hold
-  // their gate fragments, then the up ones.
-  auto first_row = [&](int fn) {
-    if constexpr (GATED) return (fn < FN / 2 ? 0 : f) + n0 + (fn % (FN / 2)) * 16;
-    return n0 + fn * 16;
-  };
-  auto valid_rows = [&](int fn) {
-    const int end = GATED ? f - (n0 + (fn % (FN > 1 ? FN / 2 : 1)) * 16) : p.n - (n0 + fn * 16);
-    return min(max(end, 0), 16);
-  };
-  const uint32_t w_off = (uint32_t)(lane & 15) * (uint32_t)p.ldw + (uint32_t)kch;
+  const int rounds = (blocks + WK - 1) / WK;  // K blocks of every wave; those past the end are zeros
+  const int units = p.groups * p.n_tiles;
   const int last_n = (p.n + kScaleBlock - 1) / kScaleBlock - 1;
 
-  for (int m0 = 0; m0 < m; m0 += T::BM) {
-    const int valid_m = min(T::BM, m - m0);
-    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a) + ((int64_t)row0 + m0) * p.lda,
-                                                      (short)0, (int)((uint32_t)valid_m * (uint32_t)p.lda),
-                                                      (int)kBufferFlags);
-    f32x4_t acc[FM][FN];
-#pragma unroll
-    for (int fm = 0; fm < FM; ++fm)
-#pragma unroll
-      for (int fn = 0; fn < FN; ++fn) acc[fm][fn] = f32x4_t{};
+  // A place in the workgroup's stream of (unit, row tile, K block).
+  struct Cursor {
+    int unit, e, tn, row0, m, m0, round;
+  };
+  auto find_rows = [&](Cursor& c) {  // the first unit from c.unit on whose group has rows
+    for (; c.unit < units; c.unit += gridDim.x) {
+      c.e = c.unit / p.n_tiles;
+      c.tn = c.unit - c.e * p.n_tiles;
+      c.row0 = group_rows(p.offs, p.rows, c.e, c.m);
+      if (c.m > 0) break;
+    }
+    c.m0 = 0;
+    c.round = 0;
+  };
+  auto advance = [&](Cursor& c) {
+    if (++c.round < rounds) return;
+    c.round = 0;
+    c.m0 += T::BM;
+    if (c.m0 < c.m) return;
+    c.unit += gridDim.x;
+    find_rows(c);
+  };
+  auto first_col = [&](const Cursor& c) { return c.tn * T::OUT_COLS + wn * (GATED ? 8 : 16) * FN; };
 
-    i32x4_t wv[U][FN][2], av[U][FM][2];
-    float sv[U][FM];
-    // Blocks at or past the end load zeros (values and row scales) and add nothing.
-    auto load = [&](int u, int kb) {
-      const uint32_t k0 = (uint32_t)kb * kScaleBlock;
+  // Copies: eight rows of 128 bytes each, chunk c of row r at c ^ swz_a(r, 8).
+  const int copy_row = lane >> 3;
+  const uint32_t ring = (uint32_t)(wave * STAGES * T::SLOT_BYTES);
+  const uint32_t ring_lds = lds_address(smem) + ring;
+  const uint32_t row_bytes = ((uint32_t)p.k + 15u) & ~15u;
+  auto issue = [&](const Cursor& c, int slot) {
+    const uint32_t to = ring_lds + (uint32_t)(slot * T::SLOT_BYTES);
+    const int kb = wk + c.round * WK;
+    const uint32_t k0 = (uint32_t)kb * kScaleBlock;
+    const int n0 = first_col(c);
+    const int valid_m = min(T::BM, c.m - c.m0);
+    const uint8_t* w = p.w + (int64_t)c.e * p.swg + (int64_t)n0 * p.ldw;
+    const int valid_n = min(GATED ? f - n0 : p.n - n0, GATED ? 8 * FN : 16 * FN);
+    const uint32_t w_bytes = valid_n > 0 && kb < blocks ? (uint32_t)(valid_n - 1) * (uint32_t)p.ldw + row_bytes : 0;
+    const u32x4_t rw = make_rsrc(w, w_bytes);
+    const u32x4_t rw2 = GATED ? make_rsrc(w + (int64_t)f * p.ldw, w_bytes) : rw;
 #pragma unroll
-      for (int fn = 0; fn < FN; ++fn) {
-        const auto rw = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(w) + (int64_t)first_row(fn) * p.ldw, (short)0,
-            (int)((uint32_t)valid_rows(fn) * (uint32_t)p.ldw), (int)kBufferFlags);
+    for (int q = 0; q < 2 * FN; ++q) {
+      const int row = q * 8 + copy_row;
+      const uint32_t ch = (uint32_t)((lane & 7) ^ swz_a(row, 8)) * 16u;
+      const bool up = GATED && q >= FN;
+      const uint32_t off = (uint32_t)(up ? row - 8 * FN : row) * (uint32_t)p.ldw + ch + k0;
+      dma_copy16(up ? rw2 : rw, (int)(k0 + ch) < p.k ? off : kOutOfRange, to + (uint32_t)(q * 1024));
+    }
+    const u32x4_t ra = make_rsrc(p.a + ((int64_t)c.row0 + c.m0) * p.lda,
+                                 kb < blocks ? (uint32_t)(valid_m - 1) * (uint32_t)p.lda + row_bytes : 0);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const bool in = (int)k0 + kch + j * 64 < p.k;
-          wv[u][fn][j] = __builtin_bit_cast(
-              i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? w_off + k0 + j * 64 : kOutOfRange, 0, kNonTemporal));
-        }
-      }
+    for (int q = 0; q < 2 * FM; ++q) {
+      const int row = q * 8 + copy_row;
+      const uint32_t ch = (uint32_t)((lane & 7) ^ swz_a(row, 8)) * 16u;
+      const bool in = (int)(k0 + ch) < p.k && row < valid_m;
+      dma_copy16(ra, in ? (uint32_t)row * (uint32_t)p.lda + ch + k0 : kOutOfRange,
+                 to + (uint32_t)(T::W_BYTES + q * 1024));
+    }
+    const int kb_in = min(kb, blocks - 1);
+    dma_copy4(make_rsrc(p.sa + ((int64_t)c.row0 + c.m0) * p.sam + (int64_t)kb_in * p.sak, kOutOfRange),
+              lane < valid_m && kb < blocks ? (uint32_t)lane * (uint32_t)p.sam * 4u : kOutOfRange,
+              to + (uint32_t)(T::W_BYTES + T::A_BYTES));
+    // The weight's scales: one block for the wave's columns; gated: lanes 0 to 3 eight up rows each, lane 4 the gate's.
+    const int block = min((GATED && lane < 4 ? f + n0 + 8 * lane : n0) / kScaleBlock, last_n);
+    dma_copy4(make_rsrc(p.sw + (int64_t)c.e * p.ssg + (int64_t)kb_in * p.ssk, kOutOfRange),
+              lane < 5 && kb < blocks ? (uint32_t)block * (uint32_t)p.ssn * 4u : kOutOfRange,
+              to + (uint32_t)(T::W_BYTES + T::A_BYTES + 256));
+  };
+
+  Cursor next{(int)blockIdx.x, 0, 0, 0, 0, 0, 0};
+  find_rows(next);
+  Cursor at = next;
+  for (int s = 0; s < STAGES; ++s) {
+    if (next.unit >= units) break;
+    issue(next, s);
+    advance(next);
+  }
+
+  // This lane's chunks of a fragment: row lane % 16, chunks lane / 16 and 4 + lane / 16.
+  const int frag_row = lane & 15, group = lane >> 4;
+  auto frag = [&](const char* rows, int i, int left) {
+    const int row = i * 16 + frag_row, s = swz_a(row, 8);
+    i32x4_t lo = *reinterpret_cast<const i32x4_t*>(rows + row * kScaleBlock + ((group ^ s) << 4));
+    i32x4_t hi = *reinterpret_cast<const i32x4_t*>(rows + row * kScaleBlock + (((4 + group) ^ s) << 4));
+    if (left < kScaleBlock) {  // K ends inside the block, perhaps inside a chunk
+      lo = keep_bytes(lo, left - group * 16);
+      hi = keep_bytes(hi, left - 64 - group * 16);
+    }
+    return join(lo, hi);
+  };
+
+  f32x4_t acc[FM][FN];
+#pragma unroll
+  for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn) acc[fm][fn] = f32x4_t{};
+
+  for (int slot = 0; at.unit < units; slot = slot + 1 == STAGES ? 0 : slot + 1) {
+    // The slot has landed once only the younger ones' copies are outstanding (near the end there are fewer).
+    if (next.unit < units) wait_vmcnt<(STAGES - 1) * T::COPIES>();
+    else wait_vmcnt<0>();
+    compiler_fence();
+    const char* from = smem + ring + slot * T::SLOT_BYTES;
+    const int left = (p.k & 15) ? p.k - (wk + at.round * WK) * kScaleBlock : kScaleBlock;
+    i32x8_t av[FM], wv[FN];
+    float sa[FM], sw[FN];
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn) wv[fn] = frag(from, fn, left);
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      av[fm] = frag(from + T::W_BYTES, fm, left);
+      sa[fm] = reinterpret_cast<const float*>(from + T::W_BYTES + T::A_BYTES)[fm * 16 + frag_row];
+    }
+    const float* scales = reinterpret_cast<const float*>(from + T::W_BYTES + T::A_BYTES + 256);
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn)
+      // A lane's four columns of an up fragment lie in one eight.
+      sw[fn] = scales[!GATED ? 0 : fn < FN / 2 ? 4 : (fn - FN / 2) * 2 + (group >> 1)];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next.unit < units) {
+      issue(next, slot);
+      advance(next);
+    }
+    Fragment<false> a[FM];
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) a[fm].set(av[fm]);
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn) {
+      Fragment<false> b;
+      b.set(wv[fn]);
 #pragma unroll
       for (int fm = 0; fm < FM; ++fm) {
-        const int r = fm * 16 + (lane & 15);
+        const f32x4_t t = block_sum(b, a[fm], f32x4_t{});
+        const float s = sa[fm] * sw[fn];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const bool in = (int)k0 + kch + j * 64 < p.k;
-          av[u][fm][j] = __builtin_bit_cast(
-              i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                           ra, in ? (uint32_t)r * (uint32_t)p.lda + kch + k0 + j * 64 : kOutOfRange, 0, 0));
-        }
-        sv[u][fm] = 0.0f;
-        if (kb < blocks && r < valid_m)
-          sv[u][fm] = p.sa[((int64_t)row0 + m0 + r) * p.sam + (int64_t)kb * p.sak];
-      }
-    };
-    auto consume = [&](int u, int kb) {
-      if (kb >= blocks) return;
-      if (kb + 1 == blocks && (p.k & 15)) {
-        const int left = p.k - kb * kScaleBlock - kch;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int fn = 0; fn < FN; ++fn) wv[u][fn][j] = keep_bytes(wv[u][fn][j], left - j * 64);
-#pragma unroll
-          for (int fm = 0; fm < FM; ++fm) av[u][fm][j] = keep_bytes(av[u][fm][j], left - j * 64);
-        }
-      }
-      Fragment<false> a[FM];
-#pragma unroll
-      for (int fm = 0; fm < FM; ++fm) a[fm].set(join(av[u][fm][0], av[u][fm][1]));
-#pragma unroll
-      for (int fn = 0; fn < FN; ++fn) {
-        Fragment<false> b;
-        b.set(join(wv[u][fn][0], wv[u][fn][1]));
-        // A fragment's 16 weight rows lie in one scale block, except up rows that start at a multiple of 8.
-        const int r = first_row(fn);
-        const float s0 = sw[(int64_t)min(r / kScaleBlock, last_n) * p.ssn + (int64_t)kb * p.ssk];
-        float s_w = s0;
-        if constexpr (GATED) {
-          if (fn >= FN / 2) {
-            const float s1 = sw[(int64_t)min((r + 15) / kScaleBlock, last_n) * p.ssn + (int64_t)kb * p.ssk];
-            s_w = (r + (lane >> 4) * 4) / kScaleBlock == r / kScaleBlock ? s0 : s1;
-          }
-        }
-#pragma unroll
-        for (int fm = 0; fm < FM; ++fm) {
-          const f32x4_t t = block_sum(b, a[fm], f32x4_t{});
-          const float s = sv[u][fm] * s_w;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[fm][fn][i] += t[i] * s;
-        }
-      }
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u) load(u, wk + u * WK);
-    for (int kb = wk; kb < blocks; kb += U * WK) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        consume(u, kb + u * WK);
-        load(u, kb + (u + U) * WK);
+        for (int i = 0; i < 4; ++i) acc[fm][fn][i] += t[i] * s;
       }
     }
+    if (at.round + 1 < rounds) {
+      ++at.round;
+      continue;
+    }
 
-    // Join the WK sums of every fragment in wave order: fragment id (fm, fn, wn) is summed by wave id % NW.
-    f32x4_t* red = reinterpret_cast<f32x4_t*>(smem);
-#pragma unroll
-    for (int fm = 0; fm < FM; ++fm)
-#pragma unroll
-      for (int fn = 0; fn < FN; ++fn) red[((wk * T::FRAGS) + (fm * FN + fn) * WN + wn) * 64 + lane] = acc[fm][fn];
-    __syncthreads();
-    auto total = [&](int id) {
-      f32x4_t v = red[id * 64 + lane];
-#pragma unroll
-      for (int x = 1; x < WK; ++x) v += red[(x * T::FRAGS + id) * 64 + lane];
-      return v;
-    };
+    const int valid_m = min(T::BM, at.m - at.m0);
+    const int64_t first = (int64_t)at.row0 + at.m0;
     if constexpr (!GATED) {
       constexpr int ES = sizeof(typename E::raw);
       const bool vec = p.n % 4 == 0 && p.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (4 * ES - 1)) == 0;
-      for (int id = wave; id < T::FRAGS; id += T::NW) {
-        const int fw = id % WN, fn = id / WN % FN, fm = id / WN / FN;
-        const f32x4_t v = total(id);
-        const int row = fm * 16 + (lane & 15);
-        const int n = tn * T::BN + fw * 16 * FN + fn * 16 + (lane >> 4) * 4;
-        if (row >= valid_m || n >= p.n) continue;
-        char* out = static_cast<char*>(p.out) + (((int64_t)row0 + m0 + row) * p.ldo + n) * ES;
+      auto store = [&](const f32x4_t& v, int fm, int fn, int fw) {
+        const int row = fm * 16 + frag_row;
+        const int n = at.tn * T::BN + fw * 16 * FN + fn * 16 + group * 4;
+        if (row >= valid_m || n >= p.n) return;
+        char* out = static_cast<char*>(p.out) + ((first + row) * p.ldo + n) * ES;
         if (vec) {
           store4<E>(out, v);
         } else {
@@ -855,49 +888,80 @@ __global__ void __launch_bounds__(T::NT) fp8_stream_kernel(Fp8Params p) {
           for (int i = 0; i < 4; ++i)
             if (n + i < p.n) store1<E>(out + i * ES, v[i]);
         }
+      };
+      if constexpr (WK == 1) {
+#pragma unroll
+        for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+          for (int fn = 0; fn < FN; ++fn) store(acc[fm][fn], fm, fn, wn);
+      } else {
+        // Join the WK sums of every fragment in wave order: fragment id (fm, fn, wn) is summed by wave id % NW.
+        // The barriers leave the copies in flight alone.
+        f32x4_t* red = reinterpret_cast<f32x4_t*>(smem + T::RING_BYTES);
+#pragma unroll
+        for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+          for (int fn = 0; fn < FN; ++fn) red[((wk * T::FRAGS) + (fm * FN + fn) * WN + wn) * 64 + lane] = acc[fm][fn];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        compiler_fence();
+        for (int id = wave; id < T::FRAGS; id += T::NW) {
+          f32x4_t v = red[id * 64 + lane];
+#pragma unroll
+          for (int x = 1; x < WK; ++x) v += red[(x * T::FRAGS + id) * 64 + lane];
+          store(v, id / WN / FN, id / WN % FN, id % WN);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        compiler_fence();
       }
     } else {
-      // Output fragment id (fm, fn < FN / 2, wn): 8 of them make up a row's 128 columns.
-      constexpr int OUTS = T::FRAGS / 2, MINE = (OUTS + T::NW - 1) / T::NW;
-      uint32_t* tops = reinterpret_cast<uint32_t*>(smem + T::RED_BYTES);  // [row][8]
-      f32x4_t h[MINE];
+      // silu(gate) * up; a row's 128 columns are four waves' two fragments, whose maxima meet in LDS.
+      uint32_t* tops = reinterpret_cast<uint32_t*>(smem + T::RING_BYTES);  // [row][8]
 #pragma unroll
-      for (int x = 0; x < MINE; ++x) {
-        const int id = wave + x * T::NW;
-        if (id >= OUTS) continue;
-        const int fw = id % WN, fn = id / WN % (FN / 2), fm = id / WN / (FN / 2);
-        const f32x4_t gate = total((fm * FN + fn) * WN + fw), up = total((fm * FN + fn + FN / 2) * WN + fw);
-        uint32_t top = 0;
+      for (int fm = 0; fm < FM; ++fm)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          h[x][i] = gated(gate[i], up[i]);
-          top = max(top, abs_bits(h[x][i]));
+        for (int fn = 0; fn < FN / 2; ++fn) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[fm][fn][i] = gated(acc[fm][fn][i], acc[fm][fn + FN / 2][i]);
+            top = max(top, abs_bits(acc[fm][fn][i]));
+          }
+          top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+          top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+          if (lane < 16) tops[(fm * 16 + lane) * 8 + wn * (FN / 2) + fn] = top;
         }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-        if (lane < 16) tops[(fm * 16 + lane) * 8 + fw * (FN / 2) + fn] = top;
-      }
-      __syncthreads();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      compiler_fence();
 #pragma unroll
-      for (int x = 0; x < MINE; ++x) {
-        const int id = wave + x * T::NW;
-        if (id >= OUTS) continue;
-        const int fw = id % WN, fn = id / WN % (FN / 2), fm = id / WN / (FN / 2);
-        const int row = fm * 16 + (lane & 15);
+      for (int fm = 0; fm < FM; ++fm) {
+        const int row = fm * 16 + frag_row;
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, tops[row * 8 + i]);
         const float amax = floored(top), inverse = kE4m3Max / amax;
         if (row >= valid_m) continue;
-        if (fw == 0 && fn == 0 && lane < 16)
-          p.out_scale[((int64_t)row0 + m0 + row) * p.osm + (int64_t)tn * p.osk] = amax / kE4m3Max;
-        const int n = tn * T::OUT_COLS + fw * 8 * FN + fn * 16 + (lane >> 4) * 4;
-        if (n < f)
-          *MOEGEMM_GLOBAL(int32_t, static_cast<uint8_t*>(p.out) + ((int64_t)row0 + m0 + row) * p.ldo + n) =
-              pack_e4m3(h[x] * inverse);
+        if (wn == 0 && lane < 16)
+          p.out_scale[(first + row) * p.osm + (int64_t)at.tn * p.osk] = amax / kE4m3Max;
+#pragma unroll
+        for (int fn = 0; fn < FN / 2; ++fn) {
+          const int n = at.tn * T::OUT_COLS + wn * 8 * FN + fn * 16 + group * 4;
+          if (n < f)
+            *MOEGEMM_GLOBAL(int32_t, static_cast<uint8_t*>(p.out) + (first + row) * p.ldo + n) =
+                pack_e4m3(acc[fm][fn] * inverse);
+        }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      compiler_fence();
     }
-    __syncthreads();  // the sums are read before the next rows' are written
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn) acc[fm][fn] = f32x4_t{};
+    advance(at);
   }
 }
 

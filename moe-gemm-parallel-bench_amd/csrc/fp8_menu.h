@@ -9,7 +9,7 @@ typedef hipError_t (*Fp8LaunchFn)(const Fp8Params&, int grid, hipStream_t stream
 
 struct Fp8Variant {
   int block_m, block_n;  // rows and weight rows of a tile
-  int stream;            // 1: a workgroup per (group, column tile); 0: persistent over tiles
+  int stream;            // 1: units of (group, column tile); 0: tiles of each group's rows and columns
   int fast;              // sums on the 8-bit matrix instructions
   Fp8LaunchFn launch;
 };
@@ -25,14 +25,14 @@ hipError_t launch_fp8_stream(const Fp8Params& p, int grid, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// X(E, BM, BN, WAVES_M, WAVES_N, STAGES, FAST) and Y(E, FM, FN, WAVES_N, WAVES_K, BLOCKS_IN_FLIGHT, unused).
+// X(E, BM, BN, WAVES_M, WAVES_N, STAGES, FAST) and Y(E, FM, FN, WAVES_N, WAVES_K, STAGES, unused).
 #define MOEGEMM_MENU_FP8(X, Y, E)                                                               \
   X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, true) X(E, 128, 128, 2, 2, 2, true)     \
   X(E, 128, 256, 2, 4, 2, false) X(E, 128, 128, 2, 2, 2, false)                                 \
-  Y(E, 1, 1, 1, 8, 4, 0) Y(E, 1, 4, 1, 4, 3, 0) Y(E, 2, 4, 1, 4, 2, 0) Y(E, 4, 4, 1, 4, 1, 0)
+  Y(E, 1, 1, 1, 8, 4, 0) Y(E, 1, 4, 1, 4, 3, 0) Y(E, 2, 4, 1, 4, 2, 0) Y(E, 4, 2, 1, 4, 2, 0)
 #define MOEGEMM_MENU_FP8_GATED(X, Y, E)                                                         \
   X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, false)    \
-  Y(E, 1, 4, 4, 2, 3, 0) Y(E, 2, 4, 4, 2, 2, 0)
+  Y(E, 1, 4, 4, 1, 3, 0) Y(E, 2, 4, 4, 1, 3, 0)
 
 #define MOEGEMM_FP8_X(E, BM, BN, WM, WN, S, FAST) \
   Fp8Variant{BM, BN, 0, FAST, &launch_fp8_tile<Fp8Tile<E, BM, BN, WM, WN, S, false, FAST>>},
