@@ -58,27 +58,45 @@ int check_scales(int64_t stride_sam, int64_t stride_ssn, int32_t n) {
   return MOEGEMM_OK;
 }
 
-// Variant for `rows` rows over `groups` groups.  Up to 64 rows a group on average (32 gated), weights are
-// what a call reads: the stream kernels read each once, at 16, 32 or 64 rows a tile.
-int choose(const Fp8Variant* table, int count, int64_t rows, int64_t groups, int64_t out_cols, int gated, int fast,
-           int cus) {
-  auto find = [&](int bm, int bn, int stream) {
-    for (int i = 0; i < count; ++i)
-      if (table[i].block_m == bm && (bn == 0 || table[i].block_n == bn) && table[i].stream == stream &&
-          (stream || table[i].fast == fast))
-        return i;
-    return -1;
-  };
-  const int64_t mean = cdiv(rows, groups), cols = out_cols * (gated ? 2 : 1);
-  if (mean <= (gated ? 32 : 64)) {
-    const int bm = mean <= 12 ? 16 : mean <= 24 || gated ? 32 : 64;
-    if (bm == 16 && !gated && groups * cdiv(out_cols, 64) < 2 * cus) return find(16, 16, 1);
-    if (bm == 16 && !gated) return find(16, 64, 1);
-    return find(bm, 0, 1);
+// Variant for `rows` rows over `groups` groups.
+//
+// Up to about 32 rows a group (20 with fast sums, whose tiles are faster) a call is bound by reading the weights, and
+// the stream kernels read them once where a group's rows fit their 16 or 32; routed groups are taken to hold up to
+// 1.6 times the mean.  32 experts of [4096, 7168], us: 8 rows each stream 145, tile 240; 32 rows stream 166, exact
+// tile 243; 64 rows stream 315, exact tile 243, fast tile 195.
+// Among stream kernels: units run in rounds of one per CU, at a cost of their weights and about 200 rows of one
+// block for the join and the stores.  [7168, 2048] x 32: 256 columns 89, 128 columns 79 (7 whole rounds), 64
+// columns 92; one group of [4096, 7168]: 256 columns 52, 16 columns 14.4.
+// Among tiles: rounds by the time of a slice, in units of 10 ns (1000 rows of [4096, 4096]: 256x256 51 us, 128x256 35,
+// 128x128 31; 16384 rows of 32 x [4096, 7168]: 473, 597, 843).
+int choose(const Fp8Variant* table, int count, int64_t rows, int64_t groups, int64_t cols, int64_t k, int gated,
+           int fast, int cus) {
+  const int64_t active = std::min(groups, rows), mean = cdiv(rows, active);
+  const int64_t high = active == 1 ? rows : cdiv(mean * 8, 5);
+  const bool stream = active == 1 ? rows <= 32 : mean <= (fast ? 20 : 32);
+  const int64_t blocks = cdiv(k, kScaleBlock);
+  int best = -1;
+  int64_t least = 0;
+  for (int i = 0; i < count; ++i) {
+    const Fp8Variant& v = table[i];
+    if ((v.stream != 0) != stream || (!stream && v.fast != fast)) continue;
+    const int64_t n_tiles = cdiv(cols, v.block_n);
+    int64_t cost;
+    if (stream) {
+      if (v.block_m != (high <= 16 ? 16 : 32)) continue;
+      const int64_t padded = cdiv(blocks, v.waves_k) * v.waves_k;
+      cost = cdiv(active * n_tiles, cus) * (v.block_n * padded + 200);
+    } else {
+      const int64_t tiles = std::max(active, rows / v.block_m + active / 2 + (active == 1 && rows % v.block_m != 0)) * n_tiles;
+      const int slice = v.block_m == 256 ? 170 : v.block_n == 256 ? (v.fast ? 115 : 190) : (v.fast ? 90 : 115);
+      cost = cdiv(tiles, cus) * slice;
+    }
+    if (best < 0 || cost < least) {
+      best = i;
+      least = cost;
+    }
   }
-  if (fast && rows / groups >= 192 && cdiv(rows, 256) * cdiv(cols, 256) * 4 >= 3 * cus) return find(256, 256, 0);
-  if (!gated && cdiv(rows, 128) * cdiv(cols, 256) < cus) return find(128, 128, 0);
-  return find(128, 256, 0);
+  return best;
 }
 
 int launch_product(const Fp8Variant* table, int count, Fp8Params& p, int64_t out_cols, int gated, int fast,
@@ -88,7 +106,7 @@ int launch_product(const Fp8Variant* table, int count, Fp8Params& p, int64_t out
     return report(MOEGEMM_ERR_NO_KERNEL, "fp8 variant %d is not compiled (0 to %d, or -1)", variant, count - 1);
   if (p.rows == 0) return MOEGEMM_OK;
   const int cus = grid_size > 0 ? grid_size : 256;
-  if (variant < 0) variant = choose(table, count, p.rows, p.groups, out_cols, gated, fast, cus);
+  if (variant < 0) variant = choose(table, count, p.rows, p.groups, gated ? cdiv(out_cols, 128) * 256 : p.n, p.k, gated, fast, cus);
   if (variant < 0) return report(MOEGEMM_ERR_NO_KERNEL, "no fp8 variant for this shape");
   const Fp8Variant& v = table[variant];
   const int64_t n_tiles = cdiv(p.n, v.block_n);  // gated: n = 2F weight rows in tiles of 128 + 128

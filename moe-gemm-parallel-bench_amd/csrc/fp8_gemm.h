@@ -709,6 +709,7 @@ struct Fp8Stream {
   static constexpr int RING_BYTES = NW * STAGES * SLOT_BYTES;
   static constexpr int RED_BYTES = WK > 1 ? WK * FRAGS * 1024 : 0;
   static constexpr int LDS_BYTES = RING_BYTES + RED_BYTES + (GATED ? BM * 8 * 4 : 0);
+  static_assert(kScaleBlock % (16 * FN) == 0, "a wave's columns lie in one scale block");
   static_assert(!GATED || (OUT_COLS == kScaleBlock && FN == 4 && WK == 1), "a gated tile is one block of the output");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS of one CU");
   static_assert(STAGES * COPIES < 64, "vmcnt is 6 bits");
@@ -742,77 +743,90 @@ __global__ void __launch_bounds__(T::NT) fp8_stream_kernel(Fp8Params p) {
     c.m0 = 0;
     c.round = 0;
   };
-  auto advance = [&](Cursor& c) {
-    if (++c.round < rounds) return;
+  auto advance = [&](Cursor& c) {  // true at a new unit or row tile
+    if (++c.round < rounds) return false;
     c.round = 0;
     c.m0 += T::BM;
-    if (c.m0 < c.m) return;
+    if (c.m0 < c.m) return true;
     c.unit += gridDim.x;
     find_rows(c);
+    return true;
   };
-  auto first_col = [&](const Cursor& c) { return c.tn * T::OUT_COLS + wn * (GATED ? 8 : 16) * FN; };
 
-  // Copies: eight rows of 128 bytes each, chunk c of row r at c ^ swz_a(r, 8).
-  const int copy_row = lane >> 3;
+  // Copies: eight rows of 128 bytes each.  Chunk c of row r lies at c ^ (r / 2 % 8), which puts the 16 rows a
+  // fragment reads at one chunk on all banks; two copies further on it is the same, next door it differs in bit 2.
   const uint32_t ring = (uint32_t)(wave * STAGES * T::SLOT_BYTES);
   const uint32_t ring_lds = lds_address(smem) + ring;
   const uint32_t row_bytes = ((uint32_t)p.k + 15u) & ~15u;
+  const uint32_t copy_chunk = (uint32_t)((lane & 7) ^ (lane >> 4)) * 16u;
+  const uint32_t w_row = (uint32_t)(lane >> 3) * (uint32_t)p.ldw, a_row = (uint32_t)(lane >> 3) * (uint32_t)p.lda;
+  const uint32_t w_even = w_row + copy_chunk, w_odd = w_row + (copy_chunk ^ 64u);
+  const uint32_t a_even = a_row + copy_chunk, a_odd = a_row + (copy_chunk ^ 64u);
+  // What a unit's copies are made of.  A panel ends with the chunk that holds its last row's last k; what a copy
+  // reads past K inside it is cut from the fragments.
+  u32x4_t rw, rw2, ra, rs, rt;
+  uint32_t rw_bytes = 0, ra_bytes = 0, s_off = 0, t_off = 0;
+  const float *s_base = nullptr, *t_base = nullptr;
+  auto set_unit = [&](const Cursor& c) {
+    const int n0 = c.tn * T::OUT_COLS + wn * (GATED ? 8 : 16) * FN;
+    const int valid_m = min(T::BM, c.m - c.m0);
+    const int valid_n = min(GATED ? f - n0 : p.n - n0, GATED ? 8 * FN : 16 * FN);
+    const uint8_t* w = p.w + (int64_t)c.e * p.swg + (int64_t)n0 * p.ldw;
+    rw_bytes = valid_n > 0 ? (uint32_t)(valid_n - 1) * (uint32_t)p.ldw + row_bytes : 0;
+    ra_bytes = (uint32_t)(valid_m - 1) * (uint32_t)p.lda + row_bytes;
+    rw = make_rsrc(w, rw_bytes);
+    if constexpr (GATED) rw2 = make_rsrc(w + (int64_t)f * p.ldw, rw_bytes);
+    ra = make_rsrc(p.a + ((int64_t)c.row0 + c.m0) * p.lda, ra_bytes);
+    s_base = p.sa + ((int64_t)c.row0 + c.m0) * p.sam + (int64_t)wk * p.sak;
+    s_off = lane < valid_m ? (uint32_t)lane * (uint32_t)p.sam * 4u : kOutOfRange;
+    // The weight's scales: one block for the wave's columns; gated: lanes 0 to 3 eight up rows each, lane 4 the gate's.
+    const int block = min((GATED && lane < 4 ? f + n0 + 8 * lane : n0) / kScaleBlock, last_n);
+    t_base = p.sw + (int64_t)c.e * p.ssg + (int64_t)wk * p.ssk;
+    t_off = lane < 5 ? (uint32_t)block * (uint32_t)p.ssn * 4u : kOutOfRange;
+  };
   auto issue = [&](const Cursor& c, int slot) {
     const uint32_t to = ring_lds + (uint32_t)(slot * T::SLOT_BYTES);
     const int kb = wk + c.round * WK;
     const uint32_t k0 = (uint32_t)kb * kScaleBlock;
-    const int n0 = first_col(c);
-    const int valid_m = min(T::BM, c.m - c.m0);
-    const uint8_t* w = p.w + (int64_t)c.e * p.swg + (int64_t)n0 * p.ldw;
-    const int valid_n = min(GATED ? f - n0 : p.n - n0, GATED ? 8 * FN : 16 * FN);
-    const uint32_t w_bytes = valid_n > 0 && kb < blocks ? (uint32_t)(valid_n - 1) * (uint32_t)p.ldw + row_bytes : 0;
-    const u32x4_t rw = make_rsrc(w, w_bytes);
-    const u32x4_t rw2 = GATED ? make_rsrc(w + (int64_t)f * p.ldw, w_bytes) : rw;
+    const bool in = kb < blocks;  // else zeros: values, and scales of either side
+    rw[2] = in ? rw_bytes : 0;
+    if constexpr (GATED) rw2[2] = rw[2];
+    ra[2] = in ? ra_bytes : 0;
+    uint32_t w0 = w_even + k0, w1 = w_odd + k0, a0 = a_even + k0, a1 = a_odd + k0;
+    asm volatile("" : "+v"(w0), "+v"(w1), "+v"(a0), "+v"(a1));  // the rows' steps are added here
 #pragma unroll
     for (int q = 0; q < 2 * FN; ++q) {
-      const int row = q * 8 + copy_row;
-      const uint32_t ch = (uint32_t)((lane & 7) ^ swz_a(row, 8)) * 16u;
       const bool up = GATED && q >= FN;
-      const uint32_t off = (uint32_t)(up ? row - 8 * FN : row) * (uint32_t)p.ldw + ch + k0;
-      dma_copy16(up ? rw2 : rw, (int)(k0 + ch) < p.k ? off : kOutOfRange, to + (uint32_t)(q * 1024));
+      dma_copy16_nt(up ? rw2 : rw, (q & 1 ? w1 : w0) + (uint32_t)((up ? q - FN : q) * 8) * (uint32_t)p.ldw,
+                 to + (uint32_t)(q * 1024));
     }
-    const u32x4_t ra = make_rsrc(p.a + ((int64_t)c.row0 + c.m0) * p.lda,
-                                 kb < blocks ? (uint32_t)(valid_m - 1) * (uint32_t)p.lda + row_bytes : 0);
 #pragma unroll
-    for (int q = 0; q < 2 * FM; ++q) {
-      const int row = q * 8 + copy_row;
-      const uint32_t ch = (uint32_t)((lane & 7) ^ swz_a(row, 8)) * 16u;
-      const bool in = (int)(k0 + ch) < p.k && row < valid_m;
-      dma_copy16(ra, in ? (uint32_t)row * (uint32_t)p.lda + ch + k0 : kOutOfRange,
-                 to + (uint32_t)(T::W_BYTES + q * 1024));
-    }
-    const int kb_in = min(kb, blocks - 1);
-    dma_copy4(make_rsrc(p.sa + ((int64_t)c.row0 + c.m0) * p.sam + (int64_t)kb_in * p.sak, kOutOfRange),
-              lane < valid_m && kb < blocks ? (uint32_t)lane * (uint32_t)p.sam * 4u : kOutOfRange,
-              to + (uint32_t)(T::W_BYTES + T::A_BYTES));
-    // The weight's scales: one block for the wave's columns; gated: lanes 0 to 3 eight up rows each, lane 4 the gate's.
-    const int block = min((GATED && lane < 4 ? f + n0 + 8 * lane : n0) / kScaleBlock, last_n);
-    dma_copy4(make_rsrc(p.sw + (int64_t)c.e * p.ssg + (int64_t)kb_in * p.ssk, kOutOfRange),
-              lane < 5 && kb < blocks ? (uint32_t)block * (uint32_t)p.ssn * 4u : kOutOfRange,
-              to + (uint32_t)(T::W_BYTES + T::A_BYTES + 256));
+    for (int q = 0; q < 2 * FM; ++q)
+      dma_copy16(ra, (q & 1 ? a1 : a0) + (uint32_t)(q * 8) * (uint32_t)p.lda, to + (uint32_t)(T::W_BYTES + q * 1024));
+    rs = make_rsrc(s_base + (int64_t)c.round * WK * p.sak, in ? kOutOfRange : 0);
+    dma_copy4(rs, s_off, to + (uint32_t)(T::W_BYTES + T::A_BYTES));
+    rt = make_rsrc(t_base + (int64_t)c.round * WK * p.ssk, in ? kOutOfRange : 0);
+    dma_copy4(rt, t_off, to + (uint32_t)(T::W_BYTES + T::A_BYTES + 256));
   };
 
   Cursor next{(int)blockIdx.x, 0, 0, 0, 0, 0, 0};
   find_rows(next);
+  if (next.unit >= units) return;
   Cursor at = next;
+  set_unit(next);
   for (int s = 0; s < STAGES; ++s) {
     if (next.unit >= units) break;
     issue(next, s);
-    advance(next);
+    if (advance(next) && next.unit < units) set_unit(next);
   }
 
   // This lane's chunks of a fragment: row lane % 16, chunks lane / 16 and 4 + lane / 16.
   const int frag_row = lane & 15, group = lane >> 4;
+  const uint32_t frag_lo = (uint32_t)(frag_row * kScaleBlock + ((group ^ (frag_row >> 1)) << 4)), frag_hi = frag_lo ^ 64u;
   auto frag = [&](const char* rows, int i, int left) {
-    const int row = i * 16 + frag_row, s = swz_a(row, 8);
-    i32x4_t lo = *reinterpret_cast<const i32x4_t*>(rows + row * kScaleBlock + ((group ^ s) << 4));
-    i32x4_t hi = *reinterpret_cast<const i32x4_t*>(rows + row * kScaleBlock + (((4 + group) ^ s) << 4));
-    if (left < kScaleBlock) {  // K ends inside the block, perhaps inside a chunk
+    i32x4_t lo = *reinterpret_cast<const i32x4_t*>(rows + i * 16 * kScaleBlock + frag_lo);
+    i32x4_t hi = *reinterpret_cast<const i32x4_t*>(rows + i * 16 * kScaleBlock + frag_hi);
+    if (left < kScaleBlock) {  // K ends inside the block
       lo = keep_bytes(lo, left - group * 16);
       hi = keep_bytes(hi, left - 64 - group * 16);
     }
@@ -831,7 +845,7 @@ __global__ void __launch_bounds__(T::NT) fp8_stream_kernel(Fp8Params p) {
     else wait_vmcnt<0>();
     compiler_fence();
     const char* from = smem + ring + slot * T::SLOT_BYTES;
-    const int left = (p.k & 15) ? p.k - (wk + at.round * WK) * kScaleBlock : kScaleBlock;
+    const int left = p.k - (wk + at.round * WK) * kScaleBlock;
     i32x8_t av[FM], wv[FN];
     float sa[FM], sw[FN];
 #pragma unroll
@@ -849,7 +863,7 @@ __global__ void __launch_bounds__(T::NT) fp8_stream_kernel(Fp8Params p) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (next.unit < units) {
       issue(next, slot);
-      advance(next);
+      if (advance(next) && next.unit < units) set_unit(next);
     }
     Fragment<false> a[FM];
 #pragma unroll

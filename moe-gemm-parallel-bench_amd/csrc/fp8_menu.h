@@ -10,6 +10,7 @@ typedef hipError_t (*Fp8LaunchFn)(const Fp8Params&, int grid, hipStream_t stream
 struct Fp8Variant {
   int block_m, block_n;  // rows and weight rows of a tile
   int stream;            // 1: units of (group, column tile); 0: tiles of each group's rows and columns
+  int waves_k;           // stream: waves that share K
   int fast;              // sums on the 8-bit matrix instructions
   Fp8LaunchFn launch;
 };
@@ -25,23 +26,25 @@ hipError_t launch_fp8_stream(const Fp8Params& p, int grid, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// X(E, BM, BN, WAVES_M, WAVES_N, STAGES, FAST) and Y(E, FM, FN, WAVES_N, WAVES_K, STAGES, unused).
+// X(E, BM, BN, WAVES_M, WAVES_N, STAGES, FAST) and Y(E, FM, FN, WAVES_N, WAVES_K, STAGES, unused).  Stream tiles are
+// 16 or 32 rows by 256 to 16 columns: wide ones for many units, narrow ones with K split over the waves for few.
 #define MOEGEMM_MENU_FP8(X, Y, E)                                                               \
   X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, true) X(E, 128, 128, 2, 2, 2, true)     \
   X(E, 128, 256, 2, 4, 2, false) X(E, 128, 128, 2, 2, 2, false)                                 \
-  Y(E, 1, 1, 1, 8, 4, 0) Y(E, 1, 4, 1, 4, 3, 0) Y(E, 2, 4, 1, 4, 2, 0) Y(E, 4, 2, 1, 4, 2, 0)
+  Y(E, 1, 4, 4, 1, 3, 0) Y(E, 1, 2, 4, 2, 2, 0) Y(E, 1, 4, 1, 4, 3, 0) Y(E, 1, 1, 1, 8, 4, 0)   \
+  Y(E, 2, 4, 4, 1, 2, 0) Y(E, 2, 1, 1, 8, 2, 0)
 #define MOEGEMM_MENU_FP8_GATED(X, Y, E)                                                         \
   X(E, 256, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, true) X(E, 128, 256, 2, 4, 2, false)    \
   Y(E, 1, 4, 4, 1, 3, 0) Y(E, 2, 4, 4, 1, 3, 0)
 
 #define MOEGEMM_FP8_X(E, BM, BN, WM, WN, S, FAST) \
-  Fp8Variant{BM, BN, 0, FAST, &launch_fp8_tile<Fp8Tile<E, BM, BN, WM, WN, S, false, FAST>>},
+  Fp8Variant{BM, BN, 0, 1, FAST, &launch_fp8_tile<Fp8Tile<E, BM, BN, WM, WN, S, false, FAST>>},
 #define MOEGEMM_FP8_Y(E, FM, FN, WN, WK, U, F) \
-  Fp8Variant{16 * FM, 16 * FN * WN, 1, 0, &launch_fp8_stream<Fp8Stream<E, FM, FN, WN, WK, U, false>, E>},
+  Fp8Variant{16 * FM, 16 * FN * WN, 1, WK, 0, &launch_fp8_stream<Fp8Stream<E, FM, FN, WN, WK, U, false>, E>},
 #define MOEGEMM_FP8_GX(E, BM, BN, WM, WN, S, FAST) \
-  Fp8Variant{BM, BN, 0, FAST, &launch_fp8_tile<Fp8Tile<E, BM, BN, WM, WN, S, true, FAST>>},
+  Fp8Variant{BM, BN, 0, 1, FAST, &launch_fp8_tile<Fp8Tile<E, BM, BN, WM, WN, S, true, FAST>>},
 #define MOEGEMM_FP8_GY(E, FM, FN, WN, WK, U, F) \
-  Fp8Variant{16 * FM, 16 * FN * WN, 1, 0, &launch_fp8_stream<Fp8Stream<E, FM, FN, WN, WK, U, true>, E>},
+  Fp8Variant{16 * FM, 16 * FN * WN, 1, WK, 0, &launch_fp8_stream<Fp8Stream<E, FM, FN, WN, WK, U, true>, E>},
 
 // The kernels of a menu, for the device pass.
 #define MOEGEMM_FP8_XK(E, BM, BN, WM, WN, S, FAST) \
