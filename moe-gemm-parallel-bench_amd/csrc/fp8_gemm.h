@@ -120,6 +120,67 @@ __device__ __forceinline__ bool find_group_tile(const int32_t* offs, int groups,
   return false;
 }
 
+// The same lookup from tables in LDS, for up to kTableGroups groups: find_group_tile loads the offsets into vector
+// registers and so waits for every copy and store in flight, which a loop that prefetches across tiles must not.
+constexpr int kTableGroups = 1024;
+struct TileTable {
+  int32_t tiles[kTableGroups];  // cumulative tile counts
+  int32_t ends[kTableGroups];   // offsets, clamped
+};
+
+// Every thread of the workgroup calls it; ends with a barrier.
+__device__ __forceinline__ void build_tile_table(TileTable& table, const int32_t* offs, int groups, int rows, int bm,
+                                                 int n_tiles) {
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x < 64 && groups <= kTableGroups) {
+    int64_t base = 0;
+    for (int first = 0; first < groups; first += 64) {
+      int m = 0;
+      if (first + lane < groups) group_rows(offs, rows, first + lane, m);
+      int64_t sum = (int64_t)((m + bm - 1) / bm) * n_tiles;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int64_t below = value_of(sum, lane - d);
+        if (lane >= d) sum += below;
+      }
+      sum = min(base + sum, (int64_t)INT32_MAX);  // overlapping groups of decreasing offsets
+      if (first + lane < groups) {
+        table.tiles[first + lane] = (int32_t)sum;
+        table.ends[first + lane] = offs ? min(max(offs[first + lane], 0), rows) : rows;
+      }
+      base = uniform(value_of(sum, 63));
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ bool find_tile(const TileTable& table, const int32_t* offs, int groups, int rows, int bm,
+                                          int n_tiles, int t, GroupTile& g) {
+  if (groups > kTableGroups) return find_group_tile(offs, groups, rows, bm, n_tiles, t, g);
+  const int lane = thread_here() & 63;
+  int before = 0, row0 = 0;
+  for (int first = 0; first < groups; first += 64) {
+    const int at = min(first + lane, groups - 1);
+    const int tiles = table.tiles[at], end = table.ends[at];
+    const uint64_t past = __builtin_amdgcn_ballot_w64(tiles > t);
+    if (past) {
+      const int hit = __builtin_ctzll(past);
+      if (hit > 0) {
+        before = __builtin_amdgcn_readlane(tiles, hit - 1);
+        row0 = __builtin_amdgcn_readlane(end, hit - 1);
+      }
+      g.e = first + hit;
+      g.local = t - before;
+      g.row0 = row0;
+      g.m = __builtin_amdgcn_readlane(end, hit) - row0;  // a group with tiles has rows
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(tiles, 63);
+    row0 = __builtin_amdgcn_readlane(end, 63);
+  }
+  return false;
+}
+
 __device__ __forceinline__ f32x16_t mfma_fp8(i32x8_t w, i32x8_t a, f32x16_t c) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, 0, 0, 0, 0, 0, 0);
 }
@@ -230,7 +291,8 @@ struct Fp8Tile {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SCALE_BYTES;
   static constexpr int PER_STAGE = QA + QB + QS;  // copies of a wave per stage
   static constexpr int RED_BYTES = GATED ? BM * WN * 4 : 0;  // row maxima of the waves that share a row
-  static constexpr int LDS_BYTES = STAGES * STAGE_BYTES + RED_BYTES;
+  static constexpr int TABLE_OFFSET = STAGES * STAGE_BYTES + RED_BYTES;
+  static constexpr int LDS_BYTES = TABLE_OFFSET + (int)sizeof(TileTable);
   static constexpr int OUT_COLS = GATED ? BN / 2 : BN;  // output columns of a tile
   static_assert(IA % NW == 0 && IB % NW == 0, "every wave issues the same copies");
   static_assert(!GATED || (BN == 256 && FN == 2), "a gated tile is one 128-column block of the output");
@@ -598,8 +660,10 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   const int blocks = (p.k + kScaleBlock - 1) / kScaleBlock;
   const int kt_count = max(blocks, 2);
   const bool cut = p.k % kScaleBlock != 0;  // slices from K / 128 on are cut in LDS
+  TileTable& table = *reinterpret_cast<TileTable*>(smem + T::TABLE_OFFSET);
+  build_tile_table(table, p.offs, p.groups, p.rows, T::BM, p.n_tiles);
   GroupTile g;
-  if (!find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g)) return;
+  if (!find_tile(table, p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g)) return;
   int tm, tn;
   group_m_order(g.local, (g.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm, tn);
   typename T::Copies c;
@@ -634,7 +698,7 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
     GroupTile g_next{};
     int tm_next = 0, tn_next = 0;
     t += grid;
-    more = find_group_tile(p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g_next);
+    more = find_tile(table, p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g_next);
     if (more) group_m_order(g_next.local, (g_next.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm_next, tn_next);
     f32x16_t acc[T::FM][T::FN];
 #pragma unroll

@@ -153,6 +153,113 @@ struct TileSums {
   }
 };
 
+// Cross-tile chaining of the ping-pong tile (see PingPongTile::run_tile_chained) with an epilogue of the caller's.
+// A tile's last three refills copy the next tile's slices 0 to 2; then the outputs leave in exactly Finish::STORES vector
+// stores per wave, and slice 3 of the next tile follows.  A wave's vector memory operations complete in issue
+// order, so the next tile waits for its slices by counting what is younger, stores included, and never for the stores
+// before it needs slice 3.  `finish.chained(acc, pd, m0, n0, wave_m, wave_n, buffer)` may stage through the wave's
+// slots of the last slice's buffer; `finish.last(...)` ends a tile without a successor.
+struct ChainState {
+  int rot;
+  bool prefetched;
+};
+
+template <class T, bool SECOND, class Finish>
+__device__ __forceinline__ void chained_tile(const ProblemDesc& pd, int m0, int n0, const ProblemDesc& next, int m1,
+                                             int n1, bool has_next, char* smem, ChainState& ch, Finish&& finish) {
+  constexpr int FM = T::FM, FN = T::FN, KK = T::KK, BK = T::BK, STAGES = T::STAGES, XMIN = T::XMIN;
+  using F = typename std::remove_reference<Finish>::type;
+  static_assert(STAGES == 4 && 3 * XMIN + F::STORES < 64, "outstanding operations must fit the 6-bit vmcnt");
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wave_m = wave / T::WN, wave_n = wave % T::WN;
+  typename T::Dma d;
+  T::setup_dma(d, pd, m0, n0, smem);
+  typename T::acc_t acc[FM][FN];
+  TileSums<T>::clear(acc);
+  const bool pre = ch.prefetched;
+  const int rot = pre ? ch.rot : 0;
+  if (pre) {
+    wait_vmcnt<3 * XMIN + F::STORES>();
+  } else {
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) T::template issue_stage<0>(d, s, s * BK);
+    wait_vmcnt<(STAGES - 1) * XMIN>();
+  }
+  phase_barrier();
+  if constexpr (SECOND) phase_barrier();
+  const int kt_count = (pd.k + BK - 1) / BK;
+  const bool chain = has_next && kt_count >= STAGES;
+  // The second group holds rows 128 to 255: of a row tile with fewer (the last one of a group of rows) it skips the
+  // fragments and products, and the first group's compute phases follow one another.
+  const bool idle = SECOND && pd.m - m0 <= T::BM / 2;
+  i16x8_t af[KK][FM], bf[KK][FN];
+  // ISSUE: 0 none, 1 this tile's slice kt + 3 (zeros past K), 2 the next tile's once that index passes K.
+  auto step = [&](int kt, auto issue, auto edge) {
+    constexpr int ISSUE = decltype(issue)::value;
+    constexpr bool EDGE = decltype(edge)::value;
+    const char* cur = smem + ((kt + rot) & (STAGES - 1)) * T::STAGE_BYTES;
+    const int buffer = (kt - 1 + rot) & (STAGES - 1), s = kt - 1 + STAGES;
+    if constexpr (ISSUE == 1) {
+      T::template issue_stage<0>(d, buffer, s * BK);
+    } else if constexpr (ISSUE == 2) {
+      if (chain && s >= kt_count) {
+        typename T::Dma dn;
+        T::setup_dma(dn, next, m1, n1, smem);
+        T::template issue_stage<0>(dn, buffer, (s - kt_count) * BK);
+      } else {
+        T::template issue_stage<0>(d, buffer, s * BK);
+      }
+    }
+    if (!idle) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        T::load_frags(af[kk], bf[kk], cur, cur + T::A_BYTES, kk, wave_m, wave_n, pd.swiglu != 0);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    auto wait_next = [&] {  // slice kt + 1 has landed
+      if constexpr (EDGE) {
+        if (!chain || kt + 1 < kt_count) {
+          if (pre && kt < 2) wait_vmcnt<(STAGES - 2) * XMIN + F::STORES>();
+          else wait_vmcnt<(STAGES - 2) * XMIN>();
+        }
+      } else {
+        wait_vmcnt<(STAGES - 2) * XMIN>();
+      }
+    };
+    if constexpr (SECOND) wait_next();
+    phase_barrier();
+    if (!idle) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) T::template mfma_rows<0, FM>(acc, af[kk], bf[kk]);
+    }
+    if constexpr (!SECOND) wait_next();
+    phase_barrier();
+  };
+  using none = std::integral_constant<int, 0>;
+  using own = std::integral_constant<int, 1>;
+  using either = std::integral_constant<int, 2>;
+  step(0, none{}, std::true_type{});
+  int kt = 1;
+  for (; kt < 2 && kt < kt_count; ++kt) step(kt, either{}, std::true_type{});
+  for (; kt + STAGES - 1 < kt_count; ++kt) step(kt, own{}, std::false_type{});
+  for (; kt < kt_count; ++kt) step(kt, either{}, std::true_type{});
+  if (chain) {
+    const int last = (kt_count - 1 + rot) & (STAGES - 1);
+    finish.chained(acc, pd, m0, n0, wave_m, wave_n, last);
+    typename T::Dma dn;
+    T::setup_dma(dn, next, m1, n1, smem);
+    T::template issue_stage<0>(dn, last, (STAGES - 1) * BK);
+    if constexpr (!SECOND) phase_barrier();
+    ch.rot = (kt_count + rot) & (STAGES - 1);
+    ch.prefetched = true;
+  } else {
+    wait_vmcnt<0>();
+    finish.last(acc, pd, m0, n0, wave_m, wave_n);
+    if constexpr (!SECOND) phase_barrier();
+    ch.prefetched = false;
+  }
+}
+
 // The tiles with their element type's name, which TileSums asks for.
 template <class E, int BM, int BN, int BK, int WM, int WN, int S, int LAY>
 struct GatedTile
@@ -162,39 +269,114 @@ struct GatedTile
 
 enum GatedProduct : int { GATED_FORWARD = 0, GATED_DX = 1, GATED_DW = 2 };
 
-// h = silu(g) u and [g | u] of a tile: gate fragments and the up fragments FN / 2 further on, four
-// consecutive columns of one row per lane and register quad.
+// h = silu(g) u and [g | u] of a tile, in a fixed number of buffer stores (out-of-range lanes are dropped): gate
+// fragments and the up fragments FN / 2 further on.  A lane holds four consecutive columns of one row per register quad;
+// 32x32 fragments go through the wave's slots of one stage in LDS, so that stores write 128 (fp32) and 64 bytes of a
+// row at a time instead of 32 (16-byte chunk c of a row at c ^ row).
 template <class T>
-__device__ __forceinline__ void store_gate_up(const typename T::acc_t (&acc)[T::FM][T::FN], const ProblemDesc& pd,
-                                              float* saved, int64_t f, int m0, int n0, int wave_m, int wave_n) {
+struct StoreGateUp {
   using E = typename T::Element;
-  const int lane = threadIdx.x & 63;
-  constexpr int MI = T::MI;
+  static constexpr int FRAGS = T::FM * (T::FN / 2);
+  static constexpr int STORES = T::MI == 32 ? 10 * FRAGS : 3 * FRAGS;
+  float* saved;  // the group's first row
+  int64_t f;
+  char* smem;
+
+  __device__ __forceinline__ void last(const typename T::acc_t (&acc)[T::FM][T::FN], const ProblemDesc& pd, int m0,
+                                       int n0, int wave_m, int wave_n) const {
+    chained(acc, pd, m0, n0, wave_m, wave_n, 0);
+  }
+  __device__ __forceinline__ void chained(const typename T::acc_t (&acc)[T::FM][T::FN], const ProblemDesc& pd, int m0,
+                                          int n0, int wave_m, int wave_n, int stage) const {
+    const int lane = thread_here() & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    constexpr int MI = T::MI;
+    const int rows = min(T::BM, pd.m - m0), cols = (int)f - n0 / 2;
+    const uint32_t pitch = (uint32_t)pd.scm * 2u, pitch32 = (uint32_t)f * 8u;
+    float* keep = saved + (int64_t)m0 * 2 * f + n0 / 2;
+    const auto rh = __builtin_amdgcn_make_buffer_rsrc(pd.c + ((int64_t)m0 * pd.scm + n0 / 2) * 2, (short)0,
+                                                      (int)kOutOfRange, (int)kBufferFlags);
+    const auto rg = __builtin_amdgcn_make_buffer_rsrc(keep, (short)0, (int)kOutOfRange, (int)kBufferFlags);
+    const auto ru = __builtin_amdgcn_make_buffer_rsrc(keep + f, (short)0, (int)kOutOfRange, (int)kBufferFlags);
 #pragma unroll
-  for (int fm = 0; fm < T::FM; ++fm) {
-    const int row = m0 + wave_m * T::WTM + fm * MI + (lane % MI);
-    if (row >= pd.m) continue;
-    char* out = pd.c + (int64_t)row * pd.scm * 2;
-    float* keep = saved + (int64_t)row * 2 * f;
+    for (int fm = 0; fm < T::FM; ++fm)
 #pragma unroll
-    for (int fn = 0; fn < T::FN / 2; ++fn)
+      for (int fn = 0; fn < T::FN / 2; ++fn) {
+        const int row0 = wave_m * T::WTM + fm * MI, n1 = wave_n * (T::WTN / 2) + fn * MI;
+        f32x4_t v[2][T::ACC / 4];
+        u32x2_t h[T::ACC / 4];
 #pragma unroll
-      for (int q = 0; q < T::ACC / 4; ++q) {
-        const int n = n0 / 2 + wave_n * (T::WTN / 2) + fn * MI + (MI == 32 ? q * 8 + (lane >> 5) * 4 : (lane >> 4) * 4);
-        if (n >= f) continue;
-        f32x4_t g, u, h;
+        for (int q = 0; q < T::ACC / 4; ++q) {
+          f32x4_t x;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          g[i] = acc[fm][fn][q * 4 + i];
-          u[i] = acc[fm][fn + T::FN / 2][q * 4 + i];
-          h[i] = gated(g[i], u[i]);
+          for (int i = 0; i < 4; ++i) {
+            v[0][q][i] = acc[fm][fn][q * 4 + i];
+            v[1][q][i] = acc[fm][fn + T::FN / 2][q * 4 + i];
+            x[i] = gated(v[0][q][i], v[1][q][i]);
+          }
+          h[q] = pack4<E>(x);
         }
-        store4<E>(out + (int64_t)n * 2, h);
-        *MOEGEMM_GLOBAL(f32x4_t, keep + n) = g;
-        *MOEGEMM_GLOBAL(f32x4_t, keep + f + n) = u;
+        if constexpr (MI == 16) {
+          const int row = row0 + lane % 16, n = n1 + (lane >> 4) * 4;
+          const bool in = row < rows && n < cols;
+          const uint32_t at = in ? (uint32_t)row * pitch32 + (uint32_t)n * 4u : kOutOfRange;
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v[0][0]), rg, at, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v[1][0]), ru, at, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b64(h[0], rh, in ? (uint32_t)row * pitch + (uint32_t)n * 2u : kOutOfRange, 0, 0);
+        } else {
+          static_assert(MI == 16 || T::XMIN >= 4, "a 32 x 32 fp32 fragment takes four 1 KiB slots");
+          auto slot = [&](int linear) {
+            return smem + T::owned_slot(stage * T::XMIN + (linear >> 10), wave) + (linear & 1023);
+          };
+          const int r = lane & 31;
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<f32x4_t*>(slot(r * 128 + (((q * 2 + (lane >> 5)) ^ (r & 7)) << 4))) = v[part][q];
+            compiler_fence();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int row = j * 8 + (lane >> 3), c = lane & 7;
+              const u32x4_t x = *reinterpret_cast<const u32x4_t*>(slot(row * 128 + ((c ^ (row & 7)) << 4)));
+              const bool in = row0 + row < rows && n1 + c * 4 < cols;
+              __builtin_amdgcn_raw_buffer_store_b128(
+                  x, part ? ru : rg, in ? (uint32_t)(row0 + row) * pitch32 + (uint32_t)(n1 + c * 4) * 4u : kOutOfRange, 0, 0);
+            }
+            compiler_fence();
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<u32x2_t*>(slot(r * 64 + ((q ^ (r & 3)) << 4) + (lane >> 5) * 8)) = h[q];
+          compiler_fence();
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int row = j * 16 + (lane >> 2), c = lane & 3;
+            const u32x4_t x = *reinterpret_cast<const u32x4_t*>(slot(row * 64 + ((c ^ (row & 3)) << 4)));
+            const bool in = row0 + row < rows && n1 + c * 8 < cols;
+            __builtin_amdgcn_raw_buffer_store_b128(
+                x, rh, in ? (uint32_t)(row0 + row) * pitch + (uint32_t)(n1 + c * 8) * 2u : kOutOfRange, 0, 0);
+          }
+          compiler_fence();
+        }
       }
   }
-}
+};
+
+// C of a plain product.
+template <class T>
+struct StorePlain {
+  static constexpr int STORES = T::CHAIN_STORES;
+  char* smem;
+  __device__ __forceinline__ void last(const typename T::acc_t (&acc)[T::FM][T::FN], const ProblemDesc& pd, int m0,
+                                       int n0, int wave_m, int wave_n) const {
+    T::template store_tile<EPI_C>(acc, pd, m0, n0, wave_m, wave_n, smem);
+  }
+  __device__ __forceinline__ void chained(const typename T::acc_t (&acc)[T::FM][T::FN], const ProblemDesc& pd, int m0,
+                                          int n0, int wave_m, int wave_n, int buffer) const {
+    T::staged_store_counted(acc, pd, m0, n0, wave_m, wave_n, smem, buffer);
+  }
+};
 
 // Zeros to rows [first, rows) of a [rows, width] 16-bit matrix (row pitch in elements, width and pitch
 // multiples of 8, 16-byte aligned), every thread of the launch.
@@ -215,12 +397,17 @@ constexpr int kWholeK = 1 << 30;  // no segments
 
 template <class T, int PRODUCT>
 __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
+  __shared__ __attribute__((aligned(16))) char smem[T::PREFIX_OFFSET];
+  __shared__ TileTable table;
+  static_assert(T::PREFIX_OFFSET + sizeof(TileTable) <= 160 * 1024, "LDS of one CU");
   const int grid = gridDim.x;
   int t = (int)blockIdx.x;
   if ((grid & 7) == 0) t = (t & 7) * (grid >> 3) + (t >> 3);  // eight contiguous runs a round, one per XCD
   const int n = PRODUCT == GATED_DX ? p.h : 2 * p.f;
-  const int n_tiles = (n + T::BN - 1) / T::BN;
+  // dW: every expert with rows holds the same number of tiles.
+  constexpr int ROWS_PER_TILE = PRODUCT == GATED_DW ? 1 << 30 : T::BM;
+  const int n_tiles = (n + T::BN - 1) / T::BN, m_tiles = (p.h + T::BM - 1) / T::BM;
+  const int per_row_tile = PRODUCT == GATED_DW ? m_tiles * n_tiles : n_tiles;
   const char* x = static_cast<const char*>(p.x);
   const char* w = static_cast<const char*>(p.w);
   char* out = static_cast<char*>(p.out);
@@ -237,72 +424,96 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
   } else {
     zero_rows(out, p.so, PRODUCT == GATED_DX ? p.h : p.f, rows_end(p), p.rows);
   }
+  build_tile_table(table, p.offs, p.groups, p.rows, ROWS_PER_TILE, per_row_tile);
 
-  auto whole = [](const ProblemDesc& pd, int, int) { return pd; };
-  if constexpr (PRODUCT == GATED_DW) {
-    // Every expert with rows holds the same number of tiles.
-    const int m_tiles = (p.h + T::BM - 1) / T::BM;
+  auto describe = [&](int tile, ProblemDesc& pd, int& m0, int& n0, float*& saved) {
     GroupTile g;
-    for (; find_group_tile(p.offs, p.groups, p.rows, 1 << 30, m_tiles * n_tiles, t, g); t += grid) {
-      int tm, tn;
-      group_m_order(g.local, m_tiles, n_tiles, 8, tm, tn);
-      ProblemDesc pd{};
+    if (!find_tile(table, p.offs, p.groups, p.rows, ROWS_PER_TILE, per_row_tile, tile, g)) return false;
+    int tm, tn;
+    group_m_order(g.local, PRODUCT == GATED_DW ? m_tiles : (g.m + T::BM - 1) / T::BM, n_tiles, 8, tm, tn);
+    pd = ProblemDesc{};
+    pd.splits = 1;
+    pd.scn = 1;
+    pd.scm = p.so;
+    pd.n = n;
+    if constexpr (PRODUCT == GATED_DW) {
       pd.a = x + (int64_t)g.row0 * p.sx * 2;
       pd.b = static_cast<const char*>(p.dp) + (int64_t)g.row0 * p.sdp * 2;
       pd.c = out + (int64_t)g.e * p.sog * 2;
-      pd.m = p.h; pd.n = n; pd.k = g.m;
-      pd.sam = 1; pd.sak = p.sx; pd.sbk = p.sdp; pd.sbn = 1; pd.scm = p.so; pd.scn = 1;
-      pd.splits = 1;
-      const int m0 = tm * T::BM, n0 = tn * T::BN;
-      auto store = [&](const typename T::acc_t (&acc)[T::FM][T::FN], int wave_m, int wave_n) {
-        T::template store_tile<EPI_C>(acc, pd, m0, n0, wave_m, wave_n, smem);
-      };
-      if (p.long_k) {
-        // 2^30 bytes of rows at a time.
-        const int64_t pitch = max(p.sx, p.sdp) * 2;
-        const int segment = (int)(((int64_t)1 << 30) / pitch / T::BK) * T::BK;
-        TileSums<T>::run(pd, m0, n0, segment, smem, [](const ProblemDesc& whole, int k0, int length) {
-          ProblemDesc part = whole;
-          part.a += (int64_t)k0 * whole.sak * 2;
-          part.b += (int64_t)k0 * whole.sbk * 2;
-          part.k = min(length, whole.k - k0);
-          return part;
-        }, store);
-      } else {
-        TileSums<T>::run(pd, m0, n0, kWholeK, smem, whole, store);
-      }
-    }
-  } else {
-    GroupTile g;
-    for (; find_group_tile(p.offs, p.groups, p.rows, T::BM, n_tiles, t, g); t += grid) {
-      int tm, tn;
-      group_m_order(g.local, (g.m + T::BM - 1) / T::BM, n_tiles, 8, tm, tn);
-      ProblemDesc pd{};
+      pd.m = p.h; pd.k = g.m;
+      pd.sam = 1; pd.sak = p.sx; pd.sbk = p.sdp; pd.sbn = 1;
+    } else {
       pd.a = x + (int64_t)g.row0 * p.sx * 2;
       pd.b = w + (int64_t)g.e * p.swg * 2;
       pd.c = out + (int64_t)g.row0 * p.so * 2;
-      pd.m = g.m; pd.n = n;
-      pd.sam = p.sx; pd.sak = 1; pd.scm = p.so; pd.scn = 1;
-      pd.splits = 1;
-      const int m0 = tm * T::BM, n0 = tn * T::BN;
+      pd.m = g.m;
+      pd.sam = p.sx; pd.sak = 1;
       if constexpr (PRODUCT == GATED_FORWARD) {
         pd.k = p.h;
         pd.sbk = p.swh; pd.sbn = 1;
         pd.swiglu = 1;
-        TileSums<T>::run(pd, m0, n0, kWholeK, smem, whole,
-                         [&](const typename T::acc_t (&acc)[T::FM][T::FN], int wave_m, int wave_n) {
-                           store_gate_up<T>(acc, pd, p.saved + (int64_t)g.row0 * 2 * p.f, p.f, m0, n0, wave_m, wave_n);
-                         });
+        saved = p.saved + (int64_t)g.row0 * 2 * p.f;
       } else {
         pd.k = 2 * p.f;
         pd.sbk = 1; pd.sbn = p.swh;
-        TileSums<T>::run(pd, m0, n0, kWholeK, smem, whole,
-                         [&](const typename T::acc_t (&acc)[T::FM][T::FN], int wave_m, int wave_n) {
-                           T::template store_tile<EPI_C>(acc, pd, m0, n0, wave_m, wave_n, smem);
-                         });
       }
     }
+    make_uniform(pd);
+    m0 = uniform(tm) * T::BM;
+    n0 = uniform(tn) * T::BN;
+    return true;
+  };
+  auto finish = [&](float* saved) {
+    if constexpr (PRODUCT == GATED_FORWARD) return StoreGateUp<T>{saved, p.f, smem};
+    else return StorePlain<T>{smem};
+  };
+
+  ProblemDesc pd;
+  int m0 = 0, n0 = 0;
+  float* saved = nullptr;
+  if (!describe(t, pd, m0, n0, saved)) return;
+  constexpr bool PING_PONG = T::BM == 256 && T::BN == 256;
+  if (PING_PONG && !p.long_k) {
+    if constexpr (PING_PONG) {
+      ChainState ch{0, false};
+      bool more = true;
+      while (more) {
+        ProblemDesc next;
+        int m1 = 0, n1 = 0;
+        float* saved_next = nullptr;
+        t += grid;
+        more = describe(t, next, m1, n1, saved_next);
+        if (__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) >= T::NW / 2)
+          chained_tile<T, true>(pd, m0, n0, next, m1, n1, more, smem, ch, finish(saved));
+        else
+          chained_tile<T, false>(pd, m0, n0, next, m1, n1, more, smem, ch, finish(saved));
+        pd = next;
+        m0 = m1;
+        n0 = n1;
+        saved = saved_next;
+      }
+    }
+    return;
   }
+  do {
+    auto store = [&](const typename T::acc_t (&acc)[T::FM][T::FN], int wave_m, int wave_n) {
+      finish(saved).last(acc, pd, m0, n0, wave_m, wave_n);
+    };
+    if (PRODUCT == GATED_DW && p.long_k) {
+      const int64_t pitch = max(p.sx, p.sdp) * 2;
+      const int segment = (int)(((int64_t)1 << 30) / pitch / T::BK) * T::BK;  // 2^30 bytes of rows at a time
+      TileSums<T>::run(pd, m0, n0, segment, smem, [](const ProblemDesc& whole, int k0, int length) {
+        ProblemDesc part = whole;
+        part.a += (int64_t)k0 * whole.sak * 2;
+        part.b += (int64_t)k0 * whole.sbk * 2;
+        part.k = min(length, whole.k - k0);
+        return part;
+      }, store);
+    } else {
+      TileSums<T>::run(pd, m0, n0, kWholeK, smem, [](const ProblemDesc& whole, int, int) { return whole; }, store);
+    }
+    t += grid;
+  } while (describe(t, pd, m0, n0, saved));
 }
 
 // dP = [dg | du] from dh and the saved [g | u], 8 columns of each half a thread; rows past the last group
