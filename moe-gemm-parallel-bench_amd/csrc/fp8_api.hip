@@ -112,18 +112,20 @@ int launch_product(const Fp8Variant* table, int count, Fp8Params& p, int64_t out
   const int64_t n_tiles = cdiv(p.n, v.block_n);  // gated: n = 2F weight rows in tiles of 128 + 128
   const int64_t col_tiles = gated ? cdiv(out_cols, v.block_n / 2) : n_tiles;
   p.n_tiles = (int32_t)col_tiles;
-  int64_t grid;
-  if (v.stream) {
-    if ((int64_t)p.groups * col_tiles > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "unit count exceeds int32");
-    grid = std::min<int64_t>((int64_t)p.groups * col_tiles, cus);
-  } else {
-    const int64_t bound = std::min(p.rows / v.block_m + (int64_t)p.groups, p.groups * cdiv(p.rows, v.block_m)) * col_tiles;
-    if (bound > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
-    grid = std::min<int64_t>(bound, cus);
+  const int64_t bound = (v.stream ? (int64_t)p.groups  // units, or tiles at most
+                                  : std::min(p.rows / v.block_m + (int64_t)p.groups, p.groups * cdiv(p.rows, v.block_m))) *
+                        col_tiles;
+  if (bound > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
+  const int64_t grid = std::min<int64_t>(bound, cus);
+  const int32_t groups = p.groups, most = v.stream ? groups : kTableGroups;
+  for (; p.first < groups; p.first += most) {
+    p.groups = std::min(groups - p.first, most);
+    for (p.round = 0; p.round * grid < bound; p.round += kListTiles) {
+      const hipError_t err = v.launch(p, (int)grid, reinterpret_cast<hipStream_t>(stream));
+      if (err != hipSuccess) return report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+      if (v.stream) break;  // goes on to its last unit
+    }
   }
-  if (grid > INT32_MAX) return report(MOEGEMM_ERR_INVALID, "grid exceeds int32");
-  const hipError_t err = v.launch(p, (int)grid, reinterpret_cast<hipStream_t>(stream));
-  if (err != hipSuccess) return report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
   return MOEGEMM_OK;
 }
 

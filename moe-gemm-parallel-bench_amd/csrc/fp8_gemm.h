@@ -53,6 +53,8 @@ struct Fp8Params {
   int64_t ldo, osm, osk;            // output row pitch in elements, output scale strides
   int32_t groups, rows, n, k;
   int32_t n_tiles;                  // column tiles (the launch's)
+  int32_t first = 0;  // tile kernels: a launch's groups are [first, first + groups), its rounds start at `round`
+  int32_t round = 0;
 };
 
 // Rows of group e: [row0, row0 + m), offsets clamped to [0, rows], a decreasing offset empty.
@@ -68,19 +70,19 @@ __device__ __forceinline__ int group_rows(const int32_t* offs, int rows, int e, 
 }
 
 struct GroupTile {
-  int e, row0, m, local;
+  int e, row0, m, tm, tn;
 };
 
 __device__ __forceinline__ float uniform(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
 }
 
-// threadIdx.x, computed where it is used.  The tile loops' lookups, tails and epilogues depend on the lane and not on
-// the tile: hoisted out of the loop, their offsets took a hundred spilled registers.
-__device__ __forceinline__ int thread_here() {
-  int thread = threadIdx.x;
-  asm volatile("" : "+v"(thread));
-  return thread;
+// The lane, computed where it is used.  The tile loops' lookups, tails and epilogues depend on the lane and not on the
+// tile: hoisted out of the loop, their offsets took a hundred spilled registers.
+__device__ __forceinline__ int lane_here() {
+  uint32_t none = 0;
+  asm volatile("" : "+s"(none));
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
 }
 
 __device__ __forceinline__ int64_t value_of(int64_t x, int lane) {
@@ -89,54 +91,26 @@ __device__ __forceinline__ int64_t value_of(int64_t x, int lane) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-// The group of tile t when each group holds ceil(m / bm) * n_tiles tiles; false past the last one.
-// Each wave looks it up for itself, 64 groups at a time (wave-uniform result).
-__device__ __forceinline__ bool find_group_tile(const int32_t* offs, int groups, int rows, int bm, int n_tiles, int t,
-                                                GroupTile& g) {
-  const int lane = thread_here() & 63;
-  int64_t base = 0;
-  for (int first = 0; first < groups; first += 64) {
-    int m = 0, row0 = 0;
-    if (first + lane < groups) row0 = group_rows(offs, rows, first + lane, m);
-    const int64_t count = (int64_t)((m + bm - 1) / bm) * n_tiles;
-    int64_t sum = count;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t below = value_of(sum, lane - d);
-      if (lane >= d) sum += below;
-    }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > t);
-    if (past) {
-      const int hit = __builtin_ctzll(past);
-      g.e = first + hit;
-      g.row0 = __builtin_amdgcn_readlane(row0, hit);
-      g.m = __builtin_amdgcn_readlane(m, hit);
-      const int before = __builtin_amdgcn_readlane((int)(base + sum - count), hit);  // at most t
-      g.local = t - before;
-      return true;
-    }
-    base = uniform(value_of(base + sum, 63));
-  }
-  return false;
-}
-
-// The same lookup from tables in LDS, for up to kTableGroups groups: find_group_tile loads the offsets into vector
-// registers and so waits for every copy and store in flight, which a loop that prefetches across tiles must not.
+// The tiles of a launch's groups, ceil(m / bm) * n_tiles each, in LDS: a search over the offsets in memory would load them
+// into vector registers and wait for every copy and store in flight, which a loop that prefetches across tiles
+// must not.  A call with more groups is several launches.
 constexpr int kTableGroups = 1024;
 struct TileTable {
   int32_t tiles[kTableGroups];  // cumulative tile counts
   int32_t ends[kTableGroups];   // offsets, clamped
+  int32_t start;                // the first group's first row
 };
 
-// Every thread of the workgroup calls it; ends with a barrier.
-__device__ __forceinline__ void build_tile_table(TileTable& table, const int32_t* offs, int groups, int rows, int bm,
-                                                 int n_tiles) {
+// Groups [first, first + groups).  Every thread of the workgroup calls it; ends with a barrier.
+__device__ __forceinline__ void build_tile_table(TileTable& table, const int32_t* offs, int first, int groups, int rows,
+                                                 int bm, int n_tiles) {
   const int lane = threadIdx.x & 63;
-  if (threadIdx.x < 64 && groups <= kTableGroups) {
+  if (threadIdx.x < 64) {
     int64_t base = 0;
-    for (int first = 0; first < groups; first += 64) {
-      int m = 0;
-      if (first + lane < groups) group_rows(offs, rows, first + lane, m);
+    for (int chunk = 0; chunk < groups; chunk += 64) {
+      const int i = chunk + lane;
+      int m = 0, row0 = 0;
+      if (i < groups) row0 = group_rows(offs, rows, first + i, m);
       int64_t sum = (int64_t)((m + bm - 1) / bm) * n_tiles;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
@@ -144,41 +118,63 @@ __device__ __forceinline__ void build_tile_table(TileTable& table, const int32_t
         if (lane >= d) sum += below;
       }
       sum = min(base + sum, (int64_t)INT32_MAX);  // overlapping groups of decreasing offsets
-      if (first + lane < groups) {
-        table.tiles[first + lane] = (int32_t)sum;
-        table.ends[first + lane] = offs ? min(max(offs[first + lane], 0), rows) : rows;
+      if (i < groups) {
+        table.tiles[i] = (int32_t)sum;
+        table.ends[i] = offs ? min(max(offs[first + i], 0), rows) : rows;
       }
+      if (i == 0) table.start = row0;
       base = uniform(value_of(sum, 63));
     }
   }
   __syncthreads();
 }
 
-__device__ __forceinline__ bool find_tile(const TileTable& table, const int32_t* offs, int groups, int rows, int bm,
-                                          int n_tiles, int t, GroupTile& g) {
-  if (groups > kTableGroups) return find_group_tile(offs, groups, rows, bm, n_tiles, t, g);
-  const int lane = thread_here() & 63;
-  int before = 0, row0 = 0;
-  for (int first = 0; first < groups; first += 64) {
-    const int at = min(first + lane, groups - 1);
-    const int tiles = table.tiles[at], end = table.ends[at];
-    const uint64_t past = __builtin_amdgcn_ballot_w64(tiles > t);
-    if (past) {
-      const int hit = __builtin_ctzll(past);
-      if (hit > 0) {
-        before = __builtin_amdgcn_readlane(tiles, hit - 1);
-        row0 = __builtin_amdgcn_readlane(end, hit - 1);
+// The tiles of a workgroup, one a round of the grid, up to kListTiles of them a launch: looked up by one thread each
+// before their loop starts.  The search and its divisions inside the loop cost a microsecond a tile, and their registers
+// spilled those of the 256 x 256 tiles.
+//
+// Each round is eight contiguous runs, one per XCD (workgroup b runs on XCD b mod 8), so that an XCD's L2 holds the rows
+// and weights its tiles share; the last round's tiles are dealt to all XCDs alike.  A grid that eight does not divide
+// takes every grid-th tile.
+constexpr int kListTiles = 256;
+struct TileList {
+  GroupTile tile[kListTiles];  // e < 0: none
+};
+
+// Rounds from `round` on.  `order(tile, local)` places the group's local-th tile.  Every thread of the workgroup calls
+// it; ends with a barrier.
+template <class Order>
+__device__ __forceinline__ void build_tile_list(TileList& list, const TileTable& table, int first, int groups, int round,
+                                                Order&& order) {
+  if (threadIdx.x < kListTiles) {  // workgroups have as many threads or more
+    const uint32_t grid = gridDim.x, b = blockIdx.x;
+    const int64_t base = ((int64_t)round + threadIdx.x) * grid, left = table.tiles[groups - 1] - base;
+    const uint32_t count = (uint32_t)min((int64_t)grid, left), shift = grid & 7 ? 0 : 3, xcd = b & ((1u << shift) - 1);
+    const uint32_t at = (xcd * count >> shift) + (b >> shift);
+    GroupTile tile{-1, 0, 0, 0, 0};
+    if (left > 0 && at < ((xcd + 1) * count >> shift)) {
+      const int t = (int)base + (int)at;
+      int lo = 0, hi = groups - 1;  // the first group with tiles[i] > t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (table.tiles[mid] > t) hi = mid;
+        else lo = mid + 1;
       }
-      g.e = first + hit;
-      g.local = t - before;
-      g.row0 = row0;
-      g.m = __builtin_amdgcn_readlane(end, hit) - row0;  // a group with tiles has rows
-      return true;
+      const int row0 = lo ? table.ends[lo - 1] : table.start;
+      tile = GroupTile{first + lo, row0, table.ends[lo] - row0, 0, 0};  // a group with tiles has rows
+      order(tile, t - (lo ? table.tiles[lo - 1] : 0));
     }
-    before = __builtin_amdgcn_readlane(tiles, 63);
-    row0 = __builtin_amdgcn_readlane(end, 63);
+    list.tile[threadIdx.x] = tile;
   }
-  return false;
+  __syncthreads();
+}
+
+// The i-th tile of the list, wave-uniform; false past its end.
+__device__ __forceinline__ bool listed_tile(const TileList& list, int i, GroupTile& g) {
+  if (i >= kListTiles) return false;
+  const GroupTile& x = list.tile[i];
+  g = {uniform(x.e), uniform(x.row0), uniform(x.m), uniform(x.tm), uniform(x.tn)};
+  return g.e >= 0;
 }
 
 __device__ __forceinline__ f32x16_t mfma_fp8(i32x8_t w, i32x8_t a, f32x16_t c) {
@@ -292,7 +288,7 @@ struct Fp8Tile {
   static constexpr int PER_STAGE = QA + QB + QS;  // copies of a wave per stage
   static constexpr int RED_BYTES = GATED ? BM * WN * 4 : 0;  // row maxima of the waves that share a row
   static constexpr int TABLE_OFFSET = STAGES * STAGE_BYTES + RED_BYTES;
-  static constexpr int LDS_BYTES = TABLE_OFFSET + (int)sizeof(TileTable);
+  static constexpr int LDS_BYTES = TABLE_OFFSET + (int)(sizeof(TileTable) + sizeof(TileList));
   static constexpr int OUT_COLS = GATED ? BN / 2 : BN;  // output columns of a tile
   static_assert(IA % NW == 0 && IB % NW == 0, "every wave issues the same copies");
   static_assert(!GATED || (BN == 256 && FN == 2), "a gated tile is one 128-column block of the output");
@@ -320,15 +316,20 @@ struct Fp8Tile {
     // Row r of a panel keeps chunk c at c ^ swz_a(r, 8); wave w copies rows 8 (w + q NW) .. + 7.
     const int r0 = wave * 8 + lane / 8;
     const int ch = (lane & 7) ^ swz_a(r0, 8);  // swz_a of 8 chunks repeats every 32 rows, and NW * 8 is 32 or 64
-    c.a_off = (uint32_t)r0 * (uint32_t)p.lda + (uint32_t)ch * 16u;
-    c.b_off = (uint32_t)r0 * (uint32_t)p.ldw + (uint32_t)ch * 16u;
+    // The products stand apart from the sums: a 64-bit multiply-add would hold four registers over the loop.
+    c.a_off = (uint32_t)r0 * (uint32_t)p.lda;
+    c.b_off = (uint32_t)r0 * (uint32_t)p.ldw;
+    asm volatile("" : "+v"(c.a_off), "+v"(c.b_off));
+    c.a_off += (uint32_t)ch * 16u;
+    c.b_off += (uint32_t)ch * 16u;
+    asm volatile("" : "+v"(c.a_off), "+v"(c.b_off));
     c.a_step = (uint32_t)p.lda * (NW * 8);
     c.b_step = (uint32_t)p.ldw * (NW * 8);
   }
 
-  __device__ static __forceinline__ void set_tile(Copies& c, const Fp8Params& p, const GroupTile& g, int tm, int tn) {
-    const int lane = thread_here() & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  __device__ static __forceinline__ void set_tile(Copies& c, const Fp8Params& p, const GroupTile& g, int wave) {
+    const int tm = g.tm, tn = g.tn;
+    const int lane = lane_here();
     const int m0 = tm * BM;
     const int valid_m = min(BM, g.m - m0);
     // A panel ends with the chunk that holds its last row's last k; what a copy reads past K inside it
@@ -371,7 +372,8 @@ struct Fp8Tile {
   template <int PART0, int PART1>
   __device__ static __forceinline__ void issue(const Copies& c, int stage, int kt) {
     const uint32_t base = c.lds + (uint32_t)(stage * STAGE_BYTES);
-    const uint32_t k0 = (uint32_t)kt * kScaleBlock;
+    uint32_t k0 = (uint32_t)kt * kScaleBlock;
+    asm volatile("" : "+s"(k0));  // no running sums of it and the offsets in vector registers
     uint32_t a0 = c.a_off + k0, b0 = c.b_off + k0;
     // The steps are added here: hoisted out of the loop, the offsets of eight copies took spilled registers.
     asm volatile("" : "+v"(a0), "+v"(b0));
@@ -420,8 +422,8 @@ struct Fp8Tile {
 
   // Zeros to the bytes of a landed slice from `left` (< 128, any sign) on: a K that is no multiple of 128
   // ends inside it.  A thread per panel row.
-  __device__ static __forceinline__ void cut_tail(char* stage, int left) {
-    for (int r = thread_here(); r < BM + BN; r += NT) {
+  __device__ static __forceinline__ void cut_tail(char* stage, int left, int wave) {
+    for (int r = wave * 64 + lane_here(); r < BM + BN; r += NT) {
       // Panel rows of A, then of B, are 128 bytes each; swz_a repeats every 32 rows and BM is a multiple of it.
       for (int c = max(left, 0) >> 4; c < 8; ++c) {
         i32x4_t* chunk = reinterpret_cast<i32x4_t*>(stage + r * kScaleBlock + ((c ^ swz_a(r, 8)) << 4));
@@ -441,13 +443,13 @@ struct Fp8Tile {
     float sa[2];
     float sw[GATED ? 5 : 1];  // wave-uniform; gated: of each eight up rows of the wave's 32, then the gate's
   };
-  // `a`: the chunks of the wave's first row group of the slice; `stage` its LDS offset.
-  __device__ static __forceinline__ void load_a(Slice& s, const char* smem, const Chunks& a, uint32_t stage, int wave_m,
-                                                int fm) {
+  // `a`: the chunks of the wave's first row group of the slice; `lane` lane_offset(); `stage` the slice's LDS offset.
+  __device__ static __forceinline__ void load_a(Slice& s, const char* smem, const Chunks& a, uint32_t lane, uint32_t stage,
+                                                int wave_m, int fm) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) s.a[fm & 1][j].set(frag(smem, a, fm, j));
     s.sa[fm & 1] = *reinterpret_cast<const float*>(smem + stage + A_BYTES + B_BYTES + (wave_m * WTM + fm * 32) * 4 +
-                                                   (threadIdx.x & 31) * 4);
+                                                   ((lane / (kScaleBlock / 4)) & 124));  // 4 (lane's row)
   }
   __device__ static __forceinline__ void load_b(Slice& s, const char* smem, const Chunks& b, int fn) {
     constexpr int UP = GATED ? (BN / 2 - WTN / 2) / 32 : 0;  // row groups from a wave's gate rows' end to its up rows
@@ -491,13 +493,14 @@ struct Fp8Tile {
   // The last sum of a slice is added in the next one.  `copies(part)` issues a part of a slice's copies.
   template <int X0, int X1, class Issue>
   __device__ static __forceinline__ void steps(f32x16_t (&acc)[FM][FN], Slice& s, Pending (&pend)[2], const char* smem,
-                                               const Chunks& a, uint32_t stage, Issue&& copies, int wave_m) {
+                                               const Chunks& a, uint32_t lane, uint32_t stage, Issue&& copies,
+                                               int wave_m) {
     unroll_steps<X0, X1>([&](auto step) {
       constexpr int x = decltype(step)::value;
       constexpr int fm = x / FN, fn = x % FN, last = x == 0 ? FM * FN - 1 : x - 1;
       constexpr int part = x >= BEFORE ? x - BEFORE : x < EARLY ? FN + x : -1;
       if constexpr (part >= 0) copies(std::integral_constant<int, part>{});
-      if (fn == 0 && fm + 1 < FM) load_a(s, smem, a, stage, wave_m, fm + 1);
+      if (fn == 0 && fm + 1 < FM) load_a(s, smem, a, lane, stage, wave_m, fm + 1);
       Pending& p = pend[x & 1];
       p.t = f32x16_t{};
 #pragma unroll
@@ -533,7 +536,7 @@ struct Fp8Tile {
 
   __device__ static __forceinline__ void store_plain(const f32x16_t (&acc)[FM][FN], const Fp8Params& p,
                                                      const GroupTile& g, int tm, int tn, int wave_m, int wave_n) {
-    const int lane = thread_here() & 63;
+    const int lane = lane_here();
     constexpr int ES = sizeof(typename E::raw);
     const int m0 = tm * BM, n0 = tn * BN;
     char* base = static_cast<char*>(p.out) + (((int64_t)g.row0 + m0) * p.ldo + n0) * ES;
@@ -593,7 +596,7 @@ struct Fp8Tile {
   // it (through `red`), and the quantised row.
   __device__ static __forceinline__ void store_gated(f32x16_t (&acc)[FM][FN], const Fp8Params& p, const GroupTile& g,
                                                      int tm, int tn, int wave_m, int wave_n, uint32_t* red) {
-    const int lane = thread_here() & 63;
+    const int lane = lane_here();
     const int f = p.n >> 1;
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
@@ -652,30 +655,27 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wave_m = wave / T::WN, wave_n = wave % T::WN;
-  const int grid = gridDim.x;
-  // Each round of `grid` tiles is split into eight contiguous runs, one per XCD (workgroup b runs on
-  // XCD b % 8), so that the tiles that share an expert's panels read them through one L2.
-  int t = (int)blockIdx.x;
-  if ((grid & 7) == 0) t = (t & 7) * (grid >> 3) + (t >> 3);
   const int blocks = (p.k + kScaleBlock - 1) / kScaleBlock;
   const int kt_count = max(blocks, 2);
   const bool cut = p.k % kScaleBlock != 0;  // slices from K / 128 on are cut in LDS
   TileTable& table = *reinterpret_cast<TileTable*>(smem + T::TABLE_OFFSET);
-  build_tile_table(table, p.offs, p.groups, p.rows, T::BM, p.n_tiles);
+  TileList& list = *reinterpret_cast<TileList*>(smem + T::TABLE_OFFSET + sizeof(TileTable));
+  build_tile_table(table, p.offs, p.first, p.groups, p.rows, T::BM, p.n_tiles);
+  build_tile_list(list, table, p.first, p.groups, p.round, [&](GroupTile& tile, int local) {
+    group_m_order(local, (tile.m + T::BM - 1) / T::BM, p.n_tiles, 8, tile.tm, tile.tn);
+  });
   GroupTile g;
-  if (!find_tile(table, p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g)) return;
-  int tm, tn;
-  group_m_order(g.local, (g.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm, tn);
+  if (!listed_tile(list, 0, g)) return;
   typename T::Copies c;
   T::start(c, p, smem);
-  T::set_tile(c, p, g, tm, tn);
+  T::set_tile(c, p, g, wave);
   T::template issue<0, T::PARTS>(c, 0, 0);
   T::template issue<0, T::FN>(c, 1, 1);  // the rest of it under slice 0's first steps
   wait_vmcnt<T::first_copy(T::FN)>();
   __builtin_amdgcn_s_barrier();
   compiler_fence();
   if (cut && blocks == 1) {
-    T::cut_tail(smem, p.k);
+    T::cut_tail(smem, p.k, wave);
     __syncthreads();
   }
   const uint32_t lane = T::lane_offset();
@@ -684,22 +684,16 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
   auto load_first = [&](uint32_t stage) {
     T::load_weight_scales(s, smem, stage, wave_n);
     ca = T::chunks(lane, stage + (uint32_t)(wave_m * T::WTM * kScaleBlock));
-    T::load_a(s, smem, ca, stage, wave_m, 0);
+    T::load_a(s, smem, ca, lane, stage, wave_m, 0);
     const typename T::Chunks cb = T::chunks(lane, stage + (uint32_t)(T::A_BYTES + T::b_row(wave_n) * kScaleBlock));
 #pragma unroll
     for (int fn = 0; fn < T::FN; ++fn) T::load_b(s, smem, cb, fn);
   };
   load_first(0);
 
-  int buffer = 0;
+  int buffer = 0, i = 0;
   bool more = true;
   while (more) {
-    // The next tile is looked up before this one's sums take the registers.
-    GroupTile g_next{};
-    int tm_next = 0, tn_next = 0;
-    t += grid;
-    more = find_tile(table, p.offs, p.groups, p.rows, T::BM, p.n_tiles, t, g_next);
-    if (more) group_m_order(g_next.local, (g_next.m + T::BM - 1) / T::BM, p.n_tiles, 8, tm_next, tn_next);
     f32x16_t acc[T::FM][T::FN];
 #pragma unroll
     for (int fm = 0; fm < T::FM; ++fm)
@@ -710,17 +704,17 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
     // the first of slice i + 2's into this one; `left()` says how many bytes of the next slice's rows lie inside K.
     auto slice = [&](auto&& early, auto&& late, auto&& left) {
       const uint32_t cur = (uint32_t)(buffer * T::STAGE_BYTES), next = (uint32_t)((buffer ^ 1) * T::STAGE_BYTES);
-      T::template steps<0, T::BEFORE>(acc, s, pend, smem, ca, cur, early, wave_m);
+      T::template steps<0, T::BEFORE>(acc, s, pend, smem, ca, lane, cur, early, wave_m);
       // Every fragment of this slice is in registers, and the next slice has landed.
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       compiler_fence();
       if (const int bytes = left(); bytes < kScaleBlock) {
-        T::cut_tail(smem + next, bytes);
+        T::cut_tail(smem + next, bytes, wave);
         __syncthreads();
       }
       // Fragments of the next slice (of the next tile, behind the last one) as this one's fall free.
-      T::template steps<T::BEFORE, T::FM * T::FN>(acc, s, pend, smem, ca, cur, late, wave_m);
+      T::template steps<T::BEFORE, T::FM * T::FN>(acc, s, pend, smem, ca, lane, cur, late, wave_m);
       load_first(next);
       buffer ^= 1;
     };
@@ -732,22 +726,22 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
       slice([&](auto part) { issue(part, buffer ^ 1, kt + 1); }, [&](auto part) { issue(part, buffer, kt + 2); },
             [] { return kScaleBlock; });
     // The last two slices refill with the next tile's first two.
+    GroupTile g_next{};
+    more = listed_tile(list, ++i, g_next);
     for (int ahead = 0; ahead < 2; ++ahead)
       slice([&](auto part) { if (ahead == 0 || more) issue(part, buffer ^ 1, ahead == 0 ? kt_count - 1 : 0); },
             [&](auto part) { if (more) issue(part, buffer, ahead); },
             [&] {
-              if (ahead == 0 && more) T::set_tile(c, p, g_next, tm_next, tn_next);
+              if (ahead == 0 && more) T::set_tile(c, p, g_next, wave);
               return p.k - (ahead == 0 ? kt_count - 1 : 0) * kScaleBlock;
             });
     T::add(acc[T::FM - 1][T::FN - 1], pend[(T::FM * T::FN - 1) & 1], T::FN - 1);
     if constexpr (T::GATED)
-      T::store_gated(acc, p, g, tm, tn, wave_m, wave_n,
+      T::store_gated(acc, p, g, g.tm, g.tn, wave_m, wave_n,
                      reinterpret_cast<uint32_t*>(smem + T::STAGES * T::STAGE_BYTES));
     else
-      T::store_plain(acc, p, g, tm, tn, wave_m, wave_n);
+      T::store_plain(acc, p, g, g.tm, g.tn, wave_m, wave_n);
     g = g_next;
-    tm = tm_next;
-    tn = tn_next;
   }
 }
 

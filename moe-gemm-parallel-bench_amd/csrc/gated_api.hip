@@ -38,16 +38,32 @@ int check_operand(const char* name, const void* base, int64_t pitch, int64_t wid
   return MOEGEMM_OK;
 }
 
-// The largest tile that about three quarters of the CUs get one of and that `rows` rows of a group fill
-// more than half; the last one otherwise.
-const GatedVariant* choose(const GatedVariant* list, int64_t row_tiles_of, int64_t groups, int64_t cols, int cus) {
-  const GatedVariant* v = list;
-  for (; v[1].launch; ++v) {
-    const int64_t tiles = groups * cdiv(row_tiles_of, v->block_m) * cdiv(cols, v->block_n);
-    if (2 * row_tiles_of > v->block_m && 4 * tiles >= 3 * cus) break;
-    if (v[2].launch == nullptr && row_tiles_of > 2 * v[1].block_m) break;  // few tiles, but long rows
+// Row tiles of forward and dX: exact for one group, else about half a tile a group more than the rows fill.
+int64_t row_tiles(const GatedVariant& v, int64_t rows, int64_t groups) {
+  const int64_t active = std::min(groups, rows);
+  return active == 1 ? cdiv(rows, v.block_m) : std::max(active, rows / v.block_m + active / 2);
+}
+
+// The variant of the least estimated time: rounds of tiles over the CUs, but no less than reading the weights
+// (dW: writing their gradients) takes.  The rounds decide more than a tile's rate does.  16 experts, 4001 rows, 2880 ->
+// 2x2880: dX 282 us in two rounds of 256x256 tiles, 187 in two of 128x256; forward 231 against 206.  32 experts, 16384
+// rows, 7168 -> 2x2048: forward 977 against 1086.  64 experts of 32 rows, 2048 -> 2x768, bound by the weights: forward
+// 102, 92 (128x256), 95, 121 (16x128).  One row, 4096 -> 2x4096: 70, 52, 28, 25.
+const GatedVariant* choose(const GatedVariant* list, int product, const GatedParams& p, int64_t cols, int cus) {
+  const int64_t k = product == GATED_FORWARD ? p.h : product == GATED_DX ? 2 * (int64_t)p.f : cdiv(p.rows, p.groups);
+  const double weights = 4.0 * std::min(p.groups, p.rows) * p.h * p.f;  // bytes
+  const GatedVariant* best = nullptr;
+  double least = 0;
+  for (const GatedVariant* v = list; v->launch; ++v) {
+    const int64_t rows = product == GATED_DW ? p.groups * cdiv(p.h, v->block_m) : row_tiles(*v, p.rows, p.groups);
+    const int64_t rounds = cdiv(rows * cdiv(cols, v->block_n), (int64_t)cus * v->per_cu);
+    const double ns = std::max(rounds * (k * v->slice_ps * 1e-3 + v->tile_ns), weights / v->gbps);
+    if (!best || ns < least) {
+      best = v;
+      least = ns;
+    }
   }
-  return v;
+  return best;
 }
 
 const GatedTable& table_of(int32_t dtype) { return dtype == DT_BF16 ? kGatedBf16 : kGatedF16; }
@@ -56,10 +72,9 @@ int launch_product(const GatedParams& p, int product, int32_t dtype, int32_t var
   const GatedVariant* list = table_of(dtype).products[product];
   const int cus = grid_size > 0 ? grid_size : 256;
   const int64_t cols = product == GATED_DX ? p.h : 2 * (int64_t)p.f;
-  const int64_t extent = product == GATED_DW ? p.h : cdiv(p.rows, p.groups);
   const GatedVariant* v = nullptr;
   if (variant < 0) {
-    v = choose(list, extent, p.groups, cols, cus);
+    v = choose(list, product, p, cols, cus);
   } else {
     for (int i = 0; list[i].launch; ++i)
       if (i == variant) v = &list[i];
@@ -70,9 +85,16 @@ int launch_product(const GatedParams& p, int product, int32_t dtype, int32_t var
                                 : std::min(p.rows / v->block_m + (int64_t)p.groups, p.groups * cdiv(p.rows, v->block_m));
   const int64_t bound = row_tiles * cdiv(cols, v->block_n);
   if (bound > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
-  const hipError_t err = v->launch(p, (int)std::min<int64_t>(std::max<int64_t>(bound, 1), cus),
-                                   reinterpret_cast<hipStream_t>(stream));
-  if (err != hipSuccess) return report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>(bound, 1), (int64_t)cus * v->per_cu);
+  GatedParams part = p;
+  for (; part.first < p.groups; part.first += kTableGroups) {
+    part.groups = std::min(p.groups - part.first, kTableGroups);
+    for (part.round = 0; (int64_t)part.round * grid < std::max<int64_t>(bound, 1); part.round += kListTiles) {
+      part.closes = part.first + part.groups == p.groups && part.round == 0;
+      const hipError_t err = v->launch(part, grid, reinterpret_cast<hipStream_t>(stream));
+      if (err != hipSuccess) return report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+    }
+  }
   return MOEGEMM_OK;
 }
 

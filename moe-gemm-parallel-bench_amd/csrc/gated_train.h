@@ -29,8 +29,11 @@ struct GatedParams {
   const void* dp;     // dW: dP [rows, 2 f]
   const int32_t* offs;
   int64_t sx, swg, swh, so, sog, sdp;  // element strides; so: row pitch of out, sog: dW's group stride
-  int32_t groups, rows, h, f;
+  int32_t groups, rows, h, f;  // groups: of this launch, [first, first + groups) of the call's
   int32_t long_k;     // dW: an expert's rows may span 2 GiB: K runs in segments
+  int32_t first = 0;
+  int32_t round = 0;   // the launch's first round of tiles
+  int32_t closes = 1;  // the launch that clears what no tile writes past the last group
 };
 
 // Sums of one tile, as the tiles' run_tile forms them (FastTile::run_tile, PingPongTile::group_tile), with
@@ -265,6 +268,7 @@ template <class E, int BM, int BN, int BK, int WM, int WN, int S, int LAY>
 struct GatedTile
     : std::conditional<BM == 256 && BN == 256, PingPongTile<E, BK, S, LAY>, FastTile<E, BM, BN, BK, WM, WN, S, LAY>>::type {
   using Element = E;
+  static constexpr int PER_CU = 2 * (GatedTile::PREFIX_OFFSET + (int)(sizeof(TileTable) + sizeof(TileList))) <= 160 * 1024 ? 2 : 1;
 };
 
 enum GatedProduct : int { GATED_FORWARD = 0, GATED_DX = 1, GATED_DW = 2 };
@@ -288,7 +292,7 @@ struct StoreGateUp {
   }
   __device__ __forceinline__ void chained(const typename T::acc_t (&acc)[T::FM][T::FN], const ProblemDesc& pd, int m0,
                                           int n0, int wave_m, int wave_n, int stage) const {
-    const int lane = thread_here() & 63;
+    const int lane = lane_here();
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     constexpr int MI = T::MI;
     const int rows = min(T::BM, pd.m - m0), cols = (int)f - n0 / 2;
@@ -390,7 +394,7 @@ __device__ __forceinline__ void zero_rows(void* base, int64_t pitch, int width, 
 
 // First row past the last group, in [0, rows].
 __device__ __forceinline__ int rows_end(const GatedParams& p) {
-  return p.offs ? min(max(p.offs[p.groups - 1], 0), p.rows) : p.rows;
+  return p.offs ? min(max(p.offs[p.first + p.groups - 1], 0), p.rows) : p.rows;
 }
 
 constexpr int kWholeK = 1 << 30;  // no segments
@@ -399,10 +403,8 @@ template <class T, int PRODUCT>
 __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
   __shared__ __attribute__((aligned(16))) char smem[T::PREFIX_OFFSET];
   __shared__ TileTable table;
-  static_assert(T::PREFIX_OFFSET + sizeof(TileTable) <= 160 * 1024, "LDS of one CU");
-  const int grid = gridDim.x;
-  int t = (int)blockIdx.x;
-  if ((grid & 7) == 0) t = (t & 7) * (grid >> 3) + (t >> 3);  // eight contiguous runs a round, one per XCD
+  __shared__ TileList list;
+  static_assert(T::PREFIX_OFFSET + sizeof(TileTable) + sizeof(TileList) <= 160 * 1024, "LDS of one CU");
   const int n = PRODUCT == GATED_DX ? p.h : 2 * p.f;
   // dW: every expert with rows holds the same number of tiles.
   constexpr int ROWS_PER_TILE = PRODUCT == GATED_DW ? 1 << 30 : T::BM;
@@ -414,23 +416,21 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
 
   // What no tile writes: rows past the last group, gradients of experts without rows.
   if constexpr (PRODUCT == GATED_DW) {
-    for (int first = 0; first < p.groups; first += 64) {
+    for (int first = 0; p.round == 0 && first < p.groups; first += 64) {
       const int e = first + (int)(threadIdx.x & 63);
       int m = 1;
-      if (e < p.groups) group_rows(p.offs, p.rows, e, m);
+      if (e < p.groups) group_rows(p.offs, p.rows, p.first + e, m);
       for (uint64_t empty = __builtin_amdgcn_ballot_w64(m == 0); empty; empty &= empty - 1)
-        zero_rows(out + (int64_t)(first + __builtin_ctzll(empty)) * p.sog * 2, p.so, n, 0, p.h);
+        zero_rows(out + (int64_t)(p.first + first + __builtin_ctzll(empty)) * p.sog * 2, p.so, n, 0, p.h);
     }
-  } else {
+  } else if (p.closes) {
     zero_rows(out, p.so, PRODUCT == GATED_DX ? p.h : p.f, rows_end(p), p.rows);
   }
-  build_tile_table(table, p.offs, p.groups, p.rows, ROWS_PER_TILE, per_row_tile);
+  build_tile_table(table, p.offs, p.first, p.groups, p.rows, ROWS_PER_TILE, per_row_tile);
 
-  auto describe = [&](int tile, ProblemDesc& pd, int& m0, int& n0, float*& saved) {
+  auto describe = [&](int i, ProblemDesc& pd, int& m0, int& n0, float*& saved) {  // the list's i-th tile
     GroupTile g;
-    if (!find_tile(table, p.offs, p.groups, p.rows, ROWS_PER_TILE, per_row_tile, tile, g)) return false;
-    int tm, tn;
-    group_m_order(g.local, PRODUCT == GATED_DW ? m_tiles : (g.m + T::BM - 1) / T::BM, n_tiles, 8, tm, tn);
+    if (!listed_tile(list, i, g)) return false;
     pd = ProblemDesc{};
     pd.splits = 1;
     pd.scn = 1;
@@ -459,30 +459,32 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
       }
     }
     make_uniform(pd);
-    m0 = uniform(tm) * T::BM;
-    n0 = uniform(tn) * T::BN;
+    m0 = g.tm * T::BM;
+    n0 = g.tn * T::BN;
     return true;
   };
+  constexpr bool PING_PONG = T::BM == 256 && T::BN == 256;
   auto finish = [&](float* saved) {
     if constexpr (PRODUCT == GATED_FORWARD) return StoreGateUp<T>{saved, p.f, smem};
     else return StorePlain<T>{smem};
   };
 
+  build_tile_list(list, table, p.first, p.groups, p.round, [&](GroupTile& tile, int local) {
+    group_m_order(local, PRODUCT == GATED_DW ? m_tiles : (tile.m + T::BM - 1) / T::BM, n_tiles, 8, tile.tm, tile.tn);
+  });
   ProblemDesc pd;
-  int m0 = 0, n0 = 0;
+  int m0 = 0, n0 = 0, i = 0;
   float* saved = nullptr;
-  if (!describe(t, pd, m0, n0, saved)) return;
-  constexpr bool PING_PONG = T::BM == 256 && T::BN == 256;
+  bool more = describe(0, pd, m0, n0, saved);
+  if (!more) return;
   if (PING_PONG && !p.long_k) {
     if constexpr (PING_PONG) {
       ChainState ch{0, false};
-      bool more = true;
       while (more) {
         ProblemDesc next;
         int m1 = 0, n1 = 0;
         float* saved_next = nullptr;
-        t += grid;
-        more = describe(t, next, m1, n1, saved_next);
+        more = describe(++i, next, m1, n1, saved_next);
         if (__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) >= T::NW / 2)
           chained_tile<T, true>(pd, m0, n0, next, m1, n1, more, smem, ch, finish(saved));
         else
@@ -493,27 +495,26 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
         saved = saved_next;
       }
     }
-    return;
+  } else {
+    do {
+      auto store = [&](const typename T::acc_t (&acc)[T::FM][T::FN], int wave_m, int wave_n) {
+        finish(saved).last(acc, pd, m0, n0, wave_m, wave_n);
+      };
+      if (PRODUCT == GATED_DW && p.long_k) {
+        const int64_t pitch = max(p.sx, p.sdp) * 2;
+        const int segment = (int)(((int64_t)1 << 30) / pitch / T::BK) * T::BK;  // 2^30 bytes of rows at a time
+        TileSums<T>::run(pd, m0, n0, segment, smem, [](const ProblemDesc& whole, int k0, int length) {
+          ProblemDesc part = whole;
+          part.a += (int64_t)k0 * whole.sak * 2;
+          part.b += (int64_t)k0 * whole.sbk * 2;
+          part.k = min(length, whole.k - k0);
+          return part;
+        }, store);
+      } else {
+        TileSums<T>::run(pd, m0, n0, kWholeK, smem, [](const ProblemDesc& whole, int, int) { return whole; }, store);
+      }
+    } while (describe(++i, pd, m0, n0, saved));
   }
-  do {
-    auto store = [&](const typename T::acc_t (&acc)[T::FM][T::FN], int wave_m, int wave_n) {
-      finish(saved).last(acc, pd, m0, n0, wave_m, wave_n);
-    };
-    if (PRODUCT == GATED_DW && p.long_k) {
-      const int64_t pitch = max(p.sx, p.sdp) * 2;
-      const int segment = (int)(((int64_t)1 << 30) / pitch / T::BK) * T::BK;  // 2^30 bytes of rows at a time
-      TileSums<T>::run(pd, m0, n0, segment, smem, [](const ProblemDesc& whole, int k0, int length) {
-        ProblemDesc part = whole;
-        part.a += (int64_t)k0 * whole.sak * 2;
-        part.b += (int64_t)k0 * whole.sbk * 2;
-        part.k = min(length, whole.k - k0);
-        return part;
-      }, store);
-    } else {
-      TileSums<T>::run(pd, m0, n0, kWholeK, smem, [](const ProblemDesc& whole, int, int) { return whole; }, store);
-    }
-    t += grid;
-  } while (describe(t, pd, m0, n0, saved));
 }
 
 // dP = [dg | du] from dh and the saved [g | u], 8 columns of each half a thread; rows past the last group
@@ -557,7 +558,8 @@ __global__ void __launch_bounds__(256) gate_up_gradient_kernel(GatedParams p, co
 
 typedef hipError_t (*GatedLaunchFn)(const GatedParams&, int grid, hipStream_t stream);
 struct GatedVariant {
-  int block_m, block_n;
+  int block_m, block_n, per_cu;  // per_cu: workgroups a CU holds (LDS and registers)
+  int slice_ps, tile_ns, gbps;
   GatedLaunchFn launch;
 };
 template <class T, int PRODUCT>
@@ -571,20 +573,28 @@ hipError_t launch_gradient(const GatedParams& p, const void* dh, int64_t sdh, vo
   return hipGetLastError();
 }
 
-// X(E, BM, BN, BK, WAVES_M, WAVES_N, STAGES, layout, product), largest tiles first.
-#define MOEGEMM_MENU_GATED(X, E)                                                        \
-  X(E, 256, 256, 32, 2, 4, 4, 0, GATED_FORWARD) X(E, 128, 256, 64, 2, 4, 3, 0, GATED_FORWARD) \
-  X(E, 64, 128, 64, 2, 2, 4, 0, GATED_FORWARD) X(E, 16, 128, 128, 1, 4, 4, 0, GATED_FORWARD)
-#define MOEGEMM_MENU_DX(X, E)                                                           \
-  X(E, 256, 256, 32, 2, 4, 4, 2, GATED_DX) X(E, 128, 256, 64, 2, 4, 3, 2, GATED_DX)     \
-  X(E, 64, 64, 64, 2, 2, 4, 2, GATED_DX) X(E, 16, 64, 128, 1, 4, 4, 2, GATED_DX)
-#define MOEGEMM_MENU_DW(X, E)                                                           \
-  X(E, 256, 256, 32, 2, 4, 4, 1, GATED_DW) X(E, 128, 256, 64, 2, 4, 3, 1, GATED_DW)     \
-  X(E, 64, 64, 64, 2, 2, 4, 1, GATED_DW)
-#define MOEGEMM_GATED_KERNEL(E, BM, BN, BK, WM, WN, S, LAY, PRODUCT) \
+// X(E, BM, BN, BK, WAVES_M, WAVES_N, STAGES, layout, product, ps, ns, gbps), largest tiles first; the last three are
+// what the choice of a variant reckons with, measured on full chips: a round of one tile per workgroup takes ps
+// picoseconds per element of K and ns nanoseconds besides, and weights that few rows share arrive at gbps.
+#define MOEGEMM_MENU_GATED(X, E)                                   \
+  X(E, 256, 256, 32, 2, 4, 4, 0, GATED_FORWARD, 26000, 5000, 5400) \
+  X(E, 128, 256, 64, 2, 4, 3, 0, GATED_FORWARD, 16500, 4000, 5400) \
+  X(E, 64, 128, 64, 2, 2, 4, 0, GATED_FORWARD, 6800, 2300, 4300)   \
+  X(E, 16, 128, 128, 1, 4, 4, 0, GATED_FORWARD, 5500, 2000, 3800)
+#define MOEGEMM_MENU_DX(X, E)                                 \
+  X(E, 256, 256, 32, 2, 4, 4, 2, GATED_DX, 26000, 5000, 4500) \
+  X(E, 128, 256, 64, 2, 4, 3, 2, GATED_DX, 16500, 4000, 4850) \
+  X(E, 64, 64, 64, 2, 2, 4, 2, GATED_DX, 8200, 2300, 4850)    \
+  X(E, 16, 64, 128, 1, 4, 4, 2, GATED_DX, 2600, 2000, 4100)
+#define MOEGEMM_MENU_DW(X, E)                                 \
+  X(E, 256, 256, 32, 2, 4, 4, 1, GATED_DW, 26000, 5000, 5400) \
+  X(E, 128, 256, 64, 2, 4, 3, 1, GATED_DW, 16500, 4000, 5400) \
+  X(E, 64, 64, 64, 2, 2, 4, 1, GATED_DW, 8200, 2300, 5400)
+#define MOEGEMM_GATED_KERNEL(E, BM, BN, BK, WM, WN, S, LAY, PRODUCT, PS, NS, GBPS) \
   template __global__ void gated_product_kernel<GatedTile<E, BM, BN, BK, WM, WN, S, LAY>, PRODUCT>(GatedParams);
-#define MOEGEMM_GATED_ENTRY(E, BM, BN, BK, WM, WN, S, LAY, PRODUCT) \
-  GatedVariant{BM, BN, &launch_gated<GatedTile<E, BM, BN, BK, WM, WN, S, LAY>, PRODUCT>},
+#define MOEGEMM_GATED_ENTRY(E, BM, BN, BK, WM, WN, S, LAY, PRODUCT, PS, NS, GBPS)           \
+  GatedVariant{BM, BN, GatedTile<E, BM, BN, BK, WM, WN, S, LAY>::PER_CU, PS, NS, GBPS,      \
+               &launch_gated<GatedTile<E, BM, BN, BK, WM, WN, S, LAY>, PRODUCT>},
 
 // Per type (bf16, fp16): the variants of the three products, each list closed by a null launch.
 struct GatedTable {
