@@ -360,3 +360,36 @@ def test_offsets_past_32_bits():
     out = grouped_mm_fp8(a, sa, w, sw, offs)
     assert not out[:-40].any()
     assert_product(out[-40:], a[-40:], sa[-40:], w[1], sw[1])
+
+
+def test_more_groups_than_a_launch_lists():
+    """Over 1024 groups: several launches; groups of 0 to 2 rows, checked row by row."""
+    from kernels import grouped_mm_fp8
+
+    counts = [(i * 7) % 3 for i in range(1100)]
+    rows, n, k = sum(counts), 40, 144
+    offs = torch.tensor(counts, device="cuda").cumsum(0).to(torch.int32)
+    a, sa, w, sw = operands(3, rows, n, k, len(counts))
+    owner = torch.repeat_interleave(torch.arange(len(counts), device="cuda"), torch.tensor(counts, device="cuda"))
+    x = values(a, sa, 1)
+    y = torch.stack([values(w[e], sw[e], 128) for e in range(len(counts))])[owner]
+    exact, size = (x[:, None] * y).sum(-1), (x[:, None] * y).abs().sum(-1)
+    for variant in (None, *_variants(0)):
+        print(f"grouped_mm_fp8 1100 groups variant={variant}", flush=True)
+        out = grouped_mm_fp8(a, sa, w, sw, offs, variant=variant)
+        bound = HALF_UNIT[out.dtype] * exact.abs() + (k + 8) * 2.0 ** -23 * size + 2.0 ** -24
+        assert torch.isfinite(out).all() and ((out.double() - exact).abs() <= bound).all()
+
+
+def test_more_rounds_than_a_launch_lists(monkeypatch):
+    """300 tiles and more on one workgroup: the launches after the first start where it ended."""
+    from kernels import fp8
+
+    a, sa, w, sw = operands(4, 130, 128 * 300, 32)
+    wide = fp8.matmul_fp8(a, sa, w, sw)
+    monkeypatch.setattr(fp8, "_cu_count", lambda *_: 1)
+    for variant in _variants(0):
+        print(f"matmul_fp8 one workgroup variant={variant}", flush=True)
+        out = fp8.matmul_fp8(a, sa, w, sw, variant=variant)
+        assert_product(out[:, -640:], a, sa, w[-640:], sw[-5:])
+        torch.testing.assert_close(out.float(), wide.float(), rtol=2.0 ** -7, atol=2.0 ** -7)

@@ -246,3 +246,46 @@ def test_rows_past_two_gib_of_one_expert():
     # Rows of zeros have g = u = 0, so h, dP and their share of dW are exactly zero.
     check_group(x[keep], w[0], dh[keep], out[keep], saved[keep], dx[keep], dw[0])
     assert not dw[1].any() and not out[1:65_535].any() and not dx[1:65_535].any()
+
+
+def test_more_groups_than_a_launch_lists():
+    """Over 1024 experts: several launches; checked per group against the first launches' neighbours."""
+    from kernels import _native, gate_up_swiglu_backward, gate_up_swiglu_forward
+
+    lib = _native.library()
+    counts = [(i * 7) % 3 for i in range(1100)]
+    x, w, dh, offs = operands(5, counts, 24, 16, torch.bfloat16)
+    starts = offs.tolist()
+    for variant in (None, *range(lib.moegemm_gate_up_variant_count(0))):
+        print(f"gate_up 1100 experts variant={variant}", flush=True)
+        out, saved = gate_up_swiglu_forward(x, w, offs, variant=variant)
+        back = min(variant or 0, lib.moegemm_gate_up_variant_count(2) - 1)
+        dx, dw = gate_up_swiglu_backward(dh, x, w, offs, saved, variants=None if variant is None else (variant, back))
+        for e in [*range(0, 12), *range(1018, 1032), *range(1090, 1100)]:
+            part = slice(starts[e] - counts[e], starts[e])
+            if counts[e]:
+                check_group(x[part], w[e], dh[part], out[part], saved[part], dx[part], dw[e])
+            else:
+                assert not dw[e].any()
+
+
+def test_more_rounds_than_a_launch_lists(monkeypatch):
+    """More than 256 tiles on one workgroup: the launches after the first start where it ended."""
+    from kernels import _native, gated_ffn
+
+    lib = _native.library()
+    counts = (20, 0, 50)
+    x, w, dh, offs = operands(6, counts, 264, 128 * 140, torch.bfloat16)
+    out, saved = gated_ffn.gate_up_swiglu_forward(x, w, offs)
+    dx, dw = gated_ffn.gate_up_swiglu_backward(dh, x, w, offs, saved)
+    monkeypatch.setattr(gated_ffn, "_cu_count", lambda *_: 1)
+    close = dict(rtol=2.0 ** -6, atol=2.0 ** -6)
+    for variant in range(lib.moegemm_gate_up_variant_count(0)):
+        print(f"gate_up forward one workgroup variant={variant}", flush=True)
+        got, kept = gated_ffn.gate_up_swiglu_forward(x, w, offs, variant=variant)
+        torch.testing.assert_close(got, out, **close)
+        torch.testing.assert_close(kept, saved, rtol=1e-5, atol=1e-4)
+    for variant in range(lib.moegemm_gate_up_variant_count(2)):
+        print(f"gate_up dw one workgroup variant={variant}", flush=True)
+        _, got = gated_ffn.gate_up_swiglu_backward(dh, x, w, offs, saved, need_dx=False, variants=(variant, variant))
+        torch.testing.assert_close(got, dw, **close)
