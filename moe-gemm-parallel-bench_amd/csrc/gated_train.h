@@ -156,6 +156,23 @@ struct TileSums {
   }
 };
 
+// T::load_frags of the first half of a wave's rows.
+template <class T>
+__device__ __forceinline__ void load_half(i16x8_t (&af)[T::FM], i16x8_t (&bf)[T::FN], const char* stage, int kk, int wave_m,
+                                          int wave_n, bool swiglu) {
+#pragma unroll
+  for (int fm = 0; fm < T::FM / 2; ++fm) {
+    if constexpr (T::AT) af[fm] = T::frag_transposed(stage, T::CA, wave_m * T::WTM + fm * T::MI, kk);
+    else af[fm] = T::frag_rows(stage, T::CA, wave_m * T::WTM + fm * T::MI, kk);
+  }
+#pragma unroll
+  for (int fn = 0; fn < T::FN; ++fn) {
+    const char* b = stage + T::A_BYTES;
+    if constexpr (T::BT) bf[fn] = T::frag_rows(b, T::CB, wave_n * T::WTN + fn * T::MI, kk);
+    else bf[fn] = T::frag_transposed(b, T::CB, T::b_frag_col(fn, wave_n, swiglu), kk);
+  }
+}
+
 // Cross-tile chaining of the ping-pong tile (see PingPongTile::run_tile_chained) with an epilogue of the caller's.
 // A tile's last three refills copy the next tile's slices 0 to 2; then the outputs leave in exactly Finish::STORES vector
 // stores per wave, and slice 3 of the next tile follows.  A wave's vector memory operations complete in issue
@@ -167,7 +184,9 @@ struct ChainState {
   bool prefetched;
 };
 
-template <class T, bool SECOND, class Finish>
+// The last row tile of a group of rows is rarely full: ROWS of the wave's FM row fragments (all, half, none) are
+// loaded and multiplied, the others' outputs lie past the rows.
+template <class T, bool SECOND, int ROWS, class Finish>
 __device__ __forceinline__ void chained_tile(const ProblemDesc& pd, int m0, int n0, const ProblemDesc& next, int m1,
                                              int n1, bool has_next, char* smem, ChainState& ch, Finish&& finish) {
   constexpr int FM = T::FM, FN = T::FN, KK = T::KK, BK = T::BK, STAGES = T::STAGES, XMIN = T::XMIN;
@@ -192,9 +211,6 @@ __device__ __forceinline__ void chained_tile(const ProblemDesc& pd, int m0, int 
   if constexpr (SECOND) phase_barrier();
   const int kt_count = (pd.k + BK - 1) / BK;
   const bool chain = has_next && kt_count >= STAGES;
-  // The second group holds rows 128 to 255: of a row tile with fewer (the last one of a group of rows) it skips the
-  // fragments and products, and the first group's compute phases follow one another.
-  const bool idle = SECOND && pd.m - m0 <= T::BM / 2;
   i16x8_t af[KK][FM], bf[KK][FN];
   // ISSUE: 0 none, 1 this tile's slice kt + 3 (zeros past K), 2 the next tile's once that index passes K.
   auto step = [&](int kt, auto issue, auto edge) {
@@ -213,10 +229,13 @@ __device__ __forceinline__ void chained_tile(const ProblemDesc& pd, int m0, int 
         T::template issue_stage<0>(d, buffer, s * BK);
       }
     }
-    if (!idle) {
+    if constexpr (ROWS == FM) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
         T::load_frags(af[kk], bf[kk], cur, cur + T::A_BYTES, kk, wave_m, wave_n, pd.swiglu != 0);
+    } else if constexpr (ROWS > 0) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) load_half<T>(af[kk], bf[kk], cur, kk, wave_m, wave_n, pd.swiglu != 0);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     auto wait_next = [&] {  // slice kt + 1 has landed
@@ -231,9 +250,12 @@ __device__ __forceinline__ void chained_tile(const ProblemDesc& pd, int m0, int 
     };
     if constexpr (SECOND) wait_next();
     phase_barrier();
-    if (!idle) {
+    if constexpr (ROWS == FM) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) T::template mfma_rows<0, FM>(acc, af[kk], bf[kk]);
+    } else if constexpr (ROWS > 0) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) T::template mfma_rows<0, ROWS>(acc, af[kk], bf[kk]);
     }
     if constexpr (!SECOND) wait_next();
     phase_barrier();
@@ -485,10 +507,21 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
         int m1 = 0, n1 = 0;
         float* saved_next = nullptr;
         more = describe(++i, next, m1, n1, saved_next);
-        if (__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) >= T::NW / 2)
-          chained_tile<T, true>(pd, m0, n0, next, m1, n1, more, smem, ch, finish(saved));
-        else
-          chained_tile<T, false>(pd, m0, n0, next, m1, n1, more, smem, ch, finish(saved));
+        auto tile = [&](auto second, auto rows) {
+          chained_tile<T, decltype(second)::value, decltype(rows)::value>(pd, m0, n0, next, m1, n1, more, smem, ch,
+                                                                           finish(saved));
+        };
+        using all = std::integral_constant<int, T::FM>;
+        using half = std::integral_constant<int, T::FM / 2>;
+        const int rows = PRODUCT == GATED_DW ? T::BM : pd.m - m0;
+        if (__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) >= T::NW / 2) {
+          if (rows > T::BM / 2 + T::WTM / 2) tile(std::true_type{}, all{});
+          else if (rows > T::BM / 2) tile(std::true_type{}, half{});
+          else tile(std::true_type{}, std::integral_constant<int, 0>{});
+        } else {
+          if (rows > T::WTM / 2) tile(std::false_type{}, all{});
+          else tile(std::false_type{}, half{});
+        }
         pd = next;
         m0 = m1;
         n0 = n1;
