@@ -382,11 +382,11 @@ int moegemm_grouped_mm_fp8_swiglu(const void* a, const float* scale_a, const voi
  * [gate | up] columns (the 3-D packed W13 of moegemm_grouped_mm_offs_swiglu), offs as there; offs NULL: one group of
  * all rows.  h and f are multiples of 8, all rows 16-byte aligned with unit inner strides.
  *   forward:  [g | u] = x w[e] in fp32 -> saved [rows, 2f]; silu(g) * u -> h_out [rows, f]
- *   gradient: dp [rows, 2f] = [dh u s (1 + g (1 - s)) | dh g s], s = sigmoid(g), rounded to dtype
- *   dx:       dp w[e]^T -> dx [rows, h]
- *   dw:       x[r0:r1]^T dp[r0:r1] -> dw [group_count, h, 2f]; zeros for a group without rows
+ *   backward: dp [rows, 2f] = [dh u s (1 + g (1 - s)) | dh g s], s = sigmoid(g), rounded to dtype (a workspace);
+ *             dp w[e]^T -> dx [rows, h] unless dx is NULL;
+ *             x[r0:r1]^T dp[r0:r1] -> dw [group_count, h, 2f] unless dw is NULL; zeros for a group without rows
  * Rows at or past offs[group_count-1] get h_out = 0 and dx = 0 (their saved and dp stay unwritten and unread).
- * saved and dp are contiguous.  `variant` -1 lets the library choose the tile (moegemm_gate_up_variant_count:
+ * saved, dp, dx and dw are contiguous.  `variant` -1 lets the library choose the tile (moegemm_gate_up_variant_count:
  * product 0 forward, 1 dx, 2 dw); grid_size as in moegemm_grouped_mm_fp8.  Sums are fp32 and of one order: repeated
  * calls give the same bits.
  */
@@ -395,15 +395,10 @@ int moegemm_gate_up_forward(const void* x, const void* w, void* h_out, float* sa
                             int32_t group_count, int32_t rows, int32_t h, int32_t f, int64_t stride_xm,
                             int64_t stride_wg, int64_t stride_wh, int64_t stride_om, int32_t dtype, int32_t variant,
                             int32_t grid_size, void* stream);
-int moegemm_gate_up_gradient(const void* dh, const float* saved, void* dp, const int32_t* offs, int32_t group_count,
-                             int32_t rows, int32_t f, int64_t stride_dhm, int32_t dtype, int32_t grid_size,
-                             void* stream);
-int moegemm_gate_up_dx(const void* dp, const void* w, void* dx, const int32_t* offs, int32_t group_count, int32_t rows,
-                       int32_t h, int32_t f, int64_t stride_wg, int64_t stride_wh, int64_t stride_om, int32_t dtype,
-                       int32_t variant, int32_t grid_size, void* stream);
-int moegemm_gate_up_dw(const void* x, const void* dp, void* dw, const int32_t* offs, int32_t group_count, int32_t rows,
-                       int32_t h, int32_t f, int64_t stride_xm, int64_t stride_og, int64_t stride_oh, int32_t dtype,
-                       int32_t variant, int32_t grid_size, void* stream);
+int moegemm_gate_up_backward(const void* dh, const void* x, const void* w, const float* saved, void* dp, void* dx,
+                             void* dw, const int32_t* offs, int32_t group_count, int32_t rows, int32_t h, int32_t f,
+                             int64_t stride_dhm, int64_t stride_xm, int64_t stride_wg, int64_t stride_wh, int32_t dtype,
+                             int32_t dx_variant, int32_t dw_variant, int32_t grid_size, void* stream);
 
 #ifdef __cplusplus
 }

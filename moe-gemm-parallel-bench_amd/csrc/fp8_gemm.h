@@ -141,8 +141,8 @@ struct TileList {
   GroupTile tile[kListTiles];  // e < 0: none
 };
 
-// Rounds from `round` on.  `order(tile, local)` places the group's local-th tile.  Every thread of the workgroup calls
-// it; ends with a barrier.
+// Rounds from `round` on.  `order(tile, local)` places the group's local-th tile.  Every
+// thread of the workgroup calls it; ends with a barrier.
 template <class Order>
 __device__ __forceinline__ void build_tile_list(TileList& list, const TileTable& table, int first, int groups, int round,
                                                 Order&& order) {

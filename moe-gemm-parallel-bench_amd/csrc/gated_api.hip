@@ -56,8 +56,10 @@ const GatedVariant* choose(const GatedVariant* list, int product, const GatedPar
   double least = 0;
   for (const GatedVariant* v = list; v->launch; ++v) {
     const int64_t rows = product == GATED_DW ? p.groups * cdiv(p.h, v->block_m) : row_tiles(*v, p.rows, p.groups);
-    const int64_t rounds = cdiv(rows * cdiv(cols, v->block_n), (int64_t)cus * v->per_cu);
-    const double ns = std::max(rounds * (k * v->slice_ps * 1e-3 + v->tile_ns), weights / v->gbps);
+    const int64_t tiles = rows * cdiv(cols, v->block_n), full = tiles / (cus * v->per_cu), rest = tiles % (cus * v->per_cu);
+    // A last round that leaves every CU one workgroup takes a round's time by the number a CU holds.
+    const double rounds = full + (rest == 0 ? 0.0 : rest <= cus ? 1.0 / v->per_cu : 1.0);
+    const double ns = std::max(rounds * k * v->slice_ps * 1e-3 + (full + (rest > 0)) * v->tile_ns, weights / v->gbps);
     if (!best || ns < least) {
       best = v;
       least = ns;
@@ -68,31 +70,47 @@ const GatedVariant* choose(const GatedVariant* list, int product, const GatedPar
 
 const GatedTable& table_of(int32_t dtype) { return dtype == DT_BF16 ? kGatedBf16 : kGatedF16; }
 
-int launch_product(const GatedParams& p, int product, int32_t dtype, int32_t variant, int32_t grid_size, void* stream) {
+// A product's variant, its workgroups and a bound on its tiles.
+struct Plan {
+  const GatedVariant* v;
+  int64_t tiles;
+  int grid;
+};
+
+int plan_product(const GatedParams& p, int product, int32_t dtype, int32_t variant, int cus, Plan& plan) {
   const GatedVariant* list = table_of(dtype).products[product];
-  const int cus = grid_size > 0 ? grid_size : 256;
   const int64_t cols = product == GATED_DX ? p.h : 2 * (int64_t)p.f;
-  const GatedVariant* v = nullptr;
+  plan.v = nullptr;
   if (variant < 0) {
-    v = choose(list, product, p, cols, cus);
+    plan.v = choose(list, product, p, cols, cus);
   } else {
     for (int i = 0; list[i].launch; ++i)
-      if (i == variant) v = &list[i];
-    if (!v) return report(MOEGEMM_ERR_NO_KERNEL, "Gate+Up variant %d is not compiled", variant);
+      if (i == variant) plan.v = &list[i];
+    if (!plan.v) return report(MOEGEMM_ERR_NO_KERNEL, "Gate+Up variant %d is not compiled", variant);
   }
+  const int bm = plan.v->block_m;
   const int64_t row_tiles = product == GATED_DW
-                                ? p.groups * cdiv(p.h, v->block_m)
-                                : std::min(p.rows / v->block_m + (int64_t)p.groups, p.groups * cdiv(p.rows, v->block_m));
-  const int64_t bound = row_tiles * cdiv(cols, v->block_n);
-  if (bound > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
-  const int grid = (int)std::min<int64_t>(std::max<int64_t>(bound, 1), (int64_t)cus * v->per_cu);
+                                ? p.groups * cdiv(p.h, bm)
+                                : std::min(p.rows / bm + (int64_t)p.groups, p.groups * cdiv(p.rows, bm));
+  plan.tiles = std::max<int64_t>(row_tiles * cdiv(cols, plan.v->block_n), 1);
+  if (plan.tiles > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
+  plan.grid = (int)std::min<int64_t>(plan.tiles, (int64_t)cus * plan.v->per_cu);
+  return MOEGEMM_OK;
+}
+
+int checked(hipError_t err) {
+  return err == hipSuccess ? MOEGEMM_OK
+                           : report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+}
+
+int launch_planned(const GatedParams& p, const Plan& plan, hipStream_t stream) {
   GatedParams part = p;
   for (; part.first < p.groups; part.first += kTableGroups) {
     part.groups = std::min(p.groups - part.first, kTableGroups);
-    for (part.round = 0; (int64_t)part.round * grid < std::max<int64_t>(bound, 1); part.round += kListTiles) {
+    for (part.round = 0; (int64_t)part.round * plan.grid < plan.tiles; part.round += kListTiles) {
       part.closes = part.first + part.groups == p.groups && part.round == 0;
-      const hipError_t err = v->launch(part, grid, reinterpret_cast<hipStream_t>(stream));
-      if (err != hipSuccess) return report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+      const int rc = checked(plan.v->launch(part, plan.grid, stream));
+      if (rc != MOEGEMM_OK) return rc;
     }
   }
   return MOEGEMM_OK;
@@ -124,55 +142,51 @@ int moegemm_gate_up_forward(const void* x, const void* w, void* h_out, float* sa
     return report(MOEGEMM_ERR_INVALID, "a group's weight must start at a multiple of 16 bytes and span under 2 GiB");
   GatedParams p{x, w, h_out, saved, nullptr, offs, stride_xm, stride_wg, stride_wh, stride_om, 0, 0,
                 group_count, rows, h, f, 0};
-  return launch_product(p, GATED_FORWARD, dtype, variant, grid_size, stream);
+  Plan plan;
+  rc = plan_product(p, GATED_FORWARD, dtype, variant, grid_size > 0 ? grid_size : 256, plan);
+  return rc == MOEGEMM_OK ? launch_planned(p, plan, reinterpret_cast<hipStream_t>(stream)) : rc;
 }
 
-int moegemm_gate_up_gradient(const void* dh, const float* saved, void* dp, const int32_t* offs, int32_t group_count,
-                             int32_t rows, int32_t f, int64_t stride_dhm, int32_t dtype, int32_t grid_size,
-                             void* stream) {
-  int rc = check_shape(group_count, rows, 8, f, offs, dtype);
-  if (rc == MOEGEMM_OK && rows == 0) return MOEGEMM_OK;
-  if (rc == MOEGEMM_OK) rc = check_operand("dh", dh, stride_dhm, f);
-  if (rc == MOEGEMM_OK) rc = check_operand("saved", saved, 2 * (int64_t)f, 2 * (int64_t)f);
-  if (rc == MOEGEMM_OK) rc = check_operand("dp", dp, 2 * (int64_t)f, 2 * (int64_t)f);
-  if (rc != MOEGEMM_OK) return rc;
-  GatedParams p{nullptr, nullptr, nullptr, const_cast<float*>(saved), nullptr, offs, 0, 0, 0, 0, 0, 0,
-                group_count, rows, 8, f, 0};
-  const int64_t blocks = cdiv((int64_t)rows * (f / 8), 256), cus = grid_size > 0 ? grid_size : 256;
-  const hipError_t err = table_of(dtype).gradient(p, dh, stride_dhm, dp, (int)std::min<int64_t>(blocks, cus * 16),
-                                                  reinterpret_cast<hipStream_t>(stream));
-  if (err != hipSuccess) return report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
-  return MOEGEMM_OK;
-}
-
-int moegemm_gate_up_dx(const void* dp, const void* w, void* dx, const int32_t* offs, int32_t group_count, int32_t rows,
-                       int32_t h, int32_t f, int64_t stride_wg, int64_t stride_wh, int64_t stride_om, int32_t dtype,
-                       int32_t variant, int32_t grid_size, void* stream) {
+int moegemm_gate_up_backward(const void* dh, const void* x, const void* w, const float* saved, void* dp, void* dx,
+                             void* dw, const int32_t* offs, int32_t group_count, int32_t rows, int32_t h, int32_t f,
+                             int64_t stride_dhm, int64_t stride_xm, int64_t stride_wg, int64_t stride_wh, int32_t dtype,
+                             int32_t dx_variant, int32_t dw_variant, int32_t grid_size, void* stream) {
+  const int64_t width = 2 * (int64_t)f;
   int rc = check_shape(group_count, rows, h, f, offs, dtype);
-  if (rc == MOEGEMM_OK && rows == 0) return MOEGEMM_OK;
-  if (rc == MOEGEMM_OK) rc = check_operand("dp", dp, 2 * (int64_t)f, 2 * (int64_t)f);
-  if (rc == MOEGEMM_OK) rc = check_operand("w", w, stride_wh, 2 * (int64_t)f);
-  if (rc == MOEGEMM_OK) rc = check_operand("dx", dx, stride_om, h);
+  if (rows > 0) {
+    if (rc == MOEGEMM_OK) rc = check_operand("dh", dh, stride_dhm, f);
+    if (rc == MOEGEMM_OK) rc = check_operand("saved", saved, width, width);
+    if (rc == MOEGEMM_OK) rc = check_operand("dp", dp, width, width);
+    if (rc == MOEGEMM_OK && dx) rc = check_operand("w", w, stride_wh, width);
+    if (rc == MOEGEMM_OK && dx) rc = check_operand("dx", dx, h, h);
+    if (rc == MOEGEMM_OK && dw) rc = check_operand("x", x, stride_xm, h);
+  }
+  if (rc == MOEGEMM_OK && dw) rc = check_operand("dw", dw, width, width);
+  if (rc == MOEGEMM_OK && stride_wg % 8)
+    rc = report(MOEGEMM_ERR_INVALID, "a group's weight must start at a multiple of 16 bytes");
   if (rc != MOEGEMM_OK) return rc;
-  if (stride_wg % 8) return report(MOEGEMM_ERR_INVALID, "a group's weight must start at a multiple of 16 bytes");
-  GatedParams p{dp, w, dx, nullptr, nullptr, offs, 2 * (int64_t)f, stride_wg, stride_wh, stride_om, 0, 0,
-                group_count, rows, h, f, 0};
-  return launch_product(p, GATED_DX, dtype, variant, grid_size, stream);
-}
+  const hipStream_t queue = reinterpret_cast<hipStream_t>(stream);
+  const int cus = grid_size > 0 ? grid_size : 256;
+  const GatedTable& table = table_of(dtype);
+  const GatedParams of_x{dp, w, dx, nullptr, nullptr, offs, width, stride_wg, stride_wh, h, 0, 0, group_count, rows, h, f, 0};
+  const GatedParams of_w{x, nullptr, dw, nullptr, dp, offs, stride_xm, 0, 0, width, h * width, width, group_count, rows, h, f,
+                         (rows + (int64_t)1024) * std::max<int64_t>(stride_xm, width) * 2 >= kTwoGiB};
+  const bool want_dx = dx && rows > 0;
+  Plan plan_x{}, plan_w{};
+  if (want_dx) rc = plan_product(of_x, GATED_DX, dtype, dx_variant, cus, plan_x);
+  if (rc == MOEGEMM_OK && dw) rc = plan_product(of_w, GATED_DW, dtype, dw_variant, cus, plan_w);
+  if (rc != MOEGEMM_OK) return rc;
 
-int moegemm_gate_up_dw(const void* x, const void* dp, void* dw, const int32_t* offs, int32_t group_count, int32_t rows,
-                       int32_t h, int32_t f, int64_t stride_xm, int64_t stride_og, int64_t stride_oh, int32_t dtype,
-                       int32_t variant, int32_t grid_size, void* stream) {
-  int rc = check_shape(group_count, rows, h, f, offs, dtype);
-  if (rc == MOEGEMM_OK && rows > 0) rc = check_operand("x", x, stride_xm, h);
-  if (rc == MOEGEMM_OK && rows > 0) rc = check_operand("dp", dp, 2 * (int64_t)f, 2 * (int64_t)f);
-  if (rc == MOEGEMM_OK) rc = check_operand("dw", dw, stride_oh, 2 * (int64_t)f);
-  if (rc != MOEGEMM_OK) return rc;
-  if (stride_og % 8) return report(MOEGEMM_ERR_INVALID, "a group's dw must start at a multiple of 16 bytes");
-  const int64_t pitch = std::max<int64_t>(stride_xm, 2 * (int64_t)f);
-  GatedParams p{x, nullptr, dw, nullptr, dp, offs, stride_xm, 0, 0, stride_oh, stride_og, 2 * (int64_t)f,
-                group_count, rows, h, f, (rows + (int64_t)1024) * pitch * 2 >= kTwoGiB};
-  return launch_product(p, GATED_DW, dtype, variant, grid_size, stream);
+  if (rows > 0 && (dx || dw)) {
+    const GatedParams p{nullptr, nullptr, nullptr, const_cast<float*>(saved), nullptr, offs, 0, 0, 0, 0, 0, 0,
+                        group_count, rows, h, f, 0};
+    const int64_t blocks = cdiv((int64_t)rows * (f / 8), 256);
+    rc = checked(table.gradient(p, dh, stride_dhm, dp, (int)std::min<int64_t>(blocks, cus * 16), queue));
+    if (rc != MOEGEMM_OK) return rc;
+  }
+  if (want_dx) rc = launch_planned(of_x, plan_x, queue);
+  if (rc == MOEGEMM_OK && dw) rc = launch_planned(of_w, plan_w, queue);
+  return rc;
 }
 
 }  // extern "C"

@@ -290,7 +290,8 @@ template <class E, int BM, int BN, int BK, int WM, int WN, int S, int LAY>
 struct GatedTile
     : std::conditional<BM == 256 && BN == 256, PingPongTile<E, BK, S, LAY>, FastTile<E, BM, BN, BK, WM, WN, S, LAY>>::type {
   using Element = E;
-  static constexpr int PER_CU = 2 * (GatedTile::PREFIX_OFFSET + (int)(sizeof(TileTable) + sizeof(TileList))) <= 160 * 1024 ? 2 : 1;
+  static constexpr int PER_CU = 2 * (GatedTile::PREFIX_OFFSET + (int)(sizeof(TileTable) + sizeof(TileList))) <= 160 * 1024
+                                    ? 2 : 1;
 };
 
 enum GatedProduct : int { GATED_FORWARD = 0, GATED_DX = 1, GATED_DW = 2 };
@@ -421,12 +422,16 @@ __device__ __forceinline__ int rows_end(const GatedParams& p) {
 
 constexpr int kWholeK = 1 << 30;  // no segments
 
+// LDS of a workgroup: the tile's stages, then the tables.
+template <class T>
+constexpr int kGatedLds = T::PREFIX_OFFSET + (int)(sizeof(TileTable) + sizeof(TileList));
+
 template <class T, int PRODUCT>
 __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[T::PREFIX_OFFSET];
-  __shared__ TileTable table;
-  __shared__ TileList list;
-  static_assert(T::PREFIX_OFFSET + sizeof(TileTable) + sizeof(TileList) <= 160 * 1024, "LDS of one CU");
+  __shared__ __attribute__((aligned(16))) char smem[kGatedLds<T>];
+  static_assert(kGatedLds<T> <= 160 * 1024, "LDS of one CU");
+  TileTable& table = *reinterpret_cast<TileTable*>(smem + T::PREFIX_OFFSET);
+  TileList& list = *reinterpret_cast<TileList*>(smem + T::PREFIX_OFFSET + sizeof(TileTable));
   const int n = PRODUCT == GATED_DX ? p.h : 2 * p.f;
   // dW: every expert with rows holds the same number of tiles.
   constexpr int ROWS_PER_TILE = PRODUCT == GATED_DW ? 1 << 30 : T::BM;
@@ -436,18 +441,6 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
   const char* w = static_cast<const char*>(p.w);
   char* out = static_cast<char*>(p.out);
 
-  // What no tile writes: rows past the last group, gradients of experts without rows.
-  if constexpr (PRODUCT == GATED_DW) {
-    for (int first = 0; p.round == 0 && first < p.groups; first += 64) {
-      const int e = first + (int)(threadIdx.x & 63);
-      int m = 1;
-      if (e < p.groups) group_rows(p.offs, p.rows, p.first + e, m);
-      for (uint64_t empty = __builtin_amdgcn_ballot_w64(m == 0); empty; empty &= empty - 1)
-        zero_rows(out + (int64_t)(p.first + first + __builtin_ctzll(empty)) * p.sog * 2, p.so, n, 0, p.h);
-    }
-  } else if (p.closes) {
-    zero_rows(out, p.so, PRODUCT == GATED_DX ? p.h : p.f, rows_end(p), p.rows);
-  }
   build_tile_table(table, p.offs, p.first, p.groups, p.rows, ROWS_PER_TILE, per_row_tile);
 
   auto describe = [&](int i, ProblemDesc& pd, int& m0, int& n0, float*& saved) {  // the list's i-th tile
@@ -498,7 +491,6 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
   int m0 = 0, n0 = 0, i = 0;
   float* saved = nullptr;
   bool more = describe(0, pd, m0, n0, saved);
-  if (!more) return;
   if (PING_PONG && !p.long_k) {
     if constexpr (PING_PONG) {
       ChainState ch{0, false};
@@ -529,7 +521,7 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
       }
     }
   } else {
-    do {
+    while (more) {
       auto store = [&](const typename T::acc_t (&acc)[T::FM][T::FN], int wave_m, int wave_n) {
         finish(saved).last(acc, pd, m0, n0, wave_m, wave_n);
       };
@@ -546,7 +538,21 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
       } else {
         TileSums<T>::run(pd, m0, n0, kWholeK, smem, [](const ProblemDesc& whole, int, int) { return whole; }, store);
       }
-    } while (describe(++i, pd, m0, n0, saved));
+      more = describe(++i, pd, m0, n0, saved);
+    }
+  }
+
+  // What no tile writes: rows past the last group, gradients of experts without rows.  After the tiles, whose first
+  // loads it would delay.
+  if constexpr (PRODUCT == GATED_DW) {
+    for (int first = 0; p.round == 0 && first < p.groups; first += 64) {
+      const int e = first + (int)(threadIdx.x & 63);
+      const bool none = e < p.groups && table.tiles[e] == (e ? table.tiles[e - 1] : 0);
+      for (uint64_t empty = __builtin_amdgcn_ballot_w64(none); empty; empty &= empty - 1)
+        zero_rows(out + (int64_t)(p.first + first + __builtin_ctzll(empty)) * p.sog * 2, p.so, n, 0, p.h);
+    }
+  } else if (p.closes) {
+    zero_rows(out, p.so, PRODUCT == GATED_DX ? p.h : p.f, table.ends[p.groups - 1], p.rows);
   }
 }
 

@@ -135,17 +135,10 @@ SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
     ),
-    "moegemm_gate_up_gradient": (
+    "moegemm_gate_up_backward": (
         ctypes.c_int,
-        [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i32, _i32, _vp],
-    ),
-    "moegemm_gate_up_dx": (
-        ctypes.c_int,
-        [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
-    ),
-    "moegemm_gate_up_dw": (
-        ctypes.c_int,
-        [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+         _vp],
     ),
 }
 

@@ -20,7 +20,7 @@ from __future__ import annotations
 from functools import lru_cache
 
 from . import _native
-from .matmul import _device_signature, _require_runtime
+from .matmul import _device_signature
 
 SCALE_BLOCK = 128
 _PITCH_LIMIT = 1 << 23  # bytes; 256 rows of a tile stay under 2 GiB
@@ -72,18 +72,19 @@ def quantize_fp8(x, *, block_rows: int = 1, out=None, scale=None):
                          "multiples of 8 bytes")
     if scale is None:
         if block_rows == 1:
-            scale = torch.empty((*x.shape[:-2], scale_shape[-1], rows), dtype=torch.float32, device=x.device)
-            scale = scale.transpose(-1, -2)
+            blocks = scale_shape[-1]
+            strides = (1, rows) if x.ndim == 2 else (blocks * rows, 1, rows)
+            scale = torch.empty_strided(scale_shape, strides, dtype=torch.float32, device=x.device)
         else:
             scale = torch.empty(scale_shape, dtype=torch.float32, device=x.device)
     elif tuple(scale.shape) != scale_shape or scale.dtype != torch.float32 or scale.device != x.device:
         raise ValueError(f"scale must be a {scale_shape} float32 tensor on x's device")
-    _require_runtime(x)
-    three = x.ndim == 3
+    xs, qs, ss = x.stride(), out.stride(), scale.stride()
+    three = len(xs) == 3
     status = _native.library().moegemm_quantize_fp8(
-        x.data_ptr(), out.data_ptr(), scale.data_ptr(), batch, rows, k, x.stride(0) if three else 0, x.stride(-2),
-        out.stride(0) if three else 0, out.stride(-2), scale.stride(0) if three else 0, scale.stride(-2),
-        scale.stride(-1), code, block_rows, _native.current_stream_handle(x.device))
+        x.data_ptr(), out.data_ptr(), scale.data_ptr(), batch, rows, k, xs[0] if three else 0, xs[-2],
+        qs[0] if three else 0, qs[-2], ss[0] if three else 0, ss[-2], ss[-1], code, block_rows,
+        _native.current_stream_handle(x.device))
     _native.check(status)
     return out, scale
 
@@ -105,13 +106,14 @@ def _validate(a, scale_a, weight, scale_w, offs):
         raise ValueError("a and weight must be float8_e4m3fn")
     if groups <= 0 or n <= 0 or k <= 0:
         raise ValueError("fp8 products need at least one group and positive K and N")
-    if tuple(scale_a.shape) != (rows, _blocks(k)) or scale_a.dtype != torch.float32:
+    if scale_a.shape != (rows, _blocks(k)) or scale_a.dtype is not torch.float32:
         raise ValueError(f"scale_a must be a float32 [{rows}, {_blocks(k)}] tensor")
     expected = (groups, _blocks(n), _blocks(k)) if grouped else (_blocks(n), _blocks(k))
-    if tuple(scale_w.shape) != expected or scale_w.dtype != torch.float32:
+    if scale_w.shape != expected or scale_w.dtype is not torch.float32:
         raise ValueError(f"scale_w must be a float32 {list(expected)} tensor")
-    tensors = (a, scale_a, weight, scale_w) + ((offs,) if grouped else ())
-    if len({t.device for t in tensors}) != 1 or a.device.type != "cuda":
+    device = a.device
+    if (not a.is_cuda or weight.device != device or scale_a.device != device or scale_w.device != device
+            or (grouped and offs.device != device)):
         raise ValueError("operands, scales and offs must be on the same GPU device")
     if grouped:
         if offs.ndim != 1 or offs.dtype != torch.int32 or offs.shape[0] != groups:
@@ -119,11 +121,13 @@ def _validate(a, scale_a, weight, scale_w, offs):
         if not offs.is_contiguous():
             raise ValueError("offs must be contiguous (pass offs.contiguous())")
     for name, t in (("a", a), ("weight", weight)):
-        if t.stride(-1) != 1 and k > 1:
+        strides, shape = t.stride(), t.shape
+        if strides[-1] != 1 and k > 1:
             raise ValueError(f"{name} needs a unit stride along K")
-        if t.data_ptr() % 16 or any(s % 16 for s, d in zip(t.stride()[:-1], t.shape[:-1]) if d > 1):
+        if (t.data_ptr() & 15 or (strides[-2] & 15 and shape[-2] > 1)
+                or (len(shape) == 3 and strides[0] & 15 and shape[0] > 1)):
             raise ValueError(f"{name} rows must start at multiples of 16 bytes (quantize_fp8 pads them so)")
-    return int(rows), int(n), int(k), int(groups)
+    return rows, n, k, groups
 
 
 def _pitch(tensor, width: int) -> int:
@@ -133,9 +137,10 @@ def _pitch(tensor, width: int) -> int:
 
 def _operand_args(a, scale_a, weight, scale_w, k: int):
     grouped = weight.ndim == 3
-    return (a.shape[0], weight.shape[-2], k, _pitch(a, k), scale_a.stride(0), scale_a.stride(1),
-            weight.stride(0) if grouped and weight.shape[0] > 1 else 0, _pitch(weight, k),
-            scale_w.stride(0) if grouped else 0, scale_w.stride(-2), scale_w.stride(-1))
+    sa, sw = scale_a.stride(), scale_w.stride()
+    return (a.shape[0], weight.shape[-2], k, _pitch(a, k), sa[0], sa[1],
+            weight.stride(0) if grouped and weight.shape[0] > 1 else 0, _pitch(weight, k), sw[0] if grouped else 0, sw[-2],
+            sw[-1])
 
 
 def _product(a, scale_a, weight, scale_w, offs, out, out_dtype, fast_accum, variant):
@@ -148,7 +153,6 @@ def _product(a, scale_a, weight, scale_w, offs, out, out_dtype, fast_accum, vari
         out_dtype = out.dtype
     out_dtype = out_dtype or torch.bfloat16
     code = _native.dtype_code(out_dtype)
-    _require_runtime(a)
     if out is None:
         out = torch.empty((rows, n), dtype=out_dtype, device=a.device)
     elif tuple(out.shape) != (rows, n) or out.device != a.device or (out.stride(1) != 1 and n > 1):
@@ -203,7 +207,6 @@ def grouped_mm_fp8_swiglu(a, scale_a, weight, scale_w, offs=None, *, fast_accum:
     if n % 16:
         raise ValueError(f"packed Gate+Up width must be 2F with F a multiple of 8 (got {n} rows)")
     f = n // 2
-    _require_runtime(a)
     pitch = -(-f // 16) * 16
     buffer = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=a.device)
     out = buffer if pitch == f else buffer[:, :f]

@@ -14,13 +14,13 @@ from __future__ import annotations
 
 from . import _native
 from .fp8 import _cu_count
-from .matmul import _require_runtime
 
 
 def _rows_ok(tensor) -> bool:
     """Unit inner stride and rows at multiples of 16 bytes."""
-    return (tensor.stride(-1) == 1 and tensor.data_ptr() % 16 == 0
-            and all(s % 8 == 0 for s, d in zip(tensor.stride()[:-1], tensor.shape[:-1]) if d > 1))
+    strides, shape = tensor.stride(), tensor.shape
+    return (strides[-1] == 1 and not tensor.data_ptr() & 15 and not (strides[-2] & 7 and shape[-2] > 1)
+            and not (len(shape) == 3 and strides[0] & 7 and shape[0] > 1))
 
 
 def _validate(x, weight, offs):
@@ -28,29 +28,30 @@ def _validate(x, weight, offs):
     import torch
 
     grouped = offs is not None
-    if x.ndim != 2 or weight.ndim != (3 if grouped else 2):
+    shape = weight.shape
+    if x.ndim != 2 or len(shape) != (3 if grouped else 2):
         raise ValueError("expected a 2-D x [rows, H] and " + ("a 3-D weight [G, H, 2F]" if grouped else
                                                                "a 2-D weight [H, 2F]"))
     rows, h = x.shape
-    groups = weight.shape[0] if grouped else 1
-    if weight.shape[-2] != h:
-        raise ValueError(f"contraction mismatch: x H={h}, weight H={weight.shape[-2]}")
-    if x.dtype not in (torch.float16, torch.bfloat16) or weight.dtype != x.dtype:
+    groups = shape[0] if grouped else 1
+    if shape[-2] != h:
+        raise ValueError(f"contraction mismatch: x H={h}, weight H={shape[-2]}")
+    dtype, device = x.dtype, x.device
+    if (dtype is not torch.float16 and dtype is not torch.bfloat16) or weight.dtype is not dtype:
         raise ValueError("x and weight must both be fp16 or bf16")
-    if groups <= 0 or h <= 0 or h % 8 or weight.shape[-1] <= 0 or weight.shape[-1] % 16:
-        raise ValueError(f"H and F must be positive multiples of 8 (H={h}, packed width {weight.shape[-1]})")
-    tensors = (x, weight) + ((offs,) if grouped else ())
-    if len({t.device for t in tensors}) != 1 or x.device.type != "cuda":
+    if groups <= 0 or h <= 0 or h % 8 or shape[-1] <= 0 or shape[-1] % 16:
+        raise ValueError(f"H and F must be positive multiples of 8 (H={h}, packed width {shape[-1]})")
+    if not x.is_cuda or weight.device != device or (grouped and offs.device != device):
         raise ValueError("x, weight and offs must be on the same GPU device")
     if grouped:
-        if offs.ndim != 1 or offs.dtype != torch.int32 or offs.shape[0] != groups:
+        if offs.ndim != 1 or offs.dtype is not torch.int32 or offs.shape[0] != groups:
             raise ValueError(f"offs must be an int32 vector with one entry per group ({groups})")
         if not offs.is_contiguous():
             raise ValueError("offs must be contiguous (pass offs.contiguous())")
     for name, t in (("x", x), ("weight", weight)):
         if not _rows_ok(t):
             raise ValueError(f"{name} needs a unit inner stride and rows at multiples of 16 bytes")
-    return int(rows), int(h), weight.shape[-1] // 2, int(groups)
+    return rows, h, shape[-1] // 2, groups
 
 
 def _pitch(tensor) -> int:
@@ -60,10 +61,6 @@ def _pitch(tensor) -> int:
 
 def _group_stride(weight) -> int:
     return weight.stride(0) if weight.ndim == 3 and weight.shape[0] > 1 else 0
-
-
-def _offs(offs):
-    return None if offs is None else offs.data_ptr()
 
 
 def gate_up_swiglu_forward(x, weight, offs=None, *, variant: int | None = None):
@@ -76,15 +73,14 @@ def gate_up_swiglu_forward(x, weight, offs=None, *, variant: int | None = None):
     import torch
 
     rows, h, f, groups = _validate(x, weight, offs)
-    _require_runtime(x)
-    out = torch.empty((rows, f), dtype=x.dtype, device=x.device)
-    saved = torch.empty((rows, 2 * f), dtype=torch.float32, device=x.device)
+    lib, device = _native.library(), x.device
+    out = x.new_empty((rows, f))
+    saved = x.new_empty((rows, 2 * f), dtype=torch.float32)
     if rows:
-        status = _native.library().moegemm_gate_up_forward(
-            x.data_ptr(), weight.data_ptr(), out.data_ptr(), saved.data_ptr(), _offs(offs), groups, rows, h, f, _pitch(x),
-            _group_stride(weight), _pitch(weight), f, _native.dtype_code(x.dtype), -1 if variant is None else variant,
-            _cu_count(x.device), _native.current_stream_handle(x.device))
-        _native.check(status)
+        _native.check(lib.moegemm_gate_up_forward(
+            x.data_ptr(), weight.data_ptr(), out.data_ptr(), saved.data_ptr(), None if offs is None else offs.data_ptr(),
+            groups, rows, h, f, _pitch(x), _group_stride(weight), _pitch(weight), f, _native.dtype_code(x.dtype),
+            -1 if variant is None else variant, _cu_count(device), _native.current_stream_handle(device)))
     return out, saved
 
 
@@ -98,29 +94,24 @@ def gate_up_swiglu_backward(dh, x, weight, offs, saved, *, need_dx: bool = True,
     import torch
 
     rows, h, f, groups = _validate(x, weight, offs)
-    if tuple(dh.shape) != (rows, f) or dh.dtype != x.dtype or dh.device != x.device:
-        raise ValueError(f"dh must be a [{rows}, {f}] {x.dtype} matrix on x's device")
-    if (tuple(saved.shape) != (rows, 2 * f) or saved.dtype != torch.float32 or saved.device != x.device
+    dtype, device = x.dtype, x.device
+    if dh.shape != (rows, f) or dh.dtype is not dtype or dh.device != device:
+        raise ValueError(f"dh must be a [{rows}, {f}] {dtype} matrix on x's device")
+    if (saved.shape != (rows, 2 * f) or saved.dtype is not torch.float32 or saved.device != device
             or not saved.is_contiguous()):
         raise ValueError(f"saved must be the contiguous [{rows}, {2 * f}] float32 tensor of the forward pass")
     if not _rows_ok(dh):
         dh = dh.contiguous()  # autograd hands out expanded and transposed gradients
-    _require_runtime(x)
-    code, cus = _native.dtype_code(x.dtype), _cu_count(x.device)
-    lib, stream = _native.library(), _native.current_stream_handle(x.device)
+    lib = _native.library()
     dx_variant, dw_variant = variants or (-1, -1)
-    dp = torch.empty((rows, 2 * f), dtype=x.dtype, device=x.device)
-    _native.check(lib.moegemm_gate_up_gradient(dh.data_ptr(), saved.data_ptr(), dp.data_ptr(), _offs(offs), groups, rows,
-                                               f, _pitch(dh), code, cus, stream))
-    dx = dw = None
-    if need_dx:
-        dx = torch.empty((rows, h), dtype=x.dtype, device=x.device)
-        _native.check(lib.moegemm_gate_up_dx(dp.data_ptr(), weight.data_ptr(), dx.data_ptr(), _offs(offs), groups, rows, h,
-                                             f, _group_stride(weight), _pitch(weight), h, code, dx_variant, cus, stream))
-    if need_dw:
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
-        _native.check(lib.moegemm_gate_up_dw(x.data_ptr(), dp.data_ptr(), dw.data_ptr(), _offs(offs), groups, rows, h, f,
-                                             _pitch(x), h * 2 * f, 2 * f, code, dw_variant, cus, stream))
+    dp = x.new_empty((rows, 2 * f))
+    dx = x.new_empty((rows, h)) if need_dx else None
+    dw = x.new_empty(weight.shape) if need_dw else None
+    _native.check(lib.moegemm_gate_up_backward(
+        dh.data_ptr(), x.data_ptr(), weight.data_ptr(), saved.data_ptr(), dp.data_ptr(), dx.data_ptr() if need_dx else None,
+        dw.data_ptr() if need_dw else None, None if offs is None else offs.data_ptr(), groups, rows, h, f, _pitch(dh),
+        _pitch(x), _group_stride(weight), _pitch(weight), _native.dtype_code(dtype), dx_variant, dw_variant,
+        _cu_count(device), _native.current_stream_handle(device)))
     return dx, dw
 
 

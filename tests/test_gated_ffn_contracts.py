@@ -36,17 +36,13 @@ def _call(entry, **changes):
         return lib.moegemm_gate_up_forward(v["x"], v["w"], v["out"], v["saved"], v["offs"], v["groups"], v["rows"], v["h"],
                                            v["f"], v["sx"], v["swg"], v["swh"], v["so"], v["dtype"], v["variant"], 256,
                                            None)
-    if entry == "gradient":
-        return lib.moegemm_gate_up_gradient(v["dh"], v["saved"], v["dp"], v["offs"], v["groups"], v["rows"], v["f"],
-                                            v["sdh"], v["dtype"], 256, None)
-    if entry == "dx":
-        return lib.moegemm_gate_up_dx(v["dp"], v["w"], v["out"], v["offs"], v["groups"], v["rows"], v["h"], v["f"],
-                                      v["swg"], v["swh"], v["so"], v["dtype"], v["variant"], 256, None)
-    return lib.moegemm_gate_up_dw(v["x"], v["dp"], v["out"], v["offs"], v["groups"], v["rows"], v["h"], v["f"], v["sx"],
-                                  v["sog"], v["so"], v["dtype"], v["variant"], 256, None)
+    dx, dw = (v["out"] if entry in (name, "backward") else None for name in ("dx", "dw"))
+    return lib.moegemm_gate_up_backward(v["dh"], v["x"], v["w"], v["saved"], v["dp"], dx, dw, v["offs"], v["groups"], v["rows"],
+                                        v["h"], v["f"], v["sdh"], v["sx"], v["swg"], v["swh"], v["dtype"], v["variant"],
+                                        v["variant"], 256, None)
 
 
-ENTRIES = ("forward", "gradient", "dx", "dw")
+ENTRIES = ("forward", "backward", "dx", "dw")
 
 
 @pytest.mark.parametrize("entry", ENTRIES)
@@ -61,9 +57,9 @@ def test_c_entries_refuse_bad_shapes(entry, changes, match):
 @pytest.mark.parametrize("entry,changes", [
     ("forward", dict(x=None)), ("forward", dict(x=4104)), ("forward", dict(sx=20)), ("forward", dict(sx=8)),
     ("forward", dict(swh=24)), ("forward", dict(so=8)), ("forward", dict(saved=4100)), ("forward", dict(swg=516)),
-    ("forward", dict(sx=1 << 22)), ("gradient", dict(dh=None)), ("gradient", dict(sdh=12)), ("gradient", dict(dp=4104)),
-    ("dx", dict(w=None)), ("dx", dict(so=20)), ("dx", dict(swg=4)), ("dw", dict(out=4104)), ("dw", dict(so=24)),
-    ("dw", dict(sog=4)), ("dw", dict(x=None)),
+    ("forward", dict(sx=1 << 22)), ("backward", dict(dh=None)), ("backward", dict(sdh=12)), ("backward", dict(dp=4104)),
+    ("backward", dict(saved=None)), ("dx", dict(w=None)), ("dx", dict(out=4104)), ("dx", dict(swg=4)),
+    ("dx", dict(swh=24)), ("dw", dict(out=4104)), ("dw", dict(x=None)), ("dw", dict(sx=12)),
 ])
 def test_c_entries_refuse_bad_operands(entry, changes):
     assert _call(entry, **changes) == _native.ERR_INVALID
@@ -76,5 +72,5 @@ def test_unknown_variants_and_empty_calls():
         assert count >= 3
         assert _call(entry, variant=count) == _native.ERR_NO_KERNEL
     assert _native.library().moegemm_gate_up_variant_count(3) == _native.ERR_INVALID
-    for entry in ("forward", "gradient", "dx"):
+    for entry in ("forward", "dx"):
         assert _call(entry, rows=0) == _native.OK
