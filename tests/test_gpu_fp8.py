@@ -363,7 +363,7 @@ def test_offsets_past_32_bits():
 
 
 def test_more_groups_than_a_launch_lists():
-    """Over 1024 groups: several launches; groups of 0 to 2 rows, checked row by row."""
+    """Over 768 groups: several launches; groups of 0 to 2 rows, checked row by row."""
     from kernels import grouped_mm_fp8
 
     counts = [(i * 7) % 3 for i in range(1100)]

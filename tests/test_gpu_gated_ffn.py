@@ -249,7 +249,7 @@ def test_rows_past_two_gib_of_one_expert():
 
 
 def test_more_groups_than_a_launch_lists():
-    """Over 1024 experts: several launches; checked per group against the first launches' neighbours."""
+    """Over 768 experts: several launches; the groups around each launch's ends are checked."""
     from kernels import _native, gate_up_swiglu_backward, gate_up_swiglu_forward
 
     lib = _native.library()
@@ -261,7 +261,7 @@ def test_more_groups_than_a_launch_lists():
         out, saved = gate_up_swiglu_forward(x, w, offs, variant=variant)
         back = min(variant or 0, lib.moegemm_gate_up_variant_count(2) - 1)
         dx, dw = gate_up_swiglu_backward(dh, x, w, offs, saved, variants=None if variant is None else (variant, back))
-        for e in [*range(0, 12), *range(1018, 1032), *range(1090, 1100)]:
+        for e in [*range(0, 12), *range(760, 776), *range(1090, 1100)]:
             part = slice(starts[e] - counts[e], starts[e])
             if counts[e]:
                 check_group(x[part], w[e], dh[part], out[part], saved[part], dx[part], dw[e])
