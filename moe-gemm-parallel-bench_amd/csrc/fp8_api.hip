@@ -62,13 +62,13 @@ int check_scales(int64_t stride_sam, int64_t stride_ssn, int32_t n) {
 //
 // Up to about 32 rows a group (20 with fast sums, whose tiles are faster) a call is bound by reading the weights, and
 // the stream kernels read them once where a group's rows fit their 16 or 32; routed groups are taken to hold up to
-// 1.6 times the mean.  32 experts of [4096, 7168], us: 8 rows each stream 145, tile 240; 32 rows stream 166, exact
-// tile 243; 64 rows stream 315, exact tile 243, fast tile 195.
+// 1.6 times the mean.  32 experts of [4096, 7168], us: 8 rows each stream 142, tile 194; 32 rows stream 155, exact
+// tile 196; 64 rows stream 314, exact tile 209, fast tile 198.
 // Among stream kernels: units run in rounds of one per CU, at a cost of their weights and about 200 rows of one
-// block for the join and the stores.  [7168, 2048] x 32: 256 columns 89, 128 columns 79 (7 whole rounds), 64
-// columns 92; one group of [4096, 7168]: 256 columns 52, 16 columns 14.4.
-// Among tiles: rounds by the time of a slice, in units of 10 ns (1000 rows of [4096, 4096]: 256x256 51 us, 128x256 35,
-// 128x128 31; 16384 rows of 32 x [4096, 7168]: 473, 597, 843).
+// block for the join and the stores.  [7168, 2048] x 32: 256 columns 86, 128 columns 80 (7 whole rounds), 64
+// columns 102; one group of [4096, 7168]: 256 columns 55, 16 columns 12.8.
+// Among tiles: rounds by the time of a slice, in units of 10 ns (1000 rows of [4096, 4096]: 256x256 50 us, 128x256 35,
+// 128x128 31; 16384 rows of 32 x [4096, 7168]: 515, 621, 840; exact 128x256 57 and 868, 128x128 47 and 1069).
 int choose(const Fp8Variant* table, int count, int64_t rows, int64_t groups, int64_t cols, int64_t k, int gated,
            int fast, int cus) {
   const int64_t active = std::min(groups, rows), mean = cdiv(rows, active);
