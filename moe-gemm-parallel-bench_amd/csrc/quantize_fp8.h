@@ -24,7 +24,12 @@ struct QuantizeParams {
 constexpr int kQuantRows = 16;   // rows and blocks of columns of a workgroup in the 1 x 128 kernel
 constexpr int kQuantBlocks = 4;
 
-// Elements [col, col + 8) of a row, zeros past k.  VEC: the row is 16-byte aligned and k a multiple of 8.
+// fp32 rows in vectors: a lane's 8 elements are two runs of 4, half a block apart, so that each load of 16 lanes covers
+// 256 bytes in a row; with 8 elements in a row it covers every other 16 bytes of 512 (8 x [5760, 2880]: 127 us, not 108).
+__device__ __forceinline__ int first_run(int col) { return (col & ~(kScaleBlock - 1)) + ((col & (kScaleBlock - 1)) >> 1); }
+
+// Elements [col, col + 8) of a row (fp32 in vectors: first_run(col) and 64 further on, 4 each), zeros past k.  VEC: the row
+// is 16-byte aligned and k a multiple of 8.
 template <class E, bool VEC>
 __device__ __forceinline__ void load8(const typename E::raw* row, int col, int k, float (&v)[8]) {
   using raw = typename E::raw;
@@ -32,9 +37,12 @@ __device__ __forceinline__ void load8(const typename E::raw* row, int col, int k
   if constexpr (VEC) {
     constexpr int N = sizeof(raw) * 8 / 16;
     u32x4_t c[N] = {};
-    if (col < k) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) c[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + col) + i);
+    if constexpr (N == 1) {
+      if (col < k) c[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + col));
+    } else {
+      const int first = first_run(col);
+      if (first < k) c[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + first));
+      if (first + 64 < k) c[1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + first + 64));
     }
     __builtin_memcpy(r, c, sizeof(r));
   } else {
@@ -49,10 +57,9 @@ __device__ __forceinline__ void load8(const typename E::raw* row, int col, int k
   }
 }
 
-// The 8 values scaled and converted; whole 8-byte stores where the row allows.
-template <bool VEC>
+// The 8 values of load8 scaled and converted; vector stores where the row allows.
+template <class E, bool VEC>
 __device__ __forceinline__ void store8(uint8_t* row, int col, int k, const float (&v)[8], float inverse) {
-  if (col >= k) return;
   f32x4_t lo, hi;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -60,7 +67,13 @@ __device__ __forceinline__ void store8(uint8_t* row, int col, int k, const float
     hi[i] = v[i + 4] * inverse;
   }
   const int32_t a = pack_e4m3(lo), b = pack_e4m3(hi);
-  if (VEC || col + 8 <= k) {
+  if constexpr (VEC && E::is_f32) {
+    const int first = first_run(col);
+    if (first < k) *reinterpret_cast<int32_t*>(row + first) = a;
+    if (first + 64 < k) *reinterpret_cast<int32_t*>(row + first + 64) = b;
+  } else if (col >= k) {
+    return;
+  } else if (VEC || col + 8 <= k) {
     *reinterpret_cast<u32x2_t*>(row + col) = u32x2_t{(uint32_t)a, (uint32_t)b};
   } else {
     for (int i = 0; i < k - col; ++i) row[col + i] = (uint8_t)((i < 4 ? a >> (8 * i) : b >> (8 * (i - 4))) & 0xff);
@@ -99,7 +112,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeParams p) {
     for (int d = 1; d < 16; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
     const float amax = floored(top);
     if ((lane & 15) == 0) s_scale[blk][wave * PER + i] = amax / kE4m3Max;
-    if (row < p.rows) store8<VEC>(q + (int64_t)row * p.sqr, col, p.k, v[i], kE4m3Max / amax);
+    if (row < p.rows) store8<E, VEC>(q + (int64_t)row * p.sqr, col, p.k, v[i], kE4m3Max / amax);
   }
   __syncthreads();
   // Scales leave block by block, 16 consecutive rows each.
@@ -137,7 +150,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(QuantizeParams p) 
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int row = tile_r * kScaleBlock + i * 16 + (threadIdx.x >> 4);
-    if (row < p.rows) store8<VEC>(q + (int64_t)row * p.sqr, col, p.k, v[i], inverse);
+    if (row < p.rows) store8<E, VEC>(q + (int64_t)row * p.sqr, col, p.k, v[i], inverse);
   }
   if (threadIdx.x == 0)
     p.scale[(int64_t)batch * p.ssb + (int64_t)tile_r * p.ssr + (int64_t)tile_c * p.ssk] = amax / kE4m3Max;
