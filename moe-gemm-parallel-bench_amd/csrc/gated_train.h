@@ -276,11 +276,13 @@ __device__ __forceinline__ void chained_tile(const ProblemDesc& pd, int m0, int 
   for (; kt < kt_count; ++kt) step(kt, either{}, std::true_type{});
   if (chain) {
     const int last = (kt_count - 1 + rot) & (STAGES - 1);
+    // The first group waits out the second's last products, so that both groups' epilogues run side by side (dW of 512
+    // rows an expert 1 % faster than with one after the other).
+    if constexpr (!SECOND) phase_barrier();
     finish.chained(acc, pd, m0, n0, wave_m, wave_n, last);
     typename T::Dma dn;
     T::setup_dma(dn, next, m1, n1, smem);
     T::template issue_stage<0>(dn, last, (STAGES - 1) * BK);
-    if constexpr (!SECOND) phase_barrier();
     ch.rot = (kt_count + rot) & (STAGES - 1);
     ch.prefetched = true;
   } else {
