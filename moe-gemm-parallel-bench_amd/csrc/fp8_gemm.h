@@ -545,7 +545,8 @@ struct Fp8Tile {
     if (ES == 2 && p.n % 8 == 0 && p.ldo % 8 == 0 && p.ldo < (1 << 22) && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0) {
       // Through LDS, 16 rows of the wave's 64 columns at a time (16-byte chunk c of row r at c ^ r), so that a store
       // covers whole 128-byte lines: from the registers, 32 bytes of a row at a time, 16384 rows of [7168, 2048] x 32
-      // took 269 us instead of 252.  One buffer resource ends with the tile's last valid row.
+      // took 269 us instead of 252.  Non-temporal, so that the operands keep the L2: 128x256 tiles 339 -> 324 us there, the
+      // others unchanged.  One buffer resource ends with the tile's last valid row.
       static_assert(WTN == 64, "a wave's 16-bit rows are 128 bytes");
       const uint32_t pitch = (uint32_t)p.ldo * ES;
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(
@@ -572,7 +573,7 @@ struct Fp8Tile {
             const int at = j * 8 + (lane >> 3), row = wave_m * WTM + fm * 32 + half * 16 + at;
             const u32x4_t x = *reinterpret_cast<const u32x4_t*>(slot + at * 128 + (((lane & 7) ^ (at & 7)) << 4));
             __builtin_amdgcn_raw_buffer_store_b128(
-                x, rs, col < valid_n ? (uint32_t)row * pitch + (uint32_t)col * ES : kOutOfRange, 0, 0);
+                x, rs, col < valid_n ? (uint32_t)row * pitch + (uint32_t)col * ES : kOutOfRange, 0, kNonTemporal);
           }
           compiler_fence();
         }
