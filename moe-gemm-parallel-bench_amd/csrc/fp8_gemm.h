@@ -71,6 +71,7 @@ __device__ __forceinline__ int group_rows(const int32_t* offs, int rows, int e, 
 
 struct GroupTile {
   int e, row0, m, tm, tn;
+  int part;  // first row in the tile (see build_tile_list)
 };
 
 __device__ __forceinline__ float uniform(float x) {
@@ -136,24 +137,28 @@ __device__ __forceinline__ void build_tile_table(TileTable& table, const int32_t
 // Each round is eight contiguous runs, one per XCD (workgroup b runs on XCD b mod 8), so that an XCD's L2 holds the rows
 // and weights its tiles share; the last round's tiles are dealt to all XCDs alike.  A grid that eight does not divide
 // takes every grid-th tile.
-constexpr int kListTiles = 256;
+constexpr int kListTiles = 192;
 struct TileList {
   GroupTile tile[kListTiles];  // e < 0: none
 };
 
-// Rounds from `round` on.  `order(tile, local)` places the group's local-th tile.  Every
-// thread of the workgroup calls it; ends with a barrier.
-template <class Order>
+// Rounds from `round` on.  `order(tile, local)` places the group's local-th tile.  Every thread of the workgroup calls
+// it; ends with a barrier.  SPLIT_BM: tiles of that many rows whose loop skips rows that are not there; where
+// the last round has tiles for at most half or a quarter of the workgroups, a tile's rows go to two or four of them
+// (`part`, and `m` as the end of the part's rows).
+template <int SPLIT_BM = 0, class Order>
 __device__ __forceinline__ void build_tile_list(TileList& list, const TileTable& table, int first, int groups, int round,
                                                 Order&& order) {
   if (threadIdx.x < kListTiles) {  // workgroups have as many threads or more
     const uint32_t grid = gridDim.x, b = blockIdx.x;
     const int64_t base = ((int64_t)round + threadIdx.x) * grid, left = table.tiles[groups - 1] - base;
-    const uint32_t count = (uint32_t)min((int64_t)grid, left), shift = grid & 7 ? 0 : 3, xcd = b & ((1u << shift) - 1);
+    const int64_t here = min((int64_t)grid, left);
+    const uint32_t log_parts = SPLIT_BM == 0 || here < 0 ? 0 : here * 4 <= grid ? 2 : here * 2 <= grid ? 1 : 0;
+    const uint32_t count = (uint32_t)here << log_parts, shift = grid & 7 ? 0 : 3, xcd = b & ((1u << shift) - 1);
     const uint32_t at = (xcd * count >> shift) + (b >> shift);
-    GroupTile tile{-1, 0, 0, 0, 0};
+    GroupTile tile{-1, 0, 0, 0, 0, 0};
     if (left > 0 && at < ((xcd + 1) * count >> shift)) {
-      const int t = (int)base + (int)at;
+      const int t = (int)base + (int)(at >> log_parts);
       int lo = 0, hi = groups - 1;  // the first group with tiles[i] > t
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -161,8 +166,14 @@ __device__ __forceinline__ void build_tile_list(TileList& list, const TileTable&
         else lo = mid + 1;
       }
       const int row0 = lo ? table.ends[lo - 1] : table.start;
-      tile = GroupTile{first + lo, row0, table.ends[lo] - row0, 0, 0};  // a group with tiles has rows
+      tile = GroupTile{first + lo, row0, table.ends[lo] - row0, 0, 0, 0};  // a group with tiles has rows
       order(tile, t - (lo ? table.tiles[lo - 1] : 0));
+      if (log_parts) {
+        const int rows = SPLIT_BM >> log_parts;
+        tile.part = (int)(at & ((1u << log_parts) - 1)) * rows;
+        tile.m = min(tile.m, tile.tm * SPLIT_BM + tile.part + rows);
+        if (tile.m <= tile.tm * SPLIT_BM + tile.part) tile.e = -1;  // the last round: nothing follows
+      }
     }
     list.tile[threadIdx.x] = tile;
   }
@@ -173,7 +184,7 @@ __device__ __forceinline__ void build_tile_list(TileList& list, const TileTable&
 __device__ __forceinline__ bool listed_tile(const TileList& list, int i, GroupTile& g) {
   if (i >= kListTiles) return false;
   const GroupTile& x = list.tile[i];
-  g = {uniform(x.e), uniform(x.row0), uniform(x.m), uniform(x.tm), uniform(x.tn)};
+  g = {uniform(x.e), uniform(x.row0), uniform(x.m), uniform(x.tm), uniform(x.tn), uniform(x.part)};
   return g.e >= 0;
 }
 

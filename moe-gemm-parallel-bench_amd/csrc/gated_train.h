@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
       }
     }
     make_uniform(pd);
-    m0 = g.tm * T::BM;
+    m0 = g.tm * T::BM + g.part;
     n0 = g.tn * T::BN;
     return true;
   };
@@ -493,7 +493,10 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
     else return StorePlain<T>{smem};
   };
 
-  build_tile_list(list, table, p.first, p.groups, p.round, [&](GroupTile& tile, int local) {
+  // A short last round in parts: 4096 rows of 8 experts, H 4096, F 1536, dX 152 us whole, 142 in parts; 4001 of 16, H and
+  // F 2880, 299 and 276; forward of 16384 uneven rows, 7168 -> 2x2048 (an eighth of a round left), 994 and 987.
+  build_tile_list<PING_PONG && PRODUCT != GATED_DW ? T::BM : 0>(list, table, p.first, p.groups, p.round,
+                                                                [&](GroupTile& tile, int local) {
     group_m_order(local, PRODUCT == GATED_DW ? m_tiles : (tile.m + T::BM - 1) / T::BM, n_tiles, 8, tile.tm, tile.tn);
   });
   ProblemDesc pd;

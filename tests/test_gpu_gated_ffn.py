@@ -270,7 +270,7 @@ def test_more_groups_than_a_launch_lists():
 
 
 def test_more_rounds_than_a_launch_lists(monkeypatch):
-    """More than 256 tiles on one workgroup: the launches after the first start where it ended."""
+    """More than 192 tiles on one workgroup: the launches after the first start where it ended."""
     from kernels import _native, gated_ffn
 
     lib = _native.library()
