@@ -15,6 +15,10 @@ namespace {
 
 constexpr int64_t kPitchLimit = int64_t(1) << 23;  // 256 rows of a panel under 2 GiB
 
+// Workgroups of 256 threads that one launch takes: it counts threads in 32 bits and drops what is past them without
+// an error (2^28 + 37 rows of 16 columns wrote nothing in one launch).
+constexpr int64_t kLaunchTiles = (int64_t(1) << 24) - 1;
+
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
@@ -153,16 +157,23 @@ int moegemm_quantize_fp8(const void* x, void* q, float* scale, int32_t batch, in
                    stride_sb, stride_sr, stride_sk, rows, k, 0};
   const int64_t blocks = cdiv(k, kScaleBlock);
   const int64_t col_tiles = block_rows == 1 ? cdiv(blocks, kQuantBlocks) : blocks;
-  const int64_t tiles = cdiv(rows, block_rows == 1 ? kQuantRows : kScaleBlock) * col_tiles;
-  if (tiles > INT32_MAX) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
+  if (col_tiles > kLaunchTiles) return report(MOEGEMM_ERR_INVALID, "k must be at most 2^31 - 128 (got %d)", k);
   p.col_tiles = (int32_t)col_tiles;
   const bool vec = k % 8 == 0 && aligned(x, 16) && stride_xr * es % 16 == 0 && stride_xb * es % 16 == 0;
-  const dim3 grid((unsigned)tiles, (unsigned)batch);
   const auto s = reinterpret_cast<hipStream_t>(stream);
-  const hipError_t err = dtype == DT_F32    ? launch_quantize<EF32>(p, block_rows, vec, grid, s)
-                         : dtype == DT_BF16 ? launch_quantize<EBf16>(p, block_rows, vec, grid, s)
-                                            : launch_quantize<EF16>(p, block_rows, vec, grid, s);
-  if (err != hipSuccess) return report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  const int64_t tile_rows = block_rows == 1 ? kQuantRows : kScaleBlock;
+  const int64_t step = kLaunchTiles / col_tiles * tile_rows;  // rows of a launch
+  for (int64_t row = 0; row < rows; row += step) {
+    p.x = static_cast<const char*>(x) + row * stride_xr * es;
+    p.q = static_cast<uint8_t*>(q) + row * stride_qr;
+    p.scale = scale + row / block_rows * stride_sr;
+    p.rows = (int32_t)std::min(rows - row, step);
+    const dim3 grid((unsigned)(cdiv(p.rows, tile_rows) * col_tiles), (unsigned)batch);
+    const hipError_t err = dtype == DT_F32    ? launch_quantize<EF32>(p, block_rows, vec, grid, s)
+                           : dtype == DT_BF16 ? launch_quantize<EBf16>(p, block_rows, vec, grid, s)
+                                              : launch_quantize<EF16>(p, block_rows, vec, grid, s);
+    if (err != hipSuccess) return report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  }
   return MOEGEMM_OK;
 }
 

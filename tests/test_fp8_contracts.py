@@ -91,3 +91,9 @@ def test_quantize_entry_refuses_before_any_launch(changes, match):
     status = _native.library().moegemm_quantize_fp8(v["x"], v["q"], v["scale"], v["batch"], v["rows"], v["k"], 0, 128,
                                                     0, v["ldq"], 0, 1, 4, v["dtype"], v["block_rows"], None)
     assert status == _native.ERR_INVALID and match in _native.last_error()
+
+
+def test_quantize_entry_refuses_columns_past_one_launch():
+    status = _native.library().moegemm_quantize_fp8(4096, 4096, 4096, 1, 1, 2 ** 31 - 1, 0, 2 ** 31, 0, 2 ** 31, 0, 1, 1,
+                                                    _native.DTYPE_BF16, 128, None)
+    assert status == _native.ERR_INVALID and "2^31 - 128" in _native.last_error()

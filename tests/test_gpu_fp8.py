@@ -393,3 +393,21 @@ def test_more_rounds_than_a_launch_lists(monkeypatch):
         out = fp8.matmul_fp8(a, sa, w, sw, variant=variant)
         assert_product(out[:, -640:], a, sa, w[-640:], sw[-5:])
         torch.testing.assert_close(out.float(), wide.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
+
+
+def test_quantize_more_rows_than_one_launch_takes():
+    """2^28 rows and more are 2^24 workgroups of 256 threads: past the 2^32 threads of one launch."""
+    from kernels import quantize_fp8
+
+    rows, k = (1 << 28) + 37, 16
+    x = torch.zeros((rows, k), device="cuda", dtype=torch.bfloat16)  # 8.6 GB
+    middle = slice((1 << 27) - 5, (1 << 27) + 60)
+    for part in (middle, slice(rows - 50, rows)):
+        x[part] = normal(73, x[part].shape[0], k).to(torch.bfloat16)
+    out = torch.full((rows, k), 0x7f, device="cuda", dtype=torch.uint8).view(E4M3)
+    q, scale = quantize_fp8(x, out=out)
+    for part in (middle, slice(rows - 50, rows)):
+        expected = quantize_fp8(x[part].clone())
+        assert torch.equal(q[part].float(), expected[0].float()) and torch.equal(scale[part], expected[1])
+    for part in (slice(0, middle.start), slice(middle.stop, rows - 50)):
+        assert not q[part].view(torch.uint8).any() and bool((scale[part] == 2.0 ** -96 / 448).all())
