@@ -100,7 +100,7 @@ def gate_up_swiglu_backward(dh, x, weight, offs, saved, *, need_dx: bool = True,
     if (saved.shape != (rows, 2 * f) or saved.dtype is not torch.float32 or saved.device != device
             or not saved.is_contiguous()):
         raise ValueError(f"saved must be the contiguous [{rows}, {2 * f}] float32 tensor of the forward pass")
-    if not _rows_ok(dh):
+    if not _rows_ok(dh) or (rows > 1 and dh.stride(0) < f):
         dh = dh.contiguous()  # autograd hands out expanded and transposed gradients
     lib = _native.library()
     dx_variant, dw_variant = variants or (-1, -1)

@@ -289,3 +289,20 @@ def test_more_rounds_than_a_launch_lists(monkeypatch):
         print(f"gate_up dw one workgroup variant={variant}", flush=True)
         _, got = gated_ffn.gate_up_swiglu_backward(dh, x, w, offs, saved, need_dx=False, variants=(variant, variant))
         torch.testing.assert_close(got, dw, **close)
+
+
+def test_a_gradient_broadcast_over_rows():
+    """The gradient of h.sum(0) reaches the block with strides (0, 1): every row is the same one."""
+    from kernels import gate_up_swiglu, gate_up_swiglu_backward, gate_up_swiglu_forward
+
+    x, w, dh, offs = operands(17, (40, 0, 25), 64, 40, torch.bfloat16)
+    x1, w1 = x.clone().requires_grad_(), w.clone().requires_grad_()
+    v = dh[0].clone()
+    gate_up_swiglu(x1, w1, offs).sum(0).backward(v)
+    _, saved = gate_up_swiglu_forward(x, w, offs)
+    dx, dw = gate_up_swiglu_backward(v.repeat(65, 1), x, w, offs, saved)
+    assert torch.equal(x1.grad, dx) and torch.equal(w1.grad, dw)
+    overlapping = torch.as_strided(normal(18, 65 * 8 + 40).to(torch.bfloat16), (65, 40), (8, 1))
+    pair = gate_up_swiglu_backward(overlapping, x, w, offs, saved)
+    dense = gate_up_swiglu_backward(overlapping.clone(), x, w, offs, saved)
+    assert torch.equal(pair[0], dense[0]) and torch.equal(pair[1], dense[1])
