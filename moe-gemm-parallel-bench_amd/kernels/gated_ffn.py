@@ -101,7 +101,8 @@ def gate_up_swiglu_backward(dh, x, weight, offs, saved, *, need_dx: bool = True,
             or not saved.is_contiguous()):
         raise ValueError(f"saved must be the contiguous [{rows}, {2 * f}] float32 tensor of the forward pass")
     if not _rows_ok(dh) or (rows > 1 and dh.stride(0) < f):
-        dh = dh.contiguous()  # autograd hands out expanded and transposed gradients
+        # Autograd hands out expanded and transposed gradients, and dense views at any offset, which contiguous() returns.
+        dh = dh.clone(memory_format=torch.contiguous_format)
     lib = _native.library()
     dx_variant, dw_variant = variants or (-1, -1)
     dp = x.new_empty((rows, 2 * f))

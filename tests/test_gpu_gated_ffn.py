@@ -306,3 +306,16 @@ def test_a_gradient_broadcast_over_rows():
     pair = gate_up_swiglu_backward(overlapping, x, w, offs, saved)
     dense = gate_up_swiglu_backward(overlapping.clone(), x, w, offs, saved)
     assert torch.equal(pair[0], dense[0]) and torch.equal(pair[1], dense[1])
+
+
+def test_a_gradient_at_an_odd_offset():
+    """The gradient of a concatenation is a view of a larger buffer: dense, but not on a multiple of 16 bytes."""
+    from kernels import gate_up_swiglu, gate_up_swiglu_backward, gate_up_swiglu_forward
+
+    x, w, dh, offs = operands(19, (40, 0, 25), 64, 40, torch.float16)
+    x1, w1 = x.clone().requires_grad_(), w.clone().requires_grad_()
+    odd = torch.zeros(3, device="cuda", dtype=torch.float16)
+    torch.cat([odd, gate_up_swiglu(x1, w1, offs).flatten()]).backward(torch.cat([odd, dh.flatten()]))
+    _, saved = gate_up_swiglu_forward(x, w, offs)
+    dx, dw = gate_up_swiglu_backward(dh, x, w, offs, saved)
+    assert torch.equal(x1.grad, dx) and torch.equal(w1.grad, dw)
