@@ -93,26 +93,36 @@ def gate_up_swiglu_backward(dh, x, weight, offs, saved, *, need_dx: bool = True,
     """
     import torch
 
-    rows, h, f, groups = _validate(x, weight, offs)
-    dtype, device = x.dtype, x.device
-    if dh.shape != (rows, f) or dh.dtype is not dtype or dh.device != device:
-        raise ValueError(f"dh must be a [{rows}, {f}] {dtype} matrix on x's device")
-    if (saved.shape != (rows, 2 * f) or saved.dtype is not torch.float32 or saved.device != device
+    rows, h, f, _ = _validate(x, weight, offs)
+    if dh.shape != (rows, f) or dh.dtype is not x.dtype or dh.device != x.device:
+        raise ValueError(f"dh must be a [{rows}, {f}] {x.dtype} matrix on x's device")
+    if (saved.shape != (rows, 2 * f) or saved.dtype is not torch.float32 or saved.device != x.device
             or not saved.is_contiguous()):
         raise ValueError(f"saved must be the contiguous [{rows}, {2 * f}] float32 tensor of the forward pass")
+    return _gradients(dh, x if need_dw else None, weight if need_dx else None, offs, saved, h, weight.shape, variants,
+                      need_dx, need_dw)
+
+
+def _gradients(dh, x, weight, offs, saved, h: int, weight_shape, variants, need_dx: bool, need_dw: bool):
+    """(dx, dw) of checked operands; x is read for dw only, weight for dx only."""
+    import torch
+
+    rows, f = dh.shape
+    device = dh.device
     if not _rows_ok(dh) or (rows > 1 and dh.stride(0) < f):
         # Autograd hands out expanded and transposed gradients, and dense views at any offset, which contiguous() returns.
         dh = dh.clone(memory_format=torch.contiguous_format)
     lib = _native.library()
     dx_variant, dw_variant = variants or (-1, -1)
-    dp = x.new_empty((rows, 2 * f))
-    dx = x.new_empty((rows, h)) if need_dx else None
-    dw = x.new_empty(weight.shape) if need_dw else None
+    dp = dh.new_empty((rows, 2 * f))
+    dx = dh.new_empty((rows, h)) if need_dx else None
+    dw = dh.new_empty(weight_shape) if need_dw else None
     _native.check(lib.moegemm_gate_up_backward(
-        dh.data_ptr(), x.data_ptr(), weight.data_ptr(), saved.data_ptr(), dp.data_ptr(), dx.data_ptr() if need_dx else None,
-        dw.data_ptr() if need_dw else None, None if offs is None else offs.data_ptr(), groups, rows, h, f, _pitch(dh),
-        _pitch(x), _group_stride(weight), _pitch(weight), _native.dtype_code(dtype), dx_variant, dw_variant,
-        _cu_count(device), _native.current_stream_handle(device)))
+        dh.data_ptr(), x.data_ptr() if need_dw else None, weight.data_ptr() if need_dx else None, saved.data_ptr(),
+        dp.data_ptr(), dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None,
+        None if offs is None else offs.data_ptr(), 1 if offs is None else offs.shape[0], rows, h, f, _pitch(dh),
+        _pitch(x) if need_dw else 0, _group_stride(weight) if need_dx else 0, _pitch(weight) if need_dx else 0,
+        _native.dtype_code(dh.dtype), dx_variant, dw_variant, _cu_count(device), _native.current_stream_handle(device)))
     return dx, dw
 
 
@@ -134,17 +144,18 @@ def _function():
         @staticmethod
         def forward(ctx, x, weight, offs):
             h, saved = gate_up_swiglu_forward(x, weight, offs)
-            ctx.save_for_backward(x, weight, saved, *(() if offs is None else (offs,)))
+            need_dx, need_dw = ctx.needs_input_grad[:2]
+            # x is read for dW and the weight for dx: what is not kept may change before the backward pass.
+            ctx.save_for_backward(saved, x if need_dw else None, weight if need_dx else None, offs)
+            ctx.width, ctx.weight_shape = x.shape[1], weight.shape
             return h
 
         @staticmethod
         @torch.autograd.function.once_differentiable
         def backward(ctx, dh):
-            x, weight, saved, *offs = ctx.saved_tensors
-            need_dx, need_dw = ctx.needs_input_grad[:2]
-            dx, dw = gate_up_swiglu_backward(dh, x, weight, offs[0] if offs else None, saved, need_dx=need_dx,
-                                             need_dw=need_dw)
-            return dx, dw, None
+            saved, x, weight, offs = ctx.saved_tensors
+            return (*_gradients(dh, x, weight, offs, saved, ctx.width, ctx.weight_shape, None, *ctx.needs_input_grad[:2]),
+                    None)
 
     _FUNCTION.append(GateUpSwiglu)
     return GateUpSwiglu

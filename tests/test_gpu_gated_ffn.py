@@ -319,3 +319,24 @@ def test_a_gradient_at_an_odd_offset():
     _, saved = gate_up_swiglu_forward(x, w, offs)
     dx, dw = gate_up_swiglu_backward(dh, x, w, offs, saved)
     assert torch.equal(x1.grad, dx) and torch.equal(w1.grad, dw)
+
+
+def test_only_what_a_gradient_needs_is_kept():
+    """An operand that no wanted gradient reads may change, or be freed, before the backward pass."""
+    from kernels import gate_up_swiglu, gate_up_swiglu_backward, gate_up_swiglu_forward
+
+    x, w, dh, offs = operands(23, (40, 0, 25), 64, 40, torch.bfloat16)
+    _, saved = gate_up_swiglu_forward(x, w, offs)
+    dx, dw = gate_up_swiglu_backward(dh, x, w, offs, saved)
+    x1, w1 = x.clone().requires_grad_(), w.clone()
+    h = gate_up_swiglu(x1, w1, offs)
+    with torch.no_grad():
+        x1.zero_()  # dx is dP W^T
+    h.backward(dh)
+    assert torch.equal(x1.grad, dx) and w1.grad is None
+    x1, w1 = x.clone(), w.clone().requires_grad_()
+    h = gate_up_swiglu(x1, w1, offs)
+    with torch.no_grad():
+        w1.zero_()  # dW is x^T dP
+    h.backward(dh)
+    assert torch.equal(w1.grad, dw) and x1.grad is None
