@@ -381,7 +381,7 @@ int moegemm_grouped_mm_fp8_swiglu(const void* a, const float* scale_a, const voi
  * in the reference (it times the forward GEMMs only, README.md:55-57).  x is [rows, h], w [group_count, h, 2f] with
  * [gate | up] columns (the 3-D packed W13 of moegemm_grouped_mm_offs_swiglu), offs as there; offs NULL: one group of
  * all rows.  h and f are multiples of 8, all rows 16-byte aligned with unit inner strides.
- *   forward:  [g | u] = x w[e] in fp32 -> saved [rows, 2f]; silu(g) * u -> h_out [rows, f]
+ *   forward:  [g | u] = x w[e] in fp32 -> saved [rows, 2f] unless saved is NULL; silu(g) * u -> h_out [rows, f]
  *   backward: dp [rows, 2f] = [dh u s (1 + g (1 - s)) | dh g s], s = sigmoid(g), rounded to dtype (a workspace);
  *             dp w[e]^T -> dx [rows, h] unless dx is NULL;
  *             x[r0:r1]^T dp[r0:r1] -> dw [group_count, h, 2f] unless dw is NULL; zeros for a group without rows

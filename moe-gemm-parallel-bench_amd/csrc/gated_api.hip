@@ -136,7 +136,7 @@ int moegemm_gate_up_forward(const void* x, const void* w, void* h_out, float* sa
   if (rc == MOEGEMM_OK) rc = check_operand("x", x, stride_xm, h);
   if (rc == MOEGEMM_OK) rc = check_operand("w", w, stride_wh, 2 * (int64_t)f);
   if (rc == MOEGEMM_OK) rc = check_operand("h", h_out, stride_om, f);
-  if (rc == MOEGEMM_OK) rc = check_operand("saved", saved, 2 * (int64_t)f, 2 * (int64_t)f);
+  if (rc == MOEGEMM_OK && saved) rc = check_operand("saved", saved, 2 * (int64_t)f, 2 * (int64_t)f);
   if (rc != MOEGEMM_OK) return rc;
   if (stride_wg % 8 || (h + 1024) * stride_wh * 2 >= kTwoGiB)
     return report(MOEGEMM_ERR_INVALID, "a group's weight must start at a multiple of 16 bytes and span under 2 GiB");

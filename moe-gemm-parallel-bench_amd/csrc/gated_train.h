@@ -31,7 +31,7 @@ struct GatedParams {
   const void* x;      // [rows, h] (sx), or dP for dx
   const void* w;      // [groups, h, 2 f] (swg between groups, swh between rows)
   void* out;          // h [rows, f], dx [rows, h] or dW [groups, h, 2 f]
-  float* saved;       // [rows, 2 f] gate | up
+  float* saved;       // [rows, 2 f] gate | up, or null: not kept
   const void* dp;     // dW: dP [rows, 2 f]
   const int32_t* offs;
   int64_t sx, swg, swh, so, sog, sdp;  // element strides; so: row pitch of out, sog: dW's group stride
@@ -314,7 +314,7 @@ struct StoreGateUp {
   using E = typename T::Element;
   static constexpr int FRAGS = T::FM * (T::FN / 2);
   static constexpr int STORES = T::MI == 32 ? 10 * FRAGS : 3 * FRAGS;
-  float* saved;  // the group's first row
+  float* saved;  // the group's first row, or null
   int64_t f;
   char* smem;
 
@@ -330,10 +330,11 @@ struct StoreGateUp {
     const int rows = min(T::BM, pd.m - m0), cols = (int)f - n0 / 2;
     const uint32_t pitch = (uint32_t)pd.scm * 2u, pitch32 = (uint32_t)f * 8u;
     float* keep = saved + (int64_t)m0 * 2 * f + n0 / 2;
+    const int kept = (int)(saved ? kOutOfRange : 0);  // a resource of no bytes drops the stores, whose count stays
     const auto rh = __builtin_amdgcn_make_buffer_rsrc(pd.c + ((int64_t)m0 * pd.scm + n0 / 2) * 2, (short)0,
                                                       (int)kOutOfRange, (int)kBufferFlags);
-    const auto rg = __builtin_amdgcn_make_buffer_rsrc(keep, (short)0, (int)kOutOfRange, (int)kBufferFlags);
-    const auto ru = __builtin_amdgcn_make_buffer_rsrc(keep + f, (short)0, (int)kOutOfRange, (int)kBufferFlags);
+    const auto rg = __builtin_amdgcn_make_buffer_rsrc(keep, (short)0, kept, (int)kBufferFlags);
+    const auto ru = __builtin_amdgcn_make_buffer_rsrc(keep + f, (short)0, kept, (int)kBufferFlags);
 #pragma unroll
     for (int fm = 0; fm < T::FM; ++fm)
 #pragma unroll
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(T::NT) gated_product_kernel(GatedParams p) {
         pd.k = p.h;
         pd.sbk = p.swh; pd.sbn = 1;
         pd.swiglu = 1;
-        saved = p.saved + (int64_t)g.row0 * 2 * p.f;
+        saved = p.saved ? p.saved + (int64_t)g.row0 * 2 * p.f : nullptr;
       } else {
         pd.k = 2 * p.f;
         pd.sbk = 1; pd.sbn = p.swh;

@@ -70,17 +70,23 @@ def gate_up_swiglu_forward(x, weight, offs=None, *, variant: int | None = None):
     fp16 or bf16, H and F multiples of 8, rows at multiples of 16 bytes.  Rows at or past offs[-1] get h = 0; their
     saved values are unspecified.
     """
+    return _forward(x, weight, offs, variant, True)
+
+
+def _forward(x, weight, offs, variant, keep: bool):
+    """``gate_up_swiglu_forward``; without ``keep`` nothing but h is written (and None returned for the projections)."""
     import torch
 
     rows, h, f, groups = _validate(x, weight, offs)
     lib, device = _native.library(), x.device
     out = x.new_empty((rows, f))
-    saved = x.new_empty((rows, 2 * f), dtype=torch.float32)
+    saved = x.new_empty((rows, 2 * f), dtype=torch.float32) if keep else None
     if rows:
         _native.check(lib.moegemm_gate_up_forward(
-            x.data_ptr(), weight.data_ptr(), out.data_ptr(), saved.data_ptr(), None if offs is None else offs.data_ptr(),
-            groups, rows, h, f, _pitch(x), _group_stride(weight), _pitch(weight), f, _native.dtype_code(x.dtype),
-            -1 if variant is None else variant, _cu_count(device), _native.current_stream_handle(device)))
+            x.data_ptr(), weight.data_ptr(), out.data_ptr(), saved.data_ptr() if keep else None,
+            None if offs is None else offs.data_ptr(), groups, rows, h, f, _pitch(x), _group_stride(weight),
+            _pitch(weight), f, _native.dtype_code(x.dtype), -1 if variant is None else variant, _cu_count(device),
+            _native.current_stream_handle(device)))
     return out, saved
 
 
@@ -127,7 +133,14 @@ def _gradients(dh, x, weight, offs, saved, h: int, weight_shape, variants, need_
 
 
 def gate_up_swiglu(x, weight, offs=None):
-    """Differentiable h [rows, F] = silu(x @ W_gate) * (x @ W_up) per expert (``gate_up_swiglu_forward``'s operands)."""
+    """Differentiable h [rows, F] = silu(x @ W_gate) * (x @ W_up) per expert (``gate_up_swiglu_forward``'s operands).
+
+    The projections are kept only where a gradient is to come: grad mode is on and x or weight requires one.
+    """
+    import torch
+
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
+        return _forward(x, weight, offs, None, False)[0]
     return _function().apply(x, weight, offs)
 
 

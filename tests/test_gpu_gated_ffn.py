@@ -340,3 +340,29 @@ def test_only_what_a_gradient_needs_is_kept():
         w1.zero_()  # dW is x^T dP
     h.backward(dh)
     assert torch.equal(w1.grad, dw) and x1.grad is None
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_no_projections_are_kept_without_a_gradient(dtype):
+    """Without a gradient to come h is the same bits, and its rows are all that is allocated."""
+    from kernels import _native, gate_up_swiglu, gate_up_swiglu_forward
+
+    for counts, h, f in (((2,), 64, 72), ((300, 0, 129), 520, 320), ((1000, 600), 256, 1024)):
+        x, w, _, offs = operands(29, counts, h, f, dtype)
+        expected, _ = gate_up_swiglu_forward(x, w, offs)
+        w.requires_grad_()
+        for enabled, weight in ((False, w), (True, w.detach())):
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            torch.cuda.reset_peak_memory_stats()
+            with torch.set_grad_enabled(enabled):
+                out = gate_up_swiglu(x, weight, offs)
+            assert torch.cuda.max_memory_allocated() - before <= -(-out.numel() * 2 // 512) * 512
+            assert torch.equal(out, expected) and not out.requires_grad
+    lib = _native.library()
+    for variant in range(lib.moegemm_gate_up_variant_count(0)):  # the C entry keeps nothing where saved is null
+        out = torch.full_like(expected, float("nan"))
+        _native.check(lib.moegemm_gate_up_forward(
+            x.data_ptr(), w.data_ptr(), out.data_ptr(), None, offs.data_ptr(), 2, 1600, 256, 1024, 256, 256 * 2048, 2048,
+            1024, _native.dtype_code(dtype), variant, 256, _native.current_stream_handle(x.device)))
+        assert torch.equal(out, gate_up_swiglu_forward(x, w, offs, variant=variant)[0])
