@@ -34,6 +34,8 @@ _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 
+INT32_MAX = 2 ** 31 - 1  # ctypes passes a larger extent's low 32 bits without an error
+
 # Exported symbol -> (restype, argtypes).  tests/test_native_abi.py checks this against the header.
 SIGNATURES = {
     "moegemm_abi_version": (ctypes.c_int, []),

@@ -51,11 +51,13 @@ def quantize_fp8(x, *, block_rows: int = 1, out=None, scale=None):
         raise ValueError(f"block_rows must be 1 or {SCALE_BLOCK}, got {block_rows!r}")
     if x.ndim not in (2, 3):
         raise ValueError("quantize_fp8 expects a 2-D [rows, K] or a 3-D [G, rows, K] tensor")
+    rows, k = x.shape[-2:]
+    batch = x.shape[0] if x.ndim == 3 else 1
+    if rows | k | batch > _native.INT32_MAX:
+        raise ValueError(f"x's extents must be under 2**31 (got {tuple(x.shape)})")
     if x.device.type != "cuda":
         raise ValueError("x must be on a GPU device")
     code = _native.dtype_code(x.dtype)
-    rows, k = x.shape[-2:]
-    batch = x.shape[0] if x.ndim == 3 else 1
     if k <= 0:
         raise ValueError("quantize_fp8 needs a positive K")
     if x.stride(-1) != 1 and x.shape[-1] > 1:
@@ -106,6 +108,8 @@ def _validate(a, scale_a, weight, scale_w, offs):
         raise ValueError("a and weight must be float8_e4m3fn")
     if groups <= 0 or n <= 0 or k <= 0:
         raise ValueError("fp8 products need at least one group and positive K and N")
+    if rows | n | k | groups > _native.INT32_MAX:
+        raise ValueError(f"extents must be under 2**31 (rows={rows} N={n} K={k} groups={groups})")
     if scale_a.shape != (rows, _blocks(k)) or scale_a.dtype is not torch.float32:
         raise ValueError(f"scale_a must be a float32 [{rows}, {_blocks(k)}] tensor")
     expected = (groups, _blocks(n), _blocks(k)) if grouped else (_blocks(n), _blocks(k))

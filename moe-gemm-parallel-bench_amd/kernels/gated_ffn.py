@@ -41,6 +41,8 @@ def _validate(x, weight, offs):
         raise ValueError("x and weight must both be fp16 or bf16")
     if groups <= 0 or h <= 0 or h % 8 or shape[-1] <= 0 or shape[-1] % 16:
         raise ValueError(f"H and F must be positive multiples of 8 (H={h}, packed width {shape[-1]})")
+    if rows | h | shape[-1] | groups > _native.INT32_MAX:
+        raise ValueError(f"extents must be under 2**31 (rows={rows} H={h} packed width {shape[-1]} groups={groups})")
     if not x.is_cuda or weight.device != device or (grouped and offs.device != device):
         raise ValueError("x, weight and offs must be on the same GPU device")
     if grouped:

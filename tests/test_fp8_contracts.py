@@ -97,3 +97,26 @@ def test_quantize_entry_refuses_columns_past_one_launch():
     status = _native.library().moegemm_quantize_fp8(4096, 4096, 4096, 1, 1, 2 ** 31 - 1, 0, 2 ** 31, 0, 2 ** 31, 0, 1, 1,
                                                     _native.DTYPE_BF16, 128, None)
     assert status == _native.ERR_INVALID and "2^31 - 128" in _native.last_error()
+
+
+def _meta(shape, dtype=E4M3):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("shape", [(2 ** 32 + 5, 16), (2 ** 31, 16), (4, 2 ** 32 + 16), (2 ** 32 + 1, 4, 16)])
+def test_quantize_refuses_extents_past_32_bits(shape):
+    """The library takes 32-bit extents: 2^32 + 5 rows would arrive as 5, and the others stay unwritten."""
+    with pytest.raises(ValueError, match="2\\*\\*31"):
+        quantize_fp8(_meta(shape, torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows,n,k,groups", [(2 ** 32 + 5, 32, 16, 1), (2 ** 31, 32, 16, 1), (4, 2 ** 32 + 16, 16, 1),
+                                             (4, 32, 2 ** 32 + 16, 1), (4, 32, 16, 2 ** 32 + 1)])
+def test_products_refuse_extents_past_32_bits(rows, n, k, groups):
+    blocks, fp32 = -(-k // 128), torch.float32
+    a, sa = _meta((rows, k)), _meta((rows, blocks), fp32)
+    w, sw = _meta((groups, n, k)), _meta((groups, -(-n // 128), blocks), fp32)
+    offs = _meta((groups,), torch.int32)
+    for call in (grouped_mm_fp8, grouped_mm_fp8_swiglu):
+        with pytest.raises(ValueError, match="2\\*\\*31"):
+            call(a, sa, w, sw, offs)

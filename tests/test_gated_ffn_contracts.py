@@ -74,3 +74,12 @@ def test_unknown_variants_and_empty_calls():
     assert _native.library().moegemm_gate_up_variant_count(3) == _native.ERR_INVALID
     for entry in ("forward", "dx"):
         assert _call(entry, rows=0) == _native.OK
+
+
+@pytest.mark.parametrize("rows,h,width,groups", [(2 ** 32 + 8, 16, 32, 1), (2 ** 31, 16, 32, 1), (4, 2 ** 32 + 16, 32, 1),
+                                                 (4, 16, 2 ** 32 + 32, 1), (4, 16, 32, 2 ** 32 + 1)])
+def test_extents_past_32_bits_are_refused(rows, h, width, groups):
+    """The library takes 32-bit extents: 2^32 + 8 rows would arrive as 8, and the others stay unwritten."""
+    x, w = (torch.empty(shape, dtype=BF16, device="meta") for shape in ((rows, h), (groups, h, width)))
+    with pytest.raises(ValueError, match="2\\*\\*31"):
+        gate_up_swiglu_forward(x, w, torch.empty(groups, dtype=torch.int32, device="meta"))
