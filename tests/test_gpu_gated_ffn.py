@@ -366,3 +366,33 @@ def test_no_projections_are_kept_without_a_gradient(dtype):
             x.data_ptr(), w.data_ptr(), out.data_ptr(), None, offs.data_ptr(), 2, 1600, 256, 1024, 256, 256 * 2048, 2048,
             1024, _native.dtype_code(dtype), variant, 256, _native.current_stream_handle(x.device)))
         assert torch.equal(out, gate_up_swiglu_forward(x, w, offs, variant=variant)[0])
+
+
+def poison(*shapes_and_types):
+    """Blocks of NaN that the next allocations of the same sizes reuse: rows that stay unwritten show."""
+    blocks = [torch.full(shape, float("nan"), device="cuda", dtype=dtype) for shape, dtype in shapes_and_types]
+    del blocks
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cus", [1, 3, 8])
+def test_widest_tiles_chained_over_few_workgroups(cus, dtype, monkeypatch):
+    """Several 256x256 tiles a workgroup in all three products: dW's K is 5, 10, 4 and 2 slices of 32 rows, so that tiles
+    with a prefetched successor and ones too short for it alternate."""
+    from kernels import gated_ffn
+
+    counts, h, f = (130, 0, 300, 97, 64), 520, 320
+    x, w, dh, offs = operands(31, counts, h, f, dtype)
+    rows = sum(counts)
+    monkeypatch.setattr(gated_ffn, "_cu_count", lambda *_: cus)
+    for ends in (counts, (0, 64, 33, 0, 300)):
+        offs = torch.tensor(ends, device="cuda").cumsum(0).to(torch.int32)
+        end = sum(ends)
+        print(f"chained tiles cus={cus} counts={ends} {dtype}", flush=True)
+        poison(((rows, f), dtype), ((rows, 2 * f), torch.float32))
+        out, saved = gated_ffn.gate_up_swiglu_forward(x, w, offs, variant=0)
+        check(x, w, dh, ends, out, saved, None, None)
+        poison(((rows, 2 * f), dtype), ((rows, h), dtype), (w.shape, dtype))
+        dx, dw = gated_ffn.gate_up_swiglu_backward(dh, x, w, offs, saved, variants=(0, 0))
+        check(x, w, dh, ends, None, None, dx, dw)
+        assert not out[end:].any() and not dx[end:].any()
