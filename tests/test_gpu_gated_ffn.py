@@ -396,3 +396,22 @@ def test_widest_tiles_chained_over_few_workgroups(cus, dtype, monkeypatch):
         dx, dw = gated_ffn.gate_up_swiglu_backward(dh, x, w, offs, saved, variants=(0, 0))
         check(x, w, dh, ends, None, None, dx, dw)
         assert not out[end:].any() and not dx[end:].any()
+
+
+@pytest.mark.parametrize("cus,h,f", [(8, 256, 128), (5, 256, 128), (8, 64, 72), (8, 520, 200), (16, 256, 128)])
+def test_short_last_rounds_are_shared_by_rows(cus, h, f, monkeypatch):
+    """One full round of 256x256 tiles and 1 to 4 tiles more, whose rows go to two or four workgroups: tiles of every
+    kind of row count, one and several columns of tiles, behind chained tiles (H 256 and 520) and unchained ones (H 64)."""
+    from kernels import gated_ffn
+
+    monkeypatch.setattr(gated_ffn, "_cu_count", lambda *_: cus)
+    for last in ((1,), (63,), (64,), (65,), (129,), (256,), (129, 65), (1, 256), (63, 64, 129), (256, 1, 65), (193, 0, 128, 2, 250)):
+        counts = (256,) * cus + last
+        rows = sum(counts)
+        x, w, dh, offs = operands(37 + sum(last), counts, h, f, torch.bfloat16)
+        print(f"short last round cus={cus} h={h} f={f} last={last}", flush=True)
+        poison(((rows, f), x.dtype), ((rows, 2 * f), torch.float32))
+        out, saved = gated_ffn.gate_up_swiglu_forward(x, w, offs, variant=0)
+        poison(((rows, 2 * f), x.dtype), ((rows, h), x.dtype))
+        dx, _ = gated_ffn.gate_up_swiglu_backward(dh, x, w, offs, saved, need_dw=False, variants=(0, 0))
+        check(x, w, dh, counts, out, saved, dx, None)
