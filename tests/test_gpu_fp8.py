@@ -411,3 +411,68 @@ def test_quantize_more_rows_than_one_launch_takes():
         assert torch.equal(q[part].float(), expected[0].float()) and torch.equal(scale[part], expected[1])
     for part in (slice(0, middle.start), slice(middle.stop, rows - 50)):
         assert not q[part].view(torch.uint8).any() and bool((scale[part] == 2.0 ** -96 / 448).all())
+
+
+def test_more_rounds_than_a_launch_lists_with_fast_sums(monkeypatch):
+    """The fast tiles over 300 tiles and more on one workgroup."""
+    from kernels import fp8
+
+    a, sa, w, sw = operands(4, 130, 128 * 300, 32)
+    monkeypatch.setattr(fp8, "_cu_count", lambda *_: 1)
+    for variant in _variants(0, fast=1):
+        print(f"matmul_fp8 one workgroup, fast, variant={variant}", flush=True)
+        out = torch.full((130, 128 * 300), float("nan"), device="cuda", dtype=torch.bfloat16)
+        fp8.matmul_fp8(a, sa, w, sw, out=out, fast_accum=True, variant=variant)
+        assert_product(out, a, sa, w, sw, FAST)
+
+
+@pytest.mark.parametrize("cus", [1, 3])
+@pytest.mark.parametrize("n,k", [(520, 80), (520, 144), (264, 400), (1032, 640)])
+def test_several_tiles_a_workgroup(cus, n, k, monkeypatch):
+    """A workgroup's stream of slices runs on over tiles of other groups and columns, one to five slices each."""
+    from kernels import fp8
+
+    counts = (130, 0, 300, 1, 64)
+    rows = sum(counts)
+    offs = torch.tensor(counts, device="cuda").cumsum(0).to(torch.int32)
+    a, sa, w, sw = operands(61 + n + k, rows, n, k, len(counts))
+    monkeypatch.setattr(fp8, "_cu_count", lambda *_: cus)
+    for fast in (0, 1):
+        for variant in _variants(0, fast):
+            for dtype in (torch.bfloat16, torch.float32):
+                print(f"grouped_mm_fp8 cus={cus} n={n} k={k} fast={fast} variant={variant} {dtype}", flush=True)
+                out = torch.full((rows, n), float("nan"), device="cuda", dtype=dtype)
+                fp8.grouped_mm_fp8(a, sa, w, sw, offs, out=out, fast_accum=bool(fast), variant=variant)
+                first = 0
+                for e, count in enumerate(counts):
+                    part = slice(first, first + count)
+                    first += count
+                    if count:
+                        assert_product(out[part], a[part], sa[part], w[e], sw[e], fast * FAST)
+
+
+@pytest.mark.parametrize("cus", [1, 2])
+@pytest.mark.parametrize("f,k", [(200, 80), (264, 272), (392, 640)])
+def test_several_gated_tiles_a_workgroup(cus, f, k, monkeypatch):
+    """Gate and up rows, their scales and the row maxima change from tile to tile of one workgroup's stream."""
+    from kernels import fp8
+
+    counts = (40, 0, 150, 300, 1)
+    rows = sum(counts)
+    offs = torch.tensor(counts, device="cuda").cumsum(0).to(torch.int32)
+    a, sa, w, sw = operands(67 + f + k, rows, 2 * f, k, len(counts))
+    monkeypatch.setattr(fp8, "_cu_count", lambda *_: cus)
+    for fast, variant in (*((0, v) for v in _variants(1)), *((1, v) for v in _variants(1, 1))):
+        print(f"grouped_mm_fp8_swiglu cus={cus} f={f} k={k} fast={fast} variant={variant}", flush=True)
+        torch.full((rows, -(-f // 16) * 16), 0x7f, device="cuda", dtype=torch.uint8)  # NaN where nothing is written
+        torch.full((-(-f // 128), rows), float("nan"), device="cuda")
+        q, scale = fp8.grouped_mm_fp8_swiglu(a, sa, w, sw, offs, fast_accum=bool(fast), variant=variant)
+        first = 0
+        for e, count in enumerate(counts):
+            part = slice(first, first + count)
+            first += count
+            if not count:
+                continue
+            x, y = values(a[part], sa[part], 1), values(w[e], sw[e], 128)
+            p, size = x @ y.t(), ((k + 8) * 2.0 ** -23 + fast * FAST) * (x.abs() @ y.abs().t())
+            assert_quantised(q[part], scale[part], p[:, :f], p[:, f:], size[:, :f], size[:, f:])
