@@ -83,3 +83,8 @@ def test_extents_past_32_bits_are_refused(rows, h, width, groups):
     x, w = (torch.empty(shape, dtype=BF16, device="meta") for shape in ((rows, h), (groups, h, width)))
     with pytest.raises(ValueError, match="2\\*\\*31"):
         gate_up_swiglu_forward(x, w, torch.empty(groups, dtype=torch.int32, device="meta"))
+
+
+def test_forward_refuses_a_weight_that_spans_two_gib():
+    assert _call("forward", swh=1 << 21) == _native.ERR_INVALID
+    assert "2 GiB" in _native.last_error()

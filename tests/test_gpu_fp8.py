@@ -476,3 +476,25 @@ def test_several_gated_tiles_a_workgroup(cus, f, k, monkeypatch):
             x, y = values(a[part], sa[part], 1), values(w[e], sw[e], 128)
             p, size = x @ y.t(), ((k + 8) * 2.0 ** -23 + fast * FAST) * (x.abs() @ y.abs().t())
             assert_quantised(q[part], scale[part], p[:, :f], p[:, f:], size[:, :f], size[:, f:])
+
+
+def test_rows_far_apart_pass_32_bits():
+    """Rows of a and of the weight 8 MB apart: every kernel, streams too, past 4 GiB."""
+    from kernels import grouped_mm_fp8, grouped_mm_fp8_swiglu
+
+    rows, n, k, pitch = 600, 592, 256, (1 << 23) - 16
+    a, sa, w, sw = operands(71, rows, n, k, 1)
+    wide = torch.zeros((rows, pitch), dtype=torch.uint8, device="cuda").view(E4M3)  # 5.0 GB
+    far_a, far_w = wide[:, :k], wide[None, :n, 512:512 + k]
+    far_a.copy_(a), far_w.copy_(w)
+    offs = torch.tensor([rows], dtype=torch.int32, device="cuda")
+    for fast in (0, 1):
+        for variant in _variants(0, fast):
+            print(f"grouped_mm_fp8 rows 8 MB apart fast={fast} variant={variant}", flush=True)
+            out = grouped_mm_fp8(far_a, sa, far_w, sw, offs, fast_accum=bool(fast), variant=variant)
+            assert_product(out, a, sa, w[0], sw[0], fast * FAST)
+        for variant in _variants(1, fast):
+            print(f"grouped_mm_fp8_swiglu rows 8 MB apart fast={fast} variant={variant}", flush=True)
+            q, scale = grouped_mm_fp8_swiglu(far_a, sa, far_w, sw, offs, fast_accum=bool(fast), variant=variant)
+            near = grouped_mm_fp8_swiglu(a, sa, w, sw, offs, fast_accum=bool(fast), variant=variant)
+            assert torch.equal(q.float(), near[0].float()) and torch.equal(scale, near[1])

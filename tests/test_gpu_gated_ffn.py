@@ -415,3 +415,38 @@ def test_short_last_rounds_are_shared_by_rows(cus, h, f, monkeypatch):
         poison(((rows, 2 * f), x.dtype), ((rows, h), x.dtype))
         dx, _ = gated_ffn.gate_up_swiglu_backward(dh, x, w, offs, saved, need_dw=False, variants=(0, 0))
         check(x, w, dh, counts, out, saved, dx, None)
+
+
+def test_weights_past_32_bit_offsets():
+    """Experts whose weights and gradients start past 4 GiB."""
+    from kernels import gate_up_swiglu_backward, gate_up_swiglu_forward
+
+    groups, h, f = 5, 4096, 65536  # 1.07 GB an expert
+    x = normal(41, 7, h).to(torch.bfloat16)
+    w = torch.empty((groups, h, 2 * f), device="cuda", dtype=torch.bfloat16)
+    for e in range(groups):
+        w[e] = normal(42 + e, h, 2 * f) / h ** 0.5
+    dh = normal(47, 7, f).to(torch.bfloat16)
+    offs = torch.tensor([2, 2, 2, 2, 7], dtype=torch.int32, device="cuda")
+    out, saved = gate_up_swiglu_forward(x, w, offs)
+    dx, dw = gate_up_swiglu_backward(dh, x, w, offs, saved)
+    check_group(x[2:], w[4], dh[2:], out[2:], saved[2:], dx[2:], dw[4])
+    assert not dw[1:4].any()
+
+
+def test_rows_past_32_bit_offsets():
+    """Rows 8 MB apart: x and dh pass 4 GiB, and dW's K runs in segments of 128 rows."""
+    from kernels import _native, gate_up_swiglu_backward, gate_up_swiglu_forward
+
+    lib = _native.library()
+    pitch, counts, h, f = (1 << 22) - 8, (300, 0, 400), 72, 40
+    x, w, dh, offs = operands(53, counts, h, f, torch.bfloat16)
+    wide = torch.zeros((700, pitch), device="cuda", dtype=torch.bfloat16)  # 5.9 GB
+    far_x, far_dh = wide[:, :h], wide[:, 80:80 + f]
+    far_x.copy_(x), far_dh.copy_(dh)
+    for variant in range(lib.moegemm_gate_up_variant_count(0)):
+        print(f"rows 8 MB apart variant={variant}", flush=True)
+        out, saved = gate_up_swiglu_forward(far_x, w, offs, variant=variant)
+        back = min(variant, lib.moegemm_gate_up_variant_count(2) - 1)
+        dx, dw = gate_up_swiglu_backward(far_dh, far_x, w, offs, saved, variants=(variant, back))
+        check(x, w, dh, counts, out, saved, dx, dw)
