@@ -174,9 +174,12 @@ def run(args: argparse.Namespace, emit) -> None:
 
 
 def main(argv: list[str] | None = None) -> int:
+    from utils.benchmark import select_cuda_device
+
     args = build_parser().parse_args(argv)
     try:
         layer_sizes(args)
+        select_cuda_device(args.device)
     except (OSError, ValueError) as exc:
         print(f"expert_layer: {exc}")
         return 2

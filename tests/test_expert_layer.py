@@ -50,3 +50,9 @@ def test_all_parts_run_together(fast, capsys):
     assert len(losses) == 3 and losses[0] > losses[1] > losses[2] > 0
     distances = {line["part"]: line["distance"] for line in lines if "distance" in line}
     assert set(distances) == {"prefill", "decode"} and all(0 < d < 0.25 for d in distances.values())
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda:x", "gpu"])
+def test_a_bad_device_ends_with_status_2(device, capsys):
+    assert main(["--device", device]) == 2
+    assert "--device" in capsys.readouterr().out
