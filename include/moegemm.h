@@ -8,11 +8,13 @@
  *   - all matrix, table and stream arguments are plain device pointers / a hipStream_t as void*;
  *   - strides are in elements; dims tables are int32 (m, n, k) triples; pointer tables are int64
  *     device addresses, read by the kernel at run time (callers may rewrite them between calls);
- *   - a call performs exactly one kernel launch on `stream` (or none for an empty problem set),
+ *   - a call performs exactly one kernel launch on `stream` (or none for an empty problem set; the fp8 and Gate+Up
+ *     training entries say below where they launch again),
  *     never allocates, copies or synchronizes, and is therefore capturable in a HIP graph;
  *   - the return value is MOEGEMM_OK or a negative error code; moegemm_last_error() returns the
  *     message of the most recent failure on the calling thread;
- *   - every launching call takes `b_stream` (0 or 1) just before `stream`: 1 issues the LDS-DMA
+ *   - every launching call but the fp8 and Gate+Up training entries takes `b_stream` (0 or 1) just
+ *     before `stream`: 1 issues the LDS-DMA
  *     kernels' B copies as non-temporal loads (streamed, evicted first from the caches), 0 as
  *     ordinary loads.  It changes no result, only speed, and which is faster depends on the
  *     workload (it is a tuning choice, like the tile config; the general kernel ignores it).  It
@@ -333,7 +335,8 @@ int moegemm_matmul(const void* a, const void* b, void* c, int32_t m, int32_t n, 
  * q = e4m3(x * (448 / amax)), round to nearest even.  A block that holds a NaN or an infinity becomes NaN.
  * x is [batch, rows, k] (dtype; unit stride along k), q its bytes and scale
  * [batch, rows / block_rows, k / 128], rounded up, with the given strides (elements).  block_rows is
- * 1 or 128; q rows start at multiples of 8 bytes.
+ * 1 or 128; q rows start at multiples of 8 bytes.  One launch, and another for every further 2^24 workgroups (of 16 rows
+ * by 512 columns, or of a 128 x 128 block).
  */
 int moegemm_quantize_fp8(const void* x, void* q, float* scale, int32_t batch, int32_t rows, int32_t k,
                          int64_t stride_xb, int64_t stride_xr, int64_t stride_qb, int64_t stride_qr, int64_t stride_sb,
@@ -353,7 +356,8 @@ int moegemm_fp8_variant_fast(int32_t gated, int32_t variant);
  * bytes and pitches under 2^23.  Rows at or past offs[group_count-1] are not written.  fast_accum 1 lets the 8-bit matrix
  * instructions form the sums inside a block, which keep about 14 bits below the largest of eight products, at
  * twice the rate; 0 keeps them in fp32.  `variant` -1
- * lets the library choose by rows, groups and columns; grid_size is the persistent grid (CUs; <= 0: 256).
+ * lets the library choose by rows, groups and columns; grid_size is the persistent grid (CUs; <= 0: 256).  One launch, and
+ * another for every further 768 groups or 192 rounds of tiles.
  */
 int moegemm_grouped_mm_fp8(const void* a, const float* scale_a, const void* w, const float* scale_w, void* out,
                            const int32_t* offs, int32_t group_count, int32_t rows, int32_t n, int32_t k,
@@ -387,7 +391,8 @@ int moegemm_grouped_mm_fp8_swiglu(const void* a, const float* scale_a, const voi
  *             x[r0:r1]^T dp[r0:r1] -> dw [group_count, h, 2f] unless dw is NULL; zeros for a group without rows
  * Rows at or past offs[group_count-1] get h_out = 0 and dx = 0 (their saved and dp stay unwritten and unread).
  * saved, dp, dx and dw are contiguous.  `variant` -1 lets the library choose the tile (moegemm_gate_up_variant_count:
- * product 0 forward, 1 dx, 2 dw); grid_size as in moegemm_grouped_mm_fp8.  Sums are fp32 and of one order: repeated
+ * product 0 forward, 1 dx, 2 dw); grid_size and further launches as in moegemm_grouped_mm_fp8, one launch for dp.
+ * x and dh rows are less than 2^23 bytes apart, a group's w spans less than 2 GiB in the forward product.  Sums are fp32 and of one order: repeated
  * calls give the same bits.
  */
 int moegemm_gate_up_variant_count(int32_t product);

@@ -1,4 +1,5 @@
-// C ABI of the block-scaled fp8 operators: argument checks, the choice of a variant, one launch each.
+// C ABI of the block-scaled fp8 operators: argument checks, the choice of a variant, the launches: one a call, and
+// another for every further 2^24 workgroups (quantisation), 768 groups or 192 rounds of tiles (products on tiles).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -66,15 +67,17 @@ int check_scales(int64_t stride_sam, int64_t stride_ssn, int32_t n) {
 //
 // Up to about 32 rows a group (20 with fast sums, whose tiles are faster) a call is bound by reading the weights, and
 // the stream kernels read them once where a group's rows fit their 16 or 32; routed groups are taken to hold up to
-// 1.6 times the mean.  32 experts of [4096, 7168], us: 8 rows each stream 142, tile 194; 32 rows stream 155, exact
+// 1.6 times the mean (a group of more rows than a unit holds has its row tiles run one after another and reads its
+// weights again for each: 256 rows over 32 experts of [4096, 7168] 140 us even, 485 with half of them on one expert,
+// 791 with all).  32 experts of [4096, 7168], us: 8 rows each stream 142, tile 194; 32 rows stream 155, exact
 // tile 196; 64 rows stream 314, exact tile 209, fast tile 198.
 // Among stream kernels: units run in rounds of one per CU, at a cost of their weights and about 200 rows of one
 // block for the join and the stores.  [7168, 2048] x 32: 256 columns 86, 128 columns 80 (7 whole rounds), 64
 // columns 102; one group of [4096, 7168]: 256 columns 55, 16 columns 12.8.
 // Among tiles: rounds by the time of a slice, in units of 10 ns (1000 rows of [4096, 4096]: 256x256 50 us, 128x256 35,
 // 128x128 31; 16384 rows of 32 x [4096, 7168]: 515, 621, 840; exact 128x256 57 and 868, 128x128 47 and 1069).
-int choose(const Fp8Variant* table, int count, int64_t rows, int64_t groups, int64_t cols, int64_t k, int gated,
-           int fast, int cus) {
+int choose(const Fp8Variant* table, int count, int64_t rows, int64_t groups, int64_t cols, int64_t k, int fast,
+           int cus) {
   const int64_t active = std::min(groups, rows), mean = cdiv(rows, active);
   const int64_t high = active == 1 ? rows : cdiv(mean * 8, 5);
   const bool stream = active == 1 ? rows <= 32 : mean <= (fast ? 20 : 32);
@@ -91,7 +94,8 @@ int choose(const Fp8Variant* table, int count, int64_t rows, int64_t groups, int
       const int64_t padded = cdiv(blocks, v.waves_k) * v.waves_k;
       cost = cdiv(active * n_tiles, cus) * (v.block_n * padded + 200);
     } else {
-      const int64_t tiles = std::max(active, rows / v.block_m + active / 2 + (active == 1 && rows % v.block_m != 0)) * n_tiles;
+      const int64_t row_tiles = rows / v.block_m + active / 2 + (active == 1 && rows % v.block_m != 0);
+      const int64_t tiles = std::max(active, row_tiles) * n_tiles;
       const int slice = v.block_m == 256 ? 170 : v.block_n == 256 ? (v.fast ? 115 : 190) : (v.fast ? 90 : 115);
       cost = cdiv(tiles, cus) * slice;
     }
@@ -110,7 +114,8 @@ int launch_product(const Fp8Variant* table, int count, Fp8Params& p, int64_t out
     return report(MOEGEMM_ERR_NO_KERNEL, "fp8 variant %d is not compiled (0 to %d, or -1)", variant, count - 1);
   if (p.rows == 0) return MOEGEMM_OK;
   const int cus = grid_size > 0 ? grid_size : 256;
-  if (variant < 0) variant = choose(table, count, p.rows, p.groups, gated ? cdiv(out_cols, 128) * 256 : p.n, p.k, gated, fast, cus);
+  const int64_t cols = gated ? cdiv(out_cols, 128) * 256 : p.n;
+  if (variant < 0) variant = choose(table, count, p.rows, p.groups, cols, p.k, fast, cus);
   if (variant < 0) return report(MOEGEMM_ERR_NO_KERNEL, "no fp8 variant for this shape");
   const Fp8Variant& v = table[variant];
   const int64_t n_tiles = cdiv(p.n, v.block_n);  // gated: n = 2F weight rows in tiles of 128 + 128

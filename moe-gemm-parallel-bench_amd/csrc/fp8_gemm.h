@@ -26,7 +26,8 @@
 //  * Fp8Tile (prefill): operands reach LDS by DMA, one 128-byte K slice (= one scale block) per
 //    stage, 16-byte chunks XOR-swizzled, read with ds_read_b128;
 //  * Fp8Stream (decode, few rows a group): each wave streams weights through a ring of its own in LDS, every
-//    byte read once.  Exact sums only: HBM is the bound, and widening costs no time.
+//    byte read once where a group has no more rows than a unit (16 or 32), and once for each 16 or 32 rows
+//    of it otherwise.  Exact sums only: HBM is the bound, and widening costs no time.
 #pragma once
 
 #include "gemm_fast.h"
@@ -776,7 +777,8 @@ __global__ void __launch_bounds__(T::NT) fp8_tile_kernel(Fp8Params p) {
 }
 
 // Decode: 16 FM rows of a group by 16 FN weight rows per wave, WN waves along the columns, WK waves that take
-// the K blocks wk, wk + WK, ...  Bound by HBM: each weight byte is read once.
+// the K blocks wk, wk + WK, ...  Bound by HBM where a group's rows fit a unit: each weight byte is then read once.  A
+// group of more rows is walked by the same workgroups, 16 FM rows at a time, and its weights are read again each time.
 //
 // Every wave streams on its own: a ring of STAGES slots in LDS, one K block of its weights, rows and scales each,
 // filled by DMA in whole 128-byte lines and refilled as soon as its fragments are in registers.  No barrier

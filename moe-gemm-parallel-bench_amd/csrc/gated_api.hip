@@ -1,4 +1,5 @@
-// C ABI of the Gate+Up training form: argument checks, the choice of a tile, one launch each.
+// C ABI of the Gate+Up training form: argument checks, the choice of a tile, the launches: one a product (and one for
+// dP), another for every further 768 groups or 192 rounds of tiles.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -168,8 +169,10 @@ int moegemm_gate_up_backward(const void* dh, const void* x, const void* w, const
   const hipStream_t queue = reinterpret_cast<hipStream_t>(stream);
   const int cus = grid_size > 0 ? grid_size : 256;
   const GatedTable& table = table_of(dtype);
-  const GatedParams of_x{dp, w, dx, nullptr, nullptr, offs, width, stride_wg, stride_wh, h, 0, 0, group_count, rows, h, f, 0};
-  const GatedParams of_w{x, nullptr, dw, nullptr, dp, offs, stride_xm, 0, 0, width, h * width, width, group_count, rows, h, f,
+  const GatedParams of_x{dp, w, dx, nullptr, nullptr, offs, width, stride_wg, stride_wh, h, 0, 0,
+                         group_count, rows, h, f, 0};
+  const GatedParams of_w{x, nullptr, dw, nullptr, dp, offs, stride_xm, 0, 0, width, h * width, width,
+                         group_count, rows, h, f,
                          (rows + (int64_t)1024) * std::max<int64_t>(stride_xm, width) * 2 >= kTwoGiB};
   const bool want_dx = dx && rows > 0;
   Plan plan_x{}, plan_w{};

@@ -8,15 +8,17 @@
 // the two products of the backward pass.  [g | u] is kept in fp32: rounded to 16 bits it would put two more
 // roundings under every gradient, and recomputing it costs a third product (0.96 TFLOP, about 0.8 ms,
 // against 0.27 GB written and read for 32 experts, 16384 rows, H 7168, F 2048).  dP is rounded to the
-// operand type once, as the matrix cores take it.
+// operand type once, as the matrix cores take it: kept wider, as two 16-bit parts, it would double both products of
+// the backward pass.  The rounding takes dx and dW from 0.0017 to 0.0024 of their norm off the 64-bit gradients in
+// bf16, from 0.00021 to 0.00029 in fp16 (the lower figures are those of the outputs' own rounding).
 //
 // The products run on the LDS-DMA tiles (gemm_fast.h, gemm_pingpong.h): row-major operands forward,
 // K-contiguous weights (kBT) for dx, the M-contiguous view of x (kAT) for dW, whose K is the expert's
 // row count, read from the offsets on the device.  Rows are grouped as in MODE_OFFSETS; rows past the last
 // group get h = 0 and dx = 0, an expert without rows dW = 0.
 //
-// 32 experts, 16384 rows, H 7168, F 2048, bf16, each product 0.96 TFLOP: forward 0.90 to 1.00 ms (the fp32 pairs alone
-// 0.05), dX 0.90, dW 1.01, dP 0.079 (6.0 TB/s read and written).  The matrix instructions are busy half the time.  With
+// 32 experts, 16384 rows, H 7168, F 2048, bf16, each product 0.96 TFLOP: forward 0.90 to 1.07 ms by card (0.03 less where
+// the fp32 pairs are not kept), dX 0.90, dW 1.01, dP 0.079 (6.0 TB/s read and written).  The matrix instructions are busy half the time.  With
 // uneven experts a sixth to a fifth of the row tiles' rows is padding, and workgroups that share weights drift apart: the
 // forward pass fetches 4.0 GB where even experts fetch 2.3.  dW writes 1.9 GB, and each of its tiles (K is an
 // expert's 512 rows) takes 18 us of which 4 are its epilogue and the next tile's start.
@@ -377,8 +379,8 @@ struct StoreGateUp {
               const int row = j * 8 + (lane >> 3), c = lane & 7;
               const u32x4_t x = *reinterpret_cast<const u32x4_t*>(slot(row * 128 + ((c ^ (row & 7)) << 4)));
               const bool in = row0 + row < rows && n1 + c * 4 < cols;
-              __builtin_amdgcn_raw_buffer_store_b128(
-                  x, part ? ru : rg, in ? (uint32_t)(row0 + row) * pitch32 + (uint32_t)(n1 + c * 4) * 4u : kOutOfRange, 0, kNonTemporal);
+              const uint32_t at = (uint32_t)(row0 + row) * pitch32 + (uint32_t)(n1 + c * 4) * 4u;
+              __builtin_amdgcn_raw_buffer_store_b128(x, part ? ru : rg, in ? at : kOutOfRange, 0, kNonTemporal);
             }
             compiler_fence();
           }

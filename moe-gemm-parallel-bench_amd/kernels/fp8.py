@@ -11,8 +11,9 @@ A serving step of one expert layer::
     h, hs = grouped_mm_fp8_swiglu(q, s, w13, w13_scale, offs)       # silu(gate) * up, quantised again
     y = grouped_mm_fp8(h, hs, w2, w2_scale, offs)                   # [rows, H] bf16
 
-Each call is one kernel launch on the current stream, reads ``offs`` on the device and keeps nothing, so it can be
-captured in a HIP graph.  ``ValueError`` for operands a kernel cannot take, ``RuntimeError`` without library or GPU.
+Each call runs on the current stream, reads ``offs`` on the device and keeps nothing, so it can be captured in a HIP
+graph.  It is one kernel launch, and another for every further 2**24 workgroups of a quantisation, 768 groups or 192
+rounds of tiles of a product.  ``ValueError`` for operands a kernel cannot take, ``RuntimeError`` without library or GPU.
 """
 
 from __future__ import annotations
@@ -23,7 +24,6 @@ from . import _native
 from .matmul import _device_signature
 
 SCALE_BLOCK = 128
-_PITCH_LIMIT = 1 << 23  # bytes; 256 rows of a tile stay under 2 GiB
 
 
 def _blocks(extent: int) -> int:
@@ -143,8 +143,8 @@ def _operand_args(a, scale_a, weight, scale_w, k: int):
     grouped = weight.ndim == 3
     sa, sw = scale_a.stride(), scale_w.stride()
     return (a.shape[0], weight.shape[-2], k, _pitch(a, k), sa[0], sa[1],
-            weight.stride(0) if grouped and weight.shape[0] > 1 else 0, _pitch(weight, k), sw[0] if grouped else 0, sw[-2],
-            sw[-1])
+            weight.stride(0) if grouped and weight.shape[0] > 1 else 0, _pitch(weight, k), sw[0] if grouped else 0,
+            sw[-2], sw[-1])
 
 
 def _product(a, scale_a, weight, scale_w, offs, out, out_dtype, fast_accum, variant):
@@ -166,8 +166,8 @@ def _product(a, scale_a, weight, scale_w, offs, out, out_dtype, fast_accum, vari
     status = _native.library().moegemm_grouped_mm_fp8(
         a.data_ptr(), scale_a.data_ptr(), weight.data_ptr(), scale_w.data_ptr(), out.data_ptr(),
         offs.data_ptr() if offs is not None else None, groups, *_operand_args(a, scale_a, weight, scale_w, k),
-        out.stride(0) if rows > 1 else n, code, int(bool(fast_accum)), -1 if variant is None else variant, _cu_count(a.device),
-        _native.current_stream_handle(a.device))
+        out.stride(0) if rows > 1 else n, code, int(bool(fast_accum)), -1 if variant is None else variant,
+        _cu_count(a.device), _native.current_stream_handle(a.device))
     _native.check(status)
     return out
 
@@ -178,9 +178,11 @@ def matmul_fp8(a, scale_a, weight, scale_w, *, out=None, out_dtype=None, fast_ac
 
     a [M, K] and scale_a [M, ceil(K / 128)], weight [N, K] and scale_w [ceil(N / 128), ceil(K / 128)]; fp32 sums,
     output in ``out_dtype`` (bf16 by default; fp16 and fp32 too).  M, N and K are arbitrary; rows of a and weight
-    start at multiples of 16 bytes.  ``fast_accum=True`` lets the 8-bit matrix instructions sum inside a block of 128:
-    twice the rate where there are rows enough for it to matter (above 64 a group), with sums of eight products
-    that keep about 14 bits below the largest; by default every sum is fp32.  ``variant`` names a compiled kernel, None lets the library choose.
+    start at multiples of 16 bytes, less than 2**23 bytes apart.  By default every sum is fp32.  ``fast_accum=True`` lets
+    the 8-bit matrix instructions sum inside a block of 128, at twice the rate, with sums of eight products that keep
+    about 14 bits below the largest.  It takes effect above 32 rows of one weight and above a mean of 20 rows a group;
+    calls with fewer rows are bound by reading the weights and keep fp32 sums.  ``variant`` names a compiled kernel,
+    None lets the library choose.
     """
     return _product(a, scale_a, weight, scale_w, None, out, out_dtype, fast_accum, variant)
 
@@ -220,7 +222,7 @@ def grouped_mm_fp8_swiglu(a, scale_a, weight, scale_w, offs=None, *, fast_accum:
     status = _native.library().moegemm_grouped_mm_fp8_swiglu(
         a.data_ptr(), scale_a.data_ptr(), weight.data_ptr(), scale_w.data_ptr(), out.data_ptr(), scale.data_ptr(),
         offs.data_ptr() if offs is not None else None, groups, *_operand_args(a, scale_a, weight, scale_w, k),
-        pitch, scale.stride(0), scale.stride(1), int(bool(fast_accum)), -1 if variant is None else variant, _cu_count(a.device),
-        _native.current_stream_handle(a.device))
+        pitch, scale.stride(0), scale.stride(1), int(bool(fast_accum)), -1 if variant is None else variant,
+        _cu_count(a.device), _native.current_stream_handle(a.device))
     _native.check(status)
     return out, scale

@@ -2,7 +2,8 @@
 
 ``h = silu(x W_gate) * (x W_up)`` per expert, with W [G, H, 2F] = [gate | up] as ``grouped_mm_swiglu`` takes it.
 The forward pass is one launch that also keeps the projections [g | u] in fp32; the backward pass is three: the
-elementwise gradient of [g | u], then ``dx`` and ``dW``.  The reference times the forward GEMMs only (README.md:55-57).
+elementwise gradient of [g | u], then ``dx`` and ``dW`` (each product launches again for every further 768 groups or 192
+rounds of tiles).  The reference times the forward GEMMs only (README.md:55-57).
 
 ``gate_up_swiglu`` is the differentiable call; ``gate_up_swiglu_forward`` and ``gate_up_swiglu_backward`` are
 its two halves for programs that run their own backward pass.  Offsets are read on the device at run time, calls run
@@ -69,7 +70,8 @@ def gate_up_swiglu_forward(x, weight, offs=None, *, variant: int | None = None):
     """``(h, saved)``: h [rows, F] = silu(x @ W[:, :F]) * (x @ W[:, F:]) and the fp32 projections saved [rows, 2F].
 
     x is expert-sorted [rows, H]; weight [G, H, 2F] with int32 end rows ``offs`` [G] on the device, or [H, 2F] without.
-    fp16 or bf16, H and F multiples of 8, rows at multiples of 16 bytes.  Rows at or past offs[-1] get h = 0; their
+    fp16 or bf16, H and F multiples of 8, rows at multiples of 16 bytes, less than 2**23 bytes apart; a group's weight
+    spans less than 2 GiB.  Rows at or past offs[-1] get h = 0; their
     saved values are unspecified.
     """
     return _forward(x, weight, offs, variant, True)
