@@ -498,3 +498,86 @@ def test_rows_far_apart_pass_32_bits():
             q, scale = grouped_mm_fp8_swiglu(far_a, sa, far_w, sw, offs, fast_accum=bool(fast), variant=variant)
             near = grouped_mm_fp8_swiglu(a, sa, w, sw, offs, fast_accum=bool(fast), variant=variant)
             assert torch.equal(q.float(), near[0].float()) and torch.equal(scale, near[1])
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(37, 300), (3, 150, 264), (2, 1, 129)])
+def test_quantize_into_given_buffers(shape, dtype, block_rows):
+    """``out`` and ``scale`` of any layout get what a call without them returns, batches what each matrix alone gets, and
+    nothing is written beside them."""
+    from kernels import quantize_fp8
+
+    x = normal(81, *shape).to(dtype)
+    q, scale = quantize_fp8(x, block_rows=block_rows)
+    *batch, rows, k = shape
+    wide = torch.full((*batch, rows + 2, k // 8 * 8 + 40), 0x55, device="cuda", dtype=torch.uint8)
+    out = wide[..., 1:rows + 1, 16:16 + k].view(E4M3)
+    blocks = scale.shape[-2:]
+    for given in (torch.full((*batch, *blocks), -1.0, device="cuda"),
+                  torch.full((*batch, blocks[1], blocks[0] + 3), -1.0, device="cuda")[..., 2:2 + blocks[0]].transpose(-1, -2),
+                  torch.full((*batch, 2 * blocks[0], 3 * blocks[1]), -1.0, device="cuda")[..., ::2, 1::3]):
+        got = quantize_fp8(x, block_rows=block_rows, out=out, scale=given)
+        assert got[0] is out and got[1] is given
+        assert torch.equal(out.float(), q.float()) and torch.equal(given, scale)
+        if given._base is not None:
+            assert int((given._base != -1.0).sum()) == given.numel()
+    untouched = torch.ones_like(wide, dtype=torch.bool)
+    untouched[..., 1:rows + 1, 16:16 + k] = False
+    assert bool((wide[untouched] == 0x55).all())
+    if batch:
+        for i in range(batch[0]):
+            alone = quantize_fp8(x[i], block_rows=block_rows)
+            assert torch.equal(alone[0].float(), q[i].float()) and torch.equal(alone[1], scale[i])
+
+
+def test_refusals_of_given_buffers():
+    from kernels import grouped_mm_fp8, matmul_fp8, quantize_fp8
+
+    x = normal(83, 8, 256)
+    e4m3 = torch.zeros((8, 300), dtype=torch.uint8, device="cuda").view(E4M3)
+    for out in (e4m3, e4m3[:, 4:260], e4m3[:, :256].float(), e4m3[:, :256].cpu(), e4m3[:4, :256], e4m3[:1, :256].expand(8, 256)):
+        with pytest.raises(ValueError, match="out must be"):
+            quantize_fp8(x, out=out)
+    for scale in (torch.zeros(8, 1, device="cuda"), torch.zeros(8, 2), torch.zeros(8, 2, device="cuda").double()):
+        with pytest.raises(ValueError, match="scale must be"):
+            quantize_fp8(x, scale=scale)
+    with pytest.raises(ValueError, match="unit stride"):
+        quantize_fp8(x.t())
+    with pytest.raises(ValueError):
+        quantize_fp8(x.int())
+    a, sa, w, sw = operands(85, 8, 32, 256, 1)
+    offs = torch.tensor([8], dtype=torch.int32, device="cuda")
+    for out in (torch.zeros(8, 31, device="cuda"), torch.zeros(8, 32), torch.zeros(32, 8, device="cuda").t()):
+        with pytest.raises(ValueError, match="out must be"):
+            grouped_mm_fp8(a, sa, w, sw, offs, out=out)
+    with pytest.raises(ValueError, match="out_dtype"):
+        matmul_fp8(a, sa, w[0], sw[0], out=torch.zeros(8, 32, device="cuda"), out_dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="cover"):
+        matmul_fp8(a, sa, w[0], sw[0], out=torch.zeros(1, 32, device="cuda").expand(8, 32))
+    for bad in (offs.long(), torch.cat([offs, offs]), offs.cpu()):
+        with pytest.raises(ValueError, match="offs|device"):
+            grouped_mm_fp8(a, sa, w, sw, bad)
+    with pytest.raises(ValueError, match="16 bytes"):
+        matmul_fp8(e4m3[:, 8:264], sa, w[0], sw[0])
+
+
+def test_strided_experts_and_scales():
+    """Every other expert of a larger weight, and scales to match."""
+    from kernels import grouped_mm_fp8, grouped_mm_fp8_swiglu
+
+    counts = (5, 0, 70)
+    offs = torch.tensor(counts, device="cuda").cumsum(0).to(torch.int32)
+    a, sa, w, sw = operands(87, 75, 64, 272, 3)
+    more = torch.full((6, 128, 288), 0x7f, dtype=torch.uint8, device="cuda").view(E4M3)
+    far_w = more[::2, ::2, 16:288]
+    far_w.copy_(w)
+    far_sw = torch.full((6, 3, 7), float("nan"), device="cuda")[1::2, 1:2, ::3]
+    far_sw.copy_(sw)
+    assert torch.equal(grouped_mm_fp8(a, sa, far_w, far_sw, offs), grouped_mm_fp8(a, sa, w, sw, offs))
+    one, other = grouped_mm_fp8_swiglu(a, sa, far_w, far_sw, offs), grouped_mm_fp8_swiglu(a, sa, w, sw, offs)
+    assert torch.equal(one[0].float(), other[0].float()) and torch.equal(one[1], other[1])
+    shared = w[:1].expand(3, 64, 272), sw[:1].expand(3, 1, 3)  # one weight for all
+    alone = grouped_mm_fp8(a, sa, *shared, offs)
+    for part in (slice(0, 5), slice(5, 75)):
+        assert_product(alone[part], a[part], sa[part], w[0], sw[0])
