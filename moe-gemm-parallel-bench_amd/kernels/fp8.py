@@ -68,8 +68,8 @@ def quantize_fp8(x, *, block_rows: int = 1, out=None, scale=None):
         buffer = torch.empty((*x.shape[:-1], pitch), dtype=torch.float8_e4m3fn, device=x.device)
         out = buffer if pitch == k else buffer[..., :k]
     elif (out.shape != x.shape or out.dtype != torch.float8_e4m3fn or out.device != x.device
-          or (out.stride(-1) != 1 and k > 1) or out.data_ptr() % 8 or any(s % 8 for s in out.stride()[:-1])
-          or out.stride(-2) < k):
+          or (out.stride(-1) != 1 and k > 1) or out.data_ptr() % 8
+          or (rows > 1 and (out.stride(-2) % 8 or out.stride(-2) < k)) or (batch > 1 and out.stride(0) % 8)):
         raise ValueError(f"out must be a {tuple(x.shape)} float8_e4m3fn tensor on x's device whose rows start at "
                          "multiples of 8 bytes")
     if scale is None:
@@ -82,11 +82,11 @@ def quantize_fp8(x, *, block_rows: int = 1, out=None, scale=None):
     elif tuple(scale.shape) != scale_shape or scale.dtype != torch.float32 or scale.device != x.device:
         raise ValueError(f"scale must be a {scale_shape} float32 tensor on x's device")
     xs, qs, ss = x.stride(), out.stride(), scale.stride()
-    three = len(xs) == 3
+    three = batch > 1  # a stride that is not walked may be anything
     status = _native.library().moegemm_quantize_fp8(
         x.data_ptr(), out.data_ptr(), scale.data_ptr(), batch, rows, k, xs[0] if three else 0, xs[-2],
-        qs[0] if three else 0, qs[-2], ss[0] if three else 0, ss[-2], ss[-1], code, block_rows,
-        _native.current_stream_handle(x.device))
+        qs[0] if three else 0, qs[-2] if rows > 1 else -(-k // 8) * 8, ss[0] if three else 0, ss[-2], ss[-1], code,
+        block_rows, _native.current_stream_handle(x.device))
     _native.check(status)
     return out, scale
 

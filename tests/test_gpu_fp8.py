@@ -581,3 +581,18 @@ def test_strided_experts_and_scales():
     alone = grouped_mm_fp8(a, sa, *shared, offs)
     for part in (slice(0, 5), slice(5, 75)):
         assert_product(alone[part], a[part], sa[part], w[0], sw[0])
+
+
+def test_quantize_one_row_into_a_dense_buffer():
+    """A single row starts where the buffer does, whatever its pitch; so does the only matrix of a batch of one."""
+    from kernels import quantize_fp8
+
+    for shape in ((1, 129), (1, 1, 77), (1, 3, 40)):
+        x = normal(89, *shape)
+        out = torch.zeros(shape, dtype=torch.uint8, device="cuda").view(E4M3)
+        if shape == (1, 3, 40):
+            out = torch.as_strided(out, shape, (123, 40, 1))
+        for block_rows in (1, 128):
+            expected = quantize_fp8(x, block_rows=block_rows)
+            q, scale = quantize_fp8(x, block_rows=block_rows, out=out)
+            assert q is out and torch.equal(q.float(), expected[0].float()) and torch.equal(scale, expected[1])
