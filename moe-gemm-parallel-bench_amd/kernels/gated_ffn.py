@@ -16,6 +16,8 @@ from __future__ import annotations
 from . import _native
 from .fp8 import _cu_count
 
+_PITCH_LIMIT = 1 << 22  # elements between rows: 256 rows of a tile span under 2 GiB
+
 
 def _rows_ok(tensor) -> bool:
     """Unit inner stride and rows at multiples of 16 bytes."""
@@ -119,8 +121,9 @@ def _gradients(dh, x, weight, offs, saved, h: int, weight_shape, variants, need_
 
     rows, f = dh.shape
     device = dh.device
-    if not _rows_ok(dh) or (rows > 1 and dh.stride(0) < f):
-        # Autograd hands out expanded and transposed gradients, and dense views at any offset, which contiguous() returns.
+    if not _rows_ok(dh) or (rows > 1 and not f <= dh.stride(0) < _PITCH_LIMIT):
+        # Autograd hands out expanded and transposed gradients, slices of wide ones, and dense views at any offset, which
+        # contiguous() returns.
         dh = dh.clone(memory_format=torch.contiguous_format)
     lib = _native.library()
     dx_variant, dw_variant = variants or (-1, -1)

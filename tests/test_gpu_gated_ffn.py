@@ -450,3 +450,16 @@ def test_rows_past_32_bit_offsets():
         back = min(variant, lib.moegemm_gate_up_variant_count(2) - 1)
         dx, dw = gate_up_swiglu_backward(far_dh, far_x, w, offs, saved, variants=(variant, back))
         check(x, w, dh, counts, out, saved, dx, dw)
+
+
+def test_a_gradient_sliced_from_a_wide_one():
+    """h beside four million other columns: its gradient's rows are 8 MB apart."""
+    from kernels import gate_up_swiglu, gate_up_swiglu_backward, gate_up_swiglu_forward
+
+    x, w, dh, offs = operands(59, (3, 0, 2), 64, 40, torch.bfloat16)
+    x1, w1 = x.clone().requires_grad_(), w.clone().requires_grad_()
+    other = torch.zeros((5, 1 << 22), device="cuda", dtype=torch.bfloat16)
+    torch.cat([gate_up_swiglu(x1, w1, offs), other], dim=1).backward(torch.cat([dh, other], dim=1))
+    _, saved = gate_up_swiglu_forward(x, w, offs)
+    dx, dw = gate_up_swiglu_backward(dh, x, w, offs, saved)
+    assert torch.equal(x1.grad, dx) and torch.equal(w1.grad, dw)
