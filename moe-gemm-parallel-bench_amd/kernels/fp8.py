@@ -49,33 +49,34 @@ def quantize_fp8(x, *, block_rows: int = 1, out=None, scale=None):
 
     if block_rows not in (1, SCALE_BLOCK):
         raise ValueError(f"block_rows must be 1 or {SCALE_BLOCK}, got {block_rows!r}")
-    if x.ndim not in (2, 3):
+    shape = x.shape
+    if len(shape) not in (2, 3):
         raise ValueError("quantize_fp8 expects a 2-D [rows, K] or a 3-D [G, rows, K] tensor")
-    rows, k = x.shape[-2:]
-    batch = x.shape[0] if x.ndim == 3 else 1
+    *head, rows, k = shape
+    batch = head[0] if head else 1
     if rows | k | batch > _native.INT32_MAX:
-        raise ValueError(f"x's extents must be under 2**31 (got {tuple(x.shape)})")
+        raise ValueError(f"x's extents must be under 2**31 (got {tuple(shape)})")
     if x.device.type != "cuda":
         raise ValueError("x must be on a GPU device")
     code = _native.dtype_code(x.dtype)
     if k <= 0:
         raise ValueError("quantize_fp8 needs a positive K")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    if x.stride(-1) != 1 and k > 1:
         raise ValueError("x needs a unit stride along its last dimension")
-    scale_shape = (*x.shape[:-2], -(-rows // block_rows), _blocks(k))
+    scale_shape = (*head, -(-rows // block_rows), _blocks(k))
     if out is None:
         pitch = -(-k // 16) * 16
-        buffer = torch.empty((*x.shape[:-1], pitch), dtype=torch.float8_e4m3fn, device=x.device)
+        buffer = torch.empty((*head, rows, pitch), dtype=torch.float8_e4m3fn, device=x.device)
         out = buffer if pitch == k else buffer[..., :k]
-    elif (out.shape != x.shape or out.dtype != torch.float8_e4m3fn or out.device != x.device
+    elif (out.shape != shape or out.dtype != torch.float8_e4m3fn or out.device != x.device
           or (out.stride(-1) != 1 and k > 1) or out.data_ptr() % 8
           or (rows > 1 and (out.stride(-2) % 8 or out.stride(-2) < k)) or (batch > 1 and out.stride(0) % 8)):
-        raise ValueError(f"out must be a {tuple(x.shape)} float8_e4m3fn tensor on x's device whose rows start at "
+        raise ValueError(f"out must be a {tuple(shape)} float8_e4m3fn tensor on x's device whose rows start at "
                          "multiples of 8 bytes")
     if scale is None:
         if block_rows == 1:
             blocks = scale_shape[-1]
-            strides = (1, rows) if x.ndim == 2 else (blocks * rows, 1, rows)
+            strides = (blocks * rows, 1, rows) if head else (1, rows)
             scale = torch.empty_strided(scale_shape, strides, dtype=torch.float32, device=x.device)
         else:
             scale = torch.empty(scale_shape, dtype=torch.float32, device=x.device)
@@ -100,10 +101,10 @@ def _validate(a, scale_a, weight, scale_w, offs):
         raise ValueError("expected a 2-D a [rows, K] and " + ("a 3-D weight [G, N, K]" if grouped else
                                                                "a 2-D weight [N, K]"))
     rows, k = a.shape
-    n = weight.shape[-2]
-    groups = weight.shape[0] if grouped else 1
-    if weight.shape[-1] != k:
-        raise ValueError(f"contraction mismatch: a K={k}, weight K={weight.shape[-1]}")
+    *head, n, width = weight.shape
+    groups = head[0] if grouped else 1
+    if width != k:
+        raise ValueError(f"contraction mismatch: a K={k}, weight K={width}")
     if a.dtype != torch.float8_e4m3fn or weight.dtype != torch.float8_e4m3fn:
         raise ValueError("a and weight must be float8_e4m3fn")
     if groups <= 0 or n <= 0 or k <= 0:

@@ -105,26 +105,27 @@ def gate_up_swiglu_backward(dh, x, weight, offs, saved, *, need_dx: bool = True,
     """
     import torch
 
-    rows, h, f, _ = _validate(x, weight, offs)
+    rows, h, f, groups = _validate(x, weight, offs)
     if dh.shape != (rows, f) or dh.dtype is not x.dtype or dh.device != x.device:
         raise ValueError(f"dh must be a [{rows}, {f}] {x.dtype} matrix on x's device")
     if (saved.shape != (rows, 2 * f) or saved.dtype is not torch.float32 or saved.device != x.device
             or not saved.is_contiguous()):
         raise ValueError(f"saved must be the contiguous [{rows}, {2 * f}] float32 tensor of the forward pass")
-    return _gradients(dh, x if need_dw else None, weight if need_dx else None, offs, saved, h, weight.shape, variants,
-                      need_dx, need_dw)
+    return _gradients(dh, x, weight, offs, saved, rows, h, f, groups, weight.shape, variants, need_dx, need_dw)
 
 
-def _gradients(dh, x, weight, offs, saved, h: int, weight_shape, variants, need_dx: bool, need_dw: bool):
-    """(dx, dw) of checked operands; x is read for dw only, weight for dx only."""
-    import torch
-
-    rows, f = dh.shape
+def _gradients(dh, x, weight, offs, saved, rows: int, h: int, f: int, groups: int, weight_shape, variants, need_dx: bool,
+               need_dw: bool):
+    """(dx, dw) of checked operands; x is read for dw only, weight for dx only (else they may be None)."""
     device = dh.device
-    if not _rows_ok(dh) or (rows > 1 and not f <= dh.stride(0) < _PITCH_LIMIT):
+    pitch, inner = dh.stride()
+    if inner != 1 or dh.data_ptr() & 15 or (rows > 1 and (pitch & 7 or not f <= pitch < _PITCH_LIMIT)):
         # Autograd hands out expanded and transposed gradients, slices of wide ones, and dense views at any offset, which
         # contiguous() returns.
+        import torch
+
         dh = dh.clone(memory_format=torch.contiguous_format)
+        pitch = f
     lib = _native.library()
     dx_variant, dw_variant = variants or (-1, -1)
     dp = dh.new_empty((rows, 2 * f))
@@ -133,7 +134,7 @@ def _gradients(dh, x, weight, offs, saved, h: int, weight_shape, variants, need_
     _native.check(lib.moegemm_gate_up_backward(
         dh.data_ptr(), x.data_ptr() if need_dw else None, weight.data_ptr() if need_dx else None, saved.data_ptr(),
         dp.data_ptr(), dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None,
-        None if offs is None else offs.data_ptr(), 1 if offs is None else offs.shape[0], rows, h, f, _pitch(dh),
+        None if offs is None else offs.data_ptr(), groups, rows, h, f, pitch if rows > 1 else f,
         _pitch(x) if need_dw else 0, _group_stride(weight) if need_dx else 0, _pitch(weight) if need_dx else 0,
         _native.dtype_code(dh.dtype), dx_variant, dw_variant, _cu_count(device), _native.current_stream_handle(device)))
     return dx, dw
@@ -167,15 +168,14 @@ def _function():
             need_dx, need_dw = ctx.needs_input_grad[:2]
             # x is read for dW and the weight for dx: what is not kept may change before the backward pass.
             ctx.save_for_backward(saved, x if need_dw else None, weight if need_dx else None, offs)
-            ctx.width, ctx.weight_shape = x.shape[1], weight.shape
+            ctx.sizes = (*x.shape, h.shape[1], 1 if offs is None else weight.shape[0], weight.shape)
             return h
 
         @staticmethod
         @torch.autograd.function.once_differentiable
         def backward(ctx, dh):
             saved, x, weight, offs = ctx.saved_tensors
-            return (*_gradients(dh, x, weight, offs, saved, ctx.width, ctx.weight_shape, None, *ctx.needs_input_grad[:2]),
-                    None)
+            return (*_gradients(dh, x, weight, offs, saved, *ctx.sizes, None, *ctx.needs_input_grad[:2]), None)
 
     _FUNCTION.append(GateUpSwiglu)
     return GateUpSwiglu
