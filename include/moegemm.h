@@ -8,12 +8,12 @@
  *   - all matrix, table and stream arguments are plain device pointers / a hipStream_t as void*;
  *   - strides are in elements; dims tables are int32 (m, n, k) triples; pointer tables are int64
  *     device addresses, read by the kernel at run time (callers may rewrite them between calls);
- *   - a call performs exactly one kernel launch on `stream` (or none for an empty problem set; the fp8 and Gate+Up
- *     training entries say below where they launch again),
+ *   - a call performs exactly one kernel launch on `stream` (or none for an empty problem set; the fp8, Gate+Up
+ *     training, sort and 4-bit entries say below where they launch again),
  *     never allocates, copies or synchronizes, and is therefore capturable in a HIP graph;
  *   - the return value is MOEGEMM_OK or a negative error code; moegemm_last_error() returns the
  *     message of the most recent failure on the calling thread;
- *   - every launching call but the fp8 and Gate+Up training entries takes `b_stream` (0 or 1) just
+ *   - every launching call but the fp8, Gate+Up training, routing and 4-bit entries takes `b_stream` (0 or 1) just
  *     before `stream`: 1 issues the LDS-DMA
  *     kernels' B copies as non-temporal loads (streamed, evicted first from the caches), 0 as
  *     ordinary loads.  It changes no result, only speed, and which is faster depends on the
@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define MOEGEMM_ABI_VERSION 10
+#define MOEGEMM_ABI_VERSION 11
 
 #define MOEGEMM_OK 0
 #define MOEGEMM_ERR_INVALID (-1)   /* bad shape, pointer, dtype or parameter (Python: ValueError) */
@@ -404,6 +404,87 @@ int moegemm_gate_up_backward(const void* dh, const void* x, const void* w, const
                              void* dw, const int32_t* offs, int32_t group_count, int32_t rows, int32_t h, int32_t f,
                              int64_t stride_dhm, int64_t stride_xm, int64_t stride_wg, int64_t stride_wh, int32_t dtype,
                              int32_t dx_variant, int32_t dw_variant, int32_t grid_size, void* stream);
+
+/*
+ * Routing: each token's experts from the router's logits, and the way to expert-sorted rows and back.  No counterpart in
+ * the reference, whose routing is uniform and on the host (README.md:55-57).
+ *
+ * moegemm_route_topk: s = softmax(logits) (sigmoid 0) or sigmoid(logits) (1) over expert_count experts (at most 1024),
+ * c = s + bias (bias NULL: s).  Of `groups` equal runs of experts the top_groups ones with the largest sums of their
+ * group_best (1 or 2) best c are eligible; the k (at most 64) largest c win, ties go to the lowest index.  weights
+ * [tokens, k] = s of the chosen, over their sum if normalize (0 where that is 0), times scale; experts [tokens, k].
+ * logits is [tokens, expert_count] (dtype; unit stride along the experts).  A NaN logit ranks below every other.
+ * moegemm_route_topk_backward: the logits' gradient [tokens, expert_count] (contiguous, dtype) for dweights, through s; an
+ * index outside the experts counts for nothing.
+ */
+int moegemm_route_topk(const void* logits, const float* bias, float* weights, int32_t* experts, int32_t tokens,
+                       int32_t expert_count, int32_t k, int64_t stride_lt, int32_t dtype, int32_t sigmoid, int32_t groups,
+                       int32_t top_groups, int32_t group_best, int32_t normalize, float scale, void* stream);
+int moegemm_route_topk_backward(const float* dweights, const void* logits, const int32_t* experts, void* dlogits,
+                                int32_t tokens, int32_t expert_count, int32_t k, int64_t stride_lt, int32_t dtype,
+                                int32_t sigmoid, int32_t normalize, float scale, void* stream);
+
+/*
+ * moegemm_sort_by_expert: a stable counting sort of `entries` expert indices for experts first to first + count - 1 (count
+ * at most 1024).  offs [count]: end rows; slots [entries]: the entry of each sorted row, -1 at and past the last end
+ * row; places [entries]: the sorted row of each entry, -1 for other experts.  `workspace` holds
+ * moegemm_sort_workspace_bytes() bytes (< 0 on bad arguments) and need not be cleared; calls that share one must not overlap.
+ * Two launches.
+ */
+int64_t moegemm_sort_workspace_bytes(int64_t entries, int32_t count);
+int moegemm_sort_by_expert(const int32_t* experts, int32_t* offs, int32_t* slots, int32_t* places, int32_t entries,
+                           int32_t first, int32_t count, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Rows of tokens to expert-sorted rows and back.  places is [tokens, k], `end` the last of the offsets (on the device);
+ * places outside 0 to rows - 1 are skipped, so any content is memory-safe.
+ *   gather:   out[places[t, j]] = x[t], rows from *end on are zeros; rows of row_bytes bytes, strides in bytes
+ *   combine:  out[t] = sum_j weights[t, j] y[places[t, j]] in fp32, in the order of j (weights NULL: 1); strides in elements
+ *   backward: dy[places[t, j]] = weights[t, j] dout[t] (contiguous; rows from *end on are zeros) unless dy is NULL;
+ *             dweights[t, j] = <dout[t], y[places[t, j]]> (0 where skipped) unless dweights is NULL
+ */
+int moegemm_gather_rows(const void* x, void* out, const int32_t* places, const int32_t* end, int64_t tokens, int32_t k,
+                        int32_t rows, int64_t row_bytes, int64_t stride_x, int64_t stride_out, void* stream);
+int moegemm_combine_rows(const void* y, const float* weights, void* out, const int32_t* places, int64_t tokens, int32_t k,
+                         int32_t rows, int32_t width, int64_t stride_y, int64_t stride_out, int32_t dtype, void* stream);
+int moegemm_combine_rows_backward(const void* dout, const void* y, const float* weights, void* dy, float* dweights,
+                                  const int32_t* places, const int32_t* end, int64_t tokens, int32_t k, int32_t rows,
+                                  int32_t width, int64_t stride_dout, int64_t stride_y, int32_t dtype, void* stream);
+
+/*
+ * 4-bit weights (OCP MXFP4, the format that model_configs/gpt-oss-120b.json names): e2m1 values, two a byte with the even k
+ * in the low half, and one e8m0 scale byte s for each 32 along k; a value stands for v 2^(s - 127), s = 255 for NaN.  No
+ * counterpart in the reference.  k is a multiple of 32; strides of q, w and scales are in bytes, of values in elements.
+ *
+ * moegemm_quantize_mxfp4: for each 32 values scale = 2^(floor(log2 max|x|) - 2), at least 2^-127, q = e2m1(x / scale) to
+ * nearest even, at most 6; a group that holds a NaN or an infinity gets s = 255.  q rows start at multiples of 4 bytes.
+ * moegemm_dequantize_mxfp4: the values in dtype, contiguous and 16-byte aligned.
+ */
+int moegemm_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scale, int64_t rows, int32_t k, int64_t stride_xr,
+                           int64_t stride_qr, int64_t stride_sr, int32_t dtype, void* stream);
+int moegemm_dequantize_mxfp4(const uint8_t* q, const uint8_t* scale, void* out, int64_t rows, int32_t k, int64_t stride_qr,
+                             int64_t stride_sr, int32_t dtype, void* stream);
+
+/* Compiled variants of the 4-bit products. */
+int moegemm_mxfp4_variant_count(void);
+
+/*
+ * C[r0:r1] = A[r0:r1] @ W[e]^T for each group e of rows, offsets as in moegemm_grouped_mm_offs; offs NULL: one group of all
+ * rows.  a is [rows, k] (fp16 or bf16), w 4-bit [group_count, n, k / 2] with scale [group_count, n, k / 32]; out is
+ * out_dtype [rows, n] with unit column stride.  Rows of a and w start at multiples of 16 bytes.  Sums are fp32 and of one
+ * order.  Rows at or past offs[group_count-1] are not written.  `variant` -1 lets the library choose; grid_size is the CUs
+ * (<= 0: 256).  One launch, and another for every further 768 groups.
+ * _swiglu: w is [group_count, n = 2F, k / 2], rows [gate | up]; out [rows, F] = silu(a gate^T) * (a up^T) in fp32.
+ */
+int moegemm_grouped_mm_mxfp4(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs,
+                             int32_t group_count, int32_t rows, int32_t n, int32_t k, int64_t stride_am, int64_t stride_wg,
+                             int64_t stride_wn, int64_t stride_sg, int64_t stride_sn, int64_t stride_om, int32_t dtype,
+                             int32_t out_dtype, int32_t variant, int32_t grid_size, void* stream);
+int moegemm_grouped_mm_mxfp4_swiglu(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs,
+                                    int32_t group_count, int32_t rows, int32_t n, int32_t k, int64_t stride_am,
+                                    int64_t stride_wg, int64_t stride_wn, int64_t stride_sg, int64_t stride_sn,
+                                    int64_t stride_om, int32_t dtype, int32_t out_dtype, int32_t variant, int32_t grid_size,
+                                    void* stream);
 
 #ifdef __cplusplus
 }

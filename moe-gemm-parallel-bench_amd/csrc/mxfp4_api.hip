@@ -1,0 +1,156 @@
+// C ABI of the 4-bit (MXFP4) operators: argument checks, the choice of a variant, the launches: one a call, and another for
+// every further 768 groups of a product.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/moegemm.h"
+#include "error.h"
+#include "mxfp4_menu.h"
+
+using namespace moegemm;
+
+namespace {
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+int checked(hipError_t err) {
+  return err == hipSuccess ? MOEGEMM_OK
+                           : report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+}
+
+bool is_dtype(int32_t dtype) { return dtype == DT_F16 || dtype == DT_BF16 || dtype == DT_F32; }
+
+constexpr int64_t kMaxBlocks = 1 << 16;  // workgroups of a conversion, which go on to what is past them
+
+int check_conversion(int64_t rows, int32_t k, const void* x, const uint8_t* q, const uint8_t* scale, int64_t stride_q,
+                     int32_t dtype) {
+  if (!is_dtype(dtype)) return report(MOEGEMM_ERR_INVALID, "unsupported dtype code %d", dtype);
+  if (rows < 0 || k <= 0 || k % kMxGroup)
+    return report(MOEGEMM_ERR_INVALID, "bad shape (rows=%lld k=%d, k a multiple of 32)", (long long)rows, k);
+  if (rows && (!x || !q || !scale)) return report(MOEGEMM_ERR_INVALID, "values, q and scale must be non-null");
+  if (!aligned(q, 4) || stride_q % 4) return report(MOEGEMM_ERR_INVALID, "q rows must start at multiples of 4 bytes");
+  if (!aligned(x, dtype == DT_F32 ? 4 : 2))
+    return report(MOEGEMM_ERR_INVALID, "values must be aligned to their element size");
+  return MOEGEMM_OK;
+}
+
+dim3 conversion_grid(int64_t rows, int32_t k) { return dim3((unsigned)std::min(cdiv(rows * (k / 8), 256), kMaxBlocks)); }
+
+template <class E>
+hipError_t launch_quantize(const MxConvertParams& p, bool vec, hipStream_t s) {
+  if (vec) hipLaunchKernelGGL((mx_quantize_kernel<E, true>), conversion_grid(p.rows, p.k), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((mx_quantize_kernel<E, false>), conversion_grid(p.rows, p.k), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+template <class E>
+hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
+  hipLaunchKernelGGL((mx_dequantize_kernel<E>), conversion_grid(p.rows, p.k), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+// Variant for `rows` rows over `groups` groups of `cols` output columns.
+int choose(const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
+  const int64_t active = std::min(groups, rows);
+  const int64_t high = active == 1 ? rows : cdiv(cdiv(rows, active) * 8, 5);
+  const int need = high <= 8 ? 8 : high <= 16 ? 16 : 32;
+  int best = -1;
+  for (int i = 0; i < kNumMx; ++i) {
+    const MxVariant& v = table[i];
+    if (v.rows != need) continue;
+    // Narrow units that share K where the wide ones would leave CUs idle.
+    if (best < 0 || (v.waves_k > 1 && active * cdiv(cols, table[best].cols) < 2 * cus)) best = i;
+  }
+  return best;
+}
+
+int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs, int32_t group_count,
+                   int32_t rows, int32_t n, int32_t k, int64_t stride_am, int64_t stride_wg, int64_t stride_wn,
+                   int64_t stride_sg, int64_t stride_sn, int64_t stride_om, int32_t dtype, int32_t out_dtype, bool gated,
+                   int32_t variant, int32_t grid_size, void* stream) {
+  if (dtype != DT_F16 && dtype != DT_BF16)
+    return report(MOEGEMM_ERR_INVALID, "4-bit products need fp16 or bf16 rows (dtype code %d)", dtype);
+  if (!is_dtype(out_dtype)) return report(MOEGEMM_ERR_INVALID, "unsupported dtype code %d", out_dtype);
+  if (group_count <= 0) return report(MOEGEMM_ERR_INVALID, "group_count must be positive (got %d)", group_count);
+  if (!offs && group_count != 1)
+    return report(MOEGEMM_ERR_INVALID, "without offsets there is one group (got %d)", group_count);
+  if (rows < 0 || n <= 0 || k <= 0 || k % kMxGroup)
+    return report(MOEGEMM_ERR_INVALID, "bad shape (rows=%d n=%d k=%d, k a multiple of 32)", rows, n, k);
+  if (gated && n % 2) return report(MOEGEMM_ERR_INVALID, "packed Gate+Up width must be even (got %d)", n);
+  if (variant < -1 || variant >= kNumMx)
+    return report(MOEGEMM_ERR_NO_KERNEL, "4-bit variant %d is not compiled (0 to %d, or -1)", variant, kNumMx - 1);
+  if (rows == 0) return MOEGEMM_OK;
+  const int64_t cols = gated ? n / 2 : n;
+  if (!a || !w || !scale || !out) return report(MOEGEMM_ERR_INVALID, "operands, scales and output must be non-null");
+  if (!aligned(a, 16) || stride_am % 8 || !aligned(w, 16) || stride_wn % 16 || stride_wg % 16)
+    return report(MOEGEMM_ERR_INVALID, "rows of a and weight must start at multiples of 16 bytes");
+  if (stride_am < 0 || stride_wn < k / 2 || stride_sn < k / kMxGroup || (rows > 1 && stride_om < cols))
+    return report(MOEGEMM_ERR_INVALID, "row pitches must cover a row");
+  if (!aligned(out, out_dtype == DT_F32 ? 4 : 2))
+    return report(MOEGEMM_ERR_INVALID, "out must be aligned to its element size");
+  const int cus = grid_size > 0 ? grid_size : 256;
+  const MxVariant* table = dtype == DT_BF16 ? (gated ? kMxGatedBf16 : kMxBf16) : (gated ? kMxGatedF16 : kMxF16);
+  if (variant < 0) variant = choose(table, rows, group_count, cols, cus);
+  const MxVariant& v = table[variant];
+  MxParams p{static_cast<const uint16_t*>(a), w, scale, out, offs, stride_am, stride_wg, stride_wn, stride_sg, stride_sn,
+             stride_om, group_count, rows, n, k, (int32_t)cdiv(cols, v.cols), out_dtype};
+  const int64_t bound = std::min(rows / v.rows + (int64_t)group_count, group_count * cdiv(rows, v.rows)) * p.n_tiles;
+  if (bound > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
+  const int grid = (int)std::min<int64_t>(bound, (int64_t)cus * 4);
+  for (; p.first < group_count; p.first += kTableGroups) {
+    p.groups = std::min(group_count - p.first, kTableGroups);
+    const int rc = checked(v.launch(p, grid, reinterpret_cast<hipStream_t>(stream)));
+    if (rc != MOEGEMM_OK) return rc;
+  }
+  return MOEGEMM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moegemm_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scale, int64_t rows, int32_t k, int64_t stride_xr,
+                           int64_t stride_qr, int64_t stride_sr, int32_t dtype, void* stream) {
+  const int rc = check_conversion(rows, k, x, q, scale, stride_qr, dtype);
+  if (rc != MOEGEMM_OK || rows == 0) return rc;
+  const MxConvertParams p{x, q, scale, nullptr, stride_xr, stride_qr, stride_sr, rows, k};
+  const bool vec = aligned(x, 16) && stride_xr * (dtype == DT_F32 ? 4 : 2) % 16 == 0;
+  const auto s = reinterpret_cast<hipStream_t>(stream);
+  return checked(dtype == DT_F32    ? launch_quantize<EF32>(p, vec, s)
+                 : dtype == DT_BF16 ? launch_quantize<EBf16>(p, vec, s)
+                                    : launch_quantize<EF16>(p, vec, s));
+}
+
+int moegemm_dequantize_mxfp4(const uint8_t* q, const uint8_t* scale, void* out, int64_t rows, int32_t k, int64_t stride_qr,
+                             int64_t stride_sr, int32_t dtype, void* stream) {
+  const int rc = check_conversion(rows, k, out, q, scale, stride_qr, dtype);
+  if (rc != MOEGEMM_OK || rows == 0) return rc;
+  if (!aligned(out, 16)) return report(MOEGEMM_ERR_INVALID, "out must be 16-byte aligned");
+  const MxConvertParams p{q, nullptr, const_cast<uint8_t*>(scale), out, 0, stride_qr, stride_sr, rows, k};
+  const auto s = reinterpret_cast<hipStream_t>(stream);
+  return checked(dtype == DT_F32    ? launch_dequantize<EF32>(p, s)
+                 : dtype == DT_BF16 ? launch_dequantize<EBf16>(p, s)
+                                    : launch_dequantize<EF16>(p, s));
+}
+
+int moegemm_mxfp4_variant_count(void) { return kNumMx; }
+
+int moegemm_grouped_mm_mxfp4(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs,
+                             int32_t group_count, int32_t rows, int32_t n, int32_t k, int64_t stride_am, int64_t stride_wg,
+                             int64_t stride_wn, int64_t stride_sg, int64_t stride_sn, int64_t stride_om, int32_t dtype,
+                             int32_t out_dtype, int32_t variant, int32_t grid_size, void* stream) {
+  return launch_product(a, w, scale, out, offs, group_count, rows, n, k, stride_am, stride_wg, stride_wn, stride_sg, stride_sn,
+                        stride_om, dtype, out_dtype, false, variant, grid_size, stream);
+}
+
+int moegemm_grouped_mm_mxfp4_swiglu(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs,
+                                    int32_t group_count, int32_t rows, int32_t n, int32_t k, int64_t stride_am,
+                                    int64_t stride_wg, int64_t stride_wn, int64_t stride_sg, int64_t stride_sn,
+                                    int64_t stride_om, int32_t dtype, int32_t out_dtype, int32_t variant, int32_t grid_size,
+                                    void* stream) {
+  return launch_product(a, w, scale, out, offs, group_count, rows, n, k, stride_am, stride_wg, stride_wn, stride_sg, stride_sn,
+                        stride_om, dtype, out_dtype, true, variant, grid_size, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,38 @@
+// Compiled variants of the 4-bit products, one table per type of the rows (inst_mxfp4_*.hip).
+#pragma once
+
+#include "mxfp4.h"
+
+namespace moegemm {
+
+typedef hipError_t (*MxLaunchFn)(const MxParams&, int grid, hipStream_t stream);
+
+struct MxVariant {
+  int rows, cols;    // of a unit: output rows, and output columns
+  int waves_k;       // waves that share K
+  MxLaunchFn launch;
+};
+
+template <class T>
+hipError_t launch_mx(const MxParams& p, int grid, hipStream_t stream) {
+  hipLaunchKernelGGL((mx_stream_kernel<T>), dim3(grid), dim3(T::NT), 0, stream, p);
+  return hipGetLastError();
+}
+
+// X(A, ROWS8, FN, WAVES_N, WAVES_K, GATED)
+#define MOEGEMM_MENU_MX(X, A, GATED)                                                             \
+  X(A, 1, 4, 4, 1, GATED) X(A, 1, 2, 1, 8, GATED) X(A, 2, 4, 4, 1, GATED) X(A, 2, 2, 1, 8, GATED) \
+  X(A, 4, 4, 4, 1, GATED)
+
+#define MOEGEMM_MX_X(A, R, FN, WN, WK, GATED) \
+  MxVariant{8 * R, 8 * FN * WN / (GATED ? 2 : 1), WK, &launch_mx<MxStream<A, R, FN, WN, WK, GATED>>},
+// The kernels of a menu, for the device pass.
+#define MOEGEMM_MX_XK(A, R, FN, WN, WK, GATED) \
+  template __global__ void mx_stream_kernel<MxStream<A, R, FN, WN, WK, GATED>>(MxParams);
+
+#define MOEGEMM_MX_COUNT(...) +1
+constexpr int kNumMx = 0 MOEGEMM_MENU_MX(MOEGEMM_MX_COUNT, , false);
+
+extern const MxVariant kMxBf16[], kMxF16[], kMxGatedBf16[], kMxGatedF16[];
+
+}  // namespace moegemm

@@ -1,0 +1,236 @@
+// C ABI of the routing operators: argument checks and launches.  One launch a call; a sort of more than one chunk is two.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/moegemm.h"
+#include "error.h"
+#include "routing.h"
+
+using namespace moegemm;
+
+namespace {
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+int checked(hipError_t err) {
+  return err == hipSuccess ? MOEGEMM_OK
+                           : report(MOEGEMM_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+}
+
+int64_t element_bytes(int32_t dtype) { return dtype == DT_F32 ? 4 : 2; }
+
+int check_route(const RouteParams& p, int32_t dtype) {
+  if (dtype != DT_F16 && dtype != DT_BF16 && dtype != DT_F32)
+    return report(MOEGEMM_ERR_INVALID, "unsupported dtype code %d", dtype);
+  if (p.tokens < 0 || p.experts <= 0 || p.experts > kRouteExperts)
+    return report(MOEGEMM_ERR_INVALID, "bad shape (tokens=%d experts=%d, at most %d experts)", p.tokens, p.experts,
+                  kRouteExperts);
+  if (p.k <= 0 || p.k > kRouteTop || p.k > p.experts)
+    return report(MOEGEMM_ERR_INVALID, "k must be 1 to min(experts, %d) (got %d)", kRouteTop, p.k);
+  if ((p.sigmoid != 0 && p.sigmoid != 1) || (p.normalize != 0 && p.normalize != 1))
+    return report(MOEGEMM_ERR_INVALID, "sigmoid and normalize must be 0 or 1");
+  if (!p.logits && p.tokens) return report(MOEGEMM_ERR_INVALID, "logits must be non-null");
+  if (!aligned(p.logits, element_bytes(dtype)))
+    return report(MOEGEMM_ERR_INVALID, "logits must be aligned to their element size");
+  return MOEGEMM_OK;
+}
+
+constexpr int64_t kMaxBlocks = 1 << 16;  // workgroups of a launch; they go on to the tokens and rows past them
+
+template <class E, int PER>
+hipError_t launch_route(const RouteParams& p, bool backward, hipStream_t stream) {
+  const dim3 grid((unsigned)std::min(cdiv(p.tokens, 4), kMaxBlocks));
+  if (backward) hipLaunchKernelGGL((route_backward_kernel<E, PER>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((route_kernel<E, PER>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+template <class E>
+hipError_t launch_route(const RouteParams& p, bool backward, hipStream_t stream) {
+  const int per = (int)cdiv(p.experts, 64);
+  return per <= 1   ? launch_route<E, 1>(p, backward, stream)
+         : per <= 2 ? launch_route<E, 2>(p, backward, stream)
+         : per <= 4 ? launch_route<E, 4>(p, backward, stream)
+         : per <= 8 ? launch_route<E, 8>(p, backward, stream)
+                    : launch_route<E, 16>(p, backward, stream);
+}
+int launch_route(const RouteParams& p, bool backward, int32_t dtype, void* stream) {
+  const auto s = reinterpret_cast<hipStream_t>(stream);
+  return checked(dtype == DT_F32    ? launch_route<EF32>(p, backward, s)
+                 : dtype == DT_BF16 ? launch_route<EBf16>(p, backward, s)
+                                    : launch_route<EF16>(p, backward, s));
+}
+
+// Entries of a workgroup: at most kSortBlocks workgroups, each of which reads all counts.
+constexpr int64_t kSortChunk = 2048, kSortBlocks = 256;
+int64_t sort_chunk(int64_t n) { return cdiv(std::max(kSortChunk, cdiv(n, kSortBlocks)), 256) * 256; }
+
+// The widest unit that rows and their pitches allow.
+int64_t unit_bytes(int64_t width, std::initializer_list<std::pair<const void*, int64_t>> rows) {
+  int64_t unit = 16;
+  auto fits = [&](int64_t u) {
+    if (width % u) return false;
+    for (const auto& r : rows)
+      if (r.first && (!aligned(r.first, u) || r.second % u)) return false;
+    return true;
+  };
+  while (unit > 1 && !fits(unit)) unit >>= 1;
+  return unit;
+}
+
+struct U16 {
+  uint32_t v[4];
+} __attribute__((aligned(16)));
+
+// `end` may be null where no rows are cleared.
+int check_rows(int64_t tokens, int32_t k, int32_t rows, int64_t width, const int32_t* places, const int32_t* end, bool clears) {
+  if (tokens < 0 || k <= 0 || rows < 0 || width <= 0 || width > INT32_MAX)
+    return report(MOEGEMM_ERR_INVALID, "bad shape (tokens=%lld k=%d rows=%d, rows of %lld bytes)", (long long)tokens, k,
+                  rows, (long long)width);
+  if ((!places && tokens) || (!end && clears)) return report(MOEGEMM_ERR_INVALID, "places and offs must be non-null");
+  return MOEGEMM_OK;
+}
+
+template <class E>
+hipError_t launch_combine(const RowsParams& p, int64_t unit, dim3 grid, hipStream_t s) {
+  using raw = typename E::raw;
+  if (unit == 16) hipLaunchKernelGGL((combine_rows_kernel<E, U16>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((combine_rows_kernel<E, raw>), grid, dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+template <class E>
+hipError_t launch_combine_backward(const RowsParams& p, int64_t unit, dim3 grid, hipStream_t s) {
+  using raw = typename E::raw;
+  if (unit == 16) hipLaunchKernelGGL((combine_rows_backward_kernel<E, U16>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((combine_rows_backward_kernel<E, raw>), grid, dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+int moegemm_route_topk(const void* logits, const float* bias, float* weights, int32_t* experts, int32_t tokens,
+                       int32_t expert_count, int32_t k, int64_t stride_lt, int32_t dtype, int32_t sigmoid, int32_t groups,
+                       int32_t top_groups, int32_t group_best, int32_t normalize, float scale, void* stream) {
+  RouteParams p{logits, bias, weights, experts, nullptr, nullptr, stride_lt, tokens, expert_count, k, sigmoid, groups,
+                top_groups, group_best, normalize, scale};
+  const int rc = check_route(p, dtype);
+  if (rc != MOEGEMM_OK) return rc;
+  if (groups <= 0 || expert_count % groups || top_groups <= 0 || top_groups > groups || (group_best != 1 && group_best != 2))
+    return report(MOEGEMM_ERR_INVALID, "bad expert groups (%d of %d over %d experts, group_best %d)", top_groups, groups,
+                  expert_count, group_best);
+  if (k > top_groups * (expert_count / groups))
+    return report(MOEGEMM_ERR_INVALID, "k = %d experts do not fit %d groups of %d", k, top_groups, expert_count / groups);
+  if (tokens == 0) return MOEGEMM_OK;
+  if (!weights || !experts) return report(MOEGEMM_ERR_INVALID, "weights and experts must be non-null");
+  return launch_route(p, false, dtype, stream);
+}
+
+int moegemm_route_topk_backward(const float* dweights, const void* logits, const int32_t* experts, void* dlogits,
+                                int32_t tokens, int32_t expert_count, int32_t k, int64_t stride_lt, int32_t dtype,
+                                int32_t sigmoid, int32_t normalize, float scale, void* stream) {
+  RouteParams p{logits, nullptr, nullptr, const_cast<int32_t*>(experts), dweights, dlogits, stride_lt, tokens, expert_count,
+                k, sigmoid, 1, 1, 1, normalize, scale};
+  const int rc = check_route(p, dtype);
+  if (rc != MOEGEMM_OK || tokens == 0) return rc;
+  if (!dweights || !experts || !dlogits) return report(MOEGEMM_ERR_INVALID, "dweights, experts and dlogits must be non-null");
+  if (!aligned(dlogits, element_bytes(dtype)))
+    return report(MOEGEMM_ERR_INVALID, "dlogits must be aligned to its element size");
+  return launch_route(p, true, dtype, stream);
+}
+
+int64_t moegemm_sort_workspace_bytes(int64_t entries, int32_t count) {
+  if (entries < 0 || entries > INT32_MAX || count <= 0 || count > kSortExperts)
+    return report(MOEGEMM_ERR_INVALID, "bad sort (%lld entries, %d experts of at most %d)", (long long)entries, count,
+                  kSortExperts);
+  return std::max<int64_t>(cdiv(entries, sort_chunk(entries)), 1) * count * 4;
+}
+
+int moegemm_sort_by_expert(const int32_t* experts, int32_t* offs, int32_t* slots, int32_t* places, int32_t entries,
+                           int32_t first, int32_t count, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int64_t need = moegemm_sort_workspace_bytes(entries, count);
+  if (need < 0) return (int)need;
+  if (first < 0) return report(MOEGEMM_ERR_INVALID, "the first expert must not be negative (got %d)", first);
+  if (!offs || !workspace || (entries && (!experts || !slots || !places)))
+    return report(MOEGEMM_ERR_INVALID, "experts, offs, slots, places and workspace must be non-null");
+  if (workspace_bytes < need)
+    return report(MOEGEMM_ERR_INVALID, "the workspace holds %lld bytes of %lld", (long long)workspace_bytes, (long long)need);
+  const int64_t chunk = sort_chunk(entries);
+  SortParams p{experts, offs, slots, places, static_cast<int32_t*>(workspace), entries, first, count, (int32_t)chunk};
+  const dim3 grid((unsigned)std::max<int64_t>(cdiv(entries, chunk), 1));
+  const auto s = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(sort_count_kernel, grid, dim3(256), 0, s, p);
+  const int rc = checked(hipGetLastError());
+  if (rc != MOEGEMM_OK) return rc;
+  hipLaunchKernelGGL(sort_place_kernel, grid, dim3(256), 0, s, p);
+  return checked(hipGetLastError());
+}
+
+int moegemm_gather_rows(const void* x, void* out, const int32_t* places, const int32_t* end, int64_t tokens, int32_t k,
+                        int32_t rows, int64_t row_bytes, int64_t stride_x, int64_t stride_out, void* stream) {
+  const int rc = check_rows(tokens, k, rows, row_bytes, places, end, true);
+  if (rc != MOEGEMM_OK || rows == 0) return rc;
+  if ((!x && tokens) || !out) return report(MOEGEMM_ERR_INVALID, "x and out must be non-null");
+  const int64_t unit = unit_bytes(row_bytes, {{x, stride_x}, {out, stride_out}});
+  const int64_t spans = cdiv(row_bytes, 4 * 64 * unit);
+  const RowsParams p{static_cast<const char*>(x), static_cast<char*>(out), places, end, nullptr, nullptr, nullptr, stride_x,
+                     stride_out, 0, tokens, k, rows, (int32_t)row_bytes, (int32_t)spans};
+  const dim3 grid((unsigned)(kClearBlocks + std::min(cdiv(tokens * spans, 4), kMaxBlocks)));
+  const auto s = reinterpret_cast<hipStream_t>(stream);
+  switch (unit) {
+    case 16: hipLaunchKernelGGL(gather_rows_kernel<U16>, grid, dim3(256), 0, s, p); break;
+    case 8: hipLaunchKernelGGL(gather_rows_kernel<uint64_t>, grid, dim3(256), 0, s, p); break;
+    case 4: hipLaunchKernelGGL(gather_rows_kernel<uint32_t>, grid, dim3(256), 0, s, p); break;
+    case 2: hipLaunchKernelGGL(gather_rows_kernel<uint16_t>, grid, dim3(256), 0, s, p); break;
+    default: hipLaunchKernelGGL(gather_rows_kernel<uint8_t>, grid, dim3(256), 0, s, p);
+  }
+  return checked(hipGetLastError());
+}
+
+int moegemm_combine_rows(const void* y, const float* weights, void* out, const int32_t* places, int64_t tokens, int32_t k,
+                         int32_t rows, int32_t width, int64_t stride_y, int64_t stride_out, int32_t dtype, void* stream) {
+  if (dtype != DT_F16 && dtype != DT_BF16 && dtype != DT_F32)
+    return report(MOEGEMM_ERR_INVALID, "unsupported dtype code %d", dtype);
+  const int64_t es = element_bytes(dtype);
+  const int rc = check_rows(tokens, k, rows, width * es, places, nullptr, false);
+  if (rc != MOEGEMM_OK || tokens == 0) return rc;
+  if ((!y && rows) || !out) return report(MOEGEMM_ERR_INVALID, "y and out must be non-null");
+  if (!aligned(y, es) || !aligned(out, es))
+    return report(MOEGEMM_ERR_INVALID, "y and out must be aligned to their element size");
+  const int64_t unit = unit_bytes(width * es, {{y, stride_y * es}, {out, stride_out * es}}) == 16 ? 16 : es;
+  const int64_t spans = cdiv(width * es, 2 * 64 * unit);
+  const RowsParams p{static_cast<const char*>(y), static_cast<char*>(out), places, nullptr, weights, nullptr, nullptr,
+                     stride_y * es, stride_out * es, 0, tokens, k, rows, (int32_t)(width * es), (int32_t)spans};
+  const dim3 grid((unsigned)std::min(cdiv(tokens * spans, 4), kMaxBlocks));
+  const auto s = reinterpret_cast<hipStream_t>(stream);
+  return checked(dtype == DT_F32    ? launch_combine<EF32>(p, unit, grid, s)
+                 : dtype == DT_BF16 ? launch_combine<EBf16>(p, unit, grid, s)
+                                    : launch_combine<EF16>(p, unit, grid, s));
+}
+
+int moegemm_combine_rows_backward(const void* dout, const void* y, const float* weights, void* dy, float* dweights,
+                                  const int32_t* places, const int32_t* end, int64_t tokens, int32_t k, int32_t rows,
+                                  int32_t width, int64_t stride_dout, int64_t stride_y, int32_t dtype, void* stream) {
+  if (dtype != DT_F16 && dtype != DT_BF16 && dtype != DT_F32)
+    return report(MOEGEMM_ERR_INVALID, "unsupported dtype code %d", dtype);
+  const int64_t es = element_bytes(dtype);
+  const int rc = check_rows(tokens, k, rows, width * es, places, end, true);
+  if (rc != MOEGEMM_OK || (!dy && !dweights)) return rc;
+  if ((!dout && tokens) || (dweights && rows && !y))
+    return report(MOEGEMM_ERR_INVALID, "dout, and y where dweights is wanted, must be non-null");
+  if (!aligned(y, es) || !aligned(dout, es) || !aligned(dy, es))
+    return report(MOEGEMM_ERR_INVALID, "dout, y and dy must be aligned to their element size");
+  const int64_t unit =
+      unit_bytes(width * es, {{dweights ? y : nullptr, stride_y * es}, {dout, stride_dout * es}, {dy, 0}}) == 16 ? 16 : es;
+  const RowsParams p{static_cast<const char*>(y), static_cast<char*>(dy), places, end, weights, static_cast<const char*>(dout),
+                     dweights, stride_y * es, width * es, stride_dout * es, tokens, k, rows, (int32_t)(width * es), 1};
+  const dim3 grid((unsigned)(kClearBlocks + std::min(cdiv(tokens * k, 4), kMaxBlocks)));
+  const auto s = reinterpret_cast<hipStream_t>(stream);
+  return checked(dtype == DT_F32    ? launch_combine_backward<EF32>(p, unit, grid, s)
+                 : dtype == DT_BF16 ? launch_combine_backward<EBf16>(p, unit, grid, s)
+                                    : launch_combine_backward<EF16>(p, unit, grid, s));
+}
+
+}  // extern "C"

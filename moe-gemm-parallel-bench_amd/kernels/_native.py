@@ -16,7 +16,7 @@ from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().with_name("libmoegemm.so")
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 OK = 0
 ERR_INVALID = -1
 ERR_NO_KERNEL = -2
@@ -32,6 +32,7 @@ DTYPE_NAMES = {DTYPE_F16: "fp16", DTYPE_BF16: "bf16", DTYPE_F32: "fp32"}
 
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
+_f32 = ctypes.c_float
 _vp = ctypes.c_void_p
 
 INT32_MAX = 2 ** 31 - 1  # ctypes passes a larger extent's low 32 bits without an error
@@ -141,6 +142,33 @@ SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
          _vp],
+    ),
+    "moegemm_route_topk": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp],
+    ),
+    "moegemm_route_topk_backward": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _vp],
+    ),
+    "moegemm_sort_workspace_bytes": (_i64, [_i64, _i32]),
+    "moegemm_sort_by_expert": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "moegemm_gather_rows": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _i64, _i64, _vp]),
+    "moegemm_combine_rows": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i64, _i32, _vp]),
+    "moegemm_combine_rows_backward": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i64, _i32, _vp],
+    ),
+    "moegemm_quantize_mxfp4": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _i32, _vp]),
+    "moegemm_dequantize_mxfp4": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, _i64, _i64, _i32, _vp]),
+    "moegemm_mxfp4_variant_count": (ctypes.c_int, []),
+    "moegemm_grouped_mm_mxfp4": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp],
+    ),
+    "moegemm_grouped_mm_mxfp4_swiglu": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp],
     ),
 }
 
@@ -490,3 +518,16 @@ def current_stream_handle(device) -> int:
     # The raw handle: building a torch.cuda.Stream object for it took about 2 us of a 11 us call.
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def launch(device, entry, *args) -> None:
+    """``entry(*args, stream)`` on ``device``'s current stream; a kernel goes to the current device, so that is made
+    ``device`` where it is another."""
+    import torch
+
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        check(entry(*args, current_stream_handle(device)))
+        return
+    with torch.cuda.device(index):
+        check(entry(*args, current_stream_handle(device)))
