@@ -81,65 +81,53 @@ __device__ __forceinline__ double sigmoid64(double x) { return 1.0 / (1.0 + exp(
 // max of a softmax: 0 where nothing is above -inf, so that exp(x - max) is 0 there and not NaN.
 __device__ __forceinline__ float softmax_base(float top) { return top == -__builtin_inff() ? 0.0f : top; }
 
-// One token a wave.  Selection runs on 64-bit scores, so that which of two close ones is larger never hangs on a
-// rounding of exp; PER scores a lane, expert lane + 64 i.
-template <class E, int PER>
-__device__ __forceinline__ void route_token(const RouteParams& p, int64_t t, int lane, double* s_score) {
+// One token a wave, on 64-bit scores, so that which of two close ones is larger never hangs on a rounding of exp.  The keys
+// lie in LDS (two arrays of the experts' number): the loops are short and hold few registers.
+template <class E>
+__device__ void route_token(const RouteParams& p, int64_t t, int lane, uint64_t* key, uint64_t* group) {
   const typename E::raw* x = static_cast<const typename E::raw*>(p.logits) + t * p.ldl;
-  float v[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) v[i] = lane + 64 * i < p.experts ? to_float<E>(x[lane + 64 * i]) : -__builtin_inff();
+  float top = -__builtin_inff();
   bool nan = false;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) nan |= v[i] != v[i];
+  for (int e = lane; e < p.experts; e += 64) {
+    const float v = to_float<E>(x[e]);
+    nan |= v != v;
+    top = fmaxf(top, v);
+  }
   nan = __ballot(nan) != 0;
   // Without a bias, and unless scores are added up, they rank as the logits do.
   const bool by_logit = !p.bias && p.group_best == 1;
-  double s[PER];
   float base = 0;
   double total = 1;
-  if (p.sigmoid) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = by_logit ? (double)v[i] : sigmoid64(v[i]);
-  } else {
-    float top = v[0];
-#pragma unroll
-    for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
+  if (!p.sigmoid) {
     base = softmax_base(wave_max(top));
     total = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      s[i] = exp((double)v[i] - base);
-      total += s[i];
-    }
+    for (int e = lane; e < p.experts; e += 64) total += exp((double)to_float<E>(x[e]) - base);
     total = wave_sum(total);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = by_logit ? (double)v[i] : total == 0 ? 0 : s[i] / total;
   }
-  uint64_t key[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = lane + 64 * i;
-    key[i] = e < p.experts ? order_of(p.bias ? s[i] + p.bias[e] : s[i]) : 0;
+  for (int e = lane; e < p.experts; e += 64) {
+    const double v = to_float<E>(x[e]);
+    double c = v;
+    if (!by_logit) c = p.sigmoid ? sigmoid64(v) : total == 0 ? 0 : exp(v - base) / total;
+    key[e] = order_of(p.bias ? c + p.bias[e] : c);
   }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  auto take = [&](uint64_t* keys, int count) {  // the best of them, struck out
+    Best b{0, 0};
+    for (int i = lane; i < count; i += 64) better(b, keys[i], i);
+    b = wave_best(b);
+    if (lane == 0) keys[b.index] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return b.index;
+  };
   if (p.groups > 1) {
-    // A group a lane in turn: its best scores one after the other, then the best groups.
     const int size = p.experts / p.groups;
     auto score_of = [](uint64_t k) {
       return k == 1 ? __builtin_nan("") : __builtin_bit_cast(double, k >> 63 ? k ^ (1ull << 63) : ~k);
     };
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 64 * i < p.experts) s_score[lane + 64 * i] = score_of(key[i]);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    uint64_t kept[PER] = {};  // of groups lane + 64 i
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int g = lane + 64 * i;
-      if (g >= p.groups) continue;
+    for (int g = lane; g < p.groups; g += 64) {
       uint64_t first = 0, second = 0;
       for (int e = 0; e < size; ++e) {
-        const uint64_t c = order_of(s_score[g * size + e]);
+        const uint64_t c = key[g * size + e];
         if (c > first) {
           second = first;
           first = c;
@@ -147,39 +135,18 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int64_t t, int
           second = c;
         }
       }
-      const double sum = p.group_best == 2 && size > 1 ? score_of(first) + score_of(second) : score_of(first);
-      kept[i] = order_of(sum);
+      group[g] = order_of(p.group_best == 2 && size > 1 ? score_of(first) + score_of(second) : score_of(first));
     }
-    uint32_t of_group[PER] = {};
-    for (int n = 0; n < p.top_groups; ++n) {
-      Best b{0, 0};
-#pragma unroll
-      for (int i = 0; i < PER; ++i) better(b, kept[i], lane + 64 * i);
-      b = wave_best(b);
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (b.index == lane + 64 * i) {
-          kept[i] = 0;
-          of_group[i] = 1;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s_score[lane + 64 * i] = of_group[i];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 64 * i < p.experts && s_score[(lane + 64 * i) / size] == 0) key[i] = 0;
+    for (int n = 0; n < p.top_groups; ++n) take(group, p.groups);  // kept groups are 0 now
+    for (int e = lane; e < p.experts; e += 64)
+      if (group[e / size] != 0) key[e] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   int mine = 0;
   for (int j = 0; j < p.k; ++j) {
-    Best b{0, 0};
-#pragma unroll
-    for (int i = 0; i < PER; ++i) better(b, key[i], lane + 64 * i);
-    b = wave_best(b);
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (b.index == lane + 64 * i) key[i] = 0;
-    if (lane == j) mine = b.index;
+    const int e = take(key, p.experts);
+    if (lane == j) mine = e;
   }
   const bool used = lane < p.k;
   const float logit = used ? to_float<E>(x[mine]) : -__builtin_inff();
@@ -203,66 +170,336 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int64_t t, int
   }
 }
 
-template <class E, int PER>
-__global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
-  __shared__ double s_score[4][PER * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < p.tokens; t += (int64_t)gridDim.x * 4)
-    route_token<E, PER>(p, t, lane, s_score[wave]);
+// Lanes of a token: rows of 16 lanes exchange values at full rate (DPP), the wave's four rows in two more steps.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
 }
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140, kRor = 0x120;  // quad_perm, row_*
 
-// Gradient of the logits through the chosen scores.  One token a wave; a lane of the first k holds a chosen expert.
-template <class E, int PER>
-__device__ __forceinline__ void route_token_backward(const RouteParams& p, int64_t t, int lane, float* s_row) {
-  const typename E::raw* x = static_cast<const typename E::raw*>(p.logits) + t * p.ldl;
-  typename E::raw* dx = static_cast<typename E::raw*>(p.dlogits) + t * p.experts;
-  const int e = lane < p.k ? p.chosen[t * p.k + lane] : -1;
-  const bool used = e >= 0 && e < p.experts;
-  const double dw = used ? (double)p.dweights[t * p.k + lane] * p.scale : 0;
-  const float logit = used ? to_float<E>(x[e]) : -__builtin_inff();
-  double s, mean = 0, base = 0, total = 1;
-  const bool dense = !p.sigmoid && !p.normalize;
-  if (p.sigmoid) {
-    s = used ? sigmoid64(logit) : 0;
-    const double slope = s * (1 - s);
-    if (p.normalize) {
-      total = wave_sum(s);
-      mean = wave_sum(s * dw);
-      s = total == 0 ? 0 : (dw - mean / total) / total * slope;
-    } else {
-      s = dw * slope;
-    }
-  } else {
-    if (dense) {
-      float top = -__builtin_inff();
-      for (int i = lane; i < p.experts; i += 64) top = fmaxf(top, to_float<E>(x[i]));
-      base = softmax_base(wave_max(top));
-      total = 0;
-      for (int i = lane; i < p.experts; i += 64) total += exp((double)to_float<E>(x[i]) - base);
-      total = wave_sum(total);
-    } else {
-      base = softmax_base(wave_max(logit));
-    }
-    s = used ? exp((double)logit - base) : 0;
-    if (!dense) total = wave_sum(s);
-    s = total == 0 ? 0 : s / total;
-    mean = wave_sum(s * dw);
-    s *= dense ? dw : dw - mean;
+// f over the LPT lanes of a token, f commutative and associative.
+template <int LPT, class F>
+__device__ __forceinline__ uint32_t token_reduce(uint32_t x, F&& f) {
+  x = f(x, dpp<kXor1>(x));
+  x = f(x, dpp<kXor2>(x));
+  x = f(x, dpp<kHalfMirror>(x));
+  x = f(x, dpp<kMirror>(x));
+  if constexpr (LPT == 64) {
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = f(b[0], b[1]);
   }
-  for (int i = lane; i < p.experts; i += 64)
-    s_row[i] = dense && total != 0 ? (float)(-mean * (exp((double)to_float<E>(x[i]) - base) / total)) : 0.0f;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  if (used) s_row[e] += (float)s;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  for (int i = lane; i < p.experts; i += 64) dx[i] = from_float<E>(s_row[i]);
+  return x;
+}
+template <int LPT>
+__device__ __forceinline__ uint32_t token_max(uint32_t x) {
+  return token_reduce<LPT>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+template <int LPT>
+__device__ __forceinline__ float token_max(float x) {
+  return __builtin_bit_cast(float, token_reduce<LPT>(__builtin_bit_cast(uint32_t, x), [](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+  }));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint64_t lo = dpp<CTRL>((uint32_t)u), hi = dpp<CTRL>((uint32_t)(u >> 32));
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+template <int LPT>
+__device__ __forceinline__ double token_sum(double x) {
+  x += dpp<kXor1>(x);
+  x += dpp<kXor2>(x);
+  x += dpp<kHalfMirror>(x);
+  x += dpp<kMirror>(x);
+  if constexpr (LPT == 64) {
+    x += __shfl_xor(x, 16);
+    x += __shfl_xor(x, 32);
+  }
+  return x;
 }
 
-template <class E, int PER>
-__global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
-  __shared__ float s_row[4][PER * 64];
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float score_of(uint32_t key) {
+  return __builtin_bit_cast(float, key >> 31 ? key ^ 0x80000000u : ~key);
+}
+// Whether fp32 scores a >= b, each within 2^-20 (1 + its size) of the exact one, cut below by up to 16 units, may stand in
+// the wrong order (or one of them is no number).  An exp of |x| 2^-24 relative error costs sigmoid and softmax at most 2^-22, a
+// sum of up to 1024 exps by 16 + 6 additions 2^-19 of a softmax.
+__device__ __forceinline__ bool too_close(float a, float b, float margin) {
+  return !(a - b > margin * fmaxf(1.0f, fmaxf(fabsf(a), fabsf(b))));
+}
+constexpr float kRouteMargin = 0x1p-17f;
+
+// 64 / LPT tokens a wave, expert lane * per + i.  Scores are taken in fp32 and compared as integers whose lowest bits tell a
+// lane's experts apart; tokens with two scores too close for that to be sure of go to route_token, one after the
+// other.  Normal scores send one token in some hundred there.  16-bit logits that rank by themselves leave 13 bits free, which
+// hold the whole index: their order is exact, and equal ones are no reason.
+//
+// Bound by the vector instructions: the k rounds of a maximum over PER registers and LPT lanes.
+template <class E, int LPT, int PER>
+__global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
+  constexpr int TOKENS = 64 / LPT;
+  constexpr uint32_t MASK = PER - 1, WHOLE = 0x1fff;
+  extern __shared__ uint64_t s_key[];  // route_token's arrays, for each wave
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int li = lane & (LPT - 1), sub = lane / LPT;
+  const int per = (p.experts + LPT - 1) / LPT, e0 = li * per;
+  uint64_t* keys = s_key + wave * (p.experts + p.groups);
+  const bool by_logit = !p.bias && p.group_best == 1;
+  const bool whole = by_logit && !E::is_f32;
+  const bool needs_total = !p.sigmoid && !p.normalize;
+  const bool vec = per == PER && PER * sizeof(typename E::raw) % 16 == 0 && p.experts == LPT * PER &&
+                   (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0 && p.ldl * sizeof(typename E::raw) % 16 == 0;
+  const int group_lanes = LPT / p.groups;  // the caller's promise where groups > 1: see fast_route
+  float bias[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) bias[i] = p.bias && i < per && e0 + i < p.experts ? p.bias[e0 + i] : 0.0f;
+
+  const int64_t step = (int64_t)gridDim.x * 4 * TOKENS;
+  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * TOKENS; t0 < p.tokens; t0 += step) {
+    const int64_t t = min(t0 + sub, (int64_t)p.tokens - 1);  // a wave's missing tokens repeat the last one
+    const typename E::raw* x = static_cast<const typename E::raw*>(p.logits) + t * p.ldl;
+    float v[PER];
+    if (vec) {
+      typename E::raw raw[PER];
+      constexpr int N = PER * sizeof(typename E::raw) / 16;
+      u32x4_t c[N > 0 ? N : 1];
+#pragma unroll
+      for (int i = 0; i < N; ++i) c[i] = reinterpret_cast<const u32x4_t*>(x + e0)[i];
+      __builtin_memcpy(raw, c, N > 0 ? sizeof(raw) : 0);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = to_float<E>(raw[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = i < per && e0 + i < p.experts ? to_float<E>(x[e0 + i]) : -__builtin_inff();
+    }
+    bool doubt = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) doubt |= v[i] != v[i];
+    float c[PER];
+    double total = 1;
+    float base = 0;
+    if (needs_total || (!p.sigmoid && !by_logit)) {
+      float top = v[0];
+#pragma unroll
+      for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
+      base = softmax_base(token_max<LPT>(top));
+    }
+    if (needs_total) {
+      total = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (i < per) total += exp((double)v[i] - base);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: sixteen side by side take all registers
+      }
+      total = token_sum<LPT>(total);
+    }
+    if (by_logit) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) c[i] = v[i];
+    } else if (p.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) c[i] = __builtin_amdgcn_rcpf(1.0f + __expf(-v[i])) + bias[i];
+    } else {
+      double sum = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        c[i] = __expf(v[i] - base);
+        sum += c[i];
+      }
+      const float inverse = (float)(1.0 / token_sum<LPT>(sum));
+#pragma unroll
+      for (int i = 0; i < PER; ++i) c[i] = c[i] * inverse + bias[i];
+    }
+    bool mine_in = true;  // a lane's experts are of one group
+    if (p.groups > 1) {
+      float first = -__builtin_inff(), second = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (i < per) {
+          second = fmaxf(second, fminf(first, c[i]));
+          first = fmaxf(first, c[i]);
+        }
+      auto merge = [&](float f, float s) {
+        second = fmaxf(fminf(first, f), fmaxf(second, s));
+        first = fmaxf(first, f);
+      };
+      // Row by row: groups of 2, 4, 8 or 16 lanes; 64 lanes have groups of 4 or more.
+      auto bits = [](float f) { return __builtin_bit_cast(uint32_t, f); };
+      auto real = [](uint32_t u) { return __builtin_bit_cast(float, u); };
+      if (group_lanes >= 2) merge(real(dpp<kXor1>(bits(first))), real(dpp<kXor1>(bits(second))));
+      if (group_lanes >= 4) merge(real(dpp<kXor2>(bits(first))), real(dpp<kXor2>(bits(second))));
+      if (group_lanes >= 8) merge(real(dpp<kHalfMirror>(bits(first))), real(dpp<kHalfMirror>(bits(second))));
+      if (group_lanes >= 16) merge(real(dpp<kMirror>(bits(first))), real(dpp<kMirror>(bits(second))));
+      if (LPT == 64 && group_lanes >= 32) merge(__shfl_xor(first, 16), __shfl_xor(second, 16));
+      const float score = p.group_best == 2 && p.experts > p.groups ? first + second : first;
+      int rank = 0;
+      for (int g = 1; g < p.groups; ++g) {
+        const int from = (lane & ~(LPT - 1)) | ((li + g * group_lanes) & (LPT - 1));
+        const float other = __shfl(score, from);
+        rank += other > score || (other == score && (from & (LPT - 1)) < li) ? 1 : 0;
+      }
+      mine_in = rank < p.top_groups;
+      if (p.top_groups < p.groups) {
+        const float least = -token_max<LPT>(mine_in ? -score : -__builtin_inff());
+        const float most = token_max<LPT>(mine_in ? -__builtin_inff() : score);
+        doubt |= too_close(least, most, 2 * kRouteMargin);
+      }
+    }
+    uint32_t key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint32_t low = whole ? WHOLE - (uint32_t)(e0 + i) : MASK - (uint32_t)i;
+      const uint32_t o = (order_of(c[i]) & ~(whole ? WHOLE : MASK)) | low;
+      key[i] = i < per && e0 + i < p.experts && mine_in ? o : 0;
+    }
+    int mine = 0;
+    float last = 0;
+    for (int j = 0; j <= p.k; ++j) {
+      uint32_t top = key[0];
+#pragma unroll
+      for (int i = 1; i < PER; ++i) top = max(top, key[i]);
+      const uint32_t best = token_max<LPT>(top);
+      const float score = score_of(best & ~MASK);
+      if (!whole && j > 0 && best) doubt |= too_close(last, score, kRouteMargin);
+      last = score;
+      if (j == p.k) break;
+      uint64_t hits = __ballot(top == best);
+      if constexpr (LPT == 16) hits = hits >> (lane & 48) & 0xffff;
+      doubt |= !whole && (hits & (hits - 1)) != 0;
+      const int e = whole ? (int)(WHOLE - (best & WHOLE)) : (int)__builtin_ctzll(hits) * per + (int)(MASK - (best & MASK));
+      if (li == j) mine = min(e, p.experts - 1);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) key[i] = key[i] == best ? 0 : key[i];
+    }
+    const uint64_t doubts = __ballot(doubt);
+    const bool used = li < p.k;
+    const float logit = used ? to_float<E>(x[mine]) : -__builtin_inff();
+    double w;
+    if (p.sigmoid) {
+      w = used ? sigmoid64(logit) : 0;
+      if (p.normalize) {
+        const double sum = token_sum<LPT>(w);
+        w = sum == 0 ? 0 : w / sum;
+      }
+    } else {
+      if (p.normalize) base = softmax_base(token_max<LPT>(logit));
+      w = used ? exp((double)logit - base) : 0;
+      if (p.normalize) total = token_sum<LPT>(w);
+      w = total == 0 ? 0 : w / total;
+    }
+    constexpr uint64_t LANES = LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1;
+    if (used && t0 + sub < p.tokens && (doubts >> (sub * LPT) & LANES) == 0) {
+      p.weights[t * p.k + li] = (float)(w * p.scale);
+      p.chosen[t * p.k + li] = mine;
+    }
+    if (doubts == 0) continue;
+    for (int n = 0; n < TOKENS; ++n)
+      if (t0 + n < p.tokens && (doubts >> (n * LPT) & LANES) != 0) route_token<E>(p, t0 + n, lane, keys, keys + p.experts);
+  }
+}
+
+// Every token on 64-bit scores, one a wave: more than 64 experts to choose in rows of 16 lanes, or groups that lanes cannot hold.
+template <class E>
+__global__ void __launch_bounds__(256) route_exact_kernel(RouteParams p) {
+  extern __shared__ uint64_t s_key[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t* keys = s_key + wave * (p.experts + p.groups);
   for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < p.tokens; t += (int64_t)gridDim.x * 4)
-    route_token_backward<E, PER>(p, t, lane, s_row[wave]);
+    route_token<E>(p, t, lane, keys, keys + p.experts);
+}
+
+// Gradient of the logits through the chosen scores.  64 / LPT tokens a wave; a lane of a token's first k holds a chosen expert.
+// Where the gradient is not dense it is k numbers among zeros, put together in LDS and stored in whole lines.
+template <class E, int LPT, int PER>
+__global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
+  constexpr int TOKENS = 64 / LPT;
+  __shared__ __attribute__((aligned(16))) float s_row[4][TOKENS][LPT * PER];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int li = lane & (LPT - 1), sub = lane / LPT;
+  const bool dense = !p.sigmoid && !p.normalize;
+  float* row = s_row[wave][sub];
+  const int64_t step = (int64_t)gridDim.x * 4 * TOKENS;
+  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * TOKENS; t0 < p.tokens; t0 += step) {
+    const int64_t t = min(t0 + sub, (int64_t)p.tokens - 1);
+    const typename E::raw* x = static_cast<const typename E::raw*>(p.logits) + t * p.ldl;
+    const int e = li < p.k ? p.chosen[t * p.k + li] : -1;
+    const bool used = e >= 0 && e < p.experts;
+    const double dw = used ? (double)p.dweights[t * p.k + li] * p.scale : 0;
+    const float logit = used ? to_float<E>(x[e]) : -__builtin_inff();
+    double s;
+    if (p.sigmoid) {
+      s = used ? sigmoid64(logit) : 0;
+      const double slope = s * (1 - s);
+      if (p.normalize) {
+        const double total = token_sum<LPT>(s), mean = token_sum<LPT>(s * dw);
+        s = total == 0 ? 0 : (dw - mean / total) / total * slope;
+      } else {
+        s = dw * slope;
+      }
+    } else if (dense) {
+      double all[PER], total = 0;
+      float v[PER], top = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        v[i] = li + i * LPT < p.experts ? to_float<E>(x[li + i * LPT]) : -__builtin_inff();
+        top = fmaxf(top, v[i]);
+      }
+      const float base = softmax_base(token_max<LPT>(top));
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        all[i] = li + i * LPT < p.experts ? exp((double)v[i] - base) : 0;
+        total += all[i];
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      total = token_sum<LPT>(total);
+      const double inverse = total == 0 ? 0 : 1 / total;
+      s = used ? exp((double)logit - base) * inverse * dw : 0;
+      const double mean = token_sum<LPT>(s);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) row[li + i * LPT] = (float)(-mean * (all[i] * inverse));
+    } else {
+      const float base = softmax_base(token_max<LPT>(logit));
+      s = used ? exp((double)logit - base) : 0;
+      const double total = token_sum<LPT>(s);
+      s = total == 0 ? 0 : s / total;
+      s *= dw - token_sum<LPT>(s * dw);
+    }
+    if (!dense) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) row[li + i * LPT] = 0;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (used) row[e] += (float)s;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    // The rows of the wave's tokens one after the other, 16 bytes a lane where they allow it.
+    constexpr int N = 16 / sizeof(typename E::raw);
+    const bool vec = p.experts % N == 0 && (reinterpret_cast<uintptr_t>(p.dlogits) & 15) == 0;
+    for (int n = 0; n < TOKENS; ++n) {
+      if (t0 + n >= p.tokens) break;
+      typename E::raw* dx = static_cast<typename E::raw*>(p.dlogits) + (t0 + n) * p.experts;
+      const float* from = s_row[wave][n];
+      if (vec) {
+        for (int i = lane * N; i < p.experts; i += 64 * N) {
+          typename E::raw out[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) out[j] = from_float<E>(from[i + j]);
+          u32x4_t packed;
+          __builtin_memcpy(&packed, out, 16);
+          *MOEGEMM_GLOBAL(u32x4_t, dx + i) = packed;
+        }
+      } else {
+        for (int i = lane; i < p.experts; i += 64) dx[i] = from_float<E>(from[i]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // read before the next tokens' rows are written
+  }
 }
 
 struct SortParams {

@@ -39,21 +39,37 @@ int check_route(const RouteParams& p, int32_t dtype) {
 
 constexpr int64_t kMaxBlocks = 1 << 16;  // workgroups of a launch; they go on to the tokens and rows past them
 
-template <class E, int PER>
+// Whether route_kernel's lanes hold the choice: one chosen expert a lane, and groups that are whole lanes' experts, as many
+// to each.  Else every token takes the 64-bit path (16384 tokens over 256 experts, 4 of 8 groups, 8 experts: REPLACE).
+bool fast_route(const RouteParams& p, int lanes) {
+  return p.k <= lanes && (p.groups == 1 || (p.groups <= 16 && lanes % p.groups == 0 && p.experts % lanes == 0));
+}
+
+template <class E, int LPT, int PER>
 hipError_t launch_route(const RouteParams& p, bool backward, hipStream_t stream) {
-  const dim3 grid((unsigned)std::min(cdiv(p.tokens, 4), kMaxBlocks));
-  if (backward) hipLaunchKernelGGL((route_backward_kernel<E, PER>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((route_kernel<E, PER>), grid, dim3(256), 0, stream, p);
+  constexpr int WIDE = LPT * PER <= 64 ? 1 : LPT * PER / 64;
+  const size_t lds = 4 * (p.experts + p.groups) * sizeof(uint64_t);  // route_token's arrays, at most 64 KiB
+  auto grid = [&](int64_t tokens) { return dim3((unsigned)std::min(cdiv(p.tokens, tokens), kMaxBlocks)); };
+  if (backward) {
+    if (p.k <= LPT) hipLaunchKernelGGL((route_backward_kernel<E, LPT, PER>), grid(256 / LPT), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((route_backward_kernel<E, 64, WIDE>), grid(4), dim3(256), 0, stream, p);
+  } else if (fast_route(p, LPT)) {
+    hipLaunchKernelGGL((route_kernel<E, LPT, PER>), grid(256 / LPT), dim3(256), lds, stream, p);
+  } else {
+    hipLaunchKernelGGL((route_exact_kernel<E>), grid(4), dim3(256), lds, stream, p);
+  }
   return hipGetLastError();
 }
+// 16 lanes a token up to 256 experts, then all 64.
 template <class E>
 hipError_t launch_route(const RouteParams& p, bool backward, hipStream_t stream) {
-  const int per = (int)cdiv(p.experts, 64);
-  return per <= 1   ? launch_route<E, 1>(p, backward, stream)
-         : per <= 2 ? launch_route<E, 2>(p, backward, stream)
-         : per <= 4 ? launch_route<E, 4>(p, backward, stream)
-         : per <= 8 ? launch_route<E, 8>(p, backward, stream)
-                    : launch_route<E, 16>(p, backward, stream);
+  const int64_t per = cdiv(p.experts, 16);
+  return per <= 2    ? launch_route<E, 16, 2>(p, backward, stream)
+         : per <= 4  ? launch_route<E, 16, 4>(p, backward, stream)
+         : per <= 8  ? launch_route<E, 16, 8>(p, backward, stream)
+         : per <= 16 ? launch_route<E, 16, 16>(p, backward, stream)
+         : per <= 32 ? launch_route<E, 64, 8>(p, backward, stream)
+                     : launch_route<E, 64, 16>(p, backward, stream);
 }
 int launch_route(const RouteParams& p, bool backward, int32_t dtype, void* stream) {
   const auto s = reinterpret_cast<hipStream_t>(stream);
