@@ -10,6 +10,8 @@
 //              dy[places[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], y[places[t, j]]>.
 #pragma once
 
+#include <type_traits>
+
 #include "gemm_kernel.h"
 
 namespace moegemm {
@@ -30,6 +32,8 @@ __device__ __forceinline__ typename E::raw from_float(float v) {
   else if constexpr (E::dtype == DT_BF16) return __builtin_bit_cast(uint16_t, (__bf16)v);
   else return __builtin_bit_cast(uint16_t, (_Float16)v);
 }
+
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 struct RouteParams {
   const void* logits;  // [tokens, experts], ldl elements between rows
@@ -84,7 +88,7 @@ __device__ __forceinline__ float softmax_base(float top) { return top == -__buil
 // One token a wave, on 64-bit scores, so that which of two close ones is larger never hangs on a rounding of exp.  The keys
 // lie in LDS (two arrays of the experts' number): the loops are short and hold few registers.
 template <class E>
-__device__ void route_token(const RouteParams& p, int64_t t, int lane, uint64_t* key, uint64_t* group) {
+__device__ __forceinline__ void route_token(const RouteParams& p, int64_t t, int lane, uint64_t* key, uint64_t* group) {
   const typename E::raw* x = static_cast<const typename E::raw*>(p.logits) + t * p.ldl;
   float top = -__builtin_inff();
   bool nan = false;
@@ -228,159 +232,278 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float score_of(uint32_t key) {
   return __builtin_bit_cast(float, key >> 31 ? key ^ 0x80000000u : ~key);
 }
-// Whether fp32 scores a >= b, each within 2^-20 (1 + its size) of the exact one, cut below by up to 16 units, may stand in
-// the wrong order (or one of them is no number).  An exp of |x| 2^-24 relative error costs sigmoid and softmax at most 2^-22, a
-// sum of up to 1024 exps by 16 + 6 additions 2^-19 of a softmax.
-__device__ __forceinline__ bool too_close(float a, float b, float margin) {
-  return !(a - b > margin * fmaxf(1.0f, fmaxf(fabsf(a), fabsf(b))));
-}
-constexpr float kRouteMargin = 0x1p-17f;
+// fp32 scores are within 2^-22 of sigmoid (exp of x is off by (|x| + 2) 2^-24 of itself, the sum and the reciprocal by 2^-24 and
+// 2^-23, and s (1 - s) |x| < 1/4) and within 2^-18 of softmax (|x| up to 88 counts 2^-17 |x| e^-|x|); a bias adds 2^-24 of the
+// sum.  Keys drop up to 1023 units of 2^-23 of their size.  Scores further apart than these margins, times their size or 1,
+// are in order.
+constexpr float kRouteMargin = 0x1p-12f, kGroupMargin = 0x1p-16f;
 
-// 64 / LPT tokens a wave, expert lane * per + i.  Scores are taken in fp32 and compared as integers whose lowest bits tell a
-// lane's experts apart; tokens with two scores too close for that to be sure of go to route_token, one after the
-// other.  Normal scores send one token in some hundred there.  16-bit logits that rank by themselves leave 13 bits free, which
-// hold the whole index: their order is exact, and equal ones are no reason.
+// Whether a, the larger in fp32, may not be the larger one (or is no number).
+__device__ __forceinline__ bool too_close(double a, double b, double margin) {
+  return !(a - b > margin * fmax(1.0, fmax(fabs(a), fabs(b))));
+}
+
+// The two largest of a token's group, GROUP lanes with their own two largest.
+template <class F, class M>
+__device__ __forceinline__ void group_two(F& first, F& second, int group_lanes, bool wide, M&& row) {
+  auto merge = [&](F f, F s) {
+    second = fmax(fmin(first, f), fmax(second, s));
+    first = fmax(first, f);
+  };
+  if (group_lanes >= 2) merge(row(first, std::integral_constant<int, kXor1>{}), row(second, std::integral_constant<int, kXor1>{}));
+  if (group_lanes >= 4) merge(row(first, std::integral_constant<int, kXor2>{}), row(second, std::integral_constant<int, kXor2>{}));
+  if (group_lanes >= 8)
+    merge(row(first, std::integral_constant<int, kHalfMirror>{}), row(second, std::integral_constant<int, kHalfMirror>{}));
+  if (group_lanes >= 16)
+    merge(row(first, std::integral_constant<int, kMirror>{}), row(second, std::integral_constant<int, kMirror>{}));
+  if (wide && group_lanes >= 32) merge(__shfl_xor(first, 16), __shfl_xor(second, 16));
+}
+
+// Descending order of N registers by compare and exchange: runs that fall and rise in turn, merged to twice their length.
+template <int N>
+__device__ __forceinline__ void sort_descending(uint32_t (&a)[N]) {
+#pragma unroll
+  for (int k = 2; k <= N; k *= 2)
+#pragma unroll
+    for (int j = k / 2; j > 0; j /= 2)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (!(i & j)) {
+          const uint32_t x = a[i], y = a[i + j];
+          const bool falls = (i & k) == 0 || k == N;
+          a[i] = falls ? max(x, y) : min(x, y);
+          a[i + j] = falls ? min(x, y) : max(x, y);
+        }
+}
+// The same where a rises and then falls, or falls and then rises.
+template <int N>
+__device__ __forceinline__ void merge_descending(uint32_t (&a)[N]) {
+#pragma unroll
+  for (int j = N / 2; j > 0; j /= 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!(i & j)) {
+        const uint32_t x = a[i], y = a[i + j];
+        a[i] = max(x, y);
+        a[i + j] = min(x, y);
+      }
+}
+// Each lane's list becomes the largest N of its own and its partner's: both fall, so the larger of one from the front and
+// one from the back are those.
+template <int CTRL, int N>
+__device__ __forceinline__ void join_lists(uint32_t (&a)[N]) {
+  uint32_t b[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) b[i] = max(a[i], (uint32_t)__builtin_amdgcn_mov_dpp((int)a[N - 1 - i], CTRL, 0xf, 0xf, true));
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = b[i];
+  merge_descending(a);
+}
+template <bool HALVES, int N>
+__device__ __forceinline__ void join_lists_across(uint32_t (&a)[N]) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    // swap(x, y) leaves (x0, y0) and (x1, y1) of the two rows (halves).
+    const uint32_t x = a[i], y = a[N - 1 - i];
+    const auto f = HALVES ? __builtin_amdgcn_permlane32_swap(x, y, false, false) : __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    const auto g = HALVES ? __builtin_amdgcn_permlane32_swap(y, x, false, false) : __builtin_amdgcn_permlane16_swap(y, x, false, false);
+    a[i] = max(f[0], g[1]);
+    a[N - 1 - i] = max(g[0], f[1]);
+  }
+  merge_descending(a);
+}
+
+// 64 / LPT tokens a wave, expert lane * per + i.  Scores are taken in fp32 as integers whose lowest bits name the expert; each
+// lane sorts its own, and the lanes' lists are joined to the token's TOP best, which every lane then holds: compares
+// and exchanges between registers, with no round of a maximum for each of the k.  Where two scores are too close for
+// their order to be sure of, those in question are taken again in 64 bits: the groups', and of the TOP best the order.  What even
+// that leaves open (a NaN, or the k-th too close to what is not on the list) goes to route_token, one token after
+// the other.  16-bit logits that rank by themselves leave 13 bits free: their order is exact, and equal ones are in order.
 //
-// Bound by the vector instructions: the k rounds of a maximum over PER registers and LPT lanes.
-template <class E, int LPT, int PER>
+// Bound by the vector instructions, about 250 a token of 256 experts.
+enum RouteRank {
+  RANK_LOGITS,      // scores rank as the logits do
+  RANK_LOGITS_SUM,  // and a softmax's sum over all experts is needed for the weights
+  RANK_SIGMOID,
+  RANK_SOFTMAX,
+};
+template <class E, int LPT, int PER, int TOP, RouteRank RANK>
 __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
+  using raw_t = typename E::raw;
+  constexpr bool SCORES = RANK >= RANK_SIGMOID;
   constexpr int TOKENS = 64 / LPT;
-  constexpr uint32_t MASK = PER - 1, WHOLE = 0x1fff;
+  constexpr bool WHOLE = !SCORES && !E::is_f32;
+  constexpr uint32_t MASK = WHOLE ? 0x1fff : LPT * PER - 1;
+  constexpr uint64_t LANES = LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1;
   extern __shared__ uint64_t s_key[];  // route_token's arrays, for each wave
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int li = lane & (LPT - 1), sub = lane / LPT;
+  const int li = lane & (LPT - 1), sub = lane / LPT, lane0 = lane & ~(LPT - 1);
   const int per = (p.experts + LPT - 1) / LPT, e0 = li * per;
-  uint64_t* keys = s_key + wave * (p.experts + p.groups);
-  const bool by_logit = !p.bias && p.group_best == 1;
-  const bool whole = by_logit && !E::is_f32;
-  const bool needs_total = !p.sigmoid && !p.normalize;
-  const bool vec = per == PER && PER * sizeof(typename E::raw) % 16 == 0 && p.experts == LPT * PER &&
-                   (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0 && p.ldl * sizeof(typename E::raw) % 16 == 0;
-  const int group_lanes = LPT / p.groups;  // the caller's promise where groups > 1: see fast_route
-  float bias[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) bias[i] = p.bias && i < per && e0 + i < p.experts ? p.bias[e0 + i] : 0.0f;
+  const int count = max(min(per, p.experts - e0), 0);  // the lane's experts
+  const int group_lanes = LPT / p.groups;              // divides where groups > 1 (see fast_route)
+  const bool vec = p.experts == LPT * PER && PER * sizeof(raw_t) % 16 == 0 &&
+                   (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0 && p.ldl * sizeof(raw_t) % 16 == 0;
 
-  const int64_t step = (int64_t)gridDim.x * 4 * TOKENS;
-  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * TOKENS; t0 < p.tokens; t0 += step) {
-    const int64_t t = min(t0 + sub, (int64_t)p.tokens - 1);  // a wave's missing tokens repeat the last one
-    const typename E::raw* x = static_cast<const typename E::raw*>(p.logits) + t * p.ldl;
-    float v[PER];
+  // No loop over tokens: it would hold the constants of exp in registers throughout.
+  const int t0 = ((int)blockIdx.x * 4 + wave) * TOKENS;
+  if (t0 < p.tokens) {
+    const int64_t t = min(t0 + sub, p.tokens - 1);  // a wave's missing tokens repeat the last one
+    const raw_t* x = static_cast<const raw_t*>(p.logits) + t * p.ldl;
+    float c[PER];
     if (vec) {
-      typename E::raw raw[PER];
-      constexpr int N = PER * sizeof(typename E::raw) / 16;
-      u32x4_t c[N > 0 ? N : 1];
+      constexpr int N = PER * sizeof(raw_t) / 16;
+      if constexpr (N > 0) {
+        raw_t raw[PER];
+        u32x4_t chunk[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) c[i] = reinterpret_cast<const u32x4_t*>(x + e0)[i];
-      __builtin_memcpy(raw, c, N > 0 ? sizeof(raw) : 0);
+        for (int i = 0; i < N; ++i) chunk[i] = reinterpret_cast<const u32x4_t*>(x + e0)[i];
+        __builtin_memcpy(raw, chunk, sizeof(raw));
 #pragma unroll
-      for (int i = 0; i < PER; ++i) v[i] = to_float<E>(raw[i]);
+        for (int i = 0; i < PER; ++i) c[i] = to_float<E>(raw[i]);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) v[i] = i < per && e0 + i < p.experts ? to_float<E>(x[e0 + i]) : -__builtin_inff();
-    }
-    bool doubt = false;
+      for (int i = 0; i < PER; ++i) c[i] = to_float<E>(x[min(e0 + i, p.experts - 1)]);  // no branch around a load
 #pragma unroll
-    for (int i = 0; i < PER; ++i) doubt |= v[i] != v[i];
-    float c[PER];
+      for (int i = 0; i < PER; ++i) c[i] = i < count ? c[i] : -__builtin_inff();
+    }
+    bool lost = false;  // for route_token to settle
+#pragma unroll
+    for (int i = 0; i < PER; ++i) lost |= c[i] != c[i];
     double total = 1;
     float base = 0;
-    if (needs_total || (!p.sigmoid && !by_logit)) {
-      float top = v[0];
+    if constexpr (RANK == RANK_LOGITS_SUM || RANK == RANK_SOFTMAX) {
+      float top = c[0];
 #pragma unroll
-      for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
+      for (int i = 1; i < PER; ++i) top = fmaxf(top, c[i]);
       base = softmax_base(token_max<LPT>(top));
-    }
-    if (needs_total) {
       total = 0;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        if (i < per) total += exp((double)v[i] - base);
+        if (i < per) total += exp((double)c[i] - base);
         if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: sixteen side by side take all registers
       }
       total = token_sum<LPT>(total);
     }
-    if (by_logit) {
+    // The score of an expert in 64 bits.
+    auto score64 = [&](float logit, int e) {
+      double s = logit;
+      if constexpr (SCORES) s = RANK == RANK_SIGMOID ? sigmoid64(s) : total == 0 ? 0 : exp(s - base) / total;
+      return SCORES && p.bias ? s + p.bias[e] : s;
+    };
+    if constexpr (SCORES) {
+      if constexpr (RANK == RANK_SIGMOID) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) c[i] = v[i];
-    } else if (p.sigmoid) {
+        for (int i = 0; i < PER; ++i) c[i] = __builtin_amdgcn_rcpf(1.0f + __expf(-c[i]));
+      } else {
+        const float inverse = total != 0 ? (float)(1 / total) : 0.0f;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) c[i] = __builtin_amdgcn_rcpf(1.0f + __expf(-v[i])) + bias[i];
-    } else {
-      double sum = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        c[i] = __expf(v[i] - base);
-        sum += c[i];
+        for (int i = 0; i < PER; ++i) c[i] = __expf(c[i] - base) * inverse;
       }
-      const float inverse = (float)(1.0 / token_sum<LPT>(sum));
+      if (p.bias) {
+        if (vec) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) c[i] = c[i] * inverse + bias[i];
+          for (int i = 0; i < PER; i += 4) {
+            const f32x4_t b = *reinterpret_cast<const f32x4_a4*>(p.bias + e0 + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[i + j] += b[j];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) c[i] += p.bias[min(e0 + i, p.experts - 1)];
+        }
+      }
     }
     bool mine_in = true;  // a lane's experts are of one group
     if (p.groups > 1) {
+      // A group's place among the groups: how many are before it.
+      auto place = [&](auto score) {
+        int rank = 0;
+#pragma unroll
+        for (int g = 1; g < 16; ++g) {
+          const int from = lane0 | ((li + g * group_lanes) & (LPT - 1));
+          const auto other = __shfl(score, from);
+          rank += (int)(g < p.groups) & ((int)(other > score) | ((int)(other == score) & (int)(from < lane)));
+        }
+        return rank;
+      };
+      const bool two = p.group_best == 2 && p.experts > p.groups;
       float first = -__builtin_inff(), second = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i < per) {
-          second = fmaxf(second, fminf(first, c[i]));
-          first = fmaxf(first, c[i]);
-        }
-      auto merge = [&](float f, float s) {
-        second = fmaxf(fminf(first, f), fmaxf(second, s));
-        first = fmaxf(first, f);
-      };
-      // Row by row: groups of 2, 4, 8 or 16 lanes; 64 lanes have groups of 4 or more.
-      auto bits = [](float f) { return __builtin_bit_cast(uint32_t, f); };
-      auto real = [](uint32_t u) { return __builtin_bit_cast(float, u); };
-      if (group_lanes >= 2) merge(real(dpp<kXor1>(bits(first))), real(dpp<kXor1>(bits(second))));
-      if (group_lanes >= 4) merge(real(dpp<kXor2>(bits(first))), real(dpp<kXor2>(bits(second))));
-      if (group_lanes >= 8) merge(real(dpp<kHalfMirror>(bits(first))), real(dpp<kHalfMirror>(bits(second))));
-      if (group_lanes >= 16) merge(real(dpp<kMirror>(bits(first))), real(dpp<kMirror>(bits(second))));
-      if (LPT == 64 && group_lanes >= 32) merge(__shfl_xor(first, 16), __shfl_xor(second, 16));
-      const float score = p.group_best == 2 && p.experts > p.groups ? first + second : first;
-      int rank = 0;
-      for (int g = 1; g < p.groups; ++g) {
-        const int from = (lane & ~(LPT - 1)) | ((li + g * group_lanes) & (LPT - 1));
-        const float other = __shfl(score, from);
-        rank += other > score || (other == score && (from & (LPT - 1)) < li) ? 1 : 0;
+      for (int i = 0; i < PER; ++i) {
+        const float each = i < per ? c[i] : -__builtin_inff();
+        second = fmaxf(second, fminf(first, each));
+        first = fmaxf(first, each);
       }
-      mine_in = rank < p.top_groups;
-      if (p.top_groups < p.groups) {
-        const float least = -token_max<LPT>(mine_in ? -score : -__builtin_inff());
-        const float most = token_max<LPT>(mine_in ? -__builtin_inff() : score);
-        doubt |= too_close(least, most, 2 * kRouteMargin);
+      group_two(first, second, group_lanes, LPT == 64, [](float f, auto ctrl) {
+        return __builtin_bit_cast(float, dpp<decltype(ctrl)::value>(__builtin_bit_cast(uint32_t, f)));
+      });
+      const float score = two ? first + second : first;
+      mine_in = place(score) < p.top_groups;
+      const float least = -token_max<LPT>(mine_in ? -score : -__builtin_inff());
+      const float most = token_max<LPT>(mine_in ? -__builtin_inff() : score);
+      if (__ballot(p.top_groups < p.groups && too_close(least, most, kGroupMargin))) {
+        double first = -__builtin_inf(), second = -__builtin_inf();
+#pragma unroll 1
+        for (int i = 0; i < per; ++i) {
+          const double each = score64(to_float<E>(x[e0 + i]), e0 + i);
+          second = fmax(second, fmin(first, each));
+          first = fmax(first, each);
+        }
+        group_two(first, second, group_lanes, LPT == 64, [](double f, auto ctrl) { return dpp<decltype(ctrl)::value>(f); });
+        mine_in = place(two ? first + second : first) < p.top_groups;
       }
     }
-    uint32_t key[PER];
+    uint32_t key[PER], list[TOP] = {};
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const uint32_t low = whole ? WHOLE - (uint32_t)(e0 + i) : MASK - (uint32_t)i;
-      const uint32_t o = (order_of(c[i]) & ~(whole ? WHOLE : MASK)) | low;
-      key[i] = i < per && e0 + i < p.experts && mine_in ? o : 0;
+      const uint32_t o = (order_of(c[i]) & ~MASK) | (MASK - (uint32_t)(e0 + i));
+      key[i] = (int)(i < count) & (int)mine_in ? o : 0;
     }
-    int mine = 0;
-    float last = 0;
-    for (int j = 0; j <= p.k; ++j) {
-      uint32_t top = key[0];
+    sort_descending(key);
 #pragma unroll
-      for (int i = 1; i < PER; ++i) top = max(top, key[i]);
-      const uint32_t best = token_max<LPT>(top);
-      const float score = score_of(best & ~MASK);
-      if (!whole && j > 0 && best) doubt |= too_close(last, score, kRouteMargin);
-      last = score;
-      if (j == p.k) break;
-      uint64_t hits = __ballot(top == best);
-      if constexpr (LPT == 16) hits = hits >> (lane & 48) & 0xffff;
-      doubt |= !whole && (hits & (hits - 1)) != 0;
-      const int e = whole ? (int)(WHOLE - (best & WHOLE)) : (int)__builtin_ctzll(hits) * per + (int)(MASK - (best & MASK));
-      if (li == j) mine = min(e, p.experts - 1);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) key[i] = key[i] == best ? 0 : key[i];
+    for (int i = 0; i < min(PER, TOP); ++i) list[i] = key[i];
+    join_lists<kXor1>(list);
+    join_lists<kXor2>(list);
+    join_lists<kHalfMirror>(list);
+    join_lists<kMirror>(list);
+    if constexpr (LPT == 64) {
+      join_lists_across<false>(list);
+      join_lists_across<true>(list);
     }
-    const uint64_t doubts = __ballot(doubt);
+    uint32_t own = 0, next = 0;  // the li-th best and the one behind it
+#pragma unroll
+    for (int i = 0; i < TOP; ++i) {
+      own = li == i ? list[i] : own;
+      next = li == i - 1 ? list[i] : next;
+    }
+    int mine = own ? (int)(MASK - (own & MASK)) : 0;
+    float logit = own ? to_float<E>(x[mine]) : -__builtin_inff();
+    if constexpr (!WHOLE) {
+      const bool close = own != 0 && next != 0 && too_close(score_of(own & ~MASK), score_of(next & ~MASK), kRouteMargin);
+      if (__ballot(close && li < p.k)) {
+        // The list's order by 64-bit scores; what is not on it has to be smaller than the k-th by more than its error.
+        const double score = own ? score64(logit, mine) : -__builtin_inf();
+        int rank = 0;
+#pragma unroll 1
+        for (int j = 0; j < TOP; ++j) {
+          const double other = __shfl(score, lane0 + j);
+          const int index = __shfl(own ? mine : 0x7fffffff, lane0 + j);
+          rank += (int)(other > score) | ((int)(other == score) & (int)(index < mine));
+        }
+        const int to = (lane0 + (own ? rank : li)) * 4;
+        mine = __builtin_amdgcn_ds_permute(to, mine);
+        logit = __builtin_bit_cast(float, __builtin_amdgcn_ds_permute(to, __builtin_bit_cast(int, logit)));
+        const uint64_t bits = __builtin_bit_cast(uint64_t, score);
+        const uint64_t lo = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)bits);
+        const uint64_t hi = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)(bits >> 32));
+        lost |= li == p.k - 1 && list[TOP - 1] != 0 &&
+                too_close(__builtin_bit_cast(double, hi << 32 | lo), score_of(list[TOP - 1] & ~MASK), kRouteMargin);
+      }
+    }
     const bool used = li < p.k;
-    const float logit = used ? to_float<E>(x[mine]) : -__builtin_inff();
+    if (!used) logit = -__builtin_inff();
+    const uint64_t left = __ballot(lost);
     double w;
     if (p.sigmoid) {
       w = used ? sigmoid64(logit) : 0;
@@ -394,25 +517,25 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
       if (p.normalize) total = token_sum<LPT>(w);
       w = total == 0 ? 0 : w / total;
     }
-    constexpr uint64_t LANES = LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1;
-    if (used && t0 + sub < p.tokens && (doubts >> (sub * LPT) & LANES) == 0) {
+    if (used && t0 + sub < p.tokens && (left >> lane0 & LANES) == 0) {
       p.weights[t * p.k + li] = (float)(w * p.scale);
       p.chosen[t * p.k + li] = mine;
     }
-    if (doubts == 0) continue;
+    if (left == 0) return;
+    uint64_t* keys = s_key + wave * (p.experts + p.groups);
     for (int n = 0; n < TOKENS; ++n)
-      if (t0 + n < p.tokens && (doubts >> (n * LPT) & LANES) != 0) route_token<E>(p, t0 + n, lane, keys, keys + p.experts);
+      if (t0 + n < p.tokens && (left >> (n * LPT) & LANES) != 0) route_token<E>(p, t0 + n, lane, keys, keys + p.experts);
   }
 }
 
-// Every token on 64-bit scores, one a wave: more than 64 experts to choose in rows of 16 lanes, or groups that lanes cannot hold.
+// Every token on 64-bit scores, one a wave: for lists longer than route_kernel's, and groups that its lanes cannot hold.
 template <class E>
 __global__ void __launch_bounds__(256) route_exact_kernel(RouteParams p) {
   extern __shared__ uint64_t s_key[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint64_t* keys = s_key + wave * (p.experts + p.groups);
-  for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < p.tokens; t += (int64_t)gridDim.x * 4)
-    route_token<E>(p, t, lane, keys, keys + p.experts);
+  const int t = (int)blockIdx.x * 4 + wave;
+  if (t < p.tokens) route_token<E>(p, t, lane, keys, keys + p.experts);
 }
 
 // Gradient of the logits through the chosen scores.  64 / LPT tokens a wave; a lane of a token's first k holds a chosen expert.
@@ -425,9 +548,9 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
   const int li = lane & (LPT - 1), sub = lane / LPT;
   const bool dense = !p.sigmoid && !p.normalize;
   float* row = s_row[wave][sub];
-  const int64_t step = (int64_t)gridDim.x * 4 * TOKENS;
-  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * TOKENS; t0 < p.tokens; t0 += step) {
-    const int64_t t = min(t0 + sub, (int64_t)p.tokens - 1);
+  const int t0 = ((int)blockIdx.x * 4 + wave) * TOKENS;
+  if (t0 < p.tokens) {
+    const int64_t t = min(t0 + sub, p.tokens - 1);
     const typename E::raw* x = static_cast<const typename E::raw*>(p.logits) + t * p.ldl;
     const int e = li < p.k ? p.chosen[t * p.k + li] : -1;
     const bool used = e >= 0 && e < p.experts;
@@ -448,13 +571,17 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
       float v[PER], top = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        v[i] = li + i * LPT < p.experts ? to_float<E>(x[li + i * LPT]) : -__builtin_inff();
+        v[i] = to_float<E>(x[min(li + i * LPT, p.experts - 1)]);  // no branch around a load
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        v[i] = li + i * LPT < p.experts ? v[i] : -__builtin_inff();
         top = fmaxf(top, v[i]);
       }
       const float base = softmax_base(token_max<LPT>(top));
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        all[i] = li + i * LPT < p.experts ? exp((double)v[i] - base) : 0;
+        all[i] = exp((double)v[i] - base);
         total += all[i];
         if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
@@ -483,7 +610,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
     const bool vec = p.experts % N == 0 && (reinterpret_cast<uintptr_t>(p.dlogits) & 15) == 0;
     for (int n = 0; n < TOKENS; ++n) {
       if (t0 + n >= p.tokens) break;
-      typename E::raw* dx = static_cast<typename E::raw*>(p.dlogits) + (t0 + n) * p.experts;
+      typename E::raw* dx = static_cast<typename E::raw*>(p.dlogits) + (int64_t)(t0 + n) * p.experts;
       const float* from = s_row[wave][n];
       if (vec) {
         for (int i = lane * N; i < p.experts; i += 64 * N) {
@@ -498,7 +625,6 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
         for (int i = lane; i < p.experts; i += 64) dx[i] = from_float<E>(from[i]);
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // read before the next tokens' rows are written
   }
 }
 

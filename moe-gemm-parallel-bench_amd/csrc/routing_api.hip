@@ -39,43 +39,84 @@ int check_route(const RouteParams& p, int32_t dtype) {
 
 constexpr int64_t kMaxBlocks = 1 << 16;  // workgroups of a launch; they go on to the tokens and rows past them
 
-// Whether route_kernel's lanes hold the choice: one chosen expert a lane, and groups that are whole lanes' experts, as many
-// to each.  Else every token takes the 64-bit path (16384 tokens over 256 experts, 4 of 8 groups, 8 experts: REPLACE).
-bool fast_route(const RouteParams& p, int lanes) {
-  return p.k <= lanes && (p.groups == 1 || (p.groups <= 16 && lanes % p.groups == 0 && p.experts % lanes == 0));
+// Whether route_kernel can choose: k on a list of `top` with two to spare where scores may be too close to call, and groups
+// that are whole lanes' experts, as many to each.
+template <class E, RouteRank RANK>
+bool fast_route(const RouteParams& p, int lanes, int top) {
+  return p.k <= (RANK >= RANK_SIGMOID || E::is_f32 ? top - 2 : top) &&
+         (p.groups == 1 || (p.groups <= 16 && lanes % p.groups == 0 && p.experts % lanes == 0));
 }
 
-template <class E, int LPT, int PER>
-hipError_t launch_route(const RouteParams& p, bool backward, hipStream_t stream) {
-  constexpr int WIDE = LPT * PER <= 64 ? 1 : LPT * PER / 64;
-  const size_t lds = 4 * (p.experts + p.groups) * sizeof(uint64_t);  // route_token's arrays, at most 64 KiB
-  auto grid = [&](int64_t tokens) { return dim3((unsigned)std::min(cdiv(p.tokens, tokens), kMaxBlocks)); };
-  if (backward) {
-    if (p.k <= LPT) hipLaunchKernelGGL((route_backward_kernel<E, LPT, PER>), grid(256 / LPT), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((route_backward_kernel<E, 64, WIDE>), grid(4), dim3(256), 0, stream, p);
-  } else if (fast_route(p, LPT)) {
-    hipLaunchKernelGGL((route_kernel<E, LPT, PER>), grid(256 / LPT), dim3(256), lds, stream, p);
-  } else {
-    hipLaunchKernelGGL((route_exact_kernel<E>), grid(4), dim3(256), lds, stream, p);
-  }
+dim3 route_grid(const RouteParams& p, int64_t tokens) { return dim3((unsigned)cdiv(p.tokens, tokens)); }
+size_t route_lds(const RouteParams& p) { return 4 * (p.experts + p.groups) * sizeof(uint64_t); }  // at most 64 KiB
+
+template <class E, int LPT, int PER, int TOP, RouteRank RANK>
+hipError_t launch_choice(const RouteParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL((route_kernel<E, LPT, PER, TOP, RANK>), route_grid(p, 256 / LPT), dim3(256), route_lds(p), stream, p);
   return hipGetLastError();
 }
-// 16 lanes a token up to 256 experts, then all 64.
+// 16 lanes a token for lists of 16 from up to 256 experts, else all 64.
+template <class E, RouteRank RANK>
+hipError_t launch_choice(const RouteParams& p, hipStream_t stream) {
+  if (p.experts <= 256 && fast_route<E, RANK>(p, 16, 16)) {
+    const int64_t per = cdiv(p.experts, 16);
+    return per <= 4   ? launch_choice<E, 16, 4, 16, RANK>(p, stream)
+           : per <= 8 ? launch_choice<E, 16, 8, 16, RANK>(p, stream)
+                      : launch_choice<E, 16, 16, 16, RANK>(p, stream);
+  }
+  if (p.experts > 256 && fast_route<E, RANK>(p, 64, 16))
+    return p.experts <= 512 ? launch_choice<E, 64, 8, 16, RANK>(p, stream) : launch_choice<E, 64, 16, 16, RANK>(p, stream);
+  if (fast_route<E, RANK>(p, 64, 32))
+    return p.experts <= 256 ? launch_choice<E, 64, 4, 32, RANK>(p, stream) : launch_choice<E, 64, 16, 32, RANK>(p, stream);
+  hipLaunchKernelGGL((route_exact_kernel<E>), route_grid(p, 4), dim3(256), route_lds(p), stream, p);
+  return hipGetLastError();
+}
+template <class E, int LPT, int PER>
+hipError_t launch_gradient(const RouteParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL((route_backward_kernel<E, LPT, PER>), route_grid(p, 256 / LPT), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+// 16 lanes a token up to 16 chosen of 256 experts, else all 64.
+template <class E>
+hipError_t launch_gradient(const RouteParams& p, hipStream_t stream) {
+  if (p.k <= 16 && p.experts <= 256) {
+    const int64_t per = cdiv(p.experts, 16);
+    return per <= 4   ? launch_gradient<E, 16, 4>(p, stream)
+           : per <= 8 ? launch_gradient<E, 16, 8>(p, stream)
+                      : launch_gradient<E, 16, 16>(p, stream);
+  }
+  return p.experts <= 256   ? launch_gradient<E, 64, 4>(p, stream)
+         : p.experts <= 512 ? launch_gradient<E, 64, 8>(p, stream)
+                            : launch_gradient<E, 64, 16>(p, stream);
+}
 template <class E>
 hipError_t launch_route(const RouteParams& p, bool backward, hipStream_t stream) {
-  const int64_t per = cdiv(p.experts, 16);
-  return per <= 2    ? launch_route<E, 16, 2>(p, backward, stream)
-         : per <= 4  ? launch_route<E, 16, 4>(p, backward, stream)
-         : per <= 8  ? launch_route<E, 16, 8>(p, backward, stream)
-         : per <= 16 ? launch_route<E, 16, 16>(p, backward, stream)
-         : per <= 32 ? launch_route<E, 64, 8>(p, backward, stream)
-                     : launch_route<E, 64, 16>(p, backward, stream);
+  if (backward) return launch_gradient<E>(p, stream);
+  if (p.bias || p.group_best == 2)
+    return p.sigmoid ? launch_choice<E, RANK_SIGMOID>(p, stream) : launch_choice<E, RANK_SOFTMAX>(p, stream);
+  return p.sigmoid || p.normalize ? launch_choice<E, RANK_LOGITS>(p, stream) : launch_choice<E, RANK_LOGITS_SUM>(p, stream);
 }
-int launch_route(const RouteParams& p, bool backward, int32_t dtype, void* stream) {
+int launch_route(RouteParams p, bool backward, int32_t dtype, void* stream) {
+  constexpr int32_t kTokens = 1 << 25;  // of a launch: it counts threads in 32 bits, at most 64 a token
   const auto s = reinterpret_cast<hipStream_t>(stream);
-  return checked(dtype == DT_F32    ? launch_route<EF32>(p, backward, s)
-                 : dtype == DT_BF16 ? launch_route<EBf16>(p, backward, s)
-                                    : launch_route<EF16>(p, backward, s));
+  const int64_t es = element_bytes(dtype);
+  for (int32_t left = p.tokens; left > 0; left -= kTokens) {
+    p.tokens = std::min(left, kTokens);
+    const int rc = checked(dtype == DT_F32    ? launch_route<EF32>(p, backward, s)
+                           : dtype == DT_BF16 ? launch_route<EBf16>(p, backward, s)
+                                              : launch_route<EF16>(p, backward, s));
+    if (rc != MOEGEMM_OK) return rc;
+    const int64_t picks = (int64_t)p.tokens * p.k;
+    p.logits = static_cast<const char*>(p.logits) + p.tokens * p.ldl * es;
+    p.chosen += picks;
+    if (backward) {
+      p.dweights += picks;
+      p.dlogits = static_cast<char*>(p.dlogits) + (int64_t)p.tokens * p.experts * es;
+    } else {
+      p.weights += picks;
+    }
+  }
+  return MOEGEMM_OK;
 }
 
 // Entries of a workgroup: at most kSortBlocks workgroups, each of which reads all counts.
