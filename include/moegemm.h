@@ -429,7 +429,7 @@ int moegemm_route_topk_backward(const float* dweights, const void* logits, const
  * at most 1024).  offs [count]: end rows; slots [entries]: the entry of each sorted row, -1 at and past the last end
  * row; places [entries]: the sorted row of each entry, -1 for other experts.  `workspace` holds
  * moegemm_sort_workspace_bytes() bytes (< 0 on bad arguments) and need not be cleared; calls that share one must not overlap.
- * Two launches.
+ * One launch up to 8192 entries (and no workspace), else two.
  */
 int64_t moegemm_sort_workspace_bytes(int64_t entries, int32_t count);
 int moegemm_sort_by_expert(const int32_t* experts, int32_t* offs, int32_t* slots, int32_t* places, int32_t entries,

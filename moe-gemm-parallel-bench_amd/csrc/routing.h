@@ -643,6 +643,87 @@ __device__ __forceinline__ int local_expert(const SortParams& p, int64_t i) {
   return e >= 0 && e < p.count ? (int)e : -1;
 }
 
+// Entries [from, from + span) of a wave, 64 at a time: an entry's place is its expert's next one in `next` plus the entries of
+// its expert on lower lanes, found by matching the experts' bits across the lanes.
+__device__ __forceinline__ void place_entries(const SortParams& p, int64_t begin, int span, int32_t* next) {
+  const int lane = threadIdx.x & 63;
+  const int bits = 32 - __builtin_clz((unsigned)p.count);
+  for (int i = 0; i < span; i += 64) {
+    const int64_t from = begin + i + lane;
+    const int e = local_expert(p, from);
+    uint64_t same = __ballot(e >= 0);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((e >> b) & 1);
+      same &= (e >> b) & 1 ? set : ~set;
+    }
+    int base = 0;
+    const int leader = e >= 0 ? __builtin_ctzll(same) : lane;
+    if (e >= 0 && lane == leader) base = atomicAdd(&next[e], __builtin_popcountll(same));
+    base = __shfl(base, leader);
+    const int place = e >= 0 ? base + __builtin_popcountll(same & ((1ull << lane) - 1)) : -1;
+    if (from < p.n) p.places[from] = place;
+    if (place >= 0) p.slots[place] = (int32_t)from;
+  }
+}
+
+// Exclusive sums over the workgroup's threads; `sums` holds one number a wave.  Every thread calls it.
+template <int WAVES>
+__device__ __forceinline__ int exclusive_sum(int x, int32_t* sums, int& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int sum = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int below = __shfl_up(sum, d);
+    sum += lane >= d ? below : 0;
+  }
+  if (lane == 63) sums[wave] = sum;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int n = sums[w];
+    before += w < wave ? n : 0;
+    all += n;
+  }
+  return before + sum - x;
+}
+
+// All entries in one workgroup of 16 waves: count, sum, place.  Counts are sums of integers and every order is that of the
+// entries, so the result is the same at every call.
+__global__ void __launch_bounds__(1024) sort_whole_kernel(SortParams p) {
+  extern __shared__ int32_t s_next[];  // [16][count]
+  __shared__ int32_t s_sums[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, span = p.chunk / 16;
+  for (int e = threadIdx.x; e < 16 * p.count; e += 1024) s_next[e] = 0;
+  __syncthreads();
+  int32_t* own = s_next + wave * p.count;
+  for (int i = lane; i < span; i += 64) {
+    const int e = local_expert(p, wave * span + i);
+    if (e >= 0) atomicAdd(&own[e], 1);
+  }
+  __syncthreads();
+  const int e = threadIdx.x;  // at most 1024 experts
+  int counts[16], total = 0, used;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    counts[w] = e < p.count ? s_next[w * p.count + e] : 0;
+    total += counts[w];
+  }
+  int at = exclusive_sum<16>(total, s_sums, used);
+  if (e < p.count) {
+    p.offs[e] = at + total;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      s_next[w * p.count + e] = at;
+      at += counts[w];
+    }
+  }
+  __syncthreads();
+  place_entries(p, wave * span, span, own);
+  for (int i = used + threadIdx.x; i < p.n; i += 1024) p.slots[i] = -1;  // rows behind the last expert's
+}
+
 // How often each expert occurs in a workgroup's chunk.
 __global__ void __launch_bounds__(256) sort_count_kernel(SortParams p) {
   __shared__ int32_t s_count[kSortExperts];
@@ -658,75 +739,70 @@ __global__ void __launch_bounds__(256) sort_count_kernel(SortParams p) {
 }
 
 // Places of a workgroup's chunk: behind the smaller experts, the earlier workgroups and waves, and the wave's own earlier
-// entries, which it finds 64 at a time by matching the experts' bits across its lanes.  Counts are sums of integers and
-// every order is that of the entries, so the result is the same at every call.
+// entries.  Each workgroup sums the counts of all for itself: reading them is cheaper than another launch.
 __global__ void __launch_bounds__(256) sort_place_kernel(SortParams p) {
   __shared__ int32_t s_next[4][kSortExperts];
-  __shared__ int32_t s_part[256];
+  __shared__ int32_t s_total[kSortExperts], s_sums[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t begin = (int64_t)blockIdx.x * p.chunk;
-  const int span = p.chunk / 4;
+  const int span = p.chunk / 4, blocks = (int)gridDim.x, block = (int)blockIdx.x;
   for (int e = threadIdx.x; e < 4 * kSortExperts; e += 256) (&s_next[0][0])[e] = 0;
   __syncthreads();
   for (int i = lane; i < span; i += 64) {
     const int e = local_expert(p, begin + wave * span + i);
     if (e >= 0) atomicAdd(&s_next[wave][e], 1);
   }
-  // Four consecutive experts a thread: their counts in all workgroups and in the earlier ones.
-  int total[4] = {}, before[4] = {}, sum = 0;
+  int before[kSortExperts / 256];
+#pragma unroll
+  for (int i = 0; i < kSortExperts / 256; ++i) {
+    const int e = threadIdx.x + 256 * i;
+    if (e >= p.count) break;
+    int total = 0, earlier = 0;
+    for (int b0 = 0; b0 < blocks; b0 += 16) {  // 16 counts on their way at a time
+      int n[16];
+#pragma unroll
+      for (int b = 0; b < 16; ++b) n[b] = p.counts[(int64_t)min(b0 + b, blocks - 1) * p.count + e];
+#pragma unroll
+      for (int b = 0; b < 16; ++b) {
+        total += b0 + b < blocks ? n[b] : 0;
+        earlier += b0 + b < block ? n[b] : 0;
+      }
+    }
+    s_total[e] = total;
+    before[i] = earlier;
+  }
+  __syncthreads();
+  int sum = 0, used;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int e = threadIdx.x * 4 + i;
-    if (e < p.count)
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const int n = p.counts[(int64_t)b * p.count + e];
-        total[i] += n;
-        before[i] += b < (int)blockIdx.x ? n : 0;
-      }
-    sum += total[i];
+    sum += e < p.count ? s_total[e] : 0;
   }
-  s_part[threadIdx.x] = sum;
-  __syncthreads();
-  for (int d = 1; d < 256; d <<= 1) {
-    const int below = (int)threadIdx.x >= d ? s_part[threadIdx.x - d] : 0;
-    __syncthreads();
-    s_part[threadIdx.x] += below;
-    __syncthreads();
-  }
-  int at = s_part[threadIdx.x] - sum;
+  int at = exclusive_sum<4>(sum, s_sums, used);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int e = threadIdx.x * 4 + i;
     if (e >= p.count) break;
-    int next = at + before[i];
+    const int total = s_total[e];
+    s_total[e] = at;  // where the expert starts
+    at += total;
+    if (block == 0) p.offs[e] = at;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSortExperts / 256; ++i) {
+    const int e = threadIdx.x + 256 * i;
+    if (e >= p.count) break;
+    int next = s_total[e] + before[i];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const int n = s_next[w][e];
       s_next[w][e] = next;
       next += n;
     }
-    at += total[i];
-    if (blockIdx.x == 0) p.offs[e] = at;
   }
   __syncthreads();
-  const int used = s_part[255];
-  const int bits = 32 - __builtin_clz((unsigned)p.count);
-  for (int i = 0; i < span; i += 64) {
-    const int64_t from = begin + wave * span + i + lane;
-    const int e = local_expert(p, from);
-    uint64_t same = __ballot(e >= 0);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot((e >> b) & 1);
-      same &= (e >> b) & 1 ? set : ~set;
-    }
-    int base = 0;
-    const int leader = e >= 0 ? __builtin_ctzll(same) : lane;
-    if (e >= 0 && lane == leader) base = atomicAdd(&s_next[wave][e], __builtin_popcountll(same));
-    base = __shfl(base, leader);
-    const int place = e >= 0 ? base + __builtin_popcountll(same & ((1ull << lane) - 1)) : -1;
-    if (from < p.n) p.places[from] = place;
-    if (place >= 0) p.slots[place] = (int32_t)from;
-  }
+  place_entries(p, begin + wave * span, span, s_next[wave]);
   for (int i = threadIdx.x; i < p.chunk; i += 256)  // rows behind the last expert's
     if (begin + i >= used && begin + i < p.n) p.slots[begin + i] = -1;
 }
@@ -755,6 +831,23 @@ __device__ __forceinline__ void clear_rows(const RowsParams& p, int block, int b
 
 constexpr int kClearBlocks = 256;
 
+// A token's places (and weights), one a lane; at(j) is slot j's, -1 where no row of the call belongs to it.
+struct Places {
+  int place;
+  float weight;
+  __device__ __forceinline__ void load(const RowsParams& p, int64_t t, int j0) {
+    const int j = j0 + (int)(threadIdx.x & 63);
+    const int64_t slot = t * p.k + min(j, p.k - 1);
+    const int at = p.places[slot];
+    weight = p.weights ? p.weights[slot] : 1.0f;
+    place = at >= 0 && at < p.rows ? at : -1;
+  }
+  __device__ __forceinline__ int at(int j) const { return __builtin_amdgcn_readlane(place, j); }
+  __device__ __forceinline__ float weight_at(int j) const {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), j));
+  }
+};
+
 // A wave copies up to SPAN x 64 units of one token to all its places: a token is read once.
 template <class U>
 __global__ void __launch_bounds__(256) gather_rows_kernel(RowsParams p) {
@@ -771,13 +864,18 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(RowsParams p) {
       const int64_t c = c0 + u * 64 * sizeof(U);
       if (c < p.width) v[u] = *reinterpret_cast<const U*>(p.from + t * p.ld_from + c);
     }
-    for (int j = 0; j < p.k; ++j) {
-      const int place = p.places[t * p.k + j];
-      if (place < 0 || place >= p.rows) continue;
+    for (int j0 = 0; j0 < p.k; j0 += 64) {
+      Places places;
+      places.load(p, t, j0);
+      for (int j = 0; j < min(p.k - j0, 64); ++j) {
+        const int place = places.at(j);
+        if (place < 0) continue;
+        char* to = p.to + (int64_t)place * p.ld_to;
 #pragma unroll
-      for (int u = 0; u < SPAN; ++u) {
-        const int64_t c = c0 + u * 64 * sizeof(U);
-        if (c < p.width) *reinterpret_cast<U*>(p.to + (int64_t)place * p.ld_to + c) = v[u];
+        for (int u = 0; u < SPAN; ++u) {
+          const int64_t c = c0 + u * 64 * sizeof(U);
+          if (c < p.width) *reinterpret_cast<U*>(to + c) = v[u];
+        }
       }
     }
   }
@@ -803,29 +901,47 @@ struct Unit {
   }
 };
 
-// A wave sums one span of a token's rows in the order of its slots, in fp32, and rounds once.
+// A wave sums one span of a token's rows in the order of its slots, in fp32, and rounds once.  Four rows are on their way at a
+// time.
 template <class E, class U>
 __global__ void __launch_bounds__(256) combine_rows_kernel(RowsParams p) {
   using Q = Unit<E, U>;
-  constexpr int SPAN = 2;
+  constexpr int SPAN = 2, AHEAD = 4;
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * 4;
   for (int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); item < p.tokens * p.spans; item += waves) {
     const int64_t t = item / p.spans;
     const int64_t c0 = ((item - t * p.spans) * SPAN * 64 + lane) * (int64_t)sizeof(U);
     float sum[SPAN][Q::N] = {};
-    for (int j = 0; j < p.k; ++j) {
-      const int place = p.places[t * p.k + j];
-      if (place < 0 || place >= p.rows) continue;
-      const float w = p.weights ? p.weights[t * p.k + j] : 1.0f;
+    for (int j0 = 0; j0 < p.k; j0 += 64) {
+      Places places;
+      places.load(p, t, j0);
+      const int count = min(p.k - j0, 64);
+      for (int j = 0; j < count; j += AHEAD) {
+        U v[AHEAD][SPAN] = {};
 #pragma unroll
-      for (int u = 0; u < SPAN; ++u) {
-        const int64_t c = c0 + u * 64 * sizeof(U);
-        if (c >= p.width) continue;
-        float v[Q::N];
-        Q::widen(*reinterpret_cast<const U*>(p.from + (int64_t)place * p.ld_from + c), v);
+        for (int a = 0; a < AHEAD; ++a) {
+          const int place = places.at(min(j + a, count - 1));
+          if (j + a >= count || place < 0) continue;
+          const char* from = p.from + (int64_t)place * p.ld_from;
 #pragma unroll
-        for (int i = 0; i < Q::N; ++i) sum[u][i] += w * v[i];
+          for (int u = 0; u < SPAN; ++u) {
+            const int64_t c = c0 + u * 64 * sizeof(U);
+            if (c < p.width) v[a][u] = *reinterpret_cast<const U*>(from + c);
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+          if (j + a >= count || places.at(min(j + a, count - 1)) < 0) continue;
+          const float w = places.weight_at(j + a);
+#pragma unroll
+          for (int u = 0; u < SPAN; ++u) {
+            float f[Q::N];
+            Q::widen(v[a][u], f);
+#pragma unroll
+            for (int i = 0; i < Q::N; ++i) sum[u][i] += w * f[i];
+          }
+        }
       }
     }
 #pragma unroll

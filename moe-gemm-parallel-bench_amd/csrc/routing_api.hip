@@ -119,9 +119,12 @@ int launch_route(RouteParams p, bool backward, int32_t dtype, void* stream) {
   return MOEGEMM_OK;
 }
 
-// Entries of a workgroup: at most kSortBlocks workgroups, each of which reads all counts.
-constexpr int64_t kSortChunk = 2048, kSortBlocks = 256;
-int64_t sort_chunk(int64_t n) { return cdiv(std::max(kSortChunk, cdiv(n, kSortBlocks)), 256) * 256; }
+// Up to so many entries one workgroup sorts all of them (REPLACE).
+constexpr int64_t kSortWhole = 8192;
+// Entries of a workgroup of the others: 64 workgroups, or more of 16384 entries up to 256, since each reads all counts.
+int64_t sort_chunk(int64_t n) {
+  return cdiv(std::max({std::min(cdiv(n, 64), int64_t(16384)), cdiv(n, 256), int64_t(1024)}), 256) * 256;
+}
 
 // The widest unit that rows and their pitches allow.
 int64_t unit_bytes(int64_t width, std::initializer_list<std::pair<const void*, int64_t>> rows) {
@@ -136,9 +139,7 @@ int64_t unit_bytes(int64_t width, std::initializer_list<std::pair<const void*, i
   return unit;
 }
 
-struct U16 {
-  uint32_t v[4];
-} __attribute__((aligned(16)));
+using U16 = u32x4_t;
 
 // `end` may be null where no rows are cleared.
 int check_rows(int64_t tokens, int32_t k, int32_t rows, int64_t width, const int32_t* places, const int32_t* end, bool clears) {
@@ -202,7 +203,7 @@ int64_t moegemm_sort_workspace_bytes(int64_t entries, int32_t count) {
   if (entries < 0 || entries > INT32_MAX || count <= 0 || count > kSortExperts)
     return report(MOEGEMM_ERR_INVALID, "bad sort (%lld entries, %d experts of at most %d)", (long long)entries, count,
                   kSortExperts);
-  return std::max<int64_t>(cdiv(entries, sort_chunk(entries)), 1) * count * 4;
+  return entries <= kSortWhole ? 0 : cdiv(entries, sort_chunk(entries)) * count * 4;
 }
 
 int moegemm_sort_by_expert(const int32_t* experts, int32_t* offs, int32_t* slots, int32_t* places, int32_t entries,
@@ -210,14 +211,19 @@ int moegemm_sort_by_expert(const int32_t* experts, int32_t* offs, int32_t* slots
   const int64_t need = moegemm_sort_workspace_bytes(entries, count);
   if (need < 0) return (int)need;
   if (first < 0) return report(MOEGEMM_ERR_INVALID, "the first expert must not be negative (got %d)", first);
-  if (!offs || !workspace || (entries && (!experts || !slots || !places)))
+  if (!offs || (!workspace && need) || (entries && (!experts || !slots || !places)))
     return report(MOEGEMM_ERR_INVALID, "experts, offs, slots, places and workspace must be non-null");
   if (workspace_bytes < need)
     return report(MOEGEMM_ERR_INVALID, "the workspace holds %lld bytes of %lld", (long long)workspace_bytes, (long long)need);
-  const int64_t chunk = sort_chunk(entries);
-  SortParams p{experts, offs, slots, places, static_cast<int32_t*>(workspace), entries, first, count, (int32_t)chunk};
-  const dim3 grid((unsigned)std::max<int64_t>(cdiv(entries, chunk), 1));
   const auto s = reinterpret_cast<hipStream_t>(stream);
+  const bool whole = entries <= kSortWhole;
+  const int64_t chunk = whole ? cdiv(entries, 1024) * 1024 : sort_chunk(entries);
+  SortParams p{experts, offs, slots, places, static_cast<int32_t*>(workspace), entries, first, count, (int32_t)chunk};
+  if (whole) {
+    hipLaunchKernelGGL(sort_whole_kernel, dim3(1), dim3(1024), 16 * count * sizeof(int32_t), s, p);
+    return checked(hipGetLastError());
+  }
+  const dim3 grid((unsigned)cdiv(entries, chunk));
   hipLaunchKernelGGL(sort_count_kernel, grid, dim3(256), 0, s, p);
   const int rc = checked(hipGetLastError());
   if (rc != MOEGEMM_OK) return rc;

@@ -154,10 +154,11 @@ def sort_by_expert(experts, num_experts: int, *, first: int = 0) -> ExpertOrder:
     if entries > _native.INT32_MAX or experts.shape[1] == 0:
         raise ValueError(f"sort_by_expert takes 1 or more experts a token and under 2**31 in all (got {tuple(experts.shape)})")
     nbytes = lib.moegemm_sort_workspace_bytes(entries, num_experts)
-    workspace = experts.new_empty((nbytes // 4,))
+    workspace = experts.new_empty((nbytes // 4,)) if nbytes else None
     offs, slots, places = experts.new_empty((num_experts,)), experts.new_empty((entries,)), torch.empty_like(experts)
     _native.launch(experts.device, lib.moegemm_sort_by_expert, experts.data_ptr(), offs.data_ptr(), slots.data_ptr(),
-                   places.data_ptr(), entries, first, num_experts, workspace.data_ptr(), nbytes)
+                   places.data_ptr(), entries, first, num_experts,
+                   workspace.data_ptr() if nbytes else None, nbytes)
     return ExpertOrder(offs, slots, places)
 
 

@@ -146,7 +146,7 @@ def test_other_entries_refuse():
         lib.moegemm_sort_by_expert(4096, 4096, 4096, 4096, 8, -1, 4, 4096, 4096, None),
         lib.moegemm_sort_by_expert(4096, 4096, 4096, 4096, 8, 0, 0, 4096, 4096, None),
         lib.moegemm_sort_by_expert(4096, 4096, 4096, 4096, 8, 0, 1025, 4096, 4096, None),
-        lib.moegemm_sort_by_expert(4096, 4096, 4096, 4096, 8, 0, 4, 4096, 15, None),
+        lib.moegemm_sort_by_expert(4096, 4096, 4096, 4096, 10 ** 6, 0, 4, 4096, 15, None),
         lib.moegemm_sort_by_expert(None, 4096, 4096, 4096, 8, 0, 4, 4096, 4096, None),
         lib.moegemm_sort_by_expert(4096, 4096, 4096, 4096, -1, 0, 4, 4096, 4096, None),
         lib.moegemm_gather_rows(4096, 4096, 4096, None, 4, 2, 8, 16, 16, 16, None),
@@ -161,4 +161,4 @@ def test_other_entries_refuse():
     ]
     assert bad == [_native.ERR_INVALID] * len(bad)
     assert lib.moegemm_sort_workspace_bytes(2 ** 31, 4) == _native.ERR_INVALID
-    assert lib.moegemm_sort_workspace_bytes(100, 4) > 0
+    assert lib.moegemm_sort_workspace_bytes(100, 4) == 0 and lib.moegemm_sort_workspace_bytes(10 ** 6, 4) > 15
