@@ -820,6 +820,19 @@ struct RowsParams {
   int32_t k, rows, width, spans;    // width in bytes; spans of a row
 };
 
+// Sorted rows are read and written once by a call.  NT: they are too many to stay in the caches for the next one, and go past
+// them (non-temporal), which leaves those to the tokens.
+template <bool NT, class U>
+__device__ __forceinline__ U load_row(const char* from) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const U*>(from));
+  else return *reinterpret_cast<const U*>(from);
+}
+template <bool NT, class U>
+__device__ __forceinline__ void store_row(char* to, U u) {
+  if constexpr (NT) __builtin_nontemporal_store(u, reinterpret_cast<U*>(to));
+  else *reinterpret_cast<U*>(to) = u;
+}
+
 // Rows that no token went to are zeros.
 template <class U>
 __device__ __forceinline__ void clear_rows(const RowsParams& p, int block, int blocks) {
@@ -849,7 +862,7 @@ struct Places {
 };
 
 // A wave copies up to SPAN x 64 units of one token to all its places: a token is read once.
-template <class U>
+template <class U, bool NT>
 __global__ void __launch_bounds__(256) gather_rows_kernel(RowsParams p) {
   constexpr int SPAN = 4;
   if (blockIdx.x < kClearBlocks) return clear_rows<U>(p, blockIdx.x, kClearBlocks);
@@ -874,7 +887,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(RowsParams p) {
 #pragma unroll
         for (int u = 0; u < SPAN; ++u) {
           const int64_t c = c0 + u * 64 * sizeof(U);
-          if (c < p.width) *reinterpret_cast<U*>(to + c) = v[u];
+          if (c < p.width) store_row<NT>(to + c, v[u]);
         }
       }
     }
@@ -903,7 +916,7 @@ struct Unit {
 
 // A wave sums one span of a token's rows in the order of its slots, in fp32, and rounds once.  Four rows are on their way at a
 // time.
-template <class E, class U>
+template <class E, class U, bool NT>
 __global__ void __launch_bounds__(256) combine_rows_kernel(RowsParams p) {
   using Q = Unit<E, U>;
   constexpr int SPAN = 2, AHEAD = 4;
@@ -927,7 +940,7 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(RowsParams p) {
 #pragma unroll
           for (int u = 0; u < SPAN; ++u) {
             const int64_t c = c0 + u * 64 * sizeof(U);
-            if (c < p.width) v[a][u] = *reinterpret_cast<const U*>(from + c);
+            if (c < p.width) v[a][u] = load_row<NT, U>(from + c);
           }
         }
 #pragma unroll
@@ -953,7 +966,7 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(RowsParams p) {
 }
 
 // One routed row a wave: dy = w dout and dw = <dout, y>, the product's sum over its lanes in one fixed order.
-template <class E, class U>
+template <class E, class U, bool NT>
 __global__ void __launch_bounds__(256) combine_rows_backward_kernel(RowsParams p) {
   using Q = Unit<E, U>;
   if (blockIdx.x < kClearBlocks) {
@@ -973,14 +986,14 @@ __global__ void __launch_bounds__(256) combine_rows_backward_kernel(RowsParams p
         float d[Q::N], y[Q::N];
         Q::widen(*reinterpret_cast<const U*>(dout + c), d);
         if (p.dweights) {
-          Q::widen(*reinterpret_cast<const U*>(p.from + (int64_t)place * p.ld_from + c), y);
+          Q::widen(load_row<NT, U>(p.from + (int64_t)place * p.ld_from + c), y);
 #pragma unroll
           for (int i = 0; i < Q::N; ++i) dot += d[i] * y[i];
         }
         if (p.to) {
 #pragma unroll
           for (int i = 0; i < Q::N; ++i) d[i] *= w;
-          *reinterpret_cast<U*>(p.to + (int64_t)place * p.ld_to + c) = Q::narrow(d);
+          store_row<NT>(p.to + (int64_t)place * p.ld_to + c, Q::narrow(d));
         }
       }
     }

@@ -150,18 +150,26 @@ int check_rows(int64_t tokens, int32_t k, int32_t rows, int64_t width, const int
   return MOEGEMM_OK;
 }
 
+// Whether the sorted rows go past the caches: from 128 MiB of them on (8 rows a token of 14336 bytes, us for combine, its
+// gradients and gather: 59 MB kept 11.8, 18.9, 10.1, past 12.3, 28.1, 11.9; 117 MB 25.5, 47.0, 24.0 and 23.6, 48.4, 23.8; 470 MB
+// 106, 207, 106 and 92, 194, 95).
+bool past_caches(int64_t rows, int64_t width, int64_t unit) { return unit == 16 && rows * width >= int64_t(128) << 20; }
+
 template <class E>
 hipError_t launch_combine(const RowsParams& p, int64_t unit, dim3 grid, hipStream_t s) {
   using raw = typename E::raw;
-  if (unit == 16) hipLaunchKernelGGL((combine_rows_kernel<E, U16>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((combine_rows_kernel<E, raw>), grid, dim3(256), 0, s, p);
+  if (past_caches(p.rows, p.width, unit)) hipLaunchKernelGGL((combine_rows_kernel<E, U16, true>), grid, dim3(256), 0, s, p);
+  else if (unit == 16) hipLaunchKernelGGL((combine_rows_kernel<E, U16, false>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((combine_rows_kernel<E, raw, false>), grid, dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <class E>
 hipError_t launch_combine_backward(const RowsParams& p, int64_t unit, dim3 grid, hipStream_t s) {
   using raw = typename E::raw;
-  if (unit == 16) hipLaunchKernelGGL((combine_rows_backward_kernel<E, U16>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((combine_rows_backward_kernel<E, raw>), grid, dim3(256), 0, s, p);
+  if (past_caches(p.rows, p.width, unit))
+    hipLaunchKernelGGL((combine_rows_backward_kernel<E, U16, true>), grid, dim3(256), 0, s, p);
+  else if (unit == 16) hipLaunchKernelGGL((combine_rows_backward_kernel<E, U16, false>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((combine_rows_backward_kernel<E, raw, false>), grid, dim3(256), 0, s, p);
   return hipGetLastError();
 }
 
@@ -243,11 +251,14 @@ int moegemm_gather_rows(const void* x, void* out, const int32_t* places, const i
   const dim3 grid((unsigned)(kClearBlocks + std::min(cdiv(tokens * spans, 4), kMaxBlocks)));
   const auto s = reinterpret_cast<hipStream_t>(stream);
   switch (unit) {
-    case 16: hipLaunchKernelGGL(gather_rows_kernel<U16>, grid, dim3(256), 0, s, p); break;
-    case 8: hipLaunchKernelGGL(gather_rows_kernel<uint64_t>, grid, dim3(256), 0, s, p); break;
-    case 4: hipLaunchKernelGGL(gather_rows_kernel<uint32_t>, grid, dim3(256), 0, s, p); break;
-    case 2: hipLaunchKernelGGL(gather_rows_kernel<uint16_t>, grid, dim3(256), 0, s, p); break;
-    default: hipLaunchKernelGGL(gather_rows_kernel<uint8_t>, grid, dim3(256), 0, s, p);
+    case 16:
+      if (past_caches(rows, row_bytes, unit)) hipLaunchKernelGGL((gather_rows_kernel<U16, true>), grid, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((gather_rows_kernel<U16, false>), grid, dim3(256), 0, s, p);
+      break;
+    case 8: hipLaunchKernelGGL((gather_rows_kernel<uint64_t, false>), grid, dim3(256), 0, s, p); break;
+    case 4: hipLaunchKernelGGL((gather_rows_kernel<uint32_t, false>), grid, dim3(256), 0, s, p); break;
+    case 2: hipLaunchKernelGGL((gather_rows_kernel<uint16_t, false>), grid, dim3(256), 0, s, p); break;
+    default: hipLaunchKernelGGL((gather_rows_kernel<uint8_t, false>), grid, dim3(256), 0, s, p);
   }
   return checked(hipGetLastError());
 }
