@@ -634,23 +634,39 @@ struct SortParams {
   int32_t* slots;          // [n]
   int32_t* places;         // [n]
   int32_t* counts;         // workspace [blocks][count]
-  int32_t n, first, count, chunk;  // chunk: entries of a workgroup, a multiple of 256
+  int32_t n, first, count, chunk;  // chunk: entries of a workgroup, a multiple of 1024
 };
 
-__device__ __forceinline__ int local_expert(const SortParams& p, int64_t i) {
-  if (i >= p.n) return -1;
-  const int64_t e = (int64_t)p.experts[i] - p.first;
-  return e >= 0 && e < p.count ? (int)e : -1;
+// 64 N entries from `begin` on, one a lane each time, -1 for those that are none of the call's.
+template <int N>
+__device__ __forceinline__ void load_entries(const SortParams& p, int64_t begin, int (&e)[N]) {
+  const int lane = threadIdx.x & 63;
+  int raw[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)  // no branch around a load, but no load where there is no entry at all
+    raw[i] = p.n > 0 ? p.experts[min(begin + i * 64 + lane, (int64_t)p.n - 1)] : 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t local = (int64_t)raw[i] - p.first;
+    e[i] = begin + i * 64 + lane < p.n && local >= 0 && local < p.count ? (int)local : -1;
+  }
 }
-
-// Entries [from, from + span) of a wave, 64 at a time: an entry's place is its expert's next one in `next` plus the entries of
-// its expert on lower lanes, found by matching the experts' bits across the lanes.
-__device__ __forceinline__ void place_entries(const SortParams& p, int64_t begin, int span, int32_t* next) {
+template <int N>
+__device__ __forceinline__ void count_entries(const int (&e)[N], int32_t* counts) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (e[i] >= 0) atomicAdd(&counts[e[i]], 1);
+}
+// An entry's place is its expert's next one in `next` plus the entries of its expert on lower lanes, found by matching the
+// experts' bits across the lanes.
+template <int N>
+__device__ __forceinline__ void place_entries(const SortParams& p, int64_t begin, const int (&entries)[N], int32_t* next) {
   const int lane = threadIdx.x & 63;
   const int bits = 32 - __builtin_clz((unsigned)p.count);
-  for (int i = 0; i < span; i += 64) {
-    const int64_t from = begin + i + lane;
-    const int e = local_expert(p, from);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t from = begin + i * 64 + lane;
+    const int e = entries[i];
     uint64_t same = __ballot(e >= 0);
     for (int b = 0; b < bits; ++b) {
       const uint64_t set = __ballot((e >> b) & 1);
@@ -689,19 +705,19 @@ __device__ __forceinline__ int exclusive_sum(int x, int32_t* sums, int& all) {
   return before + sum - x;
 }
 
-// All entries in one workgroup of 16 waves: count, sum, place.  Counts are sums of integers and every order is that of the
-// entries, so the result is the same at every call.
+// All of up to 1024 N entries in one workgroup of 16 waves: load, count, sum, place.  Counts are sums of integers and every
+// order is that of the entries, so the result is the same at every call.  Bound by its steps' latencies.
+template <int N>
 __global__ void __launch_bounds__(1024) sort_whole_kernel(SortParams p) {
   extern __shared__ int32_t s_next[];  // [16][count]
   __shared__ int32_t s_sums[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, span = p.chunk / 16;
+  const int wave = threadIdx.x >> 6;
+  int entries[N];
+  load_entries(p, wave * 64 * N, entries);
   for (int e = threadIdx.x; e < 16 * p.count; e += 1024) s_next[e] = 0;
   __syncthreads();
   int32_t* own = s_next + wave * p.count;
-  for (int i = lane; i < span; i += 64) {
-    const int e = local_expert(p, wave * span + i);
-    if (e >= 0) atomicAdd(&own[e], 1);
-  }
+  count_entries(entries, own);
   __syncthreads();
   const int e = threadIdx.x;  // at most 1024 experts
   int counts[16], total = 0, used;
@@ -720,7 +736,7 @@ __global__ void __launch_bounds__(1024) sort_whole_kernel(SortParams p) {
     }
   }
   __syncthreads();
-  place_entries(p, wave * span, span, own);
+  place_entries(p, wave * 64 * N, entries, own);
   for (int i = used + threadIdx.x; i < p.n; i += 1024) p.slots[i] = -1;  // rows behind the last expert's
 }
 
@@ -729,10 +745,11 @@ __global__ void __launch_bounds__(256) sort_count_kernel(SortParams p) {
   __shared__ int32_t s_count[kSortExperts];
   for (int e = threadIdx.x; e < p.count; e += 256) s_count[e] = 0;
   __syncthreads();
-  const int64_t begin = (int64_t)blockIdx.x * p.chunk;
-  for (int i = threadIdx.x; i < p.chunk; i += 256) {
-    const int e = local_expert(p, begin + i);
-    if (e >= 0) atomicAdd(&s_count[e], 1);
+  const int64_t begin = (int64_t)blockIdx.x * p.chunk + (threadIdx.x >> 6) * (p.chunk / 4);
+  for (int i = 0; i < p.chunk / 4; i += 256) {
+    int entries[4];
+    load_entries(p, begin + i, entries);
+    count_entries(entries, s_count);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < p.count; e += 256) p.counts[(int64_t)blockIdx.x * p.count + e] = s_count[e];
@@ -743,14 +760,15 @@ __global__ void __launch_bounds__(256) sort_count_kernel(SortParams p) {
 __global__ void __launch_bounds__(256) sort_place_kernel(SortParams p) {
   __shared__ int32_t s_next[4][kSortExperts];
   __shared__ int32_t s_total[kSortExperts], s_sums[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6;
   const int64_t begin = (int64_t)blockIdx.x * p.chunk;
   const int span = p.chunk / 4, blocks = (int)gridDim.x, block = (int)blockIdx.x;
   for (int e = threadIdx.x; e < 4 * kSortExperts; e += 256) (&s_next[0][0])[e] = 0;
   __syncthreads();
-  for (int i = lane; i < span; i += 64) {
-    const int e = local_expert(p, begin + wave * span + i);
-    if (e >= 0) atomicAdd(&s_next[wave][e], 1);
+  int entries[4];
+  for (int i = 0; i < span; i += 256) {
+    load_entries(p, begin + wave * span + i, entries);
+    count_entries(entries, s_next[wave]);
   }
   int before[kSortExperts / 256];
 #pragma unroll
@@ -802,7 +820,10 @@ __global__ void __launch_bounds__(256) sort_place_kernel(SortParams p) {
     }
   }
   __syncthreads();
-  place_entries(p, begin + wave * span, span, s_next[wave]);
+  for (int i = 0; i < span; i += 256) {
+    load_entries(p, begin + wave * span + i, entries);
+    place_entries(p, begin + wave * span + i, entries, s_next[wave]);
+  }
   for (int i = threadIdx.x; i < p.chunk; i += 256)  // rows behind the last expert's
     if (begin + i >= used && begin + i < p.n) p.slots[begin + i] = -1;
 }

@@ -123,7 +123,7 @@ int launch_route(RouteParams p, bool backward, int32_t dtype, void* stream) {
 constexpr int64_t kSortWhole = 8192;
 // Entries of a workgroup of the others: 64 workgroups, or more of 16384 entries up to 256, since each reads all counts.
 int64_t sort_chunk(int64_t n) {
-  return cdiv(std::max({std::min(cdiv(n, 64), int64_t(16384)), cdiv(n, 256), int64_t(1024)}), 256) * 256;
+  return cdiv(std::max({std::min(cdiv(n, 64), int64_t(16384)), cdiv(n, 256), int64_t(1024)}), 1024) * 1024;
 }
 
 // The widest unit that rows and their pitches allow.
@@ -225,10 +225,13 @@ int moegemm_sort_by_expert(const int32_t* experts, int32_t* offs, int32_t* slots
     return report(MOEGEMM_ERR_INVALID, "the workspace holds %lld bytes of %lld", (long long)workspace_bytes, (long long)need);
   const auto s = reinterpret_cast<hipStream_t>(stream);
   const bool whole = entries <= kSortWhole;
-  const int64_t chunk = whole ? cdiv(entries, 1024) * 1024 : sort_chunk(entries);
+  const int64_t chunk = sort_chunk(entries);
   SortParams p{experts, offs, slots, places, static_cast<int32_t*>(workspace), entries, first, count, (int32_t)chunk};
   if (whole) {
-    hipLaunchKernelGGL(sort_whole_kernel, dim3(1), dim3(1024), 16 * count * sizeof(int32_t), s, p);
+    const size_t lds = 16 * count * sizeof(int32_t);
+    if (entries <= 1024) hipLaunchKernelGGL(sort_whole_kernel<1>, dim3(1), dim3(1024), lds, s, p);
+    else if (entries <= 4096) hipLaunchKernelGGL(sort_whole_kernel<4>, dim3(1), dim3(1024), lds, s, p);
+    else hipLaunchKernelGGL(sort_whole_kernel<8>, dim3(1), dim3(1024), lds, s, p);
     return checked(hipGetLastError());
   }
   const dim3 grid((unsigned)cdiv(entries, chunk));
