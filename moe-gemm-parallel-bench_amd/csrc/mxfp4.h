@@ -73,133 +73,363 @@ struct RowParts<EF16> {
   }
 };
 
-// 8 ROWS8 rows of a group by 8 FN weight rows a wave (GATED: 4 FN gate rows and the 4 FN up rows that go with them), WN
-// waves along the columns, WK waves that take the K blocks wk, wk + WK, ...
+// The units of a launch's groups, in LDS behind the kernel's other arrays: cumulative counts of ceil(m / bm) * n_tiles, and the
+// groups' rows.
+constexpr int kMxTable = 1024;
+struct MxTable {
+  int32_t* units;
+  int32_t* ends;  // offsets, clamped
+  int32_t* sums;  // [16]
+  int32_t* start;  // the first group's first row
+  __device__ __forceinline__ MxTable(int32_t* at, int groups) : units(at + 17), ends(at + 17 + groups), sums(at), start(at + 16) {}
+  static size_t bytes(int groups) { return (17 + 2 * (size_t)groups) * sizeof(int32_t); }
+};
+
+// Sums stop at INT32_MAX, which only overlapping groups of decreasing offsets reach.
+__device__ __forceinline__ uint32_t add_units(uint32_t a, uint32_t b) { return min(a + b, (uint32_t)INT32_MAX); }
+
+// Every thread of the workgroup calls it; returns the number of units and ends with a barrier.
+template <int NT>
+__device__ __forceinline__ int mx_table(const MxTable& table, const MxParams& p, int bm) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t base = 0;
+  for (int g0 = 0; g0 < p.groups; g0 += NT) {
+    const int g = g0 + (int)threadIdx.x;
+    int m = 0, row0 = 0;
+    if (g < p.groups) row0 = group_rows(p.offs, p.rows, p.first + g, m);
+    if (g < p.groups) table.ends[g] = row0 + m;
+    if (g == 0) *table.start = row0;
+    uint32_t count = (uint32_t)min((int64_t)((m + bm - 1) / bm) * p.n_tiles, (int64_t)INT32_MAX);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t below = (uint32_t)__shfl_up((int)count, d);
+      count = lane >= d ? add_units(count, below) : count;
+    }
+    if (lane == 63) table.sums[wave] = (int32_t)count;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+      const uint32_t n = (uint32_t)table.sums[w];
+      if (w < wave) count = add_units(count, n);
+    }
+    if (g < p.groups) table.units[g] = (int32_t)add_units(base, count);
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) base = add_units(base, (uint32_t)table.sums[w]);
+    __syncthreads();
+  }
+  return (int)base;
+}
+
+// The group of a unit, its rows and the unit's place among the group's.
+__device__ __forceinline__ int mx_find(const MxTable& table, int groups, int unit, int& row0, int& m, int& local) {
+  int lo = 0, hi = groups - 1;  // the first group with units[i] > unit
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (table.units[mid] > unit) hi = mid;
+    else lo = mid + 1;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  row0 = __builtin_amdgcn_readfirstlane(lo ? table.ends[lo - 1] : *table.start);
+  m = __builtin_amdgcn_readfirstlane(table.ends[lo]) - row0;
+  local = unit - __builtin_amdgcn_readfirstlane(lo ? table.units[lo - 1] : 0);
+  return lo;
+}
+
+// 8 ROWS8 rows of a group by 8 FN weight rows a wave (GATED: 4 FN gate rows and the 4 FN up rows that go with them), and
+// WN waves along the columns, which share the rows through LDS, or WK waves that take a part of K each.
 template <class A_, int ROWS8_, int FN_, int WN_, int WK_, bool GATED_>
 struct MxStream {
   using A = A_;
   static constexpr int ROWS8 = ROWS8_, FN = FN_, WN = WN_, WK = WK_;
-  static constexpr bool GATED = GATED_;
+  static constexpr bool GATED = GATED_, SHARED = WN > 1;
   static constexpr int NT = WN * WK * 64;
   static constexpr int BM = 8 * ROWS8, BN = 8 * FN * WN;
   static constexpr int OUT_COLS = GATED ? BN / 2 : BN;
+  static constexpr int PARTS = RowParts<A>::N;
+  static constexpr int CHUNK_BLOCKS = PARTS == 1 ? 2 : 1;  // K blocks of the rows in LDS
+  static constexpr int CHUNK = CHUNK_BLOCKS * kMxBlock;
+  static constexpr int ROW_BYTES = CHUNK * 2 + 16;       // 16 bytes more: eight rows' pieces on all banks
+  static constexpr int STAGE_BYTES = BM * ROW_BYTES;     // of one part
+  static constexpr int COPIES = BM * CHUNK * 2 / 16 / NT;  // 16-byte pieces of a stage a thread
+  static constexpr int ROWS_BYTES = SHARED ? 2 * PARTS * STAGE_BYTES : 0;
+  static constexpr int SUM_BYTES = WK * BM * (BN + 4) * 4;
+  static constexpr int LDS_BYTES = ROWS_BYTES > SUM_BYTES ? ROWS_BYTES : SUM_BYTES;  // the sums where the rows were
+  // Two workgroups a CU where the rows are shared: more waves leave too few registers for the blocks ahead, and the groups'
+  // units come out uneven (256 rows over 32 experts, two a CU 92 us, three 104).
+  static constexpr int PER_CU = SHARED ? 2 : 4;
+  static constexpr int MIN_WAVES = 2;                             // a SIMD
+  static constexpr int AHEAD = SHARED && ROWS8 <= 2 ? 3 : 1;      // blocks of weights on their way
+  static_assert(4 % (AHEAD + 1) == 0, "a block's registers are known");
+  static_assert(WN == 1 || WK == 1, "columns or K");
+  static_assert(!SHARED || BM * CHUNK * 2 / 16 % NT == 0, "whole copies");
+  static_assert(LDS_BYTES + 17 * 4 + 8 * kMxTable <= 160 * 1024, "LDS of one CU");
 };
 
 // silu(g) * u in fp32, once rounded by the store.
 __device__ __forceinline__ float mx_gated(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
+
+typedef __amdgpu_buffer_rsrc_t mx_rsrc_t;
+__device__ __forceinline__ mx_rsrc_t mx_resource(const void* base, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
+  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, 0, 0));
+}
+__device__ __forceinline__ u32x4_t mx_load16_once(mx_rsrc_t r, uint32_t offset) {  // non-temporal
+  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, 0, 2));
+}
 
 // A wave reads whole 128-byte lines of eight weight rows at a time, straight into registers: lane (q = lane / 16, c = lane %
 // 16) holds the 16 bytes, one scale's 32 values, at chunk q + 4 (c / 8) of row c % 8.  As the operand of a 16 x 16 matrix
 // instruction, the lanes c >= 8 are eight more "rows": the same ones with the other half of K.  The activations are
 // laid out alike, so of the 16 x 16 outputs the two 8 x 8 squares on the diagonal are the halves' sums of eight rows by
 // eight rows, and the rest is not used.  That costs half the matrix rate and needs no exchange between lanes.
+//
+// The next blocks' weights are on their way while one is multiplied, and the scales of the next sixteen: a lane loads 16
+// of a row's 128 bytes and the lanes of the row exchange them, since byte loads of each lane's own cost as many
+// requests as the weights (256 rows over 32 experts of [4096, 7168]: REPLACE).  Offsets past a resource's bytes, which rows
+// past the last and K blocks past the end are given, read zeros and fetch nothing.
 template <class T>
-__global__ void __launch_bounds__(T::NT) mx_stream_kernel(MxParams p) {
+__global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams p) {
   using A = typename T::A;
-  constexpr int FN = T::FN, R = T::ROWS8, WK = T::WK, PARTS = RowParts<A>::N;
-  __shared__ TileTable table;
-  __shared__ float s_sum[WK][T::BM][T::BN + 4];
+  constexpr int FN = T::FN, R = T::ROWS8, WK = T::WK, PARTS = T::PARTS;
+  __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
+  extern __shared__ int32_t s_table[];
+  const MxTable table(s_table, p.groups);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wn = wave % T::WN, wk = wave / T::WN;
   const int c = lane & 15, chunk = (lane >> 4) + 4 * (c >> 3), row8 = c & 7;
   const int f = p.n >> 1;
-  build_tile_table(table, p.offs, p.first, p.groups, p.rows, T::BM, p.n_tiles);
-  const int units = table.tiles[p.groups - 1];
-  const int blocks = (p.k + kMxBlock - 1) / kMxBlock;
+  const int blocks = (p.k + kMxBlock - 1) / kMxBlock, part = (blocks + WK - 1) / WK;
+  const int first_b = min(wk * part, blocks), end_b = min(first_b + part, blocks);  // the wave's K blocks
+  const int scales = p.k / kMxGroup;                                                // of a row
+  const int units = mx_table<T::NT>(table, p, T::BM);
 
-  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    int lo = 0, hi = p.groups - 1;  // the first group with tiles[i] > unit
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (table.tiles[mid] > unit) hi = mid;
-      else lo = mid + 1;
-    }
-    const int row0 = lo ? table.ends[lo - 1] : table.start, m = table.ends[lo] - row0;
-    const int local = unit - (lo ? table.tiles[lo - 1] : 0), m_tiles = (m + T::BM - 1) / T::BM;
-    const int tn = local / m_tiles, m0 = (local - tn * m_tiles) * T::BM, n0 = tn * T::OUT_COLS;
-    const int e = p.first + lo;
-
-    // Rows past the last are the last again: what they give is not stored.
-    const uint8_t* w[FN];
-    const uint8_t* s[FN];
+  constexpr int WAVE_ROWS = T::GATED ? 4 * FN : 8 * FN;  // weight rows of one resource
+  constexpr int AHEAD = T::AHEAD;
+  const int byte_shift = (chunk & 3) * 8;
+  const int out_cols = T::GATED ? f : p.n;
+  // The unit whose loads are issued.
+  int first_n = 0, valid_m = 0, n0 = 0;
+  int64_t first_row = 0;
+  mx_rsrc_t rw, rw2, ra;
+  const uint8_t* s = nullptr;
+  const uint32_t w_lane = (uint32_t)row8 * (uint32_t)p.ldw + chunk * 16;
+  auto set_unit = [&](int unit) {
+    int row0, m, local;
+    const int e = p.first + mx_find(table, p.groups, unit, row0, m, local);
+    const int m_tiles = (m + T::BM - 1) / T::BM, tn = local / m_tiles, m0 = (local - tn * m_tiles) * T::BM;
+    first_row = (int64_t)row0 + m0;
+    valid_m = min(T::BM, m - m0);
+    n0 = tn * T::OUT_COLS;
+    first_n = n0 + wn * WAVE_ROWS;
+    const int valid_n = min(WAVE_ROWS, out_cols - first_n);
+    const uint8_t* w = p.w + (int64_t)e * p.swg + (int64_t)first_n * p.ldw;
+    const int64_t w_bytes = valid_n > 0 ? (valid_n - 1) * p.ldw + (p.k >> 1) : 0;
+    rw = mx_resource(w, w_bytes);
+    rw2 = T::GATED ? mx_resource(w + f * p.ldw, w_bytes) : rw;
+    ra = mx_resource(p.a + first_row * p.lda, ((valid_m - 1) * p.lda + p.k) * 2);
+    s = p.sw + (int64_t)e * p.ssg;
+  };
+  auto load = [&](u32x4_t (&q)[FN], int b) {
+    const bool in = b < end_b && b * kMxBlock + chunk * kMxGroup < p.k;  // whole groups: K is a multiple of 32
+    const uint32_t wo = in ? w_lane + (uint32_t)b * (kMxBlock / 2) : kOutOfRange;
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
-      int n;
-      if constexpr (T::GATED)
-        n = (i < FN / 2 ? 0 : f) + min(n0 + (wn * (FN / 2) + i % (FN / 2)) * 8 + row8, f - 1);
-      else
-        n = min(n0 + (wn * FN + i) * 8 + row8, p.n - 1);
-      w[i] = p.w + (int64_t)e * p.swg + n * p.ldw + chunk * 16;
-      s[i] = p.sw + (int64_t)e * p.ssg + n * p.ssn + chunk;
+      const bool up = T::GATED && i >= FN / 2;
+      q[i] = mx_load16_once(up ? rw2 : rw, wo + (uint32_t)((up ? i - FN / 2 : i) * 8) * (uint32_t)p.ldw);
     }
-    const uint16_t* a[R];
+  };
+  // The lane's 16 of the 128 bytes of blocks b to b + 15; zeros past the row's end, where nothing is read.
+  auto load_scales = [&](u32x4_t (&v)[FN], int b) {
+    const int want = b * (kMxBlock / kMxGroup) + chunk * 16, at = max(min(want, scales - 16), 0);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const bool up = T::GATED && i >= FN / 2;
+      const int n = min(first_n + (up ? i - FN / 2 : i) * 8 + row8, out_cols - 1) + (up ? f : 0);
+      const uint8_t* from = s + n * p.ssn + at;
+      if (scales >= 16) {
+        __builtin_memcpy(&v[i], from, 16);
+      } else {
+        v[i] = u32x4_t{};
+        for (int j = 0; j < scales; ++j) {
+          const uint32_t byte = (uint32_t)from[j] << (8 * (j & 3));
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[i][x] |= j >> 2 == x ? byte : 0;
+        }
+      }
+    }
+  };
+  // The same once they are here: moved to where the lane's bytes would be if the row went on.
+  auto settle_scales = [&](u32x4_t (&v)[FN], int b) {
+    const int want = b * (kMxBlock / kMxGroup) + chunk * 16, past = want - max(min(want, scales - 16), 0);
+    if (__ballot(past > 0) == 0) return;
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      u32x4_t x = v[i];
+      if (past & 8) x = u32x4_t{x[2], x[3], 0, 0};
+      if (past & 4) x = u32x4_t{x[1], x[2], x[3], 0};
+      const uint32_t bytes = past & 3;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = past >= 16 ? 0 : __builtin_amdgcn_alignbyte(j < 3 ? x[j + 1] : 0, x[j], bytes);
+    }
+  };
+  f32x4_t acc[R][FN];
+  // Block `at` of the sixteen whose scales are at hand: byte 8 at + chunk of the row's 128, which lane at / 2 of the row's holds.
+  auto multiply = [&](const u32x4_t (&q)[FN], const u32x4_t (&bytes)[FN], int at, int odd, auto&& rows_of) {
+    const int other = at >> 1, from = ((other & 3) * 16 + (other >> 2) * 8 + row8) * 4;
+    float scale[FN];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const uint32_t low = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)bytes[i][2 * odd]);
+      const uint32_t high = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)bytes[i][2 * odd + 1]);
+      scale[i] = mx_scale((chunk < 4 ? low : high) >> byte_shift & 0xff);
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      RowParts<A> rows[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) rows_of(rows[r], r, x);
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const bf16x8_t weights = mx_weights(q[i][x], scale[i]);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int h = 0; h < PARTS; ++h)
+            acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(weights, rows[r].v[h], acc[r][i], 0, 0, 0);
+      }
+    }
+  };
+  // Shared rows go through registers to LDS, CHUNK values at a time and one chunk ahead, split into their parts on the way; a
+  // wave that has its own part of K loads them as it needs them.
+  u32x4_t piece[T::SHARED ? T::COPIES : 1], av[T::SHARED ? 1 : 2][R][4];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < T::COPIES; ++j) {
+      const int at = threadIdx.x + j * T::NT, row = at / (T::CHUNK / 8), col = at % (T::CHUNK / 8);
+      const uint32_t offset = (uint32_t)row * (uint32_t)p.lda * 2 + (uint32_t)(k0 + col * 8) * 2;
+      piece[j] = mx_load16(ra, row < valid_m && k0 + col * 8 < p.k ? offset : kOutOfRange);
+    }
+  };
+  auto put = [&](int stage) {
+#pragma unroll
+    for (int j = 0; j < T::COPIES; ++j) {
+      const int at = threadIdx.x + j * T::NT, row = at / (T::CHUNK / 8), col = at % (T::CHUNK / 8);
+      RowParts<A> parts;
+      parts.set(piece[j]);
+#pragma unroll
+      for (int h = 0; h < PARTS; ++h)
+        *reinterpret_cast<bf16x8_t*>(smem + (stage * PARTS + h) * T::STAGE_BYTES + row * T::ROW_BYTES + col * 16) = parts.v[h];
+    }
+  };
+  const uint32_t a_lane = (uint32_t)row8 * (uint32_t)p.lda * 2 + chunk * (kMxGroup * 2);
+  auto fetch_own = [&](u32x4_t (&v)[R][4], int b) {
+    const bool in = b < end_b && b * kMxBlock + chunk * kMxGroup < p.k;
+    const uint32_t ao = in ? a_lane + (uint32_t)b * (kMxBlock * 2) : kOutOfRange;
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      a[r] = p.a + ((int64_t)row0 + min(m0 + r * 8 + row8, m - 1)) * p.lda + chunk * kMxGroup;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        v[r][x] = mx_load16(ra, r * 8 + row8 < valid_m ? ao + (uint32_t)(r * 8) * (uint32_t)p.lda * 2 + x * 16 : kOutOfRange);
+  };
+  // Waves meet without waiting for what is on its way from memory.
+  auto meet = [] {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    compiler_fence();
+  };
+  const uint32_t frag = (uint32_t)row8 * T::ROW_BYTES + chunk * (kMxGroup * 2);
 
-    f32x4_t acc[R][FN];
+  u32x4_t q[AHEAD + 1][FN];
+  u32x4_t bytes[FN], next_bytes[FN];  // scales of sixteen blocks
+  auto start = [&](int unit) {
+    set_unit(unit);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) load(q[j], first_b + j);
+    load_scales(bytes, first_b);
+    if constexpr (T::SHARED) fetch(0);
+    else fetch_own(av[0], first_b);
+  };
+  int unit = blockIdx.x;
+  if (unit >= units) return;
+  start(unit);
+  while (true) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < FN; ++i) acc[r][i] = f32x4_t{};
-    for (int b = wk; b < blocks; b += WK) {
-      const int k0 = b * kMxBlock;
-      const bool in = k0 + chunk * kMxGroup < p.k;  // whole groups: K is a multiple of 32
-      u32x4_t wv[FN], av[R][4];
-      uint32_t sv[FN];
+    if constexpr (T::SHARED) {
+      put(0);
+      meet();
+    }
+    settle_scales(bytes, first_b);
+    constexpr int CB = T::CHUNK_BLOCKS;
+    for (int b0 = first_b; b0 < end_b; b0 += 4) {
+      const int rel = b0 - first_b & 15;
+      if (rel == 8) load_scales(next_bytes, b0 + 8);
 #pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        wv[i] = u32x4_t{};
-        sv[i] = 0;
-        if (in) {
-          wv[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(w[i] + (k0 >> 1)));
-          sv[i] = s[i][k0 >> 5];
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          av[r][x] = u32x4_t{};
-          if (in) av[r][x] = *reinterpret_cast<const u32x4_t*>(a[r] + k0 + 8 * x);
-        }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        RowParts<A> rows[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) rows[r].set(av[r][x]);
-#pragma unroll
-        for (int i = 0; i < FN; ++i) {
-          const bf16x8_t weights = mx_weights(wv[i][x], mx_scale(sv[i]));
-#pragma unroll
-          for (int r = 0; r < R; ++r)
+      for (int j = 0; j < 4; ++j) {
+        const int b = b0 + j;
+        if (b >= end_b) break;
+        if constexpr (T::SHARED) {
+          const int stage = CB == 4 ? (b0 >> 2) & 1 : j / CB & 1, half = j % CB;
+          if (half == 0) fetch((b + CB) * kMxBlock);
+          load(q[(j + AHEAD) % (AHEAD + 1)], b + AHEAD);
+          multiply(q[j % (AHEAD + 1)], bytes, rel + j, j & 1, [&](RowParts<A>& rows, int r, int x) {
 #pragma unroll
             for (int h = 0; h < PARTS; ++h)
-              acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(weights, rows[r].v[h], acc[r][i], 0, 0, 0);
+              rows.v[h] = *reinterpret_cast<const bf16x8_t*>(smem + (stage * PARTS + h) * T::STAGE_BYTES + frag +
+                                                            r * 8 * T::ROW_BYTES + half * (kMxBlock * 2) + x * 16);
+          });
+          if (half == CB - 1 && b + 1 < end_b) {
+            put(stage ^ 1);
+            meet();
+          }
+        } else {
+          load(q[(j + AHEAD) % (AHEAD + 1)], b + AHEAD);
+          fetch_own(av[(j + 1) & 1], b + 1);
+          multiply(q[j % (AHEAD + 1)], bytes, rel + j, j & 1, [&](RowParts<A>& rows, int r, int x) { rows.set(av[j & 1][r][x]); });
         }
       }
+      if (rel == 12) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) bytes[i] = next_bytes[i];
+        settle_scales(bytes, b0 + 4);
+      }
     }
+
+    // The next unit's loads go out before this one's results.
+    const int done_m = valid_m, done_n = n0;
+    const int64_t done_row = first_row;
+    unit += gridDim.x;
+    if (unit < units) start(unit);
+
     // Lane (q, c) holds weight rows 4 q + j of row c; both halves of K meet, and the WK waves' sums in wave order.
+    if constexpr (T::SHARED) meet();  // the sums go where the rows are
+    float* sums = reinterpret_cast<float*>(smem);
+    constexpr int LD = T::BN + 4;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
+      for (int i = 0; i < FN; ++i) {
+        f32x4_t v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = acc[r][i][j] + __shfl_xor(acc[r][i][j], 40);
-          if (lane < 32 && c < 8) s_sum[wk][r * 8 + c][(wn * FN + i) * 8 + (lane >> 4) * 4 + j] = v;
-        }
-    __syncthreads();
+        for (int j = 0; j < 4; ++j) v[j] = acc[r][i][j] + __shfl_xor(acc[r][i][j], 40);
+        if (lane < 32 && c < 8)
+          *reinterpret_cast<f32x4_t*>(sums + (wk * T::BM + r * 8 + c) * LD + (wn * FN + i) * 8 + (lane >> 4) * 4) = v;
+      }
+    meet();
     for (int x = threadIdx.x; x < T::BM * T::OUT_COLS; x += T::NT) {
       const int r = x / T::OUT_COLS, n = x % T::OUT_COLS;
       auto sum = [&](int col) {
-        float v = s_sum[0][r][col];
+        float v = sums[r * LD + col];
 #pragma unroll
-        for (int k = 1; k < WK; ++k) v += s_sum[k][r][col];
+        for (int k = 1; k < WK; ++k) v += sums[(k * T::BM + r) * LD + col];
         return v;
       };
-      if (m0 + r >= m || n0 + n >= (T::GATED ? f : p.n)) continue;
+      if (r >= done_m || done_n + n >= out_cols) continue;
       float v;
       if constexpr (T::GATED) {
         const int gate = n / (4 * FN) * 8 * FN + n % (4 * FN);
@@ -207,13 +437,14 @@ __global__ void __launch_bounds__(T::NT) mx_stream_kernel(MxParams p) {
       } else {
         v = sum(n);
       }
-      const int64_t to = ((int64_t)row0 + m0 + r) * p.ldo + n0 + n;
+      const int64_t to = (done_row + r) * p.ldo + done_n + n;
       char* out = static_cast<char*>(p.out);
       if (p.out_dtype == DT_F32) store1<EF32>(out + to * 4, v);
       else if (p.out_dtype == DT_BF16) store1<EBf16>(out + to * 2, v);
       else store1<EF16>(out + to * 2, v);
     }
-    __syncthreads();
+    if (unit >= units) break;
+    meet();
   }
 }
 

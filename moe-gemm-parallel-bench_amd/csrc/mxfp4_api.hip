@@ -1,5 +1,5 @@
 // C ABI of the 4-bit (MXFP4) operators: argument checks, the choice of a variant, the launches: one a call, and another for
-// every further 768 groups of a product.
+// every further 1024 groups of a product.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -21,6 +21,8 @@ int checked(hipError_t err) {
 }
 
 bool is_dtype(int32_t dtype) { return dtype == DT_F16 || dtype == DT_BF16 || dtype == DT_F32; }
+
+constexpr int64_t kPitchLimit = int64_t(1) << 23;  // a unit's rows lie within 2 GiB
 
 constexpr int64_t kMaxBlocks = 1 << 16;  // workgroups of a conversion, which go on to what is past them
 
@@ -50,19 +52,31 @@ hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Variant for `rows` rows over `groups` groups of `cols` output columns.
+// Variant for `rows` rows over `groups` groups of `cols` output columns.  Routed groups are taken to hold up to 1.6 times the mean;
+// a group of more rows than a unit has its weights read again for each unit's rows.  Wide units (us): 256 rows over 128
+// experts of [5760, 2880], Gate+Up, 8 rows a unit 256, 16 rows 273; 256 rows over 32 of [4096, 7168] 126 and 92; 768 rows over
+// them 16 rows a unit 187, 32 rows 151.
+// Narrow units, whose waves split K, where the wide ones would not fill two workgroups a CU: one row of [5760, 2880] 6.4 wide 13,
+// four experts' rows of 128 x [5760, 2880] 12.7 and 14.8, 16 rows of [4096, 7168] 11.7 and 35; but 256 rows over 32
+// experts of [4096, 7168] 171 and 92.  Narrower ones where those leave CUs idle: 16 rows of [4096, 7168] 16 columns a unit 11.7, 32
+// columns 13.4, 32 rows 19.9 and 14.2; a row of one expert each, 4 of [2880, 2880], 8.4 and 9.3.
 int choose(const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
-  const int64_t active = std::min(groups, rows);
-  const int64_t high = active == 1 ? rows : cdiv(cdiv(rows, active) * 8, 5);
-  const int need = high <= 8 ? 8 : high <= 16 ? 16 : 32;
-  int best = -1;
-  for (int i = 0; i < kNumMx; ++i) {
-    const MxVariant& v = table[i];
-    if (v.rows != need) continue;
-    // Narrow units that share K where the wide ones would leave CUs idle.
-    if (best < 0 || (v.waves_k > 1 && active * cdiv(cols, table[best].cols) < 2 * cus)) best = i;
-  }
-  return best;
+  const int64_t active = std::min(groups, rows), mean = cdiv(rows, active);
+  const int64_t high = active == 1 ? rows : cdiv(mean * 8, 5);
+  auto find = [&](int wanted_rows, bool wide, bool widest) {
+    int best = -1;
+    for (int i = 0; i < kNumMx; ++i) {
+      const MxVariant& v = table[i];
+      if (v.rows != wanted_rows || (v.waves_k == 1) != wide) continue;
+      if (best < 0 || (v.cols > table[best].cols) == widest) best = i;
+    }
+    return best;
+  };
+  auto units = [&](int i) { return active * cdiv(mean, table[i].rows) * cdiv(cols, table[i].cols); };
+  const int wide = find(high <= 8 ? 8 : high <= 16 ? 16 : 32, true, true);
+  if (units(wide) >= 2 * cus) return wide;
+  const int few = high <= 8 ? 8 : 16, narrow = find(few, false, true);
+  return units(narrow) * (few == 8 ? 2 : 3) < 3 * cus ? find(few, false, false) : narrow;
 }
 
 int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs, int32_t group_count,
@@ -87,6 +101,8 @@ int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* 
     return report(MOEGEMM_ERR_INVALID, "rows of a and weight must start at multiples of 16 bytes");
   if (stride_am < 0 || stride_wn < k / 2 || stride_sn < k / kMxGroup || (rows > 1 && stride_om < cols))
     return report(MOEGEMM_ERR_INVALID, "row pitches must cover a row");
+  if (stride_am >= kPitchLimit / 2 || stride_wn >= kPitchLimit || stride_sn >= kPitchLimit || k > kPitchLimit / 2)
+    return report(MOEGEMM_ERR_INVALID, "rows of a, weight and scale must be less than %lld bytes apart", (long long)kPitchLimit);
   if (!aligned(out, out_dtype == DT_F32 ? 4 : 2))
     return report(MOEGEMM_ERR_INVALID, "out must be aligned to its element size");
   const int cus = grid_size > 0 ? grid_size : 256;
@@ -95,11 +111,12 @@ int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* 
   const MxVariant& v = table[variant];
   MxParams p{static_cast<const uint16_t*>(a), w, scale, out, offs, stride_am, stride_wg, stride_wn, stride_sg, stride_sn,
              stride_om, group_count, rows, n, k, (int32_t)cdiv(cols, v.cols), out_dtype};
-  const int64_t bound = std::min(rows / v.rows + (int64_t)group_count, group_count * cdiv(rows, v.rows)) * p.n_tiles;
+  const int64_t row_tiles = std::min({rows / v.rows + (int64_t)group_count, group_count * cdiv(rows, v.rows), (int64_t)rows});
+  const int64_t bound = row_tiles * p.n_tiles;
   if (bound > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
-  const int grid = (int)std::min<int64_t>(bound, (int64_t)cus * 4);
-  for (; p.first < group_count; p.first += kTableGroups) {
-    p.groups = std::min(group_count - p.first, kTableGroups);
+  const int grid = (int)std::min<int64_t>(bound, (int64_t)cus * v.per_cu);
+  for (; p.first < group_count; p.first += kMxTable) {
+    p.groups = std::min(group_count - p.first, kMxTable);
     const int rc = checked(v.launch(p, grid, reinterpret_cast<hipStream_t>(stream)));
     if (rc != MOEGEMM_OK) return rc;
   }

@@ -8,24 +8,27 @@ namespace moegemm {
 typedef hipError_t (*MxLaunchFn)(const MxParams&, int grid, hipStream_t stream);
 
 struct MxVariant {
-  int rows, cols;    // of a unit: output rows, and output columns
-  int waves_k;       // waves that share K
+  int rows, cols;  // of a unit: output rows, and output columns
+  int waves_k;     // waves that have a part of K each; 1: waves that share the rows
+  int per_cu;      // workgroups a CU
   MxLaunchFn launch;
 };
 
 template <class T>
 hipError_t launch_mx(const MxParams& p, int grid, hipStream_t stream) {
-  hipLaunchKernelGGL((mx_stream_kernel<T>), dim3(grid), dim3(T::NT), 0, stream, p);
+  hipLaunchKernelGGL((mx_stream_kernel<T>), dim3(grid), dim3(T::NT), MxTable::bytes(p.groups), stream, p);
   return hipGetLastError();
 }
 
-// X(A, ROWS8, FN, WAVES_N, WAVES_K, GATED)
+// X(A, ROWS8, FN, WAVES_N, WAVES_K, GATED): 8, 16 or 32 rows by 128 weight rows for many units, 32 or 16 weight rows with K split
+// over the waves for few.
 #define MOEGEMM_MENU_MX(X, A, GATED)                                                             \
-  X(A, 1, 4, 4, 1, GATED) X(A, 1, 2, 1, 8, GATED) X(A, 2, 4, 4, 1, GATED) X(A, 2, 2, 1, 8, GATED) \
-  X(A, 4, 4, 4, 1, GATED)
+  X(A, 1, 4, 4, 1, GATED) X(A, 2, 4, 4, 1, GATED) X(A, 4, 4, 4, 1, GATED)                         \
+  X(A, 1, 4, 1, 4, GATED) X(A, 2, 4, 1, 4, GATED) X(A, 1, 2, 1, 4, GATED) X(A, 2, 2, 1, 4, GATED)
 
-#define MOEGEMM_MX_X(A, R, FN, WN, WK, GATED) \
-  MxVariant{8 * R, 8 * FN * WN / (GATED ? 2 : 1), WK, &launch_mx<MxStream<A, R, FN, WN, WK, GATED>>},
+#define MOEGEMM_MX_X(A, R, FN, WN, WK, GATED)                                                                \
+  MxVariant{8 * R, 8 * FN * WN / (GATED ? 2 : 1), WK, MxStream<A, R, FN, WN, WK, GATED>::PER_CU, \
+            &launch_mx<MxStream<A, R, FN, WN, WK, GATED>>},
 // The kernels of a menu, for the device pass.
 #define MOEGEMM_MX_XK(A, R, FN, WN, WK, GATED) \
   template __global__ void mx_stream_kernel<MxStream<A, R, FN, WN, WK, GATED>>(MxParams);

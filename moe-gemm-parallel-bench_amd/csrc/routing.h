@@ -662,7 +662,7 @@ __device__ __forceinline__ void count_entries(const int (&e)[N], int32_t* counts
 template <int N>
 __device__ __forceinline__ void place_entries(const SortParams& p, int64_t begin, const int (&entries)[N], int32_t* next) {
   const int lane = threadIdx.x & 63;
-  const int bits = 32 - __builtin_clz((unsigned)p.count);
+  const int bits = p.count > 1 ? 32 - __builtin_clz((unsigned)(p.count - 1)) : 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int64_t from = begin + i * 64 + lane;
