@@ -10,6 +10,8 @@
 // may be subnormal, do the rest.  fp16 rows are taken as two bf16 parts, 8 bits and the 3 behind them, which is exact too.
 #pragma once
 
+#include <type_traits>
+
 #include "fp8_gemm.h"
 
 namespace moegemm {
@@ -448,7 +450,8 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
   }
 }
 
-// The format's conversions.  A lane takes 8 consecutive values, four lanes a group of 32.
+// The format's conversions.  An item is 16 bytes of values, so that a wave's loads and stores of them cover whole lines: 8
+// values of 16 bits or 4 of 32, and 4 or 8 lanes a group of 32.  Each thread has four items on their way.
 struct MxConvertParams {
   const void* x;   // quantise: values in; dequantise: e2m1 bytes
   uint8_t* q;      // quantise: e2m1 bytes out
@@ -456,69 +459,112 @@ struct MxConvertParams {
   void* out;       // dequantise: values out
   int64_t sxr, sqr, ssr;  // row strides: values' in elements, the others' in bytes
   int64_t rows;
-  int32_t k;
+  int64_t k;
 };
+template <class E>
+struct MxItem {
+  static constexpr int VALUES = 16 / sizeof(typename E::raw);
+  using packed_t = std::conditional_t<VALUES == 8, uint32_t, uint16_t>;
+};
+constexpr int kMxItems = 4;
+// Where item i lies: its row, and its first column.
+template <class E>
+__device__ __forceinline__ void mx_item(const MxConvertParams& p, int64_t i, int64_t& row, int64_t& col) {
+  const int64_t per_row = p.k / MxItem<E>::VALUES;
+  row = p.rows == 1 ? 0 : i / per_row;
+  col = (i - row * per_row) * MxItem<E>::VALUES;
+}
 
 // scale = floor(log2 max|x|) - 2 as an e8m0 byte, at least 0: e2m1's largest power of two is 4.  q = e2m1(x / scale), to
 // nearest even, at most 6.  A group that holds a NaN or an infinity gets the scale 255, a NaN.
+// Bound by HBM: fp32 8 x [5760, 2880] REPLACE.
 template <class E, bool VEC>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(MxConvertParams p) {
-  const int per_row = p.k / 8;
-  const int64_t items = p.rows * per_row, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += step) {  // four lanes of a group go together
-    const int64_t row = i / per_row;
-    const int col = (int)(i - row * per_row) * 8;
-    typename E::raw raw[8];
-    const typename E::raw* x = static_cast<const typename E::raw*>(p.x) + row * p.sxr + col;
-    if constexpr (VEC) {
-      constexpr int N = sizeof(raw) / 16;
-      u32x4_t c[N];
+  using raw_t = typename E::raw;
+  constexpr int V = MxItem<E>::VALUES;
+  const int64_t items = p.rows * (p.k / V), step = (int64_t)gridDim.x * 256 * kMxItems;
+  for (int64_t i0 = (int64_t)blockIdx.x * 256 * kMxItems + threadIdx.x; i0 < items; i0 += step) {  // a group's lanes go together
+    u32x4_t chunk[kMxItems];
 #pragma unroll
-      for (int j = 0; j < N; ++j) c[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(x) + j);
-      __builtin_memcpy(raw, c, sizeof(raw));
-    } else {
+    for (int u = 0; u < kMxItems; ++u) {
+      int64_t row, col;
+      mx_item<E>(p, min(i0 + u * 256, items - 1), row, col);
+      const raw_t* x = static_cast<const raw_t*>(p.x) + row * p.sxr + col;
+      if constexpr (VEC) {
+        chunk[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(x));
+      } else {
+        raw_t raw[V];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) raw[j] = x[j];
+        for (int j = 0; j < V; ++j) raw[j] = x[j];
+        __builtin_memcpy(&chunk[u], raw, 16);
+      }
     }
-    float v[8];
-    uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (E::dtype == DT_F32) v[j] = __builtin_bit_cast(float, raw[j]);
-      else if constexpr (E::dtype == DT_BF16) v[j] = __builtin_bit_cast(float, (uint32_t)raw[j] << 16);
-      else v[j] = (float)__builtin_bit_cast(_Float16, raw[j]);
-      top = max(top, abs_bits(v[j]));
+    for (int u = 0; u < kMxItems; ++u) {
+      if (i0 + u * 256 >= items) break;
+      int64_t row, col;
+      mx_item<E>(p, i0 + u * 256, row, col);
+      raw_t raw[V];
+      __builtin_memcpy(raw, &chunk[u], 16);
+      float v[V];
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if constexpr (E::dtype == DT_F32) v[j] = __builtin_bit_cast(float, raw[j]);
+        else if constexpr (E::dtype == DT_BF16) v[j] = __builtin_bit_cast(float, (uint32_t)raw[j] << 16);
+        else v[j] = (float)__builtin_bit_cast(_Float16, raw[j]);
+        top = max(top, abs_bits(v[j]));
+      }
+#pragma unroll
+      for (int d = 1; d < kMxGroup / V; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+      const int exponent = (int)(top >> 23);  // 255: infinity or NaN; a subnormal maximum's scale is below the least one
+      const uint32_t s = exponent == 255 ? 255u : (uint32_t)max(exponent - 2, 0);
+      const float scale = mx_scale(exponent == 255 ? 127u : s);
+      uint32_t q = 0;
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[0], v[1], scale, 0);
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[2], v[3], scale, 1);
+      if constexpr (V == 8) {
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[4], v[5], scale, 2);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], scale, 3);
+      }
+      *reinterpret_cast<typename MxItem<E>::packed_t*>(p.q + row * p.sqr + col / 2) = (typename MxItem<E>::packed_t)q;
+      if ((col & 31) == 0) p.scale[row * p.ssr + col / 32] = (uint8_t)s;
     }
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-    const int exponent = (int)(top >> 23);  // 255: infinity or NaN; a subnormal maximum's scale is below the least one
-    const uint32_t s = exponent == 255 ? 255u : (uint32_t)max(exponent - 2, 0);
-    const float scale = mx_scale(exponent == 255 ? 127u : s);
-    uint32_t q = 0;
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[0], v[1], scale, 0);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[2], v[3], scale, 1);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[4], v[5], scale, 2);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], scale, 3);
-    *reinterpret_cast<uint32_t*>(p.q + row * p.sqr + col / 2) = q;
-    if ((col & 31) == 0) p.scale[row * p.ssr + col / 32] = (uint8_t)s;
   }
 }
 
 template <class E>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(MxConvertParams p) {
-  const int per_row = p.k / 8;
-  const int64_t items = p.rows * per_row, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += step) {
-    const int64_t row = i / per_row;
-    const int col = (int)(i - row * per_row) * 8;
-    const uint32_t q = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.x) + row * p.sqr + col / 2);
-    const bf16x8_t v = mx_weights(q, mx_scale(p.scale[row * p.ssr + col / 32]));  // exact
-    char* out = static_cast<char*>(p.out) + (row * p.k + col) * sizeof(typename E::raw);
-    if constexpr (E::dtype == DT_BF16) {
-      *MOEGEMM_GLOBAL(u32x4_t, out) = __builtin_bit_cast(u32x4_t, v);
-    } else {
-      store4<E>(out, f32x4_t{(float)v[0], (float)v[1], (float)v[2], (float)v[3]});
-      store4<E>(out + 4 * sizeof(typename E::raw), f32x4_t{(float)v[4], (float)v[5], (float)v[6], (float)v[7]});
+  using raw_t = typename E::raw;
+  using packed_t = typename MxItem<E>::packed_t;
+  constexpr int V = MxItem<E>::VALUES;
+  const int64_t items = p.rows * (p.k / V), step = (int64_t)gridDim.x * 256 * kMxItems;
+  for (int64_t i0 = (int64_t)blockIdx.x * 256 * kMxItems + threadIdx.x; i0 < items; i0 += step) {
+    uint32_t q[kMxItems], s[kMxItems];
+#pragma unroll
+    for (int u = 0; u < kMxItems; ++u) {
+      int64_t row, col;
+      mx_item<E>(p, min(i0 + u * 256, items - 1), row, col);
+      q[u] = *reinterpret_cast<const packed_t*>(static_cast<const uint8_t*>(p.x) + row * p.sqr + col / 2);
+      s[u] = p.scale[row * p.ssr + col / 32];
+    }
+#pragma unroll
+    for (int u = 0; u < kMxItems; ++u) {
+      if (i0 + u * 256 >= items) break;
+      const bf16x8_t v = mx_weights(q[u], mx_scale(s[u]));  // exact
+      u32x4_t out;
+      if constexpr (E::dtype == DT_BF16) {
+        out = __builtin_bit_cast(u32x4_t, v);
+      } else {
+        raw_t raw[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if constexpr (E::is_f32) raw[j] = __builtin_bit_cast(uint32_t, (float)v[j]);
+          else raw[j] = __builtin_bit_cast(uint16_t, (_Float16)(float)v[j]);
+        }
+        __builtin_memcpy(&out, raw, 16);
+      }
+      __builtin_nontemporal_store(out, reinterpret_cast<u32x4_t*>(p.out) + i0 + u * 256);
     }
   }
 }

@@ -38,17 +38,28 @@ int check_conversion(int64_t rows, int32_t k, const void* x, const uint8_t* q, c
   return MOEGEMM_OK;
 }
 
-dim3 conversion_grid(int64_t rows, int32_t k) { return dim3((unsigned)std::min(cdiv(rows * (k / 8), 256), kMaxBlocks)); }
+template <class E>
+dim3 conversion_grid(const MxConvertParams& p) {
+  return dim3((unsigned)std::min(cdiv(p.rows * (p.k / MxItem<E>::VALUES), 256 * kMxItems), kMaxBlocks));
+}
+// Rows that follow on one another are one long row: no division by a row's length.
+MxConvertParams flat(MxConvertParams p, bool dense) {
+  if (dense) {
+    p.k *= p.rows;
+    p.rows = 1;
+  }
+  return p;
+}
 
 template <class E>
 hipError_t launch_quantize(const MxConvertParams& p, bool vec, hipStream_t s) {
-  if (vec) hipLaunchKernelGGL((mx_quantize_kernel<E, true>), conversion_grid(p.rows, p.k), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((mx_quantize_kernel<E, false>), conversion_grid(p.rows, p.k), dim3(256), 0, s, p);
+  if (vec) hipLaunchKernelGGL((mx_quantize_kernel<E, true>), conversion_grid<E>(p), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((mx_quantize_kernel<E, false>), conversion_grid<E>(p), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <class E>
 hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((mx_dequantize_kernel<E>), conversion_grid(p.rows, p.k), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((mx_dequantize_kernel<E>), conversion_grid<E>(p), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 
@@ -131,7 +142,8 @@ int moegemm_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scale, int64_t ro
                            int64_t stride_qr, int64_t stride_sr, int32_t dtype, void* stream) {
   const int rc = check_conversion(rows, k, x, q, scale, stride_qr, dtype);
   if (rc != MOEGEMM_OK || rows == 0) return rc;
-  const MxConvertParams p{x, q, scale, nullptr, stride_xr, stride_qr, stride_sr, rows, k};
+  const MxConvertParams p = flat({x, q, scale, nullptr, stride_xr, stride_qr, stride_sr, rows, k},
+                                 stride_xr == k && stride_qr == k / 2 && stride_sr == k / kMxGroup);
   const bool vec = aligned(x, 16) && stride_xr * (dtype == DT_F32 ? 4 : 2) % 16 == 0;
   const auto s = reinterpret_cast<hipStream_t>(stream);
   return checked(dtype == DT_F32    ? launch_quantize<EF32>(p, vec, s)
@@ -144,7 +156,8 @@ int moegemm_dequantize_mxfp4(const uint8_t* q, const uint8_t* scale, void* out, 
   const int rc = check_conversion(rows, k, out, q, scale, stride_qr, dtype);
   if (rc != MOEGEMM_OK || rows == 0) return rc;
   if (!aligned(out, 16)) return report(MOEGEMM_ERR_INVALID, "out must be 16-byte aligned");
-  const MxConvertParams p{q, nullptr, const_cast<uint8_t*>(scale), out, 0, stride_qr, stride_sr, rows, k};
+  const MxConvertParams p = flat({q, nullptr, const_cast<uint8_t*>(scale), out, 0, stride_qr, stride_sr, rows, k},
+                                 stride_qr == k / 2 && stride_sr == k / kMxGroup);
   const auto s = reinterpret_cast<hipStream_t>(stream);
   return checked(dtype == DT_F32    ? launch_dequantize<EF32>(p, s)
                  : dtype == DT_BF16 ? launch_dequantize<EBf16>(p, s)

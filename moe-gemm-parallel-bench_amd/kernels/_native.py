@@ -520,14 +520,24 @@ def current_stream_handle(device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
+_TORCH: list = []  # torch's current device and raw stream, bound on the first launch
+
+
 def launch(device, entry, *args) -> None:
     """``entry(*args, stream)`` on ``device``'s current stream; a kernel goes to the current device, so that is made
     ``device`` where it is another."""
-    import torch
+    if not _TORCH:
+        import torch
 
-    index = device.index
-    if index is None or index == torch.cuda.current_device():
-        check(entry(*args, current_stream_handle(device)))
-        return
-    with torch.cuda.device(index):
-        check(entry(*args, current_stream_handle(device)))
+        _TORCH.extend((torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream))
+    current_device, raw_stream = _TORCH
+    index, current = device.index, current_device()
+    if index is None or index == current:
+        status = entry(*args, raw_stream(current))
+    else:
+        import torch
+
+        with torch.cuda.device(index):
+            status = entry(*args, raw_stream(index))
+    if status != OK:
+        check(status)
