@@ -494,13 +494,18 @@ def tile_queue(device, stream_handle: int):
     return queue
 
 
-def dtype_code(dtype) -> int:
-    import torch
+_DTYPE_CODES: dict = {}  # torch dtype -> code, filled on first use
 
-    codes = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
-    if dtype not in codes:
+
+def dtype_code(dtype) -> int:
+    if not _DTYPE_CODES:
+        import torch
+
+        _DTYPE_CODES.update({torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32})
+    code = _DTYPE_CODES.get(dtype)
+    if code is None:
         raise ValueError(f"unsupported dtype {dtype}; expected float16, bfloat16 or float32")
-    return codes[dtype]
+    return code
 
 
 def precision_code(input_precision: str, dtype_code_value: int) -> int:

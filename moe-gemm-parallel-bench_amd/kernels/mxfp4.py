@@ -26,19 +26,13 @@ from .fp8 import _cu_count
 MX_GROUP = 32
 
 
-def _is_bytes(t, name: str) -> bool:
-    """uint8, or torch's own type of such bytes."""
+def _are_bytes(codes, scales) -> bool:
+    """Both uint8, or torch's own types of such bytes."""
     import torch
 
-    return t.dtype is torch.uint8 or t.dtype is getattr(torch, name, None)
-
-
-def _is_codes(t) -> bool:
-    return _is_bytes(t, "float4_e2m1fn_x2")
-
-
-def _is_scales(t) -> bool:
-    return _is_bytes(t, "float8_e8m0fnu")
+    uint8 = torch.uint8
+    return ((codes.dtype is uint8 or codes.dtype is getattr(torch, "float4_e2m1fn_x2", None))
+            and (scales.dtype is uint8 or scales.dtype is getattr(torch, "float8_e8m0fnu", None)))
 
 
 def _matrices(t) -> list:
@@ -112,16 +106,17 @@ def dequantize_mxfp4(q, scale, *, dtype=None):
 
 def _check_weight(weight, scale, k: int) -> None:
     """Shapes, types and layout of packed weights [..., K / 2] and their scales."""
-    if not _is_codes(weight) or not _is_scales(scale):
+    shape, strides = weight.shape, weight.stride()
+    if not _are_bytes(weight, scale):
         raise ValueError("4-bit weights and their scales must be uint8 (or float4_e2m1fn_x2 and float8_e8m0fnu)")
     if k <= 0 or k % MX_GROUP or k > _native.INT32_MAX:
         raise ValueError(f"K must be a positive multiple of {MX_GROUP} under 2**31 (got {k})")
-    if weight.shape[-1] * 2 != k:
-        raise ValueError(f"contraction mismatch: K={k}, weight rows hold {2 * weight.shape[-1]}")
-    if scale.shape != (*weight.shape[:-1], k // MX_GROUP):
-        raise ValueError(f"scale must be {[*weight.shape[:-1], k // MX_GROUP]} (got {list(scale.shape)})")
-    strides, shape = weight.stride(), weight.shape
-    if strides[-1] != 1 or (scale.stride(-1) != 1 and scale.shape[-1] > 1):
+    if shape[-1] * 2 != k:
+        raise ValueError(f"contraction mismatch: K={k}, weight rows hold {2 * shape[-1]}")
+    expected = (*shape[:-1], k // MX_GROUP)
+    if scale.shape != expected:
+        raise ValueError(f"scale must be {list(expected)} (got {list(scale.shape)})")
+    if strides[-1] != 1 or (k > MX_GROUP and scale.stride(-1) != 1):
         raise ValueError("weight and scale need a unit stride along K")
     if (weight.data_ptr() & 15 or (strides[-2] & 15 and shape[-2] > 1)
             or (len(shape) == 3 and strides[0] & 15 and shape[0] > 1)):

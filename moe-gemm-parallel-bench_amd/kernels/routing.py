@@ -166,26 +166,36 @@ def _check_order(order: ExpertOrder, device) -> tuple[int, int]:
     """(tokens, k) of an order on ``device``."""
     import torch
 
-    offs, places = order.offs, order.places
-    if (places.ndim != 2 or places.dtype is not torch.int32 or places.device != device or not places.is_contiguous()
-            or places.shape[1] == 0):
+    offs, places, int32 = order.offs, order.places, torch.int32
+    shape = places.shape
+    if (len(shape) != 2 or places.dtype is not int32 or places.device != device or not places.is_contiguous()
+            or shape[1] == 0):
         raise ValueError("order.places must be a contiguous int32 [tokens, k] tensor on the rows' device")
-    if (offs.ndim != 1 or offs.dtype is not torch.int32 or offs.device != device or not offs.is_contiguous()
-            or offs.shape[0] == 0):
+    if (offs.ndim != 1 or offs.dtype is not int32 or offs.device != device or not offs.is_contiguous()
+            or len(offs) == 0):
         raise ValueError("order.offs must be a contiguous int32 vector on the rows' device")
-    return places.shape
+    return shape
 
 
-def _check_rows(name: str, t, rows: int | None, width: int | None) -> None:
-    if t.ndim != 2 or (rows is not None and t.shape[0] != rows) or (width is not None and t.shape[1] != width):
+def _end_of(order: ExpertOrder) -> int:
+    """Address of the last offset."""
+    return order.offs.data_ptr() + 4 * (len(order.offs) - 1)
+
+
+def _check_rows(name: str, t, rows: int | None, width: int | None) -> tuple[int, int]:
+    """(rows, width) of a matrix whose rows the kernels can walk."""
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (width is not None and shape[1] != width):
         expected = ", ".join("any" if n is None else str(n) for n in (rows, width))
-        raise ValueError(f"{name} must be a 2-D [{expected}] tensor (got {tuple(t.shape)})")
+        raise ValueError(f"{name} must be a 2-D [{expected}] tensor (got {tuple(shape)})")
+    count, columns = shape
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a GPU device")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    if columns > 1 and t.stride(1) != 1:
         raise ValueError(f"{name} needs a unit stride along its rows")
-    if t.shape[1] == 0 or max(t.shape) > _native.INT32_MAX or t.shape[1] * t.element_size() > _native.INT32_MAX:
-        raise ValueError(f"{name} must have between 1 and 2**31 - 1 bytes a row and under 2**31 rows (got {tuple(t.shape)})")
+    if columns == 0 or (count | columns) > _native.INT32_MAX or columns * t.element_size() > _native.INT32_MAX:
+        raise ValueError(f"{name} must have between 1 and 2**31 - 1 bytes a row and under 2**31 rows (got {tuple(shape)})")
+    return count, columns
 
 
 def gather_rows(x, order: ExpertOrder, *, rows: int | None = None):
@@ -204,19 +214,18 @@ def gather_rows(x, order: ExpertOrder, *, rows: int | None = None):
 
 def _gather(x, order, rows):
     tokens, k = _check_order(order, x.device)
-    _check_rows("x", x, tokens, None)
+    _, width = _check_rows("x", x, tokens, None)
     size = x.element_size()
     if size > 4:
         raise ValueError(f"x must have elements of 1, 2 or 4 bytes (got {x.dtype})")
     rows = tokens * k if rows is None else rows
     if not 0 <= rows <= _native.INT32_MAX:
         raise ValueError(f"rows must be 0 to 2**31 - 1 (got {rows})")
-    width = x.shape[1]
     out = x.new_empty((rows, width))
     if rows:
+        width *= size
         _native.launch(x.device, _native.library().moegemm_gather_rows, x.data_ptr(), out.data_ptr(), order.places.data_ptr(),
-                       order.offs.data_ptr() + 4 * (order.offs.shape[0] - 1), tokens, k, rows, width * size,
-                       _row_stride(x) * size, width * size)
+                       _end_of(order), tokens, k, rows, width, x.stride(0) * size if tokens > 1 else width, width)
     return out
 
 
@@ -243,17 +252,17 @@ def combine_rows(y, order: ExpertOrder, weights=None):
 
 
 def _combine(y, order, weights):
-    tokens, k = _check_order(order, y.device)
-    _check_rows("y", y, None, None)
+    device = y.device
+    tokens, k = _check_order(order, device)
+    rows, width = _check_rows("y", y, None, None)
     code = _native.dtype_code(y.dtype)
     if weights is not None:
-        _check_weights(weights, tokens, k, y.device)
-    width = y.shape[1]
+        _check_weights(weights, tokens, k, device)
     out = y.new_empty((tokens, width))
     if tokens:
-        _native.launch(y.device, _native.library().moegemm_combine_rows, y.data_ptr(),
+        _native.launch(device, _native.library().moegemm_combine_rows, y.data_ptr(),
                        None if weights is None else weights.data_ptr(), out.data_ptr(), order.places.data_ptr(), tokens, k,
-                       y.shape[0], width, _row_stride(y), width, code)
+                       rows, width, y.stride(0) if rows > 1 else width, width, code)
     return out
 
 
@@ -286,8 +295,7 @@ def _combine_gradients(dout, y, order, weights, rows: int, need_dy: bool, need_d
         _native.launch(dout.device, _native.library().moegemm_combine_rows_backward, dout.data_ptr(),
                        y.data_ptr() if need_dweights else None, None if weights is None else weights.data_ptr(),
                        dy.data_ptr() if need_dy and rows else None, dweights.data_ptr() if need_dweights else None,
-                       order.places.data_ptr(), order.offs.data_ptr() + 4 * (order.offs.shape[0] - 1), tokens, k, rows,
-                       width, _row_stride(dout), _row_stride(y) if need_dweights else 0, code)
+                       order.places.data_ptr(), _end_of(order), tokens, k, rows, width, _row_stride(dout), _row_stride(y) if need_dweights else 0, code)
     return dy, dweights
 
 
