@@ -174,11 +174,9 @@ typedef __amdgpu_buffer_rsrc_t mx_rsrc_t;
 __device__ __forceinline__ mx_rsrc_t mx_resource(const void* base, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
 }
+template <bool ONCE = false>  // non-temporal
 __device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
-  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, 0, 0));
-}
-__device__ __forceinline__ u32x4_t mx_load16_once(mx_rsrc_t r, uint32_t offset) {  // non-temporal
-  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, 0, 2));
+  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, 0, ONCE ? 2 : 0));
 }
 
 // A wave reads whole 128-byte lines of eight weight rows at a time, straight into registers: lane (q = lane / 16, c = lane %
@@ -191,7 +189,11 @@ __device__ __forceinline__ u32x4_t mx_load16_once(mx_rsrc_t r, uint32_t offset) 
 // of a row's 128 bytes and the lanes of the row exchange them, since byte loads of each lane's own cost as many
 // requests as the weights (256 rows over 32 experts of [4096, 7168]: REPLACE).  Offsets past a resource's bytes, which rows
 // past the last and K blocks past the end are given, read zeros and fetch nothing.
-template <class T>
+//
+// ONCE: weights pass the caches by.  That is faster where a line belongs to one block of one row (256 rows over 32 experts of
+// [4096, 7168]: 92 us, kept 97), and slower where rows begin inside a line, whose other part the next block or row
+// reads soon after (256 rows over 128 experts of [5760, 2880]: 255 us, kept 232).
+template <class T, bool ONCE>
 __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams p) {
   using A = typename T::A;
   constexpr int FN = T::FN, R = T::ROWS8, WK = T::WK, PARTS = T::PARTS;
@@ -240,7 +242,7 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       const bool up = T::GATED && i >= FN / 2;
-      q[i] = mx_load16_once(up ? rw2 : rw, wo + (uint32_t)((up ? i - FN / 2 : i) * 8) * (uint32_t)p.ldw);
+      q[i] = mx_load16<ONCE>(up ? rw2 : rw, wo + (uint32_t)((up ? i - FN / 2 : i) * 8) * (uint32_t)p.ldw);
     }
   };
   // The lane's 16 of the 128 bytes of blocks b to b + 15; zeros past the row's end, where nothing is read.

@@ -16,7 +16,12 @@ struct MxVariant {
 
 template <class T>
 hipError_t launch_mx(const MxParams& p, int grid, hipStream_t stream) {
-  hipLaunchKernelGGL((mx_stream_kernel<T>), dim3(grid), dim3(T::NT), MxTable::bytes(p.groups), stream, p);
+  const size_t lds = MxTable::bytes(p.groups);
+  // Few units' weights are small: kept.
+  if (T::SHARED && p.ldw % 128 == 0 && (reinterpret_cast<uintptr_t>(p.w) & 127) == 0)
+    hipLaunchKernelGGL((mx_stream_kernel<T, T::SHARED>), dim3(grid), dim3(T::NT), lds, stream, p);
+  else
+    hipLaunchKernelGGL((mx_stream_kernel<T, false>), dim3(grid), dim3(T::NT), lds, stream, p);
   return hipGetLastError();
 }
 
@@ -30,8 +35,12 @@ hipError_t launch_mx(const MxParams& p, int grid, hipStream_t stream) {
   MxVariant{8 * R, 8 * FN * WN / (GATED ? 2 : 1), WK, MxStream<A, R, FN, WN, WK, GATED>::PER_CU, \
             &launch_mx<MxStream<A, R, FN, WN, WK, GATED>>},
 // The kernels of a menu, for the device pass.
-#define MOEGEMM_MX_XK(A, R, FN, WN, WK, GATED) \
-  template __global__ void mx_stream_kernel<MxStream<A, R, FN, WN, WK, GATED>>(MxParams);
+#define MOEGEMM_MX_XK(A, R, FN, WN, WK, GATED)                                                   \
+  template __global__ void mx_stream_kernel<MxStream<A, R, FN, WN, WK, GATED>, false>(MxParams); \
+  MOEGEMM_MX_ONCE_##WK(A, R, FN, WN, WK, GATED)
+#define MOEGEMM_MX_ONCE_1(A, R, FN, WN, WK, GATED) \
+  template __global__ void mx_stream_kernel<MxStream<A, R, FN, WN, WK, GATED>, true>(MxParams);
+#define MOEGEMM_MX_ONCE_4(A, R, FN, WN, WK, GATED)
 
 #define MOEGEMM_MX_COUNT(...) +1
 constexpr int kNumMx = 0 MOEGEMM_MENU_MX(MOEGEMM_MX_COUNT, , false);
