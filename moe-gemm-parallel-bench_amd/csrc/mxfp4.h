@@ -99,7 +99,7 @@ __device__ __forceinline__ int mx_table(const MxTable& table, const MxParams& p,
     const int g = g0 + (int)threadIdx.x;
     int m = 0, row0 = 0;
     if (g < p.groups) row0 = group_rows(p.offs, p.rows, p.first + g, m);
-    if (g < p.groups) table.ends[g] = row0 + m;
+    if (g < p.groups) table.ends[g] = p.offs ? min(max(p.offs[p.first + g], 0), p.rows) : p.rows;  // the next group's first row
     if (g == 0) *table.start = row0;
     uint32_t count = (uint32_t)min((int64_t)((m + bm - 1) / bm) * p.n_tiles, (int64_t)INT32_MAX);
 #pragma unroll

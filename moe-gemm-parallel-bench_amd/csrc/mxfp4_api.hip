@@ -100,7 +100,7 @@ int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* 
   if (group_count <= 0) return report(MOEGEMM_ERR_INVALID, "group_count must be positive (got %d)", group_count);
   if (!offs && group_count != 1)
     return report(MOEGEMM_ERR_INVALID, "without offsets there is one group (got %d)", group_count);
-  if (rows < 0 || n <= 0 || k <= 0 || k % kMxGroup)
+  if (rows < 0 || rows >= 1 << 30 || n <= 0 || n >= 1 << 30 || k <= 0 || k % kMxGroup)
     return report(MOEGEMM_ERR_INVALID, "bad shape (rows=%d n=%d k=%d, k a multiple of 32)", rows, n, k);
   if (gated && n % 2) return report(MOEGEMM_ERR_INVALID, "packed Gate+Up width must be even (got %d)", n);
   if (variant < -1 || variant >= kNumMx)

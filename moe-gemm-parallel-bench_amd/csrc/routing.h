@@ -233,10 +233,10 @@ __device__ __forceinline__ float score_of(uint32_t key) {
   return __builtin_bit_cast(float, key >> 31 ? key ^ 0x80000000u : ~key);
 }
 // fp32 scores are within 2^-22 of sigmoid (exp of x is off by (|x| + 2) 2^-24 of itself, the sum and the reciprocal by 2^-24 and
-// 2^-23, and s (1 - s) |x| < 1/4) and within 2^-18 of softmax (|x| up to 88 counts 2^-17 |x| e^-|x|); a bias adds 2^-24 of the
-// sum.  Keys drop up to 1023 units of 2^-23 of their size.  Scores further apart than these margins, times their size or 1,
-// are in order.
-constexpr float kRouteMargin = 0x1p-12f, kGroupMargin = 0x1p-16f;
+// 2^-23, and s (1 - s) |x| < 1/4) and of softmax (whose sum is a 64-bit one, and |x| e^-|x| < 0.4); a bias adds 2^-24 of the sum.
+// Keys drop up to `mask` units of 2^-23 of their size.  Scores further apart than this, times their size or 1, are in order;
+// for sums of two, twice the scores' part.
+__host__ __device__ constexpr float route_margin(uint32_t mask) { return (float)(mask + 1) * 0x1p-23f + 0x1p-20f; }
 
 // Whether a, the larger in fp32, may not be the larger one (or is no number).
 __device__ __forceinline__ bool too_close(double a, double b, double margin) {
@@ -414,6 +414,10 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
         }
       }
     }
+    if constexpr (SCORES) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) lost |= (int)(i < count) & (int)(c[i] != c[i]);
+    }
     bool mine_in = true;  // a lane's experts are of one group
     if (p.groups > 1) {
       // A group's place among the groups: how many are before it.
@@ -442,7 +446,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
       mine_in = place(score) < p.top_groups;
       const float least = -token_max<LPT>(mine_in ? -score : -__builtin_inff());
       const float most = token_max<LPT>(mine_in ? -__builtin_inff() : score);
-      if (__ballot(p.top_groups < p.groups && too_close(least, most, kGroupMargin))) {
+      if (__ballot(p.top_groups < p.groups && too_close(least, most, 2 * route_margin(0)))) {
         double first = -__builtin_inf(), second = -__builtin_inf();
 #pragma unroll 1
         for (int i = 0; i < per; ++i) {
@@ -480,7 +484,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
     int mine = own ? (int)(MASK - (own & MASK)) : 0;
     float logit = own ? to_float<E>(x[mine]) : -__builtin_inff();
     if constexpr (!WHOLE) {
-      const bool close = own != 0 && next != 0 && too_close(score_of(own & ~MASK), score_of(next & ~MASK), kRouteMargin);
+      const bool close = own != 0 && next != 0 && too_close(score_of(own & ~MASK), score_of(next & ~MASK), route_margin(MASK));
       if (__ballot(close && li < p.k)) {
         // The list's order by 64-bit scores; what is not on it has to be smaller than the k-th by more than its error.
         const double score = own ? score64(logit, mine) : -__builtin_inf();
@@ -498,7 +502,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
         const uint64_t lo = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)bits);
         const uint64_t hi = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)(bits >> 32));
         lost |= li == p.k - 1 && list[TOP - 1] != 0 &&
-                too_close(__builtin_bit_cast(double, hi << 32 | lo), score_of(list[TOP - 1] & ~MASK), kRouteMargin);
+                too_close(__builtin_bit_cast(double, hi << 32 | lo), score_of(list[TOP - 1] & ~MASK), route_margin(MASK));
       }
     }
     const bool used = li < p.k;
@@ -859,7 +863,7 @@ template <class U>
 __device__ __forceinline__ void clear_rows(const RowsParams& p, int block, int blocks) {
   const int used = min(max(*p.end, 0), p.rows);
   for (int64_t r = used + block; r < p.rows; r += blocks)
-    for (int c = threadIdx.x * (int)sizeof(U); c < p.width; c += 256 * (int)sizeof(U))
+    for (int64_t c = threadIdx.x * sizeof(U); c < p.width; c += 256 * sizeof(U))
       *reinterpret_cast<U*>(p.to + r * p.ld_to + c) = U{};
 }
 

@@ -143,7 +143,7 @@ using U16 = u32x4_t;
 
 // `end` may be null where no rows are cleared.
 int check_rows(int64_t tokens, int32_t k, int32_t rows, int64_t width, const int32_t* places, const int32_t* end, bool clears) {
-  if (tokens < 0 || k <= 0 || rows < 0 || width <= 0 || width > INT32_MAX)
+  if (tokens < 0 || tokens > INT32_MAX || k <= 0 || rows < 0 || width <= 0 || width > INT32_MAX)
     return report(MOEGEMM_ERR_INVALID, "bad shape (tokens=%lld k=%d rows=%d, rows of %lld bytes)", (long long)tokens, k,
                   rows, (long long)width);
   if ((!places && tokens) || (!end && clears)) return report(MOEGEMM_ERR_INVALID, "places and offs must be non-null");

@@ -494,15 +494,15 @@ def tile_queue(device, stream_handle: int):
     return queue
 
 
-_DTYPE_CODES: dict = {}  # torch dtype -> code, filled on first use
+@lru_cache(maxsize=1)
+def _dtype_codes() -> dict:
+    import torch
+
+    return {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
 
 
 def dtype_code(dtype) -> int:
-    if not _DTYPE_CODES:
-        import torch
-
-        _DTYPE_CODES.update({torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32})
-    code = _DTYPE_CODES.get(dtype)
+    code = _dtype_codes().get(dtype)
     if code is None:
         raise ValueError(f"unsupported dtype {dtype}; expected float16, bfloat16 or float32")
     return code
@@ -525,17 +525,18 @@ def current_stream_handle(device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-_TORCH: list = []  # torch's current device and raw stream, bound on the first launch
+@lru_cache(maxsize=1)
+def _device_calls():
+    """torch's calls for the current device and a device's current stream."""
+    import torch
+
+    return torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def launch(device, entry, *args) -> None:
     """``entry(*args, stream)`` on ``device``'s current stream; a kernel goes to the current device, so that is made
     ``device`` where it is another."""
-    if not _TORCH:
-        import torch
-
-        _TORCH.extend((torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream))
-    current_device, raw_stream = _TORCH
+    current_device, raw_stream = _device_calls()
     index, current = device.index, current_device()
     if index is None or index == current:
         status = entry(*args, raw_stream(current))

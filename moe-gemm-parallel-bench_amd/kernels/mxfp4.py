@@ -39,6 +39,8 @@ def _matrices(t) -> list:
     """The matrices of a 2-D or 3-D tensor: one where its rows lie evenly, else one per leading index."""
     if t.ndim == 2:
         return [t]
+    if t.shape[1] == 1:
+        return [t.select(1, 0)]
     if t.shape[0] == 1 or t.stride(0) == t.shape[1] * t.stride(1):
         return [t.as_strided((t.shape[0] * t.shape[1], t.shape[2]), (t.stride(1), t.stride(2)))]
     return list(t.unbind(0))
@@ -180,8 +182,8 @@ def matmul_mxfp4(a, weight, scale, *, out=None, out_dtype=None, variant: int | N
 
     a [M, K] is fp16 or bf16, weight [N, K / 2] and scale [N, K / 32] uint8 as ``quantize_mxfp4`` returns them (or torch's
     float4_e2m1fn_x2 and float8_e8m0fnu).  fp32 sums; output in ``out_dtype`` (fp16, bf16 or fp32; a's by default).  M and N
-    are arbitrary, K is a multiple of 32; rows of a and weight start at multiples of 16 bytes.  ``variant`` names a
-    compiled kernel, None lets the library choose.
+    are arbitrary (under 2**30), K is a multiple of 32; rows of a and weight start at multiples of 16 bytes, less than 2**23
+    bytes apart.  ``variant`` names a compiled kernel, None lets the library choose.
     """
     return _product("moegemm_grouped_mm_mxfp4", a, weight, scale, None, out, out_dtype, variant, False)
 

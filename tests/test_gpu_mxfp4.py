@@ -128,7 +128,7 @@ def test_conversion_strides():
     from kernels import dequantize_mxfp4, quantize_mxfp4
 
     base = normal(3, 6, 50, 900).to(torch.bfloat16)
-    for view in (base[:, 3:, 1:641], base[::2, ::3, :96], base[4, :, :64], base[:1, :, 8:40], base[:, :0, :32]):
+    for view in (base[:, 3:, 1:641], base[:, 7:8, :32], base[:1, :3, :64].expand(5, 3, 64), base[::2, ::3, :96], base[4, :, :64], base[:1, :, 8:40], base[:, :0, :32]):
         q, scale = quantize_mxfp4(view)
         q0, scale0 = quantize_mxfp4(view.contiguous())
         assert torch.equal(q, q0) and torch.equal(scale, scale0)
@@ -227,6 +227,14 @@ def test_offsets_past_the_rows_and_decreasing_ones_stay_in_bounds():
     for values_ in ([5, 2, 9, 1], [-4, -1, 3, 3]):
         grouped_mm_mxfp4(a, q, scale, torch.tensor(values_, device="cuda", dtype=torch.int32))
     torch.cuda.synchronize()
+    # A group that begins before the end of an earlier, larger one: rows 2 to 90 are the third's or the first's.
+    a = normal(3, 100, 96).to(torch.bfloat16)
+    for variant in _variants():
+        out = torch.zeros(100, 40, device="cuda", dtype=torch.bfloat16)
+        grouped_mm_mxfp4(a, q, scale, torch.tensor([100, 2, 90, 1], device="cuda", dtype=torch.int32), out=out, variant=variant)
+        close(out[:2], a[:2], w[0])
+        close(out[90:], a[90:], w[0])
+        assert torch.isfinite(out).all()
 
 
 def test_scales_at_both_ends_and_nan():

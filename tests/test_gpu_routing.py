@@ -169,6 +169,36 @@ def test_nan_and_infinite_logits_keep_choices_valid():
         assert ((each >= 0) & (each < 100)).all() and all(len(set(r)) == 6 for r in each.tolist())
 
 
+def test_scores_that_are_no_numbers_keep_choices_valid():
+    """inf - inf and NaN made by the bias, over few experts and many: distinct indices, whatever their order."""
+    from kernels import route_topk
+
+    for experts in (8, 16, 200, 896):
+        x = normal(experts, 3, experts)
+        x[1, 5] = INF
+        for bad in (-INF, INF, float("nan")):
+            for score in ("softmax", "sigmoid"):
+                _, chosen = route_topk(x, 4, score=score, bias=torch.full((experts,), bad, device="cuda"))
+                assert ((chosen >= 0) & (chosen < experts)).all() and all(len(set(r)) == 4 for r in chosen.tolist())
+
+
+def test_many_equal_and_nearly_equal_scores():
+    """More ties at the k-th place than any short list holds, and scores one fp32 step apart throughout."""
+    from kernels import route_topk
+
+    step = 1 + torch.arange(256, device="cuda", dtype=torch.float64) * 2.0 ** -23
+    rows = torch.stack([torch.zeros(256, device="cuda"), step.float(), step.flip(0).float(),
+                        (torch.arange(256, device="cuda") % 3).float()])
+    bias = torch.zeros(256, device="cuda")
+    bias[::5] = 2.0 ** -30
+    for score in ("softmax", "sigmoid"):
+        for b in (None, bias):
+            for groups, top, best in ((1, 1, 1), (8, 4, 2), (16, 5, 1)):
+                _, chosen = route_topk(rows, 12, score=score, bias=b, groups=groups, top_groups=top, group_best=best)
+                _, expected = route(rows, 12, score, b, groups, top, best, True, 1.0)
+                assert torch.equal(chosen.long(), expected), (score, b is None, groups)
+
+
 def test_extreme_scores_keep_their_ratios():
     """Normalised weights of logits that all underflow beside a larger, ineligible one."""
     from kernels import route_topk
