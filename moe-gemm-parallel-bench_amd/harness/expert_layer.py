@@ -1,14 +1,17 @@
 """``python -m harness.expert_layer``: one rank's expert layer, trained in bf16 and served in fp8.
 
 The experts are those of one expert-parallel rank of ``--model-config`` (``num_experts / --parallel-size`` of them), with
-expert-sorted rows routed unevenly.  Three parts run on the same weights:
+expert-sorted rows routed unevenly.  Three parts run on the same weights, and a fourth with ``--top-k``:
 
 * training: ``--steps`` steps of gradient descent of the packed Gate+Up weights towards a target (the down projection
   stays as it is): ``gate_up_swiglu_forward``, ``grouped_mm``, and back through ``grouped_mm`` and
   ``gate_up_swiglu_backward``.  Weights are updated in fp32 and used in bf16; the loss is printed per step;
 * quantisation: the trained weights as e4m3 with a scale for each 128 x 128 block (``quantize_fp8``), once;
 * serving: ``quantize_fp8`` of the rows, ``grouped_mm_fp8_swiglu`` and ``grouped_mm_fp8``, for the training's rows and for
-  ``--decode-rows`` rows an expert; its normwise distance from the bf16 layer and both times are printed.
+  ``--decode-rows`` rows an expert; its normwise distance from the bf16 layer and both times are printed;
+* tokens (``--top-k`` of the experts each): ``route_topk`` of random logits, ``sort_by_expert``, ``gather_rows``, the experts with
+  4-bit weights (``quantize_mxfp4`` once; ``grouped_mm_mxfp4_swiglu`` and ``grouped_mm_mxfp4``), and ``combine_rows``; as above against
+  the bf16 experts, for as many routed rows.
 
 Each line is one JSON object.  Exit status 2 for bad arguments.  The reference times the forward GEMMs only
 (README.md:55-57): this driver has no counterpart there.
@@ -40,6 +43,7 @@ def build_parser() -> argparse.ArgumentParser:
     add("--steps", type=int, default=4)
     add("--learning-rate", type=float, default=0.01, help="step against the squared distance's gradient over (rows + H)")
     add("--fast-accum", action="store_true", help="8-bit matrix instructions in the fp8 products")
+    add("--top-k", type=int, default=0, help="experts of a token in the part that routes tokens; 0 leaves it out")
     add("--repeat", type=int, default=50, help="timed calls per measurement; 0 skips the timing")
     add("--device", default="cuda")
     add("--seed", type=int, default=1234)
@@ -53,6 +57,7 @@ class LayerSizes:
     ffn: int
     rows: int
     decode_rows: int
+    top_k: int = 0
 
 
 def layer_sizes(args: argparse.Namespace) -> LayerSizes:
@@ -72,7 +77,11 @@ def layer_sizes(args: argparse.Namespace) -> LayerSizes:
     if hidden % 16 or ffn % 16:
         raise ValueError("hidden and ffn sizes must be multiples of 16 (e4m3 rows of 16 bytes)")
     local = experts // args.parallel_size
-    return LayerSizes(local, hidden, ffn, local * args.rows, local * args.decode_rows)
+    if not 0 <= args.top_k <= min(local, 64):
+        raise ValueError(f"--top-k must be 0 to the rank's {local} experts, at most 64")
+    if args.top_k and (hidden % 32 or ffn % 32):
+        raise ValueError("hidden and ffn sizes must be multiples of 32 with --top-k (4-bit groups)")
+    return LayerSizes(local, hidden, ffn, local * args.rows, local * args.decode_rows, args.top_k)
 
 
 def uneven_ends(rows: int, experts: int):
@@ -140,8 +149,32 @@ class Fp8ExpertLayer:
         return grouped_mm_fp8(h, scale, self.w2, self.s2, offs, fast_accum=self.fast_accum)
 
 
+class Mxfp4ExpertLayer:
+    """The layer with 4-bit weights in groups of 32; rows stay bf16."""
+
+    def __init__(self, layer: ExpertLayer):
+        from kernels import quantize_mxfp4
+
+        self.w13 = quantize_mxfp4(layer.w13.transpose(1, 2).contiguous())
+        self.w2 = quantize_mxfp4(layer.w2t)
+
+    def forward(self, x, offs):
+        from kernels import grouped_mm_mxfp4, grouped_mm_mxfp4_swiglu
+
+        return grouped_mm_mxfp4(grouped_mm_mxfp4_swiglu(x, *self.w13, offs), *self.w2, offs)
+
+
+def routed(experts, x, logits, top_k: int):
+    """Tokens x [T, H] through ``top_k`` of the experts each, weighted by the softmax of their logits [T, E]."""
+    from kernels import combine_rows, gather_rows, route_topk, sort_by_expert
+
+    weights, chosen = route_topk(logits, top_k)
+    order = sort_by_expert(chosen, logits.shape[1])
+    return combine_rows(experts.forward(gather_rows(x, order), order.offs), order, weights)
+
+
 def run(args: argparse.Namespace, emit) -> None:
-    """The three parts; ``emit`` takes a dict per line."""
+    """The parts; ``emit`` takes a dict per line."""
     import torch
 
     from utils.benchmark import normwise_relative_error, select_cuda_device, time_cuda
@@ -169,6 +202,21 @@ def run(args: argparse.Namespace, emit) -> None:
         if args.repeat:
             for kind, run_one in (("fp8", served), ("bf16", layer)):
                 timing = time_cuda(lambda _: run_one.forward(x, offs), 10, args.repeat)
+                line[f"{kind}_us"] = round(timing.median_ms * 1e3, 2)
+        emit(line)
+    if not sizes.top_k:
+        return
+    small = Mxfp4ExpertLayer(layer)
+    for name, count in (("tokens_prefill", sizes.rows), ("tokens_decode", sizes.decode_rows)):
+        tokens = max(1, count // sizes.top_k)
+        x = torch.randn(tokens, sizes.hidden, device=device, generator=generator).bfloat16()
+        logits = torch.randn(tokens, sizes.experts, device=device, generator=generator)
+        line = {"part": name, "tokens": tokens, "top_k": sizes.top_k,
+                "distance": normwise_relative_error(routed(small, x, logits, sizes.top_k),
+                                                    routed(layer, x, logits, sizes.top_k))}
+        if args.repeat:
+            for kind, run_one in (("mxfp4", small), ("bf16", layer)):
+                timing = time_cuda(lambda _: routed(run_one, x, logits, sizes.top_k), 10, args.repeat)
                 line[f"{kind}_us"] = round(timing.median_ms * 1e3, 2)
         emit(line)
 
