@@ -7,7 +7,9 @@
 //
 // A weight v 2^(s - 127) has two significant bits and fp32's exponents, so it is exact in bf16: the conversion
 // instruction takes the scale along, and the bf16 matrix instructions, whose sums keep fp32's bits and whose operands
-// may be subnormal, do the rest.  fp16 rows are taken as two bf16 parts, 8 bits and the 3 behind them, which is exact too.
+// may be subnormal, do the rest.  fp16 rows are taken as two bf16 parts, 8 bits and the 3 behind them, which is exact too; fp32
+// rows as two as well, which are within 2^-16 of a value (2^-14 above 2^127) or 2^-134: a third would cost half as many matrix instructions again for bits
+// that a 16-bit output, which such rows are an intermediate of, does not show.
 #pragma once
 
 #include <type_traits>
@@ -20,7 +22,7 @@ constexpr int kMxGroup = 32;
 constexpr int kMxBlock = 256;  // K values of a weight row in 128 bytes
 
 struct MxParams {
-  const uint16_t* a;    // [rows, k], lda elements between rows
+  const void* a;        // [rows, k], lda elements between rows
   const uint8_t* w;     // [groups, n, k / 2]
   const uint8_t* sw;    // [groups, n, k / 32]
   void* out;            // [rows, n], or [rows, n / 2] where gated
@@ -44,34 +46,45 @@ __device__ __forceinline__ bf16x8_t mx_weights(uint32_t q, float scale) {
 // 2^(s - 127) as the conversion reads it: an exponent field (0 is 2^-127 there, 255 a NaN).
 __device__ __forceinline__ float mx_scale(uint32_t s) { return __builtin_bit_cast(float, s << 23); }
 
-// Eight values of a row as bf16 parts that add up to them.
+// Eight values of a row as they lie in memory, and as bf16 parts that add up to them.
 template <class A>
-struct RowParts;
-template <>
-struct RowParts<EBf16> {
-  static constexpr int N = 1;
-  bf16x8_t v[1];
-  __device__ __forceinline__ void set(u32x4_t x) { v[0] = __builtin_bit_cast(bf16x8_t, x); }
+struct RowPiece {
+  static constexpr int LOADS = A::is_f32 ? 2 : 1;
+  u32x4_t v[LOADS];
 };
-template <>
-struct RowParts<EF16> {
-  static constexpr int N = 2;
-  bf16x8_t v[2];
-  __device__ __forceinline__ void set(u32x4_t x) {
-    typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-    typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
-    const f16x8_t h = __builtin_bit_cast(f16x8_t, x);
-    u16x8_t hi, lo;
+template <class A>
+struct RowParts {
+  static constexpr int N = A::dtype == DT_BF16 ? 1 : 2;
+  bf16x8_t v[N];
+  __device__ __forceinline__ void set(const RowPiece<A>& x) {
+    if constexpr (A::dtype == DT_BF16) {
+      v[0] = __builtin_bit_cast(bf16x8_t, x.v[0]);
+    } else {
+      typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+      typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
+      u16x8_t hi, lo;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float f = (float)h[i];
-      const uint32_t top = __builtin_bit_cast(uint32_t, f) & 0xffff0000u;
-      hi[i] = (uint16_t)(top >> 16);
-      const float rest = f - __builtin_bit_cast(float, top);  // 0 for an infinity, which hi holds whole
-      lo[i] = (top & 0x7fffffffu) == 0x7f800000u ? 0 : (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16);
+      for (int i = 0; i < 8; ++i) {
+        float f;
+        if constexpr (A::is_f32) {
+          const uint32_t word = x.v[i >> 2][i & 3];  // a bit cast of the vector's element itself takes the first one
+          f = __builtin_bit_cast(float, word);
+        } else {
+          f = (float)__builtin_bit_cast(f16x8_t, x.v[0])[i];
+        }
+        const uint32_t bits = __builtin_bit_cast(uint32_t, f), top = bits & 0xffff0000u;
+        hi[i] = (uint16_t)(top >> 16);
+        const float rest = f - __builtin_bit_cast(float, top);  // 0 for an infinity, which hi holds whole
+        uint16_t low = (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16);  // exact for fp16
+        if constexpr (A::is_f32) {
+          // Above 2^127 rounding up could take the parts' sum past the largest number.
+          if ((bits & 0x7f800000u) != 0x7f000000u) low = __builtin_bit_cast(uint16_t, (__bf16)rest);
+        }
+        lo[i] = (bits & 0x7fffffffu) == 0x7f800000u ? 0 : low;
+      }
+      v[0] = __builtin_bit_cast(bf16x8_t, hi);
+      v[1] = __builtin_bit_cast(bf16x8_t, lo);
     }
-    v[0] = __builtin_bit_cast(bf16x8_t, hi);
-    v[1] = __builtin_bit_cast(bf16x8_t, lo);
   }
 };
 
@@ -152,7 +165,8 @@ struct MxStream {
   static constexpr int CHUNK = CHUNK_BLOCKS * kMxBlock;
   static constexpr int ROW_BYTES = CHUNK * 2 + 16;       // 16 bytes more: eight rows' pieces on all banks
   static constexpr int STAGE_BYTES = BM * ROW_BYTES;     // of one part
-  static constexpr int COPIES = BM * CHUNK * 2 / 16 / NT;  // 16-byte pieces of a stage a thread
+  static constexpr int ES = sizeof(typename A::raw);
+  static constexpr int COPIES = BM * CHUNK / 8 / NT;     // pieces of a stage a thread
   static constexpr int ROWS_BYTES = SHARED ? 2 * PARTS * STAGE_BYTES : 0;
   static constexpr int SUM_BYTES = WK * BM * (BN + 4) * 4;
   static constexpr int LDS_BYTES = ROWS_BYTES > SUM_BYTES ? ROWS_BYTES : SUM_BYTES;  // the sums where the rows were
@@ -163,7 +177,7 @@ struct MxStream {
   static constexpr int AHEAD = SHARED && ROWS8 <= 2 ? 3 : 1;      // blocks of weights on their way
   static_assert(4 % (AHEAD + 1) == 0, "a block's registers are known");
   static_assert(WN == 1 || WK == 1, "columns or K");
-  static_assert(!SHARED || BM * CHUNK * 2 / 16 % NT == 0, "whole copies");
+  static_assert(!SHARED || BM * CHUNK / 8 % NT == 0, "whole copies");
   static_assert(LDS_BYTES + 17 * 4 + 8 * kMxTable <= 160 * 1024, "LDS of one CU");
 };
 
@@ -233,7 +247,7 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
     const int64_t w_bytes = valid_n > 0 ? (valid_n - 1) * p.ldw + (p.k >> 1) : 0;
     rw = mx_resource(w, w_bytes);
     rw2 = T::GATED ? mx_resource(w + f * p.ldw, w_bytes) : rw;
-    ra = mx_resource(p.a + first_row * p.lda, ((valid_m - 1) * p.lda + p.k) * 2);
+    ra = mx_resource(static_cast<const char*>(p.a) + first_row * p.lda * T::ES, ((valid_m - 1) * p.lda + p.k) * T::ES);
     s = p.sw + (int64_t)e * p.ssg;
   };
   auto load = [&](u32x4_t (&q)[FN], int b) {
@@ -308,13 +322,18 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
   };
   // Shared rows go through registers to LDS, CHUNK values at a time and one chunk ahead, split into their parts on the way; a
   // wave that has its own part of K loads them as it needs them.
-  u32x4_t piece[T::SHARED ? T::COPIES : 1], av[T::SHARED ? 1 : 2][R][4];
+  constexpr uint32_t ES = T::ES;
+  auto load_piece = [&](RowPiece<A>& v, uint32_t offset) {
+#pragma unroll
+    for (int l = 0; l < RowPiece<A>::LOADS; ++l) v.v[l] = mx_load16(ra, offset + l * 16);
+  };
+  RowPiece<A> piece[T::SHARED ? T::COPIES : 1], av[T::SHARED ? 1 : 2][R][4];
   auto fetch = [&](int k0) {
 #pragma unroll
     for (int j = 0; j < T::COPIES; ++j) {
       const int at = threadIdx.x + j * T::NT, row = at / (T::CHUNK / 8), col = at % (T::CHUNK / 8);
-      const uint32_t offset = (uint32_t)row * (uint32_t)p.lda * 2 + (uint32_t)(k0 + col * 8) * 2;
-      piece[j] = mx_load16(ra, row < valid_m && k0 + col * 8 < p.k ? offset : kOutOfRange);
+      const uint32_t offset = ((uint32_t)row * (uint32_t)p.lda + (uint32_t)(k0 + col * 8)) * ES;
+      load_piece(piece[j], row < valid_m && k0 + col * 8 < p.k ? offset : kOutOfRange);
     }
   };
   auto put = [&](int stage) {
@@ -328,15 +347,15 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
         *reinterpret_cast<bf16x8_t*>(smem + (stage * PARTS + h) * T::STAGE_BYTES + row * T::ROW_BYTES + col * 16) = parts.v[h];
     }
   };
-  const uint32_t a_lane = (uint32_t)row8 * (uint32_t)p.lda * 2 + chunk * (kMxGroup * 2);
-  auto fetch_own = [&](u32x4_t (&v)[R][4], int b) {
+  const uint32_t a_lane = ((uint32_t)row8 * (uint32_t)p.lda + chunk * kMxGroup) * ES;
+  auto fetch_own = [&](RowPiece<A> (&v)[R][4], int b) {
     const bool in = b < end_b && b * kMxBlock + chunk * kMxGroup < p.k;
-    const uint32_t ao = in ? a_lane + (uint32_t)b * (kMxBlock * 2) : kOutOfRange;
+    const uint32_t ao = a_lane + (uint32_t)b * (kMxBlock * ES);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        v[r][x] = mx_load16(ra, r * 8 + row8 < valid_m ? ao + (uint32_t)(r * 8) * (uint32_t)p.lda * 2 + x * 16 : kOutOfRange);
+        load_piece(v[r][x], in && r * 8 + row8 < valid_m ? ao + ((uint32_t)(r * 8) * (uint32_t)p.lda + x * 8) * ES : kOutOfRange);
   };
   // Waves meet without waiting for what is on its way from memory.
   auto meet = [] {

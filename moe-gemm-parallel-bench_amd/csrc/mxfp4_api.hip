@@ -94,9 +94,8 @@ int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* 
                    int32_t rows, int32_t n, int32_t k, int64_t stride_am, int64_t stride_wg, int64_t stride_wn,
                    int64_t stride_sg, int64_t stride_sn, int64_t stride_om, int32_t dtype, int32_t out_dtype, bool gated,
                    int32_t variant, int32_t grid_size, void* stream) {
-  if (dtype != DT_F16 && dtype != DT_BF16)
-    return report(MOEGEMM_ERR_INVALID, "4-bit products need fp16 or bf16 rows (dtype code %d)", dtype);
-  if (!is_dtype(out_dtype)) return report(MOEGEMM_ERR_INVALID, "unsupported dtype code %d", out_dtype);
+  if (!is_dtype(dtype) || !is_dtype(out_dtype))
+    return report(MOEGEMM_ERR_INVALID, "unsupported dtype code %d or %d", dtype, out_dtype);
   if (group_count <= 0) return report(MOEGEMM_ERR_INVALID, "group_count must be positive (got %d)", group_count);
   if (!offs && group_count != 1)
     return report(MOEGEMM_ERR_INVALID, "without offsets there is one group (got %d)", group_count);
@@ -108,19 +107,22 @@ int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* 
   if (rows == 0) return MOEGEMM_OK;
   const int64_t cols = gated ? n / 2 : n;
   if (!a || !w || !scale || !out) return report(MOEGEMM_ERR_INVALID, "operands, scales and output must be non-null");
-  if (!aligned(a, 16) || stride_am % 8 || !aligned(w, 16) || stride_wn % 16 || stride_wg % 16)
+  if (!aligned(a, 16) || stride_am % (dtype == DT_F32 ? 4 : 8) || !aligned(w, 16) || stride_wn % 16 || stride_wg % 16)
     return report(MOEGEMM_ERR_INVALID, "rows of a and weight must start at multiples of 16 bytes");
   if (stride_am < 0 || stride_wn < k / 2 || stride_sn < k / kMxGroup || (rows > 1 && stride_om < cols))
     return report(MOEGEMM_ERR_INVALID, "row pitches must cover a row");
-  if (stride_am >= kPitchLimit / 2 || stride_wn >= kPitchLimit || stride_sn >= kPitchLimit || k > kPitchLimit / 2)
+  const int64_t es = dtype == DT_F32 ? 4 : 2;
+  if (stride_am * es >= kPitchLimit || k * es >= kPitchLimit || stride_wn >= kPitchLimit || stride_sn >= kPitchLimit)
     return report(MOEGEMM_ERR_INVALID, "rows of a, weight and scale must be less than %lld bytes apart", (long long)kPitchLimit);
   if (!aligned(out, out_dtype == DT_F32 ? 4 : 2))
     return report(MOEGEMM_ERR_INVALID, "out must be aligned to its element size");
   const int cus = grid_size > 0 ? grid_size : 256;
-  const MxVariant* table = dtype == DT_BF16 ? (gated ? kMxGatedBf16 : kMxBf16) : (gated ? kMxGatedF16 : kMxF16);
+  const MxVariant* table = dtype == DT_BF16  ? (gated ? kMxGatedBf16 : kMxBf16)
+                           : dtype == DT_F16 ? (gated ? kMxGatedF16 : kMxF16)
+                                             : (gated ? kMxGatedF32 : kMxF32);
   if (variant < 0) variant = choose(table, rows, group_count, cols, cus);
   const MxVariant& v = table[variant];
-  MxParams p{static_cast<const uint16_t*>(a), w, scale, out, offs, stride_am, stride_wg, stride_wn, stride_sg, stride_sn,
+  MxParams p{a, w, scale, out, offs, stride_am, stride_wg, stride_wn, stride_sg, stride_sn,
              stride_om, group_count, rows, n, k, (int32_t)cdiv(cols, v.cols), out_dtype};
   const int64_t row_tiles = std::min({rows / v.rows + (int64_t)group_count, group_count * cdiv(rows, v.rows), (int64_t)rows});
   const int64_t bound = row_tiles * p.n_tiles;

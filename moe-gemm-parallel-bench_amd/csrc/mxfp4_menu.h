@@ -45,6 +45,6 @@ hipError_t launch_mx(const MxParams& p, int grid, hipStream_t stream) {
 #define MOEGEMM_MX_COUNT(...) +1
 constexpr int kNumMx = 0 MOEGEMM_MENU_MX(MOEGEMM_MX_COUNT, , false);
 
-extern const MxVariant kMxBf16[], kMxF16[], kMxGatedBf16[], kMxGatedF16[];
+extern const MxVariant kMxBf16[], kMxF16[], kMxF32[], kMxGatedBf16[], kMxGatedF16[], kMxGatedF32[];
 
 }  // namespace moegemm

@@ -3,7 +3,7 @@
 The format is the one ``model_configs/gpt-oss-120b.json`` names (mxfp4), the OCP microscaling one: e2m1 values, two a byte
 with the even k in the low half, and an e8m0 byte ``s`` for each 32 along K; a value stands for ``v * 2**(s - 127)``.  Weights
 are stored ``[N, K / 2]`` (``[G, N, K / 2]`` for experts) with scales ``[..., N, K / 32]``, as checkpoints store them.  Rows stay
-fp16 or bf16.  The reference has no 4-bit path; this is the expert GEMM of its kernels/torch_grouped_gemm.py:121-174 on
+16-bit (fp32 ones are taken too).  The reference has no 4-bit path; this is the expert GEMM of its kernels/torch_grouped_gemm.py:121-174 on
 such weights.
 
 A serving step of one expert layer::
@@ -11,6 +11,9 @@ A serving step of one expert layer::
     q, s = quantize_mxfp4(w)                                        # once
     h = grouped_mm_mxfp4_swiglu(x, w13, s13, offs)                  # silu(gate) * up, [rows, F]
     y = grouped_mm_mxfp4(h, w2, s2, offs)                           # [rows, H]
+
+h is rounded to x's 16 bits between the two; ``out_dtype=torch.float32`` in the first and x's in the second leaves one rounding, at
+the end.
 
 The products are made for decode, where an expert has few rows and reading its weights is the bound; they take any number
 of rows.  Each call runs on the current stream, reads ``offs`` on the device and keeps nothing, so it can be captured in a
@@ -136,8 +139,7 @@ def _product(entry: str, a, weight, scale, offs, out, out_dtype, variant, gated:
     rows, k = a.shape
     n, groups = shape[-2], shape[0] if grouped else 1
     _check_weight(weight, scale, k)
-    if a.dtype is not torch.bfloat16 and a.dtype is not torch.float16:
-        raise ValueError("a must be fp16 or bf16")
+    a_code = _native.dtype_code(a.dtype)
     if groups <= 0 or n <= 0:
         raise ValueError("4-bit products need at least one group and a positive N")
     if rows | n | groups > _native.INT32_MAX:
@@ -153,7 +155,7 @@ def _product(entry: str, a, weight, scale, offs, out, out_dtype, variant, gated:
         if not offs.is_contiguous():
             raise ValueError("offs must be contiguous (pass offs.contiguous())")
     pitch, inner = a.stride()
-    if inner != 1 or a.data_ptr() & 15 or (pitch & 7 and rows > 1):
+    if inner != 1 or a.data_ptr() & 15 or (rows > 1 and pitch & (3 if a_code == _native.DTYPE_F32 else 7)):
         raise ValueError("a needs a unit stride along K and rows at multiples of 16 bytes")
     cols = n // 2 if gated else n
     if out is not None:
@@ -172,7 +174,7 @@ def _product(entry: str, a, weight, scale, offs, out, out_dtype, variant, gated:
                        out.data_ptr(), offs.data_ptr() if grouped else None, groups, rows, n, k, pitch if rows > 1 else k,
                        weight.stride(0) if grouped and groups > 1 else 0, weight.stride(-2) if n > 1 else k // 2,
                        scale.stride(0) if grouped and groups > 1 else 0, scale.stride(-2) if n > 1 else k // MX_GROUP,
-                       out.stride(0) if rows > 1 else cols, _native.dtype_code(a.dtype), code,
+                       out.stride(0) if rows > 1 else cols, a_code, code,
                        -1 if variant is None else variant, _cu_count(device))
     return out
 
@@ -180,7 +182,8 @@ def _product(entry: str, a, weight, scale, offs, out, out_dtype, variant, gated:
 def matmul_mxfp4(a, weight, scale, *, out=None, out_dtype=None, variant: int | None = None):
     """``a @ dequantized(weight, scale).T``; returns ``out`` (allocated if None).
 
-    a [M, K] is fp16 or bf16, weight [N, K / 2] and scale [N, K / 32] uint8 as ``quantize_mxfp4`` returns them (or torch's
+    a [M, K] is fp16, bf16 or fp32 (taken to within 2**-16 of each value, 2**-14 above 2**127, or
+    2**-134), weight [N, K / 2] and scale [N, K / 32] uint8 as ``quantize_mxfp4`` returns them (or torch's
     float4_e2m1fn_x2 and float8_e8m0fnu).  fp32 sums; output in ``out_dtype`` (fp16, bf16 or fp32; a's by default).  M and N
     are arbitrary (under 2**30), K is a multiple of 32; rows of a and weight start at multiples of 16 bytes, less than 2**23
     bytes apart.  ``variant`` names a compiled kernel, None lets the library choose.

@@ -3,7 +3,8 @@
 Bounds (derived, elementwise).  Conversions are exact: quantised bytes equal the definition's, and values equal them in
 bf16 and fp32 (fp16: one rounding).  Products: a weight is exact in bf16 and a row is a sum of exact bf16 parts, so an output
 differs from the 64-bit sum by the fp32 sums' rounding alone, (K + 8) 2^-23 sum_k |a w| (a unit of 2^-23 covers
-truncating adds), plus half a unit of the output type.  Gate+Up: silu' is at most 1.1 in size, and exp, division and
+truncating adds), plus half a unit of the output type.  fp32 rows are two bf16 parts: the first is cut to 8 bits, which leaves less than
+2^-7 of a value, of which the second keeps all but 2^-9: 2^-16 sum_k |a w| more.  Gate+Up: silu' is at most 1.1 in size, and exp, division and
 products in fp32 round by 2^-19 of the result.
 """
 
@@ -45,18 +46,23 @@ def weight(seed, *shape, low=115, high=125):
     return q, torch.randint(low, high, (*head, k // 32), device="cuda", dtype=torch.uint8, generator=generator)
 
 
+def sums(a):
+    """Error of a sum of products per sum of their sizes."""
+    return (a.shape[1] + 8) * 2.0 ** -23 + (2.0 ** -16 if a.dtype is torch.float32 else 0.0)
+
+
 def close(out, a, w, extra=0.0):
     """``out`` against a @ w.T, elementwise."""
     x = a.double()
     exact, size = x @ w.t(), x.abs() @ w.abs().t()
-    bound = HALF_UNIT[out.dtype] * exact.abs() + (a.shape[1] + 8) * 2.0 ** -23 * size + SMALL[out.dtype] + extra
+    bound = HALF_UNIT[out.dtype] * exact.abs() + sums(a) * size + SMALL[out.dtype] + extra
     worst = float(((out.double() - exact).abs() - bound).max()) if out.numel() else -1.0
     assert torch.isfinite(out).all() and worst <= 0, worst
 
 
 def close_gated(h, a, w):
     x, f = a.double(), w.shape[0] // 2
-    p, size = x @ w.t(), (a.shape[1] + 8) * 2.0 ** -23 * (x.abs() @ w.abs().t())
+    p, size = x @ w.t(), sums(a) * (x.abs() @ w.abs().t())
     g, u, ge, ue = p[:, :f], p[:, f:], size[:, :f], size[:, f:]
     s = torch.sigmoid(g)
     exact = g * s * u
@@ -151,7 +157,7 @@ SHAPES = [(1, 1, 32), (1, 5760, 2880), (2, 40, 64), (5, 72, 160), (8, 130, 2880)
           (33, 33, 288), (70, 96, 256)]
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("m,n,k", SHAPES)
 def test_single_products(m, n, k, dtype):
     from kernels import grouped_mm_mxfp4_swiglu, matmul_mxfp4
@@ -173,7 +179,7 @@ def test_single_products(m, n, k, dtype):
 GROUPS = [[1], [0, 3, 0, 5], [4, 0, 0, 1, 17, 2], [8] * 32, [0] * 9 + [1] + [0] * 5, [70, 1, 33, 0], [1] * 200, [0, 0]]
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("counts", GROUPS)
 @pytest.mark.parametrize("n,k", [(48, 96), (130, 544)])
 def test_grouped_products(counts, n, k, dtype):
@@ -271,7 +277,7 @@ def test_fp16_rows_keep_all_their_bits(dtype):
 def test_infinities_and_nan_stay_in_their_row():
     from kernels import matmul_mxfp4
 
-    for dtype in (torch.bfloat16, torch.float16):
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
         a = normal(4, 11, 288).abs().to(dtype)
         q, scale = weight(6, 50, 288)
         q &= 0x77  # no negative weights: an infinity cannot meet its opposite
@@ -282,6 +288,41 @@ def test_infinities_and_nan_stay_in_their_row():
         assert (out[3] == float("inf")).all() and torch.isnan(out[7]).all()
         keep = [r for r in range(11) if r not in (3, 7)]
         assert torch.equal(out[keep], clean[keep])
+
+
+def test_fp32_rows_from_end_to_end_of_their_range():
+    """Values next to the largest and subnormal ones, and a NaN whose payload lies below bf16's bits."""
+    from kernels import matmul_mxfp4
+
+    a = torch.zeros(4, 64, device="cuda")
+    a[0, 3], a[1, 40], a[2, 5] = torch.finfo(torch.float32).max, -2.0 ** -140, 1 + 2.0 ** -15
+    a[3, 9] = torch.tensor(0x7f800001, dtype=torch.int32).view(torch.float32)
+    q = torch.full((8, 32), 0x22, dtype=torch.uint8, device="cuda")  # 1.0 throughout
+    out = matmul_mxfp4(a, q, torch.full((8, 2), 127, dtype=torch.uint8, device="cuda"))
+    exact = a.double().sum(dim=1, keepdim=True)
+    assert torch.isnan(out[3]).all()
+    # The second part is a multiple of bf16's least number, 2^-133, and rounded to it: 2^-134 at most, here of one value times 1.
+    # (Of a subnormal value the first part is 0 or such a multiple too, and nothing bounds the error by its size.)
+    assert bool(((out[:3].double() - exact[:3]).abs() <= 2.0 ** -16 * exact[:3].abs() + 2.0 ** -134).all())
+    wide = normal(2, 6, 130)[:, 2:98]  # rows at multiples of 8 bytes: refused
+    with pytest.raises(ValueError, match="16 bytes"):
+        matmul_mxfp4(wide, *weight(1, 8, 96))
+    a = normal(2, 6, 132)[:, 4:100]
+    close(matmul_mxfp4(a, *weight(1, 8, 96)), a, values(*weight(1, 8, 96)))
+
+
+def test_one_rounding_with_a_wide_intermediate():
+    """h in fp32 between the two products: off the 64-bit layer by one bf16 rounding, 2^-16 of each product's sizes and sums."""
+    from kernels import grouped_mm_mxfp4, grouped_mm_mxfp4_swiglu
+
+    a, offs = normal(1, 20, 160).to(torch.bfloat16), torch.tensor([12, 20], device="cuda", dtype=torch.int32)
+    w13, w2 = weight(2, 2, 192, 160, low=118, high=121), weight(3, 2, 40, 96)
+    h = grouped_mm_mxfp4_swiglu(a, *w13, offs, out_dtype=torch.float32)
+    out = grouped_mm_mxfp4(h, *w2, offs, out_dtype=torch.bfloat16)
+    for e, part in enumerate((slice(0, 12), slice(12, 20))):
+        close_gated(h[part], a[part], values(*w13)[e])
+        close(out[part], h[part], values(*w2)[e])
+    assert out.dtype is torch.bfloat16
 
 
 def test_strides_types_and_given_outputs():

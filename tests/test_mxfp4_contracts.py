@@ -42,7 +42,7 @@ def test_dequantize_refuses_other_types():
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(), "GPU"), (dict(a=torch.zeros(3, 64)), "fp16 or bf16"), (dict(a=torch.zeros(3, 96, dtype=BF16)), "contraction"),
+    (dict(), "GPU"), (dict(a=torch.zeros(3, 64, dtype=torch.float64)), "dtype"), (dict(a=torch.zeros(3, 96, dtype=BF16)), "contraction"),
     (dict(a=torch.zeros(64, dtype=BF16)), "2-D"), (dict(w=torch.zeros(2, 8, 32)), "uint8"),
     (dict(w=torch.zeros(8, 32, dtype=U8)), "3-D"), (dict(s=torch.zeros(2, 8, 3, dtype=U8)), "scale"),
     (dict(a=torch.zeros(3, 48, dtype=BF16), w=torch.zeros(2, 8, 24, dtype=U8)), "multiple of 32"),
@@ -80,7 +80,7 @@ def _product(gated=False, **changes):
 
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("changes", [
-    dict(dtype=_native.DTYPE_F32), dict(out_dtype=4), dict(groups=0), dict(offs=None), dict(rows=-1), dict(n=0), dict(k=0), dict(k=48),
+    dict(dtype=7), dict(out_dtype=4), dict(lda=1 << 22), dict(dtype=_native.DTYPE_F32, lda=66), dict(groups=0), dict(offs=None), dict(rows=-1), dict(n=0), dict(k=0), dict(k=48),
     dict(a=None), dict(w=None), dict(s=None), dict(out=None), dict(a=4104), dict(w=4104), dict(lda=68), dict(lda=-8), dict(ldw=24),
     dict(ldw=40), dict(swg=520), dict(ssn=1), dict(ldo=7), dict(out=4097), dict(groups=1 << 20, n=1 << 20, rows=1 << 21, ldo=1 << 20)])
 def test_product_entries_refuse(gated, changes):
