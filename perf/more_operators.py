@@ -267,13 +267,14 @@ def _own(state):
     if not case["G"]:
         if kind == "matmul":
             return ops.matmul_mxfp4(state["a"], state["w"], state["scale"])
-        return ops.matmul_mxfp4(ops.grouped_mm_mxfp4_swiglu(state["a"], state["w"], state["scale"]), state["w2"],
-                                state["scale2"])
+        h = ops.grouped_mm_mxfp4_swiglu(state["a"], state["w"], state["scale"], out_dtype=torch.float32)
+        return ops.matmul_mxfp4(h, state["w2"], state["scale2"], out_dtype=dtype)
     offs = state["offs"]
     if kind == "matmul":
         return ops.grouped_mm_mxfp4(state["a"], state["w"], state["scale"], offs)
-    h = ops.grouped_mm_mxfp4_swiglu(state["a"], state["w"], state["scale"], offs)
-    return ops.grouped_mm_mxfp4(h, state["w2"], state["scale2"], offs)
+    # The activations stay in fp32 between the products, as in the plain form: one rounding, at the end.
+    h = ops.grouped_mm_mxfp4_swiglu(state["a"], state["w"], state["scale"], offs, out_dtype=torch.float32)
+    return ops.grouped_mm_mxfp4(h, state["w2"], state["scale2"], offs, out_dtype=dtype)
 
 
 def _group_best(case):
