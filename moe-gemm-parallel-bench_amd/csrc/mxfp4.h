@@ -150,32 +150,37 @@ __device__ __forceinline__ int mx_find(const MxTable& table, int groups, int uni
   return lo;
 }
 
-// 8 ROWS8 rows of a group by 8 FN weight rows a wave (GATED: 4 FN gate rows and the 4 FN up rows that go with them), and
+// ROWS rows of a group by 8 FN weight rows a wave (GATED: 4 FN gate rows and the 4 FN up rows that go with them), and
 // WN waves along the columns, which share the rows through LDS, or WK waves that take a part of K each.
-template <class A_, int ROWS8_, int FN_, int WN_, int WK_, bool GATED_>
+template <class A_, int ROWS_, int FN_, int WN_, int WK_, bool GATED_>
 struct MxStream {
   using A = A_;
-  static constexpr int ROWS8 = ROWS8_, FN = FN_, WN = WN_, WK = WK_;
+  static constexpr int FN = FN_, WN = WN_, WK = WK_;
   static constexpr bool GATED = GATED_, SHARED = WN > 1;
   static constexpr int NT = WN * WK * 64;
-  static constexpr int BM = 8 * ROWS8, BN = 8 * FN * WN;
+  static constexpr int BM = ROWS_, BN = 8 * FN * WN;
+  static constexpr bool EIGHT = BM == 8;
+  static constexpr int FM = EIGHT ? 1 : BM / 16, TILES = EIGHT ? FN : FN / 2;  // of 16 x 16 sums
+  static constexpr int HALVES = EIGHT ? 1 : 2;                                 // pieces of a row a lane needs of a block, by four
   static constexpr int OUT_COLS = GATED ? BN / 2 : BN;
   static constexpr int PARTS = RowParts<A>::N;
   static constexpr int CHUNK_BLOCKS = PARTS == 1 ? 2 : 1;  // K blocks of the rows in LDS
   static constexpr int CHUNK = CHUNK_BLOCKS * kMxBlock;
-  static constexpr int ROW_BYTES = CHUNK * 2 + 16;       // 16 bytes more: eight rows' pieces on all banks
+  static constexpr int ROW_BYTES = CHUNK * 2 + 16;       // 16 bytes more: rows' pieces on all banks
   static constexpr int STAGE_BYTES = BM * ROW_BYTES;     // of one part
   static constexpr int ES = sizeof(typename A::raw);
   static constexpr int COPIES = BM * CHUNK / 8 / NT;     // pieces of a stage a thread
   static constexpr int ROWS_BYTES = SHARED ? 2 * PARTS * STAGE_BYTES : 0;
   static constexpr int SUM_BYTES = WK * BM * (BN + 4) * 4;
   static constexpr int LDS_BYTES = ROWS_BYTES > SUM_BYTES ? ROWS_BYTES : SUM_BYTES;  // the sums where the rows were
-  // Two workgroups a CU where the rows are shared: more waves leave too few registers for the blocks ahead, and the groups'
-  // units come out uneven (256 rows over 32 experts, two a CU 92 us, three 104).
-  static constexpr int PER_CU = SHARED ? 2 : 4;
-  static constexpr int MIN_WAVES = 2;                             // a SIMD
-  static constexpr int AHEAD = SHARED && ROWS8 <= 2 ? 3 : 1;      // blocks of weights on their way
+  static constexpr int PER_CU = SHARED ? 2 : 4;          // workgroups a CU
+  static constexpr int MIN_WAVES = 2;                    // a SIMD
+  // Blocks of weights on their way.  256 rows over 32 experts of [4096, 7168] 86 us with three, 89 with one; over [7168,
+  // 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32: 128 and 127, 71 and 65.
+  static constexpr int AHEAD = SHARED && PARTS == 1 ? 3 : 1;
   static_assert(4 % (AHEAD + 1) == 0, "a block's registers are known");
+  static_assert(EIGHT || BM % 16 == 0, "whole matrix instructions");
+  static_assert(FN % 2 == 0, "weight rows go in pairs of eights");
   static_assert(WN == 1 || WK == 1, "columns or K");
   static_assert(!SHARED || BM * CHUNK / 8 % NT == 0, "whole copies");
   static_assert(LDS_BYTES + 17 * 4 + 8 * kMxTable <= 160 * 1024, "LDS of one CU");
@@ -194,10 +199,12 @@ __device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
 }
 
 // A wave reads whole 128-byte lines of eight weight rows at a time, straight into registers: lane (q = lane / 16, c = lane %
-// 16) holds the 16 bytes, one scale's 32 values, at chunk q + 4 (c / 8) of row c % 8.  As the operand of a 16 x 16 matrix
-// instruction, the lanes c >= 8 are eight more "rows": the same ones with the other half of K.  The activations are
-// laid out alike, so of the 16 x 16 outputs the two 8 x 8 squares on the diagonal are the halves' sums of eight rows by
-// eight rows, and the rest is not used.  That costs half the matrix rate and needs no exchange between lanes.
+// 16) holds the 16 bytes, one scale's 32 values, at chunk q + 4 (c / 8) of row c % 8.  The 16 x 16 matrix instructions want one
+// row a lane c, and one K for all rows: lanes c + 8 of eight rows change places with lanes c of the next eight (a DPP move
+// of each dword), which gives sixteen rows' first halves of the block, and their second halves.  For up to EIGHT rows the
+// weights stay where they are: lanes c >= 8 are the same eight weight rows with the other half of K, the activations are
+// laid out alike, and of the 16 x 16 sums the two 8 x 8 squares on the diagonal are the halves' sums; as many matrix
+// instructions, half the rows to load and split.
 //
 // The next blocks' weights are on their way while one is multiplied, and the scales of the next sixteen: a lane loads 16
 // of a row's 128 bytes and the lanes of the row exchange them, since byte loads of each lane's own cost as many
@@ -210,14 +217,14 @@ __device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
 template <class T, bool ONCE>
 __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams p) {
   using A = typename T::A;
-  constexpr int FN = T::FN, R = T::ROWS8, WK = T::WK, PARTS = T::PARTS;
+  constexpr int FM = T::FM, FN = T::FN, WK = T::WK, PARTS = T::PARTS, TILES = T::TILES, HALVES = T::HALVES;
   __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
   extern __shared__ int32_t s_table[];
   const MxTable table(s_table, p.groups);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wn = wave % T::WN, wk = wave / T::WN;
-  const int c = lane & 15, chunk = (lane >> 4) + 4 * (c >> 3), row8 = c & 7;
+  const int c = lane & 15, quad = lane >> 4, chunk = quad + 4 * (c >> 3), row8 = c & 7;
   const int f = p.n >> 1;
   const int blocks = (p.k + kMxBlock - 1) / kMxBlock, part = (blocks + WK - 1) / WK;
   const int first_b = min(wk * part, blocks), end_b = min(first_b + part, blocks);  // the wave's K blocks
@@ -293,30 +300,54 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
       for (int j = 0; j < 4; ++j) v[i][j] = past >= 16 ? 0 : __builtin_amdgcn_alignbyte(j < 3 ? x[j + 1] : 0, x[j], bytes);
     }
   };
-  f32x4_t acc[R][FN];
+  f32x4_t acc[FM][TILES];
   // Block `at` of the sixteen whose scales are at hand: byte 8 at + chunk of the row's 128, which lane at / 2 of the row's holds.
   auto multiply = [&](const u32x4_t (&q)[FN], const u32x4_t (&bytes)[FN], int at, int odd, auto&& rows_of) {
     const int other = at >> 1, from = ((other & 3) * 16 + (other >> 2) * 8 + row8) * 4;
-    float scale[FN];
+    uint32_t scale[FN];
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       const uint32_t low = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)bytes[i][2 * odd]);
       const uint32_t high = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)bytes[i][2 * odd + 1]);
-      scale[i] = mx_scale((chunk < 4 ? low : high) >> byte_shift & 0xff);
+      scale[i] = (chunk < 4 ? low : high) >> byte_shift & 0xff;
     }
+    // Of two eights of rows: all sixteen's first halves of the block, and their second.
+    auto first = [](uint32_t a, uint32_t b) {
+      return (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xf, 0xc, false);  // row_ror:8 into lanes 8 to 15
+    };
+    auto second = [](uint32_t a, uint32_t b) {
+      return (uint32_t)__builtin_amdgcn_update_dpp((int)b, (int)a, 0x128, 0xf, 0x3, false);  // into lanes 0 to 7
+    };
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      RowParts<A> rows[R];
+      RowParts<A> rows[FM][HALVES];
 #pragma unroll
-      for (int r = 0; r < R; ++r) rows_of(rows[r], r, x);
+      for (int m = 0; m < FM; ++m)
 #pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        const bf16x8_t weights = mx_weights(q[i][x], scale[i]);
+        for (int half = 0; half < HALVES; ++half) rows_of(rows[m][half], m, half, x);
+      if constexpr (T::EIGHT) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int i = 0; i < FN; ++i) {
+          const bf16x8_t weights = mx_weights(q[i][x], mx_scale(scale[i]));
 #pragma unroll
           for (int h = 0; h < PARTS; ++h)
-            acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(weights, rows[r].v[h], acc[r][i], 0, 0, 0);
+            acc[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(weights, rows[0][0].v[h], acc[0][i], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < FN; i += 2) {
+          const uint32_t a = q[i][x], b = q[i + 1][x];
+          const bf16x8_t weights[2] = {mx_weights(first(a, b), mx_scale(first(scale[i], scale[i + 1]))),
+                                       mx_weights(second(a, b), mx_scale(second(scale[i], scale[i + 1])))};
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int m = 0; m < FM; ++m)
+#pragma unroll
+              for (int h = 0; h < PARTS; ++h)
+                acc[m][i / 2] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(weights[half], rows[m][half].v[h], acc[m][i / 2], 0, 0, 0);
+        }
       }
     }
   };
@@ -327,7 +358,7 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
 #pragma unroll
     for (int l = 0; l < RowPiece<A>::LOADS; ++l) v.v[l] = mx_load16(ra, offset + l * 16);
   };
-  RowPiece<A> piece[T::SHARED ? T::COPIES : 1], av[T::SHARED ? 1 : 2][R][4];
+  RowPiece<A> piece[T::SHARED ? T::COPIES : 1], av[T::SHARED ? 1 : 2][FM][HALVES][4];
   auto fetch = [&](int k0) {
 #pragma unroll
     for (int j = 0; j < T::COPIES; ++j) {
@@ -347,15 +378,19 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
         *reinterpret_cast<bf16x8_t*>(smem + (stage * PARTS + h) * T::STAGE_BYTES + row * T::ROW_BYTES + col * 16) = parts.v[h];
     }
   };
-  const uint32_t a_lane = ((uint32_t)row8 * (uint32_t)p.lda + chunk * kMxGroup) * ES;
-  auto fetch_own = [&](RowPiece<A> (&v)[R][4], int b) {
-    const bool in = b < end_b && b * kMxBlock + chunk * kMxGroup < p.k;
-    const uint32_t ao = a_lane + (uint32_t)b * (kMxBlock * ES);
+  const int a_row = T::EIGHT ? row8 : c, a_chunk = T::EIGHT ? chunk : quad;  // of the lane, among 8 or 16
+  const uint32_t a_lane = ((uint32_t)a_row * (uint32_t)p.lda + a_chunk * kMxGroup) * ES;
+  auto fetch_own = [&](RowPiece<A> (&v)[FM][HALVES][4], int b) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int m = 0; m < FM; ++m)
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        load_piece(v[r][x], in && r * 8 + row8 < valid_m ? ao + ((uint32_t)(r * 8) * (uint32_t)p.lda + x * 8) * ES : kOutOfRange);
+      for (int half = 0; half < HALVES; ++half) {
+        const int k0 = b * kMxBlock + half * (kMxBlock / 2);
+        const bool in = b < end_b && k0 + a_chunk * kMxGroup < p.k && m * 16 + a_row < valid_m;
+        const uint32_t ao = a_lane + ((uint32_t)(m * 16) * (uint32_t)p.lda + (uint32_t)k0) * ES;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) load_piece(v[m][half][x], in ? ao + x * 8 * ES : kOutOfRange);
+      }
   };
   // Waves meet without waiting for what is on its way from memory.
   auto meet = [] {
@@ -363,7 +398,7 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
     __builtin_amdgcn_s_barrier();
     compiler_fence();
   };
-  const uint32_t frag = (uint32_t)row8 * T::ROW_BYTES + chunk * (kMxGroup * 2);
+  const uint32_t frag = (uint32_t)a_row * T::ROW_BYTES + a_chunk * (kMxGroup * 2);
 
   u32x4_t q[AHEAD + 1][FN];
   u32x4_t bytes[FN], next_bytes[FN];  // scales of sixteen blocks
@@ -380,9 +415,9 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
   start(unit);
   while (true) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int m = 0; m < FM; ++m)
 #pragma unroll
-      for (int i = 0; i < FN; ++i) acc[r][i] = f32x4_t{};
+      for (int i = 0; i < TILES; ++i) acc[m][i] = f32x4_t{};
     if constexpr (T::SHARED) {
       put(0);
       meet();
@@ -397,23 +432,26 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
         const int b = b0 + j;
         if (b >= end_b) break;
         if constexpr (T::SHARED) {
-          const int stage = CB == 4 ? (b0 >> 2) & 1 : j / CB & 1, half = j % CB;
-          if (half == 0) fetch((b + CB) * kMxBlock);
+          const int stage = j / CB & 1, place = j % CB;
+          if (place == 0) fetch((b + CB) * kMxBlock);
           load(q[(j + AHEAD) % (AHEAD + 1)], b + AHEAD);
-          multiply(q[j % (AHEAD + 1)], bytes, rel + j, j & 1, [&](RowParts<A>& rows, int r, int x) {
+          multiply(q[j % (AHEAD + 1)], bytes, rel + j, j & 1, [&](RowParts<A>& rows, int m, int half, int x) {
 #pragma unroll
             for (int h = 0; h < PARTS; ++h)
               rows.v[h] = *reinterpret_cast<const bf16x8_t*>(smem + (stage * PARTS + h) * T::STAGE_BYTES + frag +
-                                                            r * 8 * T::ROW_BYTES + half * (kMxBlock * 2) + x * 16);
+                                                            m * 16 * T::ROW_BYTES + place * (kMxBlock * 2) +
+                                                            half * kMxBlock + x * 16);
           });
-          if (half == CB - 1 && b + 1 < end_b) {
+          if (place == CB - 1 && b + 1 < end_b) {
             put(stage ^ 1);
             meet();
           }
         } else {
           load(q[(j + AHEAD) % (AHEAD + 1)], b + AHEAD);
           fetch_own(av[(j + 1) & 1], b + 1);
-          multiply(q[j % (AHEAD + 1)], bytes, rel + j, j & 1, [&](RowParts<A>& rows, int r, int x) { rows.set(av[j & 1][r][x]); });
+          multiply(q[j % (AHEAD + 1)], bytes, rel + j, j & 1, [&](RowParts<A>& rows, int m, int half, int x) {
+            rows.set(av[j & 1][m][half][x]);
+          });
         }
       }
       if (rel == 12) {
@@ -429,19 +467,22 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
     unit += gridDim.x;
     if (unit < units) start(unit);
 
-    // Lane (q, c) holds weight rows 4 q + j of row c; both halves of K meet, and the WK waves' sums in wave order.
+    // Lane (q, c) holds weight rows 4 q + j of sixteen, of row c, or of EIGHT both halves of K meet; the WK waves' sums are
+    // added in wave order.
     if constexpr (T::SHARED) meet();  // the sums go where the rows are
     float* sums = reinterpret_cast<float*>(smem);
     constexpr int LD = T::BN + 4;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int m = 0; m < FM; ++m)
 #pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        f32x4_t v;
+      for (int i = 0; i < TILES; ++i) {
+        f32x4_t v = acc[m][i];
+        if constexpr (T::EIGHT) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = acc[r][i][j] + __shfl_xor(acc[r][i][j], 40);
-        if (lane < 32 && c < 8)
-          *reinterpret_cast<f32x4_t*>(sums + (wk * T::BM + r * 8 + c) * LD + (wn * FN + i) * 8 + (lane >> 4) * 4) = v;
+          for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], 40);
+        }
+        if (!T::EIGHT || (quad < 2 && c < 8))
+          *reinterpret_cast<f32x4_t*>(sums + (wk * T::BM + m * 16 + c) * LD + wn * 8 * FN + i * (8 * HALVES) + quad * 4) = v;
       }
     meet();
     for (int x = threadIdx.x; x < T::BM * T::OUT_COLS; x += T::NT) {

@@ -64,30 +64,26 @@ hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
 }
 
 // Variant for `rows` rows over `groups` groups of `cols` output columns.  Routed groups are taken to hold up to 1.6 times the mean;
-// a group of more rows than a unit has its weights read again for each unit's rows.  Wide units (us): 256 rows over 128
-// experts of [5760, 2880], Gate+Up, 8 rows a unit 256, 16 rows 273; 256 rows over 32 of [4096, 7168] 126 and 92; 768 rows over
-// them 16 rows a unit 187, 32 rows 151.
-// Narrow units, whose waves split K, where the wide ones would not fill two workgroups a CU: one row of [5760, 2880] 6.4 wide 13,
-// four experts' rows of 128 x [5760, 2880] 12.7 and 14.8, 16 rows of [4096, 7168] 11.7 and 35; but 256 rows over 32
-// experts of [4096, 7168] 171 and 92.  Narrower ones where those leave CUs idle: 16 rows of [4096, 7168] 16 columns a unit 11.7, 32
-// columns 13.4, 32 rows 19.9 and 14.2; a row of one expert each, 4 of [2880, 2880], 8.4 and 9.3.
+// a group of more rows than a unit has its weights read again for each unit's rows.  Wide units, Gate+Up (us): 256 rows over
+// 128 experts of [5760, 2880] 8 rows a unit 234, 16 rows 244; 256 rows over 32 of [4096, 7168] 124 and 102; 768 rows over them 16
+// rows 177, 32 rows 128.
+// Narrow units, whose waves split K, where the wide ones would not fill two workgroups a CU: one row of [5760, 2880] 5.7, wide 12.6,
+// four experts' rows of 128 x [2880, 2880] 8.3 and 13.3, 32 rows of [4096, 7168] 13.0 and 23.2; but 256 rows over 32
+// experts of [4096, 7168] 171 and 86.  Sixteen rows a narrow unit where that leaves no CU idle: 32 rows of [4096, 7168], 256 units, 13.0
+// and by eight rows 16.9, but 16 rows, 128 units, 12.6 and by eight 10.0.
 int choose(const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
   const int64_t active = std::min(groups, rows), mean = cdiv(rows, active);
   const int64_t high = active == 1 ? rows : cdiv(mean * 8, 5);
-  auto find = [&](int wanted_rows, bool wide, bool widest) {
-    int best = -1;
-    for (int i = 0; i < kNumMx; ++i) {
-      const MxVariant& v = table[i];
-      if (v.rows != wanted_rows || (v.waves_k == 1) != wide) continue;
-      if (best < 0 || (v.cols > table[best].cols) == widest) best = i;
-    }
-    return best;
+  auto find = [&](int wanted_rows, bool wide) {
+    int i = 0;
+    while (table[i].rows != wanted_rows || (table[i].waves_k == 1) != wide) ++i;
+    return i;
   };
   auto units = [&](int i) { return active * cdiv(mean, table[i].rows) * cdiv(cols, table[i].cols); };
-  const int wide = find(high <= 8 ? 8 : high <= 16 ? 16 : 32, true, true);
+  const int wide = find(high <= 8 ? 8 : high <= 16 ? 16 : 32, true);
   if (units(wide) >= 2 * cus) return wide;
-  const int few = high <= 8 ? 8 : 16, narrow = find(few, false, true);
-  return units(narrow) * (few == 8 ? 2 : 3) < 3 * cus ? find(few, false, false) : narrow;
+  const int narrow = find(16, false);
+  return high <= 8 || units(narrow) < cus ? find(8, false) : narrow;
 }
 
 int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs, int32_t group_count,

@@ -25,22 +25,22 @@ hipError_t launch_mx(const MxParams& p, int grid, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// X(A, ROWS8, FN, WAVES_N, WAVES_K, GATED): 8, 16 or 32 rows by 128 weight rows for many units, 32 or 16 weight rows with K split
-// over the waves for few.
-#define MOEGEMM_MENU_MX(X, A, GATED)                                                             \
-  X(A, 1, 4, 4, 1, GATED) X(A, 2, 4, 4, 1, GATED) X(A, 4, 4, 4, 1, GATED)                         \
-  X(A, 1, 4, 1, 4, GATED) X(A, 2, 4, 1, 4, GATED) X(A, 1, 2, 1, 4, GATED) X(A, 2, 2, 1, 4, GATED)
+// X(A, ROWS, FN, WAVES_N, WAVES_K, GATED): 8, 16 or 32 rows by 128 weight rows for many units, 8 or 16 rows by 32 weight rows with K
+// split over the waves for few.
+#define MOEGEMM_MENU_MX(X, A, GATED)                                        \
+  X(A, 8, 4, 4, 1, GATED) X(A, 16, 4, 4, 1, GATED) X(A, 32, 4, 4, 1, GATED) \
+  X(A, 8, 4, 1, 4, GATED) X(A, 16, 4, 1, 4, GATED)
 
-#define MOEGEMM_MX_X(A, R, FN, WN, WK, GATED)                                                                \
-  MxVariant{8 * R, 8 * FN * WN / (GATED ? 2 : 1), WK, MxStream<A, R, FN, WN, WK, GATED>::PER_CU, \
-            &launch_mx<MxStream<A, R, FN, WN, WK, GATED>>},
+#define MOEGEMM_MX_X(A, ROWS, FN, WN, WK, GATED)                                                                \
+  MxVariant{ROWS, 8 * FN * WN / (GATED ? 2 : 1), WK, MxStream<A, ROWS, FN, WN, WK, GATED>::PER_CU, \
+            &launch_mx<MxStream<A, ROWS, FN, WN, WK, GATED>>},
 // The kernels of a menu, for the device pass.
-#define MOEGEMM_MX_XK(A, R, FN, WN, WK, GATED)                                                   \
-  template __global__ void mx_stream_kernel<MxStream<A, R, FN, WN, WK, GATED>, false>(MxParams); \
-  MOEGEMM_MX_ONCE_##WK(A, R, FN, WN, WK, GATED)
-#define MOEGEMM_MX_ONCE_1(A, R, FN, WN, WK, GATED) \
-  template __global__ void mx_stream_kernel<MxStream<A, R, FN, WN, WK, GATED>, true>(MxParams);
-#define MOEGEMM_MX_ONCE_4(A, R, FN, WN, WK, GATED)
+#define MOEGEMM_MX_XK(A, ROWS, FN, WN, WK, GATED)                                                   \
+  template __global__ void mx_stream_kernel<MxStream<A, ROWS, FN, WN, WK, GATED>, false>(MxParams); \
+  MOEGEMM_MX_ONCE_##WK(A, ROWS, FN, WN, WK, GATED)
+#define MOEGEMM_MX_ONCE_1(A, ROWS, FN, WN, WK, GATED) \
+  template __global__ void mx_stream_kernel<MxStream<A, ROWS, FN, WN, WK, GATED>, true>(MxParams);
+#define MOEGEMM_MX_ONCE_4(A, ROWS, FN, WN, WK, GATED)
 
 #define MOEGEMM_MX_COUNT(...) +1
 constexpr int kNumMx = 0 MOEGEMM_MENU_MX(MOEGEMM_MX_COUNT, , false);
