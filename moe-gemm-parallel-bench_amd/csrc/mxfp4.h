@@ -164,7 +164,7 @@ struct MxStream {
   static constexpr int HALVES = EIGHT ? 1 : 2;                                 // pieces of a row a lane needs of a block, by four
   static constexpr int OUT_COLS = GATED ? BN / 2 : BN;
   static constexpr int PARTS = RowParts<A>::N;
-  static constexpr int CHUNK_BLOCKS = PARTS == 1 ? 2 : 1;  // K blocks of the rows in LDS
+  static constexpr int CHUNK_BLOCKS = PARTS == 1 && BM <= 32 ? 2 : 1;  // K blocks of the rows in LDS
   static constexpr int CHUNK = CHUNK_BLOCKS * kMxBlock;
   static constexpr int ROW_BYTES = CHUNK * 2 + 16;       // 16 bytes more: rows' pieces on all banks
   static constexpr int STAGE_BYTES = BM * ROW_BYTES;     // of one part
@@ -176,8 +176,9 @@ struct MxStream {
   static constexpr int PER_CU = SHARED ? 2 : 4;          // workgroups a CU
   static constexpr int MIN_WAVES = 2;                    // a SIMD
   // Blocks of weights on their way.  256 rows over 32 experts of [4096, 7168] 86 us with three, 89 with one; over [7168,
-  // 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32: 128 and 127, 71 and 65.
-  static constexpr int AHEAD = SHARED && PARTS == 1 ? 3 : 1;
+  // 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32: 128 and 127, 71 and 65; 2048
+  // rows, 64 a unit, over [4096, 7168] 219 and 210.
+  static constexpr int AHEAD = SHARED && PARTS == 1 && BM <= 32 ? 3 : 1;
   static_assert(4 % (AHEAD + 1) == 0, "a block's registers are known");
   static_assert(EIGHT || BM % 16 == 0, "whole matrix instructions");
   static_assert(FN % 2 == 0, "weight rows go in pairs of eights");
@@ -211,9 +212,10 @@ __device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
 // requests as the weights (256 rows over 32 experts of [4096, 7168]: bytes 115 us, four at a time 95, 16 92).  Offsets past a resource's bytes, which rows
 // past the last and K blocks past the end are given, read zeros and fetch nothing.
 //
-// ONCE: weights pass the caches by.  That is faster where a line belongs to one block of one row (256 rows over 32 experts of
-// [4096, 7168]: 92 us, kept 97), and slower where rows begin inside a line, whose other part the next block or row
-// reads soon after (256 rows over 128 experts of [5760, 2880]: 255 us, kept 232).
+// ONCE: weights pass the caches by.  That is faster where a line belongs to one block of one row that one unit reads (256 rows
+// over 32 experts of [4096, 7168]: 86 us, kept 102), and slower where rows begin inside a line, whose other part the next
+// block or row reads soon after (256 rows over 128 experts of [5760, 2880]: 255 us, kept 232), or where a group's other units
+// read the weights too (2048 rows over 32 of [7168, 2048], 32 a unit: 152 us, kept 134).
 template <class T, bool ONCE>
 __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams p) {
   using A = typename T::A;

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/moegemm.h"
 #include "error.h"
@@ -63,27 +64,32 @@ hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Variant for `rows` rows over `groups` groups of `cols` output columns.  Routed groups are taken to hold up to 1.6 times the mean;
-// a group of more rows than a unit has its weights read again for each unit's rows.  Wide units, Gate+Up (us): 256 rows over
-// 128 experts of [5760, 2880] 8 rows a unit 234, 16 rows 244; 256 rows over 32 of [4096, 7168] 124 and 102; 768 rows over them 16
-// rows 177, 32 rows 128.
-// Narrow units, whose waves split K, where the wide ones would not fill two workgroups a CU: one row of [5760, 2880] 5.7, wide 12.6,
-// four experts' rows of 128 x [2880, 2880] 8.3 and 13.3, 32 rows of [4096, 7168] 13.0 and 23.2; but 256 rows over 32
-// experts of [4096, 7168] 171 and 86.  Sixteen rows a narrow unit where that leaves no CU idle: 32 rows of [4096, 7168], 256 units, 13.0
-// and by eight rows 16.9, but 16 rows, 128 units, 12.6 and by eight 10.0.
-int choose(const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
-  const int64_t active = std::min(groups, rows), mean = cdiv(rows, active);
-  const int64_t high = active == 1 ? rows : cdiv(mean * 8, 5);
-  auto find = [&](int wanted_rows, bool wide) {
-    int i = 0;
-    while (table[i].rows != wanted_rows || (table[i].waves_k == 1) != wide) ++i;
-    return i;
-  };
-  auto units = [&](int i) { return active * cdiv(mean, table[i].rows) * cdiv(cols, table[i].cols); };
-  const int wide = find(high <= 8 ? 8 : high <= 16 ? 16 : 32, true);
-  if (units(wide) >= 2 * cus) return wide;
-  const int narrow = find(16, false);
-  return high <= 8 || units(narrow) < cus ? find(8, false) : narrow;
+// Variant of the least estimated time for `rows` rows over `groups` groups of `cols` output columns.  Routed groups are taken to
+// hold 0.4 to 1.6 times the mean; a group of more rows than a unit has its weights read again for each unit's rows.  A CU
+// works on two units at a time: it takes half of its units' number, at least 0.65, times what a unit of the variant takes for
+// 256 of K (us, from launches of many units, in the tables' order; rows of one part and of two):
+constexpr double kUnitTime[2][kNumMx] = {{1.15, 1.36, 1.72, 0.46, 0.67, 2.55}, {1.80, 2.05, 3.40, 0.80, 1.05, 3.40}};
+// Of 207 calls (10 weights, 1 to 1024 rows, three types) the chosen one took 1.01 times the best one's time in the mean, at most
+// 1.32.  What the variants take, in the same order (us, bf16): 32 experts of [4096, 7168] by 256 rows 122, 88, 99, 161, 135,
+// 131; by 1024 rows 340, 204, 162, 467, 369, 151; one weight of [4096, 7168] by 16 rows 22, 25, 31, 11, 13, 46; by 32 rows 23, 24, 31,
+// 18, 14, 47.
+int choose(bool two_parts, const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
+  const int64_t active = std::min(groups, rows);
+  const double mean = (double)rows / active;
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < kNumMx; ++i) {
+    double tiles = 0;
+    for (int j = 0; j < 7; ++j)
+      tiles += std::ceil(std::max(active == 1 ? mean : mean * (0.4 + 0.2 * j), 1.0) / table[i].rows - 1e-9) / 7;
+    const double units = std::ceil(active * tiles * cdiv(cols, table[i].cols) / cus - 1e-9);  // of a CU
+    const double time = std::max(units / 2, 0.65) * kUnitTime[two_parts][i];
+    if (i == 0 || time < least) {
+      best = i;
+      least = time;
+    }
+  }
+  return best;
 }
 
 int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs, int32_t group_count,
@@ -116,7 +122,7 @@ int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* 
   const MxVariant* table = dtype == DT_BF16  ? (gated ? kMxGatedBf16 : kMxBf16)
                            : dtype == DT_F16 ? (gated ? kMxGatedF16 : kMxF16)
                                              : (gated ? kMxGatedF32 : kMxF32);
-  if (variant < 0) variant = choose(table, rows, group_count, cols, cus);
+  if (variant < 0) variant = choose(dtype != DT_BF16, table, rows, group_count, cols, cus);
   const MxVariant& v = table[variant];
   MxParams p{a, w, scale, out, offs, stride_am, stride_wg, stride_wn, stride_sg, stride_sn,
              stride_om, group_count, rows, n, k, (int32_t)cdiv(cols, v.cols), out_dtype};
@@ -124,9 +130,10 @@ int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* 
   const int64_t bound = row_tiles * p.n_tiles;
   if (bound > INT32_MAX / 2) return report(MOEGEMM_ERR_INVALID, "tile count exceeds int32");
   const int grid = (int)std::min<int64_t>(bound, (int64_t)cus * v.per_cu);
+  const bool once = stride_wn % 128 == 0 && aligned(w, 128) && cdiv(rows, group_count) <= v.rows;
   for (; p.first < group_count; p.first += kMxTable) {
     p.groups = std::min(group_count - p.first, kMxTable);
-    const int rc = checked(v.launch(p, grid, reinterpret_cast<hipStream_t>(stream)));
+    const int rc = checked(v.launch(p, grid, once, reinterpret_cast<hipStream_t>(stream)));
     if (rc != MOEGEMM_OK) return rc;
   }
   return MOEGEMM_OK;
