@@ -2,14 +2,15 @@
 //
 //   C[m, n] = sum_k a[m, k] v[n, k] 2^(s[n, k / 32] - 127)
 //
-// v is e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte, the even k in the low half; s is e8m0, one for
-// each 32 along K, 255 a NaN: the OCP microscaling format that model_configs/gpt-oss-120b.json names (mxfp4).
+// v is e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte, the even k in the low half; s is e8m0, one
+// for each 32 along K, 255 a NaN: the OCP microscaling format that model_configs/gpt-oss-120b.json names (mxfp4).
 //
 // A weight v 2^(s - 127) has two significant bits and fp32's exponents, so it is exact in bf16: the conversion
 // instruction takes the scale along, and the bf16 matrix instructions, whose sums keep fp32's bits and whose operands
-// may be subnormal, do the rest.  fp16 rows are taken as two bf16 parts, 8 bits and the 3 behind them, which is exact too; fp32
-// rows as two as well, which are within 2^-16 of a value (2^-14 above 2^127) or 2^-134: a third would cost half as many matrix instructions again for bits
-// that a 16-bit output, which such rows are an intermediate of, does not show.
+// may be subnormal, do the rest.  fp16 rows are taken as two bf16 parts, 8 bits and the 3 behind them, which is exact
+// too; fp32 rows as two as well, which are within 2^-16 of a value (2^-14 above 2^127) or 2^-134: a third would cost
+// half as many matrix instructions again for bits that a 16-bit output, which such rows are an intermediate of, does
+// not show.
 #pragma once
 
 #include <type_traits>
@@ -88,8 +89,8 @@ struct RowParts {
   }
 };
 
-// The units of a launch's groups, in LDS behind the kernel's other arrays: cumulative counts of ceil(m / bm) * n_tiles, and the
-// groups' rows.
+// The units of a launch's groups, in LDS behind the kernel's other arrays: cumulative counts of ceil(m / bm) * n_tiles,
+// and the groups' rows.
 constexpr int kMxTable = 1024;
 struct MxTable {
   int32_t* units;
@@ -175,9 +176,9 @@ struct MxStream {
   static constexpr int LDS_BYTES = ROWS_BYTES > SUM_BYTES ? ROWS_BYTES : SUM_BYTES;  // the sums where the rows were
   static constexpr int PER_CU = SHARED ? 2 : 4;          // workgroups a CU
   static constexpr int MIN_WAVES = 2;                    // a SIMD
-  // Blocks of weights on their way.  256 rows over 32 experts of [4096, 7168] 86 us with three, 89 with one; over [7168,
-  // 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32: 128 and 127, 71 and 65; 2048
-  // rows, 64 a unit, over [4096, 7168] 219 and 210.
+  // Blocks of weights on their way.  256 rows over 32 experts of [4096, 7168] 86 us with three, 89 with one; over
+  // [7168, 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32: 128 and 127, 71 and
+  // 65; 2048 rows, 64 a unit, over [4096, 7168] 219 and 210.
   static constexpr int AHEAD = SHARED && PARTS == 1 && BM <= 32 ? 3 : 1;
   static_assert(4 % (AHEAD + 1) == 0, "a block's registers are known");
   static_assert(EIGHT || BM % 16 == 0, "whole matrix instructions");
@@ -199,23 +200,29 @@ __device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
   return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, 0, ONCE ? 2 : 0));
 }
 
-// A wave reads whole 128-byte lines of eight weight rows at a time, straight into registers: lane (q = lane / 16, c = lane %
-// 16) holds the 16 bytes, one scale's 32 values, at chunk q + 4 (c / 8) of row c % 8.  The 16 x 16 matrix instructions want one
-// row a lane c, and one K for all rows: lanes c + 8 of eight rows change places with lanes c of the next eight (a DPP move
-// of each dword), which gives sixteen rows' first halves of the block, and their second halves.  For up to EIGHT rows the
-// weights stay where they are: lanes c >= 8 are the same eight weight rows with the other half of K, the activations are
-// laid out alike, and of the 16 x 16 sums the two 8 x 8 squares on the diagonal are the halves' sums; as many matrix
-// instructions, half the rows to load and split.
+// A wave reads whole 128-byte lines of eight weight rows at a time, straight into registers: lane (q = lane / 16, c =
+// lane % 16) holds the 16 bytes, one scale's 32 values, at chunk q + 4 (c / 8) of row c % 8.  The 16 x 16 matrix
+// instructions want one row a lane c, and one K for all rows: lanes c + 8 of eight rows change places with lanes c of
+// the next eight (a DPP move of each dword), which gives sixteen rows' first halves of the block, and their second
+// halves.  For up to EIGHT rows the weights stay where they are: lanes c >= 8 are the same eight weight rows with the
+// other half of K, the activations are laid out alike, and of the 16 x 16 sums the two 8 x 8 squares on the diagonal
+// are the halves' sums; as many matrix instructions, half the rows to load and split.
 //
-// The next blocks' weights are on their way while one is multiplied, and the scales of the next sixteen: a lane loads 16
-// of a row's 128 bytes and the lanes of the row exchange them, since byte loads of each lane's own cost as many
-// requests as the weights (256 rows over 32 experts of [4096, 7168]: bytes 115 us, four at a time 95, 16 92).  Offsets past a resource's bytes, which rows
-// past the last and K blocks past the end are given, read zeros and fetch nothing.
+// The next blocks' weights are on their way while one is multiplied, and the scales of the next sixteen: a lane loads
+// 16 of a row's 128 bytes and the lanes of the row exchange them, since byte loads of each lane's own cost as many
+// requests as the weights (256 rows over 32 experts of [4096, 7168]: bytes 115 us, four at a time 95, 16 92).  Offsets
+// past a resource's bytes, which rows past the last and K blocks past the end are given, read zeros and fetch nothing.
 //
-// ONCE: weights pass the caches by.  That is faster where a line belongs to one block of one row that one unit reads (256 rows
-// over 32 experts of [4096, 7168]: 86 us, kept 102), and slower where rows begin inside a line, whose other part the next
-// block or row reads soon after (256 rows over 128 experts of [5760, 2880]: 255 us, kept 232), or where a group's other units
-// read the weights too (2048 rows over 32 of [7168, 2048], 32 a unit: 152 us, kept 134).
+// ONCE: weights pass the caches by.  That is faster where a line belongs to one block of one row that one unit reads
+// (256 rows over 32 experts of [4096, 7168]: 86 us, kept 102), and slower where rows begin inside a line, whose other
+// part the next block or row reads soon after (256 rows over 128 experts of [5760, 2880]: 255 us, kept 232), or where a
+// group's other units read the weights too (2048 rows over 32 of [7168, 2048], 32 a unit: 152 us, kept 134).
+//
+// Decode is bound by HBM's reads: 256 bf16 rows over 32 experts of [4096, 7168], 0.50 GB, 86 us, 5.8 TB/s; 4 rows of
+// 128 experts of [5760, 2880], 35 MB, 10.5 us, where the launch, one memory latency after the other and the table are
+// half of it.  fp32 rows cost their split and twice the matrix instructions: vector and matrix instructions fill
+// four fifths of the cycles, 256 by [7168, 2048] 65 us, bf16 50 (0.25 GB, 5.0 TB/s).  From 64 rows a group on the matrix pipes and the conversions are the bound: 16384
+// rows over 32 experts of [4096, 7168] 1191 us, 0.81 PFLOP/s.
 template <class T, bool ONCE>
 __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams p) {
   using A = typename T::A;
@@ -303,7 +310,8 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
     }
   };
   f32x4_t acc[FM][TILES];
-  // Block `at` of the sixteen whose scales are at hand: byte 8 at + chunk of the row's 128, which lane at / 2 of the row's holds.
+  // Block `at` of the sixteen whose scales are at hand: byte 8 at + chunk of the row's 128, which lane at / 2 of the
+  // row's holds.
   auto multiply = [&](const u32x4_t (&q)[FN], const u32x4_t (&bytes)[FN], int at, int odd, auto&& rows_of) {
     const int other = at >> 1, from = ((other & 3) * 16 + (other >> 2) * 8 + row8) * 4;
     uint32_t scale[FN];
@@ -353,8 +361,8 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
       }
     }
   };
-  // Shared rows go through registers to LDS, CHUNK values at a time and one chunk ahead, split into their parts on the way; a
-  // wave that has its own part of K loads them as it needs them.
+  // Shared rows go through registers to LDS, CHUNK values at a time and one chunk ahead, split into their parts on the
+  // way; a wave that has its own part of K loads them as it needs them.
   constexpr uint32_t ES = T::ES;
   auto load_piece = [&](RowPiece<A>& v, uint32_t offset) {
 #pragma unroll
@@ -469,8 +477,8 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
     unit += gridDim.x;
     if (unit < units) start(unit);
 
-    // Lane (q, c) holds weight rows 4 q + j of sixteen, of row c, or of EIGHT both halves of K meet; the WK waves' sums are
-    // added in wave order.
+    // Lane (q, c) holds weight rows 4 q + j of sixteen, of row c, or of EIGHT both halves of K meet; the WK waves' sums
+    // are added in wave order.
     if constexpr (T::SHARED) meet();  // the sums go where the rows are
     float* sums = reinterpret_cast<float*>(smem);
     constexpr int LD = T::BN + 4;
@@ -514,8 +522,8 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
   }
 }
 
-// The format's conversions.  An item is 16 bytes of values, so that a wave's loads and stores of them cover whole lines: 8
-// values of 16 bits or 4 of 32, and 4 or 8 lanes a group of 32.  Each thread has four items on their way.
+// The format's conversions.  An item is 16 bytes of values, so that a wave's loads and stores of them cover whole
+// lines: 8 values of 16 bits or 4 of 32, and 4 or 8 lanes a group of 32.  Each thread has four items on their way.
 struct MxConvertParams {
   const void* x;   // quantise: values in; dequantise: e2m1 bytes
   uint8_t* q;      // quantise: e2m1 bytes out
@@ -539,9 +547,9 @@ __device__ __forceinline__ void mx_item(const MxConvertParams& p, int64_t i, int
   col = (i - row * per_row) * MxItem<E>::VALUES;
 }
 
-// scale = floor(log2 max|x|) - 2 as an e8m0 byte, at least 0: e2m1's largest power of two is 4.  q = e2m1(x / scale), to
-// nearest even, at most 6.  A group that holds a NaN or an infinity gets the scale 255, a NaN.
-// Bound by HBM: 8 x [5760, 2880] in fp32 98 us, 6.1 TB/s read and written, and back 84 us, 7.2 TB/s.
+// scale = floor(log2 max|x|) - 2 as an e8m0 byte, at least 0: e2m1's largest power of two is 4.  q = e2m1(x / scale),
+// to nearest even, at most 6.  A group that holds a NaN or an infinity gets the scale 255, a NaN. Bound by HBM: 8 x
+// [5760, 2880] in fp32 96 us, 6.3 TB/s read and written.  Values are read once, past the caches.
 template <class E, bool VEC>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(MxConvertParams p) {
   using raw_t = typename E::raw;
@@ -597,6 +605,10 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(MxConvertParams p) {
   }
 }
 
+// Each value is exact in bf16.  Bound by HBM: 8 x [5760, 2880] to fp32 84 us, 7.2 TB/s read and written.  Stores go
+// past the caches at every size: to bf16, 17 MB 4.6 us, kept 5.0; 133 MB 24.6 and 25.1; 265 MB 48 and 59; to fp32, 531
+// MB 85 and 106.  A copy of the values right behind it gains less from kept ones (17 MB 16.4 and 15.0, 265 MB 158 and
+// 162).
 template <class E>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(MxConvertParams p) {
   using raw_t = typename E::raw;

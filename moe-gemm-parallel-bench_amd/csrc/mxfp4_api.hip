@@ -1,5 +1,5 @@
-// C ABI of the 4-bit (MXFP4) operators: argument checks, the choice of a variant, the launches: one a call, and another for
-// every further 1024 groups of a product.
+// C ABI of the 4-bit (MXFP4) operators: argument checks, the choice of a variant, the launches: one a call, and another
+// for every further 1024 groups of a product.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -64,15 +64,15 @@ hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Variant of the least estimated time for `rows` rows over `groups` groups of `cols` output columns.  Routed groups are taken to
-// hold 0.4 to 1.6 times the mean; a group of more rows than a unit has its weights read again for each unit's rows.  A CU
-// works on two units at a time: it takes half of its units' number, at least 0.65, times what a unit of the variant takes for
-// 256 of K (us, from launches of many units, in the tables' order; rows of one part and of two):
+// Variant of the least estimated time for `rows` rows over `groups` groups of `cols` output columns.  Routed groups are
+// taken to hold 0.4 to 1.6 times the mean; a group of more rows than a unit has its weights read again for each unit's
+// rows.  A CU works on two units at a time: it takes half of its units' number, at least 0.65, times what a unit of the
+// variant takes for 256 of K (us, from launches of many units, in the tables' order; rows of one part and of two):
 constexpr double kUnitTime[2][kNumMx] = {{1.15, 1.36, 1.72, 0.46, 0.67, 2.55}, {1.80, 2.05, 3.40, 0.80, 1.05, 3.40}};
-// Of 207 calls (10 weights, 1 to 1024 rows, three types) the chosen one took 1.01 times the best one's time in the mean, at most
-// 1.32.  What the variants take, in the same order (us, bf16): 32 experts of [4096, 7168] by 256 rows 122, 88, 99, 161, 135,
-// 131; by 1024 rows 340, 204, 162, 467, 369, 151; one weight of [4096, 7168] by 16 rows 22, 25, 31, 11, 13, 46; by 32 rows 23, 24, 31,
-// 18, 14, 47.
+// Of 207 calls (10 weights, 1 to 1024 rows, three types) the chosen one took 1.01 times the best one's time in the
+// mean, at most 1.32.  What the variants take, in the same order (us, bf16): 32 experts of [4096, 7168] by 256 rows
+// 122, 88, 99, 161, 135, 131; by 1024 rows 340, 204, 162, 467, 369, 151; one weight of [4096, 7168] by 16 rows 22, 25,
+// 31, 11, 13, 46; by 32 rows 23, 24, 31, 18, 14, 47.
 int choose(bool two_parts, const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
   const int64_t active = std::min(groups, rows);
   const double mean = (double)rows / active;
