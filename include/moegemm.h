@@ -415,7 +415,7 @@ int moegemm_gate_up_backward(const void* dh, const void* x, const void* w, const
  * [tokens, k] = s of the chosen, over their sum if normalize (0 where that is 0), times scale; experts [tokens, k].
  * logits is [tokens, expert_count] (dtype; unit stride along the experts).  A NaN logit ranks below every other.
  * moegemm_route_topk_backward: the logits' gradient [tokens, expert_count] (contiguous, dtype) for dweights, through s; an
- * index outside the experts counts for nothing.
+ * index outside the experts counts for nothing, a token's are distinct.
  */
 int moegemm_route_topk(const void* logits, const float* bias, float* weights, int32_t* experts, int32_t tokens,
                        int32_t expert_count, int32_t k, int64_t stride_lt, int32_t dtype, int32_t sigmoid, int32_t groups,
@@ -470,10 +470,11 @@ int moegemm_mxfp4_variant_count(void);
 
 /*
  * C[r0:r1] = A[r0:r1] @ W[e]^T for each group e of rows, offsets as in moegemm_grouped_mm_offs; offs NULL: one group of all
- * rows.  a is [rows, k] (dtype; fp32 is taken to within 2^-16 of each value), w 4-bit [group_count, n, k / 2] with scale [group_count, n, k / 32]; out is
- * out_dtype [rows, n] with unit column stride.  Rows of a and w start at multiples of 16 bytes, less than 2^23 apart; rows and n are under 2^30.  Sums are fp32 and of one
- * order.  Rows at or past offs[group_count-1] are not written.  `variant` -1 lets the library choose; grid_size is the CUs
- * (<= 0: 256).  One launch, and another for every further 768 groups.
+ * rows.  a is [rows, k] (dtype; fp32 is taken to within 2^-16 of each value), w 4-bit [group_count, n, k / 2] with scale
+ * [group_count, n, k / 32]; out is out_dtype [rows, n] with unit column stride.  Rows of a and w start at multiples of 16
+ * bytes, less than 2^23 apart; rows and n are under 2^30.  Sums are fp32 and of one order.  Rows at or past
+ * offs[group_count-1] are not written.  `variant` -1 lets the library choose; grid_size is the CUs (<= 0: 256).  One launch,
+ * and another for every further 1024 groups.
  * _swiglu: w is [group_count, n = 2F, k / 2], rows [gate | up]; out [rows, F] = silu(a gate^T) * (a up^T) in fp32.
  */
 int moegemm_grouped_mm_mxfp4(const void* a, const uint8_t* w, const uint8_t* scale, void* out, const int32_t* offs,

@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
   const int blocks = (p.k + kMxBlock - 1) / kMxBlock, part = (blocks + WK - 1) / WK;
   const int first_b = min(wk * part, blocks), end_b = min(first_b + part, blocks);  // the wave's K blocks
   const int scales = p.k / kMxGroup;                                                // of a row
-  const int units = mx_table<T::NT>(table, p, T::BM);
+  const uint32_t units = (uint32_t)mx_table<T::NT>(table, p, T::BM);
 
   constexpr int WAVE_ROWS = T::GATED ? 4 * FN : 8 * FN;  // weight rows of one resource
   constexpr int AHEAD = T::AHEAD;
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
     if constexpr (T::SHARED) fetch(0);
     else fetch_own(av[0], first_b);
   };
-  int unit = blockIdx.x;
+  uint32_t unit = blockIdx.x;  // one past INT32_MAX units is past a signed one's range
   if (unit >= units) return;
   start(unit);
   while (true) {

@@ -2,9 +2,9 @@
 
 The format is the one ``model_configs/gpt-oss-120b.json`` names (mxfp4), the OCP microscaling one: e2m1 values, two a byte
 with the even k in the low half, and an e8m0 byte ``s`` for each 32 along K; a value stands for ``v * 2**(s - 127)``.  Weights
-are stored ``[N, K / 2]`` (``[G, N, K / 2]`` for experts) with scales ``[..., N, K / 32]``, as checkpoints store them.  Rows stay
-16-bit (fp32 ones are taken too).  The reference has no 4-bit path; this is the expert GEMM of its kernels/torch_grouped_gemm.py:121-174 on
-such weights.
+are stored ``[N, K / 2]`` (``[G, N, K / 2]`` for experts) with scales ``[..., N, K / 32]``, as checkpoints store them.  Rows
+stay 16-bit (fp32 ones are taken too).  The reference has no 4-bit path; this is the expert GEMM of its
+kernels/torch_grouped_gemm.py:121-174 on such weights.
 
 A serving step of one expert layer::
 
@@ -12,11 +12,11 @@ A serving step of one expert layer::
     h = grouped_mm_mxfp4_swiglu(x, w13, s13, offs)                  # silu(gate) * up, [rows, F]
     y = grouped_mm_mxfp4(h, w2, s2, offs)                           # [rows, H]
 
-h is rounded to x's 16 bits between the two; ``out_dtype=torch.float32`` in the first and x's in the second leaves one rounding, at
-the end.
+h is rounded to x's 16 bits between the two; ``out_dtype=torch.float32`` in the first and x's in the second leaves one
+rounding, at the end (256 rows over 32 experts of [7168, 2048]: 65 us for the second, of 16-bit rows 50).
 
 The products are made for decode, where an expert has few rows and reading its weights is the bound; they take any number
-of rows.  Each call runs on the current stream, reads ``offs`` on the device and keeps nothing, so it can be captured in a
+of rows, but past 128 an expert a bf16 copy (``dequantize_mxfp4``) and ``grouped_mm`` are faster.  Each call runs on the current stream, reads ``offs`` on the device and keeps nothing, so it can be captured in a
 HIP graph; repeated calls give the same bits.  ``ValueError`` for operands a kernel cannot take, ``RuntimeError`` without
 library or GPU.
 """

@@ -295,7 +295,8 @@ def _combine_gradients(dout, y, order, weights, rows: int, need_dy: bool, need_d
         _native.launch(dout.device, _native.library().moegemm_combine_rows_backward, dout.data_ptr(),
                        y.data_ptr() if need_dweights else None, None if weights is None else weights.data_ptr(),
                        dy.data_ptr() if need_dy and rows else None, dweights.data_ptr() if need_dweights else None,
-                       order.places.data_ptr(), _end_of(order), tokens, k, rows, width, _row_stride(dout), _row_stride(y) if need_dweights else 0, code)
+                       order.places.data_ptr(), _end_of(order), tokens, k, rows, width, _row_stride(dout),
+                       _row_stride(y) if need_dweights else 0, code)
     return dy, dweights
 
 
