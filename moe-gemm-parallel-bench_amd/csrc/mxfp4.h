@@ -8,7 +8,7 @@
 // A weight v 2^(s - 127) has two significant bits and fp32's exponents, so it is exact in bf16: the conversion
 // instruction takes the scale along, and the bf16 matrix instructions, whose sums keep fp32's bits and whose operands
 // may be subnormal, do the rest.  fp16 rows are taken as two bf16 parts, 8 bits and the 3 behind them, which is exact
-// too; fp32 rows as two as well, which are within 2^-16 of a value (2^-14 above 2^127) or 2^-134: a third would cost
+// too; fp32 rows as two as well, which are within 2^-16 of a value (2^-15 above 2^127) or 2^-134: a third would cost
 // half as many matrix instructions again for bits that a 16-bit output, which such rows are an intermediate of, does
 // not show.
 #pragma once
@@ -63,25 +63,24 @@ struct RowParts {
     } else {
       typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
       typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
+      constexpr float kMost = 0x1.fep119f;
       u16x8_t hi, lo;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float f;
         if constexpr (A::is_f32) {
           const uint32_t word = x.v[i >> 2][i & 3];  // a bit cast of the vector's element itself takes the first one
-          f = __builtin_bit_cast(float, word);
+          f = __builtin_canonicalizef(__builtin_bit_cast(float, word));  // quiet, so that hi is a NaN too
         } else {
           f = (float)__builtin_bit_cast(f16x8_t, x.v[0])[i];
         }
-        const uint32_t bits = __builtin_bit_cast(uint32_t, f), top = bits & 0xffff0000u;
+        const uint32_t top = __builtin_bit_cast(uint32_t, f) & 0xffff0000u;
         hi[i] = (uint16_t)(top >> 16);
-        const float rest = f - __builtin_bit_cast(float, top);  // 0 for an infinity, which hi holds whole
-        uint16_t low = (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16);  // exact for fp16
-        if constexpr (A::is_f32) {
-          // Above 2^127 rounding up could take the parts' sum past the largest number.
-          if ((bits & 0x7f800000u) != 0x7f000000u) low = __builtin_bit_cast(uint16_t, (__bf16)rest);
-        }
-        lo[i] = (bits & 0x7fffffffu) == 0x7f800000u ? 0 : low;
+        // kMost: rounding up above it could take the parts' sum past the largest number.  What is left of an infinity,
+        // which hi holds whole, or a NaN is a NaN, of which the median makes a number.
+        const float rest = __builtin_amdgcn_fmed3f(f - __builtin_bit_cast(float, top), -kMost, kMost);
+        if constexpr (A::is_f32) lo[i] = __builtin_bit_cast(uint16_t, (__bf16)rest);
+        else lo[i] = (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16);  // exact
       }
       v[0] = __builtin_bit_cast(bf16x8_t, hi);
       v[1] = __builtin_bit_cast(bf16x8_t, lo);
@@ -174,11 +173,17 @@ struct MxStream {
   static constexpr int ROWS_BYTES = SHARED ? 2 * PARTS * STAGE_BYTES : 0;
   static constexpr int SUM_BYTES = WK * BM * (BN + 4) * 4;
   static constexpr int LDS_BYTES = ROWS_BYTES > SUM_BYTES ? ROWS_BYTES : SUM_BYTES;  // the sums where the rows were
-  static constexpr int PER_CU = SHARED ? 2 : 4;          // workgroups a CU
-  static constexpr int MIN_WAVES = 2;                    // a SIMD
+  // Workgroups a CU, and waves a SIMD that the registers allow.  Where rows are shared two: a third leaves too few
+  // registers for the blocks ahead, and the units come out uneven (256 rows over 32 experts, 8 a unit, 127 us and 135);
+  // rows of two parts, which have no more than one block ahead, three up to 16 a unit (fp16 116 and 101 us, over [7168,
+  // 2048] 59 and 50). Units of one wave's width two as well, and up to four's worth of workgroups that wait (Gate+Up of
+  // four rows over 128 experts of [5760, 2880] by two 11.6 us, by four 10.5, by eight 10.7).
+  static constexpr int MIN_WAVES = SHARED && PARTS == 2 && BM <= 16 ? 3 : 2;
+  static constexpr int PER_CU = SHARED ? MIN_WAVES : 4;
   // Blocks of weights on their way.  256 rows over 32 experts of [4096, 7168] 86 us with three, 89 with one; over
   // [7168, 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32: 128 and 127, 71 and
-  // 65; 2048 rows, 64 a unit, over [4096, 7168] 219 and 210.
+  // 65; 2048 rows, 64 a unit, over [4096, 7168] 219 and 210; waves with a part of K, one row of [5760, 2880] 6.6 and
+  // 5.7.
   static constexpr int AHEAD = SHARED && PARTS == 1 && BM <= 32 ? 3 : 1;
   static_assert(4 % (AHEAD + 1) == 0, "a block's registers are known");
   static_assert(EIGHT || BM % 16 == 0, "whole matrix instructions");
@@ -220,9 +225,9 @@ __device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
 //
 // Decode is bound by HBM's reads: 256 bf16 rows over 32 experts of [4096, 7168], 0.50 GB, 86 us, 5.8 TB/s; 4 rows of
 // 128 experts of [5760, 2880], 35 MB, 10.5 us, where the launch, one memory latency after the other and the table are
-// half of it.  fp32 rows cost their split and twice the matrix instructions: vector and matrix instructions fill
-// four fifths of the cycles, 256 by [7168, 2048] 65 us, bf16 50 (0.25 GB, 5.0 TB/s).  From 64 rows a group on the matrix pipes and the conversions are the bound: 16384
-// rows over 32 experts of [4096, 7168] 1191 us, 0.81 PFLOP/s.
+// half of it.  fp32 rows cost their split and twice the matrix instructions: vector and matrix instructions fill four
+// fifths of the cycles, 256 by [7168, 2048] 65 us, bf16 50 (0.25 GB, 5.0 TB/s).  From 64 rows a group on the matrix
+// pipes and the conversions are the bound: 16384 rows over 32 experts of [4096, 7168] 1191 us, 0.81 PFLOP/s.
 template <class T, bool ONCE>
 __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams p) {
   using A = typename T::A;

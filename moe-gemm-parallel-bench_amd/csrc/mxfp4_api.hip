@@ -68,7 +68,7 @@ hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
 // taken to hold 0.4 to 1.6 times the mean; a group of more rows than a unit has its weights read again for each unit's
 // rows.  A CU works on two units at a time: it takes half of its units' number, at least 0.65, times what a unit of the
 // variant takes for 256 of K (us, from launches of many units, in the tables' order; rows of one part and of two):
-constexpr double kUnitTime[2][kNumMx] = {{1.15, 1.36, 1.72, 0.46, 0.67, 2.55}, {1.80, 2.05, 3.40, 0.80, 1.05, 3.40}};
+constexpr double kUnitTime[2][kNumMx] = {{1.15, 1.36, 1.72, 0.46, 0.67, 2.55}, {1.57, 1.66, 2.90, 0.72, 0.95, 2.90}};
 // Of 207 calls (10 weights, 1 to 1024 rows, three types) the chosen one took 1.01 times the best one's time in the
 // mean, at most 1.32.  What the variants take, in the same order (us, bf16): 32 experts of [4096, 7168] by 256 rows
 // 122, 88, 99, 161, 135, 131; by 1024 rows 340, 204, 162, 467, 369, 151; one weight of [4096, 7168] by 16 rows 22, 25,

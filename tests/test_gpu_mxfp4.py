@@ -290,6 +290,23 @@ def test_infinities_and_nan_stay_in_their_row():
         assert torch.equal(out[keep], clean[keep])
 
 
+def test_signalling_nans_and_infinities_in_every_variant():
+    """The parts of a value that is no number give back what it is: in each kernel that splits rows, and in the one that does not."""
+    from kernels import matmul_mxfp4
+
+    q = torch.full((40, 48), 0x22, dtype=torch.uint8, device="cuda")  # 1.0 throughout
+    scale = torch.full((40, 3), 127, dtype=torch.uint8, device="cuda")
+    for dtype, whole, signalling in ((torch.float32, torch.int32, (0x7F800001, -0x7FFFFF)), (torch.float16, torch.int16, (0x7C01, -0x3FF)),
+                                     (torch.bfloat16, torch.int16, (0x7F81, -0x7F))):
+        for variant in _variants():
+            a = torch.ones(6, 96, dtype=dtype, device="cuda")
+            a[1, 7], a[2, 95] = float("inf"), -float("inf")
+            a[3, 64], a[4, 31] = torch.tensor(signalling, dtype=whole, device="cuda").view(dtype)
+            out = matmul_mxfp4(a, q, scale, variant=variant)
+            assert (out[[0, 5]] == 96).all() and (out[1] == float("inf")).all() and (out[2] == -float("inf")).all()
+            assert torch.isnan(out[3:5]).all()
+
+
 def test_fp32_rows_from_end_to_end_of_their_range():
     """Values next to the largest and subnormal ones, and a NaN whose payload lies below bf16's bits."""
     from kernels import matmul_mxfp4
