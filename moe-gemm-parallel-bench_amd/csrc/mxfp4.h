@@ -225,8 +225,8 @@ __device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
 //
 // Decode is bound by HBM's reads: 256 bf16 rows over 32 experts of [4096, 7168], 0.50 GB, 86 us, 5.8 TB/s; 4 rows of
 // 128 experts of [5760, 2880], 35 MB, 10.5 us, where the launch, one memory latency after the other and the table are
-// half of it.  fp32 rows cost their split and twice the matrix instructions: vector and matrix instructions fill four
-// fifths of the cycles, 256 by [7168, 2048] 65 us, bf16 50 (0.25 GB, 5.0 TB/s).  From 64 rows a group on the matrix
+// half of it.  fp32 rows cost their split and twice the matrix instructions: vector and matrix instructions fill seven
+// tenths of the cycles, 256 by [7168, 2048] 60 us, bf16 51 (0.25 GB, 5.0 TB/s).  From 64 rows a group on the matrix
 // pipes and the conversions are the bound: 16384 rows over 32 experts of [4096, 7168] 1191 us, 0.81 PFLOP/s.
 template <class T, bool ONCE>
 __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams p) {

@@ -13,7 +13,7 @@ A serving step of one expert layer::
     y = grouped_mm_mxfp4(h, w2, s2, offs)                           # [rows, H]
 
 h is rounded to x's 16 bits between the two; ``out_dtype=torch.float32`` in the first and x's in the second leaves one
-rounding, at the end (256 rows over 32 experts of [7168, 2048]: 65 us for the second, of 16-bit rows 50).
+rounding, at the end (256 rows over 32 experts of [7168, 2048]: 60 us for the second, of bf16 rows 51).
 
 The products are made for decode, where an expert has few rows and reading its weights is the bound; they take any number
 of rows, but past 128 an expert a bf16 copy (``dequantize_mxfp4``) and ``grouped_mm`` are faster.  Each call runs on the current stream, reads ``offs`` on the device and keeps nothing, so it can be captured in a

@@ -1,4 +1,4 @@
-"""The expert-layer driver's part that routes tokens: its arguments on the CPU, one small run on a GPU."""
+"""harness.expert_layer's part that routes tokens: its arguments on the CPU, one small run on a GPU."""
 
 from __future__ import annotations
 
