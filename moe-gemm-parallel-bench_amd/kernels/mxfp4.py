@@ -73,8 +73,8 @@ def quantize_mxfp4(x):
         raise ValueError(f"K must be a positive multiple of {MX_GROUP} under 2**31 (got {k})")
     if x.stride(-1) != 1:
         raise ValueError("x needs a unit stride along its last dimension")
-    q = torch.empty((*head, k // 2), dtype=torch.uint8, device=x.device)
-    scale = torch.empty((*head, k // MX_GROUP), dtype=torch.uint8, device=x.device)
+    q = x.new_empty((*head, k // 2), dtype=torch.uint8)
+    scale = x.new_empty((*head, k // MX_GROUP), dtype=torch.uint8)
     if x.numel():
         parts = _matrices(x)
         rows = parts[0].shape[0]
@@ -98,7 +98,7 @@ def dequantize_mxfp4(q, scale, *, dtype=None):
     _check_weight(q, scale, k)
     if not q.is_cuda or scale.device != q.device:
         raise ValueError("q and scale must be on the same GPU device")
-    out = torch.empty((*head, k), dtype=dtype, device=q.device)
+    out = q.new_empty((*head, k), dtype=dtype)
     if q.numel():
         even = q.ndim == 2 or len(_matrices(q)) == len(_matrices(scale)) == 1
         pairs = [(_matrices(q)[0], _matrices(scale)[0])] if even else list(zip(q.unbind(0), scale.unbind(0)))
@@ -168,7 +168,7 @@ def _product(entry: str, a, weight, scale, offs, out, out_dtype, variant, gated:
     out_dtype = out_dtype or a.dtype
     code = _native.dtype_code(out_dtype)
     if out is None:
-        out = torch.empty((rows, cols), dtype=out_dtype, device=device)
+        out = a.new_empty((rows, cols), dtype=out_dtype)
     if rows:
         _native.launch(device, getattr(_native.library(), entry), a.data_ptr(), weight.data_ptr(), scale.data_ptr(),
                        out.data_ptr(), offs.data_ptr() if grouped else None, groups, rows, n, k, pitch if rows > 1 else k,
