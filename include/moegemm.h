@@ -470,7 +470,7 @@ int moegemm_mxfp4_variant_count(void);
 
 /*
  * C[r0:r1] = A[r0:r1] @ W[e]^T for each group e of rows, offsets as in moegemm_grouped_mm_offs; offs NULL: one group of all
- * rows.  a is [rows, k] (dtype; fp32 is taken to within 2^-16 of each value), w 4-bit [group_count, n, k / 2] with scale
+ * rows.  a is [rows, k] (dtype; fp32 values below 2^-110 are taken to within 2^-134), w 4-bit [group_count, n, k / 2] with scale
  * [group_count, n, k / 32]; out is out_dtype [rows, n] with unit column stride.  Rows of a and w start at multiples of 16
  * bytes, less than 2^23 apart; rows and n are under 2^30.  Sums are fp32 and of one order.  Rows at or past
  * offs[group_count-1] are not written.  `variant` -1 lets the library choose; grid_size is the CUs (<= 0: 256).  One launch,

@@ -8,9 +8,9 @@
 // A weight v 2^(s - 127) has two significant bits and fp32's exponents, so it is exact in bf16: the conversion
 // instruction takes the scale along, and the bf16 matrix instructions, whose sums keep fp32's bits and whose operands
 // may be subnormal, do the rest.  fp16 rows are taken as two bf16 parts, 8 bits and the 3 behind them, which is exact
-// too; fp32 rows as two as well, which are within 2^-16 of a value (2^-15 above 2^127) or 2^-134: a third would cost
-// half as many matrix instructions again for bits that a 16-bit output, which such rows are an intermediate of, does
-// not show.
+// too; fp32 rows as three, their 24 bits, which is exact from 2^-110 up (below, the last part is rounded to 2^-133, bf16's
+// least number).  Two would hold 16 bits, which the rounding of some 16-bit outputs shows.  The third costs half as many
+// matrix instructions again: 256 rows over 32 experts of [7168, 2048] 62 and 65 us, 16384 over [4096, 7168] 2.55 and 3.4 ms.
 #pragma once
 
 #include <type_traits>
@@ -55,7 +55,7 @@ struct RowPiece {
 };
 template <class A>
 struct RowParts {
-  static constexpr int N = A::dtype == DT_BF16 ? 1 : 2;
+  static constexpr int N = A::dtype == DT_BF16 ? 1 : A::is_f32 ? 3 : 2;
   bf16x8_t v[N];
   __device__ __forceinline__ void set(const RowPiece<A>& x) {
     if constexpr (A::dtype == DT_BF16) {
@@ -63,8 +63,8 @@ struct RowParts {
     } else {
       typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
       typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
-      constexpr float kMost = 0x1.fep119f;
-      u16x8_t hi, lo;
+      constexpr float kMost = 0x1p120f;  // above what is left of any number
+      u16x8_t hi, mid, lo;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float f;
@@ -76,14 +76,15 @@ struct RowParts {
         }
         const uint32_t top = __builtin_bit_cast(uint32_t, f) & 0xffff0000u;
         hi[i] = (uint16_t)(top >> 16);
-        // kMost: rounding up above it could take the parts' sum past the largest number.  What is left of an infinity,
-        // which hi holds whole, or a NaN is a NaN, of which the median makes a number.
+        // What is left of an infinity, which hi holds whole, or a NaN is a NaN, of which the median makes a number.
         const float rest = __builtin_amdgcn_fmed3f(f - __builtin_bit_cast(float, top), -kMost, kMost);
-        if constexpr (A::is_f32) lo[i] = __builtin_bit_cast(uint16_t, (__bf16)rest);
-        else lo[i] = (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16);  // exact
+        const uint32_t next = __builtin_bit_cast(uint32_t, rest) & 0xffff0000u;
+        mid[i] = (uint16_t)(next >> 16);  // of fp16 all that is left
+        if constexpr (A::is_f32) lo[i] = __builtin_bit_cast(uint16_t, (__bf16)(rest - __builtin_bit_cast(float, next)));
       }
       v[0] = __builtin_bit_cast(bf16x8_t, hi);
-      v[1] = __builtin_bit_cast(bf16x8_t, lo);
+      v[1] = __builtin_bit_cast(bf16x8_t, mid);
+      if constexpr (A::is_f32) v[2] = __builtin_bit_cast(bf16x8_t, lo);
     }
   }
 };
@@ -170,15 +171,18 @@ struct MxStream {
   static constexpr int STAGE_BYTES = BM * ROW_BYTES;     // of one part
   static constexpr int ES = sizeof(typename A::raw);
   static constexpr int COPIES = BM * CHUNK / 8 / NT;     // pieces of a stage a thread
-  static constexpr int ROWS_BYTES = SHARED ? 2 * PARTS * STAGE_BYTES : 0;
+  // One where two would leave LDS for one workgroup a CU (16384 fp32 rows over 32 experts of [4096, 7168] 3.8 and 3.4 ms).
+  static constexpr int STAGES = PARTS == 3 && BM == 32 ? 1 : 2;
+  static constexpr int ROWS_BYTES = SHARED ? STAGES * PARTS * STAGE_BYTES : 0;
   static constexpr int SUM_BYTES = WK * BM * (BN + 4) * 4;
   static constexpr int LDS_BYTES = ROWS_BYTES > SUM_BYTES ? ROWS_BYTES : SUM_BYTES;  // the sums where the rows were
   // Workgroups a CU, and waves a SIMD that the registers allow.  Where rows are shared two: a third leaves too few
   // registers for the blocks ahead, and the units come out uneven (256 rows over 32 experts, 8 a unit, 127 us and 135);
-  // rows of two parts, which have no more than one block ahead, three up to 16 a unit (fp16 116 and 101 us, over [7168,
-  // 2048] 59 and 50). Units of one wave's width two as well, and up to four's worth of workgroups that wait (Gate+Up of
-  // four rows over 128 experts of [5760, 2880] by two 11.6 us, by four 10.5, by eight 10.7).
-  static constexpr int MIN_WAVES = SHARED && PARTS == 2 && BM <= 16 ? 3 : 2;
+  // rows of two or three parts, which have no more than one block ahead, three up to 16 a unit (fp16 116 and 101 us, over
+  // [7168, 2048] 59 and 50).  Units of one wave's width two as well, 16 rows of three parts one, whose registers spill else
+  // (32 rows of [4096, 7168] 25.8 and 22.6 us), and up to four's worth of workgroups that wait (Gate+Up of four rows over
+  // 128 experts of [5760, 2880] by two 11.6 us, by four 10.5, by eight 10.7).
+  static constexpr int MIN_WAVES = SHARED && PARTS > 1 && BM <= 16 ? 3 : !SHARED && PARTS == 3 && !EIGHT ? 1 : 2;
   static constexpr int PER_CU = SHARED ? MIN_WAVES : 4;
   // Blocks of weights on their way.  256 rows over 32 experts of [4096, 7168] 86 us with three, 89 with one; over
   // [7168, 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32: 128 and 127, 71 and
@@ -447,7 +451,7 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
         const int b = b0 + j;
         if (b >= end_b) break;
         if constexpr (T::SHARED) {
-          const int stage = j / CB & 1, place = j % CB;
+          const int stage = T::STAGES == 1 ? 0 : j / CB & 1, place = j % CB;
           if (place == 0) fetch((b + CB) * kMxBlock);
           load(q[(j + AHEAD) % (AHEAD + 1)], b + AHEAD);
           multiply(q[j % (AHEAD + 1)], bytes, rel + j, j & 1, [&](RowParts<A>& rows, int m, int half, int x) {
@@ -458,7 +462,8 @@ __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams
                                                             half * kMxBlock + x * 16);
           });
           if (place == CB - 1 && b + 1 < end_b) {
-            put(stage ^ 1);
+            if constexpr (T::STAGES == 1) meet();
+            put(T::STAGES == 1 ? 0 : stage ^ 1);
             meet();
           }
         } else {

@@ -67,13 +67,14 @@ hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
 // Variant of the least estimated time for `rows` rows over `groups` groups of `cols` output columns.  Routed groups are
 // taken to hold 0.4 to 1.6 times the mean; a group of more rows than a unit has its weights read again for each unit's
 // rows.  A CU works on two units at a time: it takes half of its units' number, at least 0.65, times what a unit of the
-// variant takes for 256 of K (us, from launches of many units, in the tables' order; rows of one part and of two):
-constexpr double kUnitTime[2][kNumMx] = {{1.15, 1.36, 1.72, 0.46, 0.67, 2.55}, {1.57, 1.66, 2.90, 0.72, 0.95, 2.90}};
+// variant takes for 256 of K (us, from launches of many units, in the tables' order; rows of one part, of two, of three):
+constexpr double kUnitTime[3][kNumMx] = {
+    {1.15, 1.36, 1.72, 0.46, 0.67, 2.55}, {1.57, 1.66, 2.90, 0.72, 0.95, 2.90}, {1.76, 1.94, 3.80, 0.80, 1.15, 3.80}};
 // Of 207 calls (10 weights, 1 to 1024 rows, three types) the chosen one took 1.01 times the best one's time in the
-// mean, at most 1.32.  What the variants take, in the same order (us, bf16): 32 experts of [4096, 7168] by 256 rows
+// mean, at most 1.32; of 144 calls of three parts (11 weights, 1 to 2048 rows) 1.01 times, at most 1.19.  What the variants take, in the same order (us, bf16): 32 experts of [4096, 7168] by 256 rows
 // 122, 88, 99, 161, 135, 131; by 1024 rows 340, 204, 162, 467, 369, 151; one weight of [4096, 7168] by 16 rows 22, 25,
 // 31, 11, 13, 46; by 32 rows 23, 24, 31, 18, 14, 47.
-int choose(bool two_parts, const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
+int choose(int parts, const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
   const int64_t active = std::min(groups, rows);
   const double mean = (double)rows / active;
   int best = 0;
@@ -83,7 +84,7 @@ int choose(bool two_parts, const MxVariant* table, int64_t rows, int64_t groups,
     for (int j = 0; j < 7; ++j)
       tiles += std::ceil(std::max(active == 1 ? mean : mean * (0.4 + 0.2 * j), 1.0) / table[i].rows - 1e-9) / 7;
     const double units = std::ceil(active * tiles * cdiv(cols, table[i].cols) / cus - 1e-9);  // of a CU
-    const double time = std::max(units / 2, 0.65) * kUnitTime[two_parts][i];
+    const double time = std::max(units / 2, 0.65) * kUnitTime[parts - 1][i];
     if (i == 0 || time < least) {
       best = i;
       least = time;
@@ -122,7 +123,7 @@ int launch_product(const void* a, const uint8_t* w, const uint8_t* scale, void* 
   const MxVariant* table = dtype == DT_BF16  ? (gated ? kMxGatedBf16 : kMxBf16)
                            : dtype == DT_F16 ? (gated ? kMxGatedF16 : kMxF16)
                                              : (gated ? kMxGatedF32 : kMxF32);
-  if (variant < 0) variant = choose(dtype != DT_BF16, table, rows, group_count, cols, cus);
+  if (variant < 0) variant = choose(dtype == DT_BF16 ? 1 : dtype == DT_F16 ? 2 : 3, table, rows, group_count, cols, cus);
   const MxVariant& v = table[variant];
   MxParams p{a, w, scale, out, offs, stride_am, stride_wg, stride_wn, stride_sg, stride_sn,
              stride_om, group_count, rows, n, k, (int32_t)cdiv(cols, v.cols), out_dtype};

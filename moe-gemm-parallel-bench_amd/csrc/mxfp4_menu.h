@@ -25,8 +25,8 @@ hipError_t launch_mx(const MxParams& p, int grid, bool once, hipStream_t stream)
 
 // X(A, ROWS, FN, WAVES_N, WAVES_K, GATED): 8, 16 or 32 rows by 128 weight rows for many units, 8 or 16 rows by 32
 // weight rows with K split over the waves for few.  A table ends with the unit of the most rows: 64 for bf16; of two
-// parts 64 would leave LDS for one workgroup a CU (2048 fp32 rows over 32 experts of [4096, 7168] 594 us, 32 rows a
-// unit 446), so there it is the 32 again.
+// parts 64 would leave LDS for one workgroup a CU (2048 rows over 32 experts of [4096, 7168] 594 us, 32 rows a unit
+// 446), of three for none, so there it is the 32 again.
 #define MOEGEMM_MENU_MX(X, A, GATED)                                        \
   X(A, 8, 4, 4, 1, GATED) X(A, 16, 4, 4, 1, GATED) X(A, 32, 4, 4, 1, GATED) \
   X(A, 8, 4, 1, 4, GATED) X(A, 16, 4, 1, 4, GATED)

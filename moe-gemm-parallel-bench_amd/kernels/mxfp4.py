@@ -182,8 +182,7 @@ def _product(entry: str, a, weight, scale, offs, out, out_dtype, variant, gated:
 def matmul_mxfp4(a, weight, scale, *, out=None, out_dtype=None, variant: int | None = None):
     """``a @ dequantized(weight, scale).T``; returns ``out`` (allocated if None).
 
-    a [M, K] is fp16, bf16 or fp32 (taken to within 2**-16 of each value, 2**-15 above 2**127, or
-    2**-134), weight [N, K / 2] and scale [N, K / 32] uint8 as ``quantize_mxfp4`` returns them (or torch's
+    a [M, K] is fp16, bf16 or fp32 (taken whole, below 2**-110 to within 2**-134), weight [N, K / 2] and scale [N, K / 32] uint8 as ``quantize_mxfp4`` returns them (or torch's
     float4_e2m1fn_x2 and float8_e8m0fnu).  fp32 sums; output in ``out_dtype`` (fp16, bf16 or fp32; a's by default).  M and N
     are arbitrary (under 2**30), K is a multiple of 32; rows of a and weight start at multiples of 16 bytes, less than 2**23
     bytes apart.  ``variant`` names a compiled kernel, None lets the library choose.
