@@ -47,9 +47,10 @@ struct RouteParams {
   float scale;
 };
 
-// Scores as integers of the same order; a NaN lies below -inf, and 0 below everything is "not to be had".
+// Scores as integers of the same order; a NaN lies below -inf, and 0 below everything is "not to be had".  -0 + 0 is 0:
+// zeros of both signs are one score.
 __device__ __forceinline__ uint64_t order_of(double x) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
   return x != x ? 1 : u >> 63 ? ~u : u | (1ull << 63);
 }
 
@@ -226,7 +227,7 @@ __device__ __forceinline__ double token_sum(double x) {
 }
 
 __device__ __forceinline__ uint32_t order_of(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float score_of(uint32_t key) {
