@@ -599,8 +599,9 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
       }
       total = token_sum<LPT>(total);
       const double inverse = total == 0 ? 0 : 1 / total;
-      s = used ? exp((double)logit - base) * inverse * dw : 0;
-      const double mean = token_sum<LPT>(s);
+      s = used ? exp((double)logit - base) * inverse : 0;
+      const double mean = token_sum<LPT>(s * dw);
+      s *= dw - mean;  // a small difference of large terms where s is close to 1
 #pragma unroll
       for (int i = 0; i < PER; ++i) row[li + i * LPT] = (float)(-mean * (all[i] * inverse));
     } else {
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
       for (int i = 0; i < PER; ++i) row[li + i * LPT] = 0;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (used) row[e] += (float)s;
+    if (used) row[e] = (float)s;  // in place of a dense gradient's part without dw
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // The rows of the wave's tokens one after the other, 16 bytes a lane where they allow it.
     constexpr int N = 16 / sizeof(typename E::raw);
