@@ -570,8 +570,9 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
     const float logit = used ? to_float<E>(x[e]) : -__builtin_inff();
     double s;
     if (p.sigmoid) {
-      s = used ? sigmoid64(logit) : 0;
-      const double slope = s * (1 - s);
+      // s = 1 / (1 + z) or, of negative logits, z / (1 + z); s (1 - s) of either, where 1 - s has no bits left past 37.
+      const double z = used ? exp(-fabs((double)logit)) : 0, inverse = 1 / (1 + z), slope = z * inverse * inverse;
+      s = logit < 0 ? z * inverse : used ? inverse : 0;
       if (p.normalize) {
         const double total = token_sum<LPT>(s), mean = token_sum<LPT>(s * dw);
         s = total == 0 ? 0 : (dw - mean / total) / total * slope;

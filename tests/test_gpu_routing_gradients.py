@@ -56,3 +56,32 @@ def test_dense_gradient_of_a_confident_router(k, experts, dtype):
     bound = rounding(dtype) * exact.abs() + 2.0 ** -47 * p * dw.abs().sum(dim=1, keepdim=True) + SMALL[dtype]
     worst = ((actual.cpu().double() - exact).abs() - bound).max()
     assert worst <= 0, float(worst)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("normalize", [False, True])
+def test_gradient_of_saturated_sigmoids(normalize, dtype):
+    """Logits far to both sides of 0: the slope s (1 - s) is e^-|x| / (1 + e^-|x|)^2, of which 1 - s keeps no bits past 37."""
+    from kernels import route_topk_backward
+
+    x = torch.tensor([[-40.0, -30.0, -20.0, -8.0, 0.0, 8.0, 14.0, 18.0, 22.0, 26.0, 30.0, 34.0, 36.0, 38.0, 42.0, 60.0]])
+    if dtype is torch.float16:
+        x = x / 4  # gradients of e^-15 at most are within its range
+    chosen = torch.stack([torch.roll(torch.arange(16), r)[:3] for r in range(16)]).int()  # each three in turn
+    x, dw = x.expand(16, 16).contiguous().to(dtype), normal(3, 16, 3)
+    how = dict(score="sigmoid", normalize=normalize, scale=2.5)
+    actual = route_topk_backward(dw.cuda(), x.cuda(), chosen.cuda(), **how)
+    y, index, dw = x.double(), chosen.long(), 2.5 * dw.double()
+    z = torch.exp(-y.abs())
+    slope, s = (z / (1 + z) ** 2).gather(1, index), torch.sigmoid(y).gather(1, index)
+    if normalize:
+        # (dw_i - sum_j s_j dw_j / S) / S = sum_j s_j (dw_i - dw_j) / S^2
+        total = s.sum(dim=1, keepdim=True)
+        d = slope * (s[:, None] * (dw[:, :, None] - dw[:, None])).sum(dim=2) / total ** 2
+        extra = 2.0 ** -47 * slope * dw.abs().sum(dim=1, keepdim=True) / total
+    else:
+        d, extra = slope * dw, 0 * dw
+    exact = torch.zeros_like(y).scatter_(1, index, d)
+    bound = rounding(dtype) * exact.abs() + torch.zeros_like(y).scatter_(1, index, extra) + SMALL[dtype]
+    worst = ((actual.cpu().double() - exact).abs() - bound).max()
+    assert worst <= 0, float(worst)
