@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
       s = logit < 0 ? z * inverse : used ? inverse : 0;
       if (p.normalize) {
         const double total = token_sum<LPT>(s), mean = token_sum<LPT>(s * dw);
-        s = total == 0 ? 0 : (dw - mean / total) / total * slope;
+        s = total == 0 ? 0 : (dw - mean / total) * (slope / total);  // dw over a tiny total may be past the largest number
       } else {
         s = dw * slope;
       }

@@ -85,3 +85,18 @@ def test_gradient_of_saturated_sigmoids(normalize, dtype):
     bound = rounding(dtype) * exact.abs() + torch.zeros_like(y).scatter_(1, index, extra) + SMALL[dtype]
     worst = ((actual.cpu().double() - exact).abs() - bound).max()
     assert worst <= 0, float(worst)
+
+
+def test_gradient_of_normalised_sigmoids_that_are_tiny():
+    """Logits near -700, whose scores are 1e-304: their ratios' gradient, w_i (dw_i - sum_j w_j dw_j) as a softmax's, is of
+    ordinary size.  The scores' own 64-bit rounding, 2^-40 of them at most, is the error before the last rounding."""
+    from kernels import route_topk_backward
+
+    x = torch.tensor([[-700.0, -701.0, -699.0, 3.0], [-300.0, -300.0, -302.0, 3.0], [-120.0, -121.0, -125.0, 3.0]])
+    chosen = torch.tensor([[0, 1, 2]] * 3, dtype=torch.int32)
+    dw = 1e8 * normal(2, 3, 3)  # over 1e-304 past the largest 64-bit number
+    actual = route_topk_backward(dw.cuda(), x.cuda(), chosen.cuda(), score="sigmoid").cpu().double()
+    w, dw = torch.softmax(x[:, :3].double(), dim=1), dw.double()
+    exact = w * (dw - (w * dw).sum(dim=1, keepdim=True))
+    bound = rounding(torch.float32) * exact.abs() + 2.0 ** -40 * w * dw.abs().sum(dim=1, keepdim=True)
+    assert bool(((actual[:, :3] - exact).abs() <= bound).all()) and not actual[:, 3].any()
