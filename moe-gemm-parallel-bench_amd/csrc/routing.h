@@ -236,7 +236,8 @@ __device__ __forceinline__ float score_of(uint32_t key) {
 // fp32 scores are within 2^-22 of sigmoid (exp of x is off by (|x| + 2) 2^-24 of itself, the sum and the reciprocal by
 // 2^-24 and 2^-23, and s (1 - s) |x| < 1/4) and of softmax (whose sum is a 64-bit one, and |x| e^-|x| < 0.4); a bias
 // adds 2^-24 of the sum. Keys drop up to `mask` units of 2^-23 of their size.  Scores further apart than this, times
-// their size or 1, are in order; for sums of two, twice the scores' part.
+// their size or 1, are in order; sums of two than twice this, times the size of the largest term or 1 (the terms' errors,
+// 2^-21 and 2^-22 of their size with the sum's rounding, of either sum).
 __host__ __device__ constexpr float route_margin(uint32_t mask) { return (float)(mask + 1) * 0x1p-23f + 0x1p-20f; }
 
 // Whether a, the larger in fp32, may not be the larger one (or is no number).
@@ -451,7 +452,10 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
       mine_in = place(score) < p.top_groups;
       const float least = -token_max<LPT>(mine_in ? -score : -__builtin_inff());
       const float most = token_max<LPT>(mine_in ? -__builtin_inff() : score);
-      if (__ballot(p.top_groups < p.groups && too_close(least, most, 2 * route_margin(0)))) {
+      // Terms that a bias made large and that cancel leave a sum as wrong as they are; an infinite one is exact.
+      auto finite_size = [](float f) { return fabsf(f) < __builtin_inff() ? fabsf(f) : 0.0f; };
+      const double size = token_max<LPT>(fmaxf(finite_size(first), two ? finite_size(second) : 0.0f));
+      if (__ballot(p.top_groups < p.groups && !((double)least - most > 2 * route_margin(0) * fmax(1.0, size)))) {
         double first = -__builtin_inf(), second = -__builtin_inf();
 #pragma unroll 1
         for (int i = 0; i < per; ++i) {
