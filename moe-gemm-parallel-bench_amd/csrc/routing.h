@@ -449,6 +449,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
         return __builtin_bit_cast(float, dpp<decltype(ctrl)::value>(__builtin_bit_cast(uint32_t, f)));
       });
       const float score = two ? first + second : first;
+      lost |= score != score;  // inf - inf
       mine_in = place(score) < p.top_groups;
       const float least = -token_max<LPT>(mine_in ? -score : -__builtin_inff());
       const float most = token_max<LPT>(mine_in ? -__builtin_inff() : score);

@@ -11,6 +11,8 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
+INF = float("inf")
+
 
 @pytest.fixture(autouse=True)
 def _gpu_only():
@@ -45,3 +47,21 @@ def test_group_sums_of_large_terms_that_cancel(step, size, experts, groups):
         first = c[:, :, 0].gather(1, kept)
         expected = kept.gather(1, first.sort(dim=1, descending=True).indices) * each
         assert torch.equal(chosen.cpu().long(), expected), top
+
+
+@pytest.mark.parametrize("experts,groups", [(32, 4), (256, 8), (896, 8), (40, 5)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_group_sum_that_is_no_number_ranks_last(score, experts, groups):
+    """A bias of inf beside -inf throughout a group: inf - inf, which no other group's sum is below."""
+    from kernels import route_topk
+
+    each = experts // groups
+    x = torch.randn(20, experts, generator=torch.Generator().manual_seed(experts))
+    bias = torch.zeros(experts)
+    bias[:each] = -INF
+    bias[1] = INF
+    for top in (1, groups - 1):
+        _, chosen = route_topk(x.cuda(), 2, score=score, bias=bias.cuda(), groups=groups, top_groups=top, group_best=2)
+        assert int(chosen.min()) >= each and (chosen[:, 0] != chosen[:, 1]).all()
+    _, chosen = route_topk(x.cuda(), 2, score=score, bias=bias.cuda(), groups=groups, group_best=2)
+    assert (chosen[:, 0] == 1).all()  # all groups kept: the largest score
