@@ -63,7 +63,7 @@ struct RowParts {
     } else {
       typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
       typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
-      constexpr float kMost = 0x1p120f;  // above what is left of any number
+      constexpr float kLargest = 0x1.fffffep127f;
       u16x8_t hi, mid, lo;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -74,10 +74,11 @@ struct RowParts {
         } else {
           f = (float)__builtin_bit_cast(f16x8_t, x.v[0])[i];
         }
-        const uint32_t top = __builtin_bit_cast(uint32_t, f) & 0xffff0000u;
-        hi[i] = (uint16_t)(top >> 16);
-        // What is left of an infinity, which hi holds whole, or a NaN is a NaN, of which the median makes a number.
-        const float rest = __builtin_amdgcn_fmed3f(f - __builtin_bit_cast(float, top), -kMost, kMost);
+        hi[i] = (uint16_t)(__builtin_bit_cast(uint32_t, f) >> 16);
+        // Of an infinity or a NaN, which hi holds whole, the median makes the largest number, and the parts behind hi are
+        // what is left of that: of an infinity's sign, so that no product of theirs opposes an infinite one.
+        const float number = __builtin_amdgcn_fmed3f(f, -kLargest, kLargest);
+        const float rest = number - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, number) & 0xffff0000u);
         const uint32_t next = __builtin_bit_cast(uint32_t, rest) & 0xffff0000u;
         mid[i] = (uint16_t)(next >> 16);  // of fp16 all that is left
         if constexpr (A::is_f32) lo[i] = __builtin_bit_cast(uint16_t, (__bf16)(rest - __builtin_bit_cast(float, next)));
