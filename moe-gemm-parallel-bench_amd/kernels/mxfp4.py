@@ -17,8 +17,8 @@ rounding, at the end (256 rows over 32 experts of [7168, 2048]: 60 us for the se
 
 The products are made for decode, where an expert has few rows and reading its weights is the bound; they take any number
 of rows, but past 128 an expert a bf16 copy (``dequantize_mxfp4``) and ``grouped_mm`` are faster.  Each call runs on the current stream, reads ``offs`` on the device and keeps nothing, so it can be captured in a
-HIP graph; repeated calls give the same bits.  ``ValueError`` for operands a kernel cannot take, ``RuntimeError`` without
-library or GPU.
+HIP graph; repeated calls give the same bits.  Serving only: the products have no gradient, and rows that ask for one are
+refused.  ``ValueError`` for operands a kernel cannot take, ``RuntimeError`` without library or GPU.
 """
 
 from __future__ import annotations
@@ -131,6 +131,8 @@ def _check_weight(weight, scale, k: int) -> None:
 def _product(entry: str, a, weight, scale, offs, out, out_dtype, variant, gated: bool):
     import torch
 
+    if a.requires_grad and torch.is_grad_enabled():
+        raise ValueError("4-bit products have no gradient: pass a.detach(), or call them under torch.no_grad()")
     grouped = offs is not None
     shape = weight.shape
     if a.ndim != 2 or len(shape) != (3 if grouped else 2):

@@ -1,7 +1,7 @@
 """Routing on gfx950: each token's experts, and the way to expert-sorted rows and back.
 
-What stands before and behind the experts' products, which take expert-sorted rows and their end offsets.  A step of a
-mixture-of-experts layer::
+What stands before and behind the experts' products, which take expert-sorted rows and their end offsets.  A serving step
+of a mixture-of-experts layer::
 
     weights, experts = route_topk(logits, 8)                # [T, 8] fp32 and int32
     order = sort_by_expert(experts, num_experts)            # end offsets, and where each token's slots went
@@ -9,10 +9,12 @@ mixture-of-experts layer::
     ys = grouped_mm(grouped_mm_swiglu(xs, w13, order.offs), w2, order.offs)
     out = combine_rows(ys, order, weights)                  # [T, H], weighted
 
-``route_topk``, ``gather_rows`` and ``combine_rows`` are differentiable; ``route_topk_backward`` and
-``combine_rows_backward`` are the gradients for programs that run their own backward pass, and the gradient of
-``gather_rows`` is ``combine_rows`` of the sorted rows' gradient.  An expert-parallel rank sorts for its own experts
-(``first``, ``num_experts``); slots of other ranks' experts get no row.
+In training ``gate_up_swiglu`` takes the place of ``grouped_mm_swiglu``; ``grouped_mm`` keeps no history, so the gradient of the
+second product is the program's own (``grouped_mm`` of the transposed weight for the rows).  ``route_topk``, ``gather_rows`` and
+``combine_rows`` are differentiable; ``route_topk_backward`` and ``combine_rows_backward`` are the
+gradients for programs that run their own backward pass, and the gradient of ``gather_rows`` is ``combine_rows`` of the
+sorted rows' gradient.  An expert-parallel rank sorts for its own experts (``first``, ``num_experts``); slots of other ranks'
+experts get no row.
 
 Calls run on the current stream of their tensors' device, read no counts back and keep nothing, so they can be captured in
 a HIP graph; repeated calls give the same bits.  ``ValueError`` for arguments the kernels cannot take, ``RuntimeError``
