@@ -533,6 +533,16 @@ def _device_calls():
     return torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
+def refuse_tangents(name: str, *tensors) -> None:
+    """``ValueError`` where a forward-mode derivative is being taken of one of the tensors (or Nones): there is none."""
+    import torch
+
+    forward_ad = torch.autograd.forward_ad
+    if forward_ad._current_level >= 0:  # else no tensor has a tangent
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise ValueError(f"{name} has no forward-mode derivative")
+
+
 def launch(device, entry, *args) -> None:
     """``entry(*args, stream)`` on ``device``'s current stream; a kernel goes to the current device, so that is made
     ``device`` where it is another."""

@@ -133,6 +133,7 @@ def _product(entry: str, a, weight, scale, offs, out, out_dtype, variant, gated:
 
     if a.requires_grad and torch.is_grad_enabled():
         raise ValueError("4-bit products have no gradient: pass a.detach(), or call them under torch.no_grad()")
+    _native.refuse_tangents("a 4-bit product", a)
     grouped = offs is not None
     shape = weight.shape
     if a.ndim != 2 or len(shape) != (3 if grouped else 2):

@@ -11,8 +11,8 @@ of a mixture-of-experts layer::
 
 In training ``gate_up_swiglu`` takes the place of ``grouped_mm_swiglu``; ``grouped_mm`` keeps no history, so the gradient of the
 second product is the program's own (``grouped_mm`` of the transposed weight for the rows).  ``route_topk``, ``gather_rows`` and
-``combine_rows`` are differentiable; ``route_topk_backward`` and ``combine_rows_backward`` are the
-gradients for programs that run their own backward pass, and the gradient of ``gather_rows`` is ``combine_rows`` of the
+``combine_rows`` are differentiable, in reverse mode only; ``route_topk_backward`` and ``combine_rows_backward`` are the
+gradients for programs that run their own backward pass (without a history of their own), and the gradient of ``gather_rows`` is ``combine_rows`` of the
 sorted rows' gradient.  An expert-parallel rank sorts for its own experts (``first``, ``num_experts``); slots of other ranks'
 experts get no row.
 
@@ -87,6 +87,7 @@ def route_topk(logits, k: int, *, score: str = "softmax", bias=None, groups: int
     """
     import torch
 
+    _native.refuse_tangents("route_topk", logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _functions()[0].apply(logits, k, score, bias, groups, top_groups, group_best, normalize, scale)
     return _route(logits, k, score, bias, groups, top_groups, group_best, normalize, scale)
@@ -209,6 +210,7 @@ def gather_rows(x, order: ExpertOrder, *, rows: int | None = None):
     """
     import torch
 
+    _native.refuse_tangents("gather_rows", x)
     if torch.is_grad_enabled() and x.requires_grad:
         return _functions()[1].apply(x, order, rows)
     return _gather(x, order, rows)
@@ -248,6 +250,7 @@ def combine_rows(y, order: ExpertOrder, weights=None):
     """
     import torch
 
+    _native.refuse_tangents("combine_rows", y, weights)
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
         return _functions()[2].apply(y, weights, order)
     return _combine(y, order, weights)
