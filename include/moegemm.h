@@ -411,8 +411,10 @@ int moegemm_gate_up_backward(const void* dh, const void* x, const void* w, const
  *
  * moegemm_route_topk: s = softmax(logits) (sigmoid 0) or sigmoid(logits) (1) over expert_count experts (at most 1024),
  * c = s + bias (bias NULL: s).  Of `groups` equal runs of experts the top_groups ones with the largest sums of their
- * group_best (1 or 2) best c are eligible; the k (at most 64) largest c win, ties go to the lowest index.  weights
- * [tokens, k] = s of the chosen, over their sum if normalize (0 where that is 0), times scale; experts [tokens, k].
+ * group_best (1 or 2) best c are eligible; the k (at most 64) largest c win, ties go to the lowest index.  c is compared in
+ * 64 bits; without a bias, and with group_best 1, the logits are, which tells apart scores that 64 bits do not.  weights
+ * [tokens, k] = s of the chosen, over their sum if normalize (sigmoid: 0 where that is 0 in 64 bits; softmax: the softmax of
+ * the chosen logits, 0 where all of them are -inf), times scale; experts [tokens, k].
  * logits is [tokens, expert_count] (dtype; unit stride along the experts).  A NaN logit ranks below every other.
  * moegemm_route_topk_backward: the logits' gradient [tokens, expert_count] (contiguous, dtype) for dweights, through s; an
  * index outside the experts counts for nothing, a token's are distinct.

@@ -78,12 +78,15 @@ def route_topk(logits, k: int, *, score: str = "softmax", bias=None, groups: int
     ``s = softmax(logits)`` or ``sigmoid(logits)`` over the experts; ``c = s + bias`` (fp32 [E], or none) chooses.  With
     ``groups`` equal runs of experts, only the ``top_groups`` (default: all) runs with the largest sums of their
     ``group_best`` (1 or 2) best ``c`` are eligible.  The ``k`` largest ``c`` win; ties go to the lowest index, of groups
-    too.  ``weights = s`` of the chosen, divided by their sum if ``normalize`` (0 where that is 0), times ``scale``.
+    too, and 0.0 and -0.0 are one number.  ``weights = s`` of the chosen, divided by their sum if ``normalize``, times ``scale``
+    (held in fp32).  Divided, a softmax's are the softmax of the chosen logits alone, also where every chosen score
+    underflows; they are 0 where the chosen logits are all -inf, and a sigmoid's where their 64-bit sum is 0.
 
     logits: fp16, bf16 or fp32 [T, E] with unit stride along E, E at most 1024 and k at most 64.  Choices are made on 64-bit
-    scores, so they do not hang on the rounding of an exponential.  A logit of -inf has score 0; a NaN ranks below every
-    other score, and makes all softmax weights of its token NaN.  Differentiable in logits (through ``s``; the choice is
-    taken as given, and no gradient goes to ``bias``).
+    scores, so they do not hang on the rounding of an exponential; without a bias, and with ``group_best`` 1, the logits rank,
+    which is the scores' order and tells apart what is equal in 64 bits (sigmoids past 37; softmax scores that underflow).  A
+    logit of -inf has score 0; a NaN ranks below every other score, and makes all softmax weights of its token NaN.
+    Differentiable in logits (through ``s``; the choice is taken as given, and no gradient goes to ``bias``).
     """
     import torch
 
