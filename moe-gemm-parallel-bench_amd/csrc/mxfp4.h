@@ -186,7 +186,7 @@ struct MxStream {
   static constexpr int MIN_WAVES = SHARED && PARTS > 1 && BM <= 16 ? 3 : !SHARED && PARTS == 3 && !EIGHT ? 1 : 2;
   static constexpr int PER_CU = SHARED ? MIN_WAVES : 4;
   // Blocks of weights on their way.  256 rows over 32 experts of [4096, 7168] 86 us with three, 89 with one; over
-  // [7168, 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32: 128 and 127, 71 and
+  // [7168, 2048] 56 and 60.  Rows of two parts, whose matrix instructions take twice as long, fp32 by two of their parts: 128 and 127, 71 and
   // 65; 2048 rows, 64 a unit, over [4096, 7168] 219 and 210; waves with a part of K, one row of [5760, 2880] 6.6 and
   // 5.7.
   static constexpr int AHEAD = SHARED && PARTS == 1 && BM <= 32 ? 3 : 1;
@@ -228,11 +228,12 @@ __device__ __forceinline__ u32x4_t mx_load16(mx_rsrc_t r, uint32_t offset) {
 // part the next block or row reads soon after (256 rows over 128 experts of [5760, 2880]: 255 us, kept 232), or where a
 // group's other units read the weights too (2048 rows over 32 of [7168, 2048], 32 a unit: 152 us, kept 134).
 //
-// Decode is bound by HBM's reads: 256 bf16 rows over 32 experts of [4096, 7168], 0.50 GB, 86 us, 5.8 TB/s; 4 rows of
-// 128 experts of [5760, 2880], 35 MB, 10.5 us, where the launch, one memory latency after the other and the table are
-// half of it.  fp32 rows cost their split and twice the matrix instructions: vector and matrix instructions fill seven
-// tenths of the cycles, 256 by [7168, 2048] 60 us, bf16 51 (0.25 GB, 5.0 TB/s).  From 64 rows a group on the matrix
-// pipes and the conversions are the bound: 16384 rows over 32 experts of [4096, 7168] 1191 us, 0.81 PFLOP/s.
+// Decode is bound by HBM's reads: 256 bf16 rows over 32 experts of [4096, 7168], 0.50 GB, 88 to 92 us, 5.4 to 5.7 TB/s;
+// 4 rows of 128 experts of [5760, 2880], 35 MB, 11.8 us, of which the launch, one memory latency after the other and
+// the table are an estimated half.  fp32 rows cost their split and three times the matrix instructions: vector and
+// matrix instructions fill nearly nine tenths of the cycles, 256 by [7168, 2048] 61 to 67 us, bf16 53 (0.25 GB, 4.8
+// TB/s).  From 64 rows a group on the matrix pipes and the conversions are the bound: 16384 rows over 32 experts of
+// [4096, 7168] 1191 us, 0.81 PFLOP/s.
 template <class T, bool ONCE>
 __global__ void __launch_bounds__(T::NT, T::MIN_WAVES) mx_stream_kernel(MxParams p) {
   using A = typename T::A;
@@ -560,7 +561,7 @@ __device__ __forceinline__ void mx_item(const MxConvertParams& p, int64_t i, int
 
 // scale = floor(log2 max|x|) - 2 as an e8m0 byte, at least 0: e2m1's largest power of two is 4.  q = e2m1(x / scale),
 // to nearest even, at most 6.  A group that holds a NaN or an infinity gets the scale 255, a NaN. Bound by HBM: 8 x
-// [5760, 2880] in fp32 96 us, 6.3 TB/s read and written.  Values are read once, past the caches.
+// [5760, 2880] in fp32 95 to 98 us, 6.1 to 6.3 TB/s read and written.  Values are read once, past the caches.
 template <class E, bool VEC>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(MxConvertParams p) {
   using raw_t = typename E::raw;

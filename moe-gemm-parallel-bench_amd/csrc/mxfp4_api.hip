@@ -71,9 +71,10 @@ hipError_t launch_dequantize(const MxConvertParams& p, hipStream_t s) {
 constexpr double kUnitTime[3][kNumMx] = {
     {1.15, 1.36, 1.72, 0.46, 0.67, 2.55}, {1.57, 1.66, 2.90, 0.72, 0.95, 2.90}, {1.76, 1.94, 3.80, 0.80, 1.15, 3.80}};
 // Of 207 calls (10 weights, 1 to 1024 rows, three types) the chosen one took 1.01 times the best one's time in the
-// mean, at most 1.32; of 144 calls of three parts (11 weights, 1 to 2048 rows) 1.01 times, at most 1.19.  What the variants take, in the same order (us, bf16): 32 experts of [4096, 7168] by 256 rows
-// 122, 88, 99, 161, 135, 131; by 1024 rows 340, 204, 162, 467, 369, 151; one weight of [4096, 7168] by 16 rows 22, 25,
-// 31, 11, 13, 46; by 32 rows 23, 24, 31, 18, 14, 47.
+// mean, at most 1.32; of 144 calls of three parts (11 weights, 1 to 2048 rows) 1.01 times, at most 1.19.  What the
+// variants take, in the same order (us, bf16): 32 experts of [4096, 7168] by 256 rows 122, 88, 99, 161, 135, 131; by
+// 1024 rows 340, 204, 162, 467, 369, 151; one weight of [4096, 7168] by 16 rows 22, 25, 31, 11, 13, 46; by 32 rows 23,
+// 24, 31, 18, 14, 47.
 int choose(int parts, const MxVariant* table, int64_t rows, int64_t groups, int64_t cols, int cus) {
   const int64_t active = std::min(groups, rows);
   const double mean = (double)rows / active;

@@ -324,9 +324,12 @@ __device__ __forceinline__ void join_lists_across(uint32_t (&a)[N]) {
 // route_token, one token after the other.  16-bit logits that rank by themselves leave 13 bits free: their order is
 // exact, and equal ones are in order.
 //
-// Bound by the vector instructions, about 250 a token of 256 experts.  16384 tokens, 8 of 256 experts: by their logits
-// 8.4 us, by sigmoid with a bias 10.0, 4 of 8 groups too 15.0 (1.1 TB/s of logits); 4097 tokens, 16 of 896 by softmax
-// unnormalised 17.5; one token 4.5, a launch and the chain of its steps.
+// Bound by the vector instructions: 320 a token of 256 experts with groups, 7 tenths of the busy cycles, and 9 tenths of 896
+// experts.  16384 tokens, 8 of 256 experts, fp32: by their logits 9.5 us, by sigmoid with a bias 11.1, 4 of 8 groups too
+// 13.3 to 15.4, by how many are close (1.1 TB/s of logits); 4097 tokens, 16 of 896 bf16 by softmax unnormalised 17.3; one
+// token 4.7, a launch and the chain of its steps.  Softmax scores with a bias pay for closeness most, since the margin is
+// that of scores up to 1: 16384 x 256 of logits N(0, 1.5) 16.8, of N(0, 0.02), a router that has not learnt yet, 77 (one
+// token after the other; by route_exact_kernel 47).
 enum RouteRank {
   RANK_LOGITS,      // scores rank as the logits do
   RANK_LOGITS_SUM,  // and a softmax's sum over all experts is needed for the weights
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams p) {
 }
 
 // Every token on 64-bit scores, one a wave: for lists longer than route_kernel's, and groups that its lanes cannot
-// hold. Bound by the k rounds of a maximum over the wave: 16384 tokens, 8 of 256 experts 42 us, 4 of 8 groups too 67.
+// hold. Bound by the k rounds of a maximum over the wave: 16384 tokens, 8 of 256 experts 44 us, 4 of 8 groups too 64.
 template <class E>
 __global__ void __launch_bounds__(256) route_exact_kernel(RouteParams p) {
   extern __shared__ uint64_t s_key[];
@@ -555,8 +558,9 @@ __global__ void __launch_bounds__(256) route_exact_kernel(RouteParams p) {
 
 // Gradient of the logits through the chosen scores.  64 / LPT tokens a wave; a lane of a token's first k holds a chosen
 // expert. Where the gradient is not dense it is k numbers among zeros, put together in LDS and stored in whole lines.
-// Bound by HBM where there are many tokens: 16384 x 256 fp32 6.5 us, 2.6 TB/s written; the dense one by 64-bit
-// exponentials, 4097 x 896 9.3 us.
+// 16384 x 256 fp32 6.4 us, 2.6 TB/s written: bound by a launch and the chain of its steps (chosen, their logits, the
+// exponential, LDS, stores), with vector instructions in 4 tenths of the busy cycles.  The dense one by 64-bit
+// exponentials, 4097 x 896 bf16 9.6 us, 7 tenths.
 template <class E, int LPT, int PER>
 __global__ void __launch_bounds__(256) route_backward_kernel(RouteParams p) {
   constexpr int TOKENS = 64 / LPT;

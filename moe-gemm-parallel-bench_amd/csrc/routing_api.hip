@@ -42,7 +42,7 @@ constexpr int64_t kMaxBlocks = 1 << 16;  // workgroups of a launch; they go on t
 
 // Whether route_kernel can choose: k on a list of `top` with two to spare where scores may be too close to call, and
 // groups that are whole lanes' experts, as many to each.  Else every token takes the 64-bit path (16384 tokens, 8 of
-// 256 experts, sigmoid with a bias: 10.0 us and 41.8; 4 of 8 groups 15.5 and 66.9).
+// 256 experts, sigmoid with a bias: 11.2 us and 43.9; 4 of 8 groups 15.2 and 63.8).
 template <class E, RouteRank RANK>
 bool fast_route(const RouteParams& p, int lanes, int top) {
   return p.k <= (RANK >= RANK_SIGMOID || E::is_f32 ? top - 2 : top) &&
@@ -57,8 +57,10 @@ hipError_t launch_choice(const RouteParams& p, hipStream_t stream) {
   hipLaunchKernelGGL((route_kernel<E, LPT, PER, TOP, RANK>), route_grid(p, 256 / LPT), dim3(256), route_lds(p), stream, p);
   return hipGetLastError();
 }
-// 16 lanes a token for lists of 16 from up to 256 experts, else all 64 (16384 tokens, 256 experts by their logits: 16
-// lanes and a list of 16 8.4 us, 64 lanes and a list of 32 42).
+// 16 lanes a token for lists of 16 from up to 256 experts, else all 64 (16384 tokens, 256 experts by fp32 logits: 14 by 16
+// lanes and a list of 16 9.4 us, 15 by 64 lanes and a list of 32 44).  A list of 32 against the 64-bit path, which it
+// stands in front of for 15 to 30 (WHOLE: 17 to 32) experts: 15 of 256 44 and 70 us, 30 of 256 45 and 127; 4097 tokens, 15
+// of 896 20 and 53, 30 of 896 19 and 93; 64 tokens, 15 of 256 5.0 and 19.7.
 template <class E, RouteRank RANK>
 hipError_t launch_choice(const RouteParams& p, hipStream_t stream) {
   if (p.experts <= 256 && fast_route<E, RANK>(p, 16, 16)) {

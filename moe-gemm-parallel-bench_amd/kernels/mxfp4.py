@@ -13,12 +13,15 @@ A serving step of one expert layer::
     y = grouped_mm_mxfp4(h, w2, s2, offs)                           # [rows, H]
 
 h is rounded to x's 16 bits between the two; ``out_dtype=torch.float32`` in the first and x's in the second leaves one
-rounding, at the end (256 rows over 32 experts of [7168, 2048]: 60 us for the second, of bf16 rows 51).
+rounding, at the end (256 rows over 32 experts of [7168, 2048]: 66 us for the second, of bf16 rows 53).
 
-The products are made for decode, where an expert has few rows and reading its weights is the bound; they take any number
-of rows, but past 128 an expert a bf16 copy (``dequantize_mxfp4``) and ``grouped_mm`` are faster.  Each call runs on the current stream, reads ``offs`` on the device and keeps nothing, so it can be captured in a
-HIP graph; repeated calls give the same bits.  Serving only: the products have no gradient, and rows that ask for one are
-refused.  ``ValueError`` for operands a kernel cannot take, ``RuntimeError`` without library or GPU.
+The products are made for decode, where an expert has few rows and reading its weights is the bound; they take any
+number of rows, but past 128 an expert a bf16 copy (``dequantize_mxfp4``) and ``grouped_mm`` are faster. Gate+Up is
+``silu(gate) * up`` of [gate | up] rows without a bias: an expert with biases, interleaved rows, a clamp or another
+activation (gpt-oss among them) takes ``grouped_mm_mxfp4`` and its own epilogue. Each call runs on the current stream,
+reads ``offs`` on the device and keeps nothing, so it can be captured in a HIP graph; repeated calls give the same bits.
+Serving only: the products have no gradient, and rows that ask for one are refused. ``ValueError`` for operands a kernel
+cannot take, ``RuntimeError`` without library or GPU.
 """
 
 from __future__ import annotations
